@@ -83,6 +83,11 @@ extern "C" {
  * factors: SVDMLP_EINVAL. */
 #define SVDMLP_FP8_ACT 0x20u
 
+/* svdmlp_rope, svdmlp_rope_append: pairs (2p, 2p + 1) instead of (p, p + rot / 2) */
+#define SVDMLP_ROPE_INTERLEAVED 0x1u
+/* svdmlp_prompt_attention: a token sees the keys up to its own */
+#define SVDMLP_CAUSAL 0x1u
+
 /* status codes */
 #define SVDMLP_OK 0
 #define SVDMLP_EINVAL (-1)
@@ -283,6 +288,92 @@ int svdmlp_svd_mlp_noalloc(const void* x, const void* ug, const void* vg, const 
  * does not belong inside graph capture.
  */
 int svdmlp_noalloc_status(int32_t reset, int64_t wait_bound, void* stream);
+
+/*
+ * The operators around the MLP block of a decoder layer: rotary positions,
+ * attention over prompts and over a paged cache, and the residual sum with its
+ * norms.  They replace the eager pieces of bench/e2e_block.py:72-75, 205-226
+ * (RMSNorm, attention) and add the decode half that it has not.  dtype is
+ * SVDMLP_BF16 or SVDMLP_F32, of every tensor but gains (fp32) and indices.
+ * Softmax statistics and sums are in 32 bits.  Strides are host arrays, in
+ * elements, in the order named (NULL: dense); the last dimension is contiguous.
+ * Query head h belongs to key/value head h / (Hq / Hk).  They need no
+ * workspace but cache attention's, hold no state between calls, and can be
+ * captured into graphs.  Indices are read on the device: one that points
+ * nowhere (a slot or page outside the cache, a sequence outside the rows, a
+ * length beyond the table) is skipped or cut, never followed.
+ */
+
+/*
+ * Rotary positions.  The first rot values of each head of q (T, Hq, D) and
+ * k (T, Hk, D) are turned in pairs (a, b) -> (a c - b s, b c + a s), with
+ * c, s = scale * cos, sin(positions[t] * inv_freq[p]) for pair p < rot / 2, the
+ * angle in 64 bits; the others are copied.  strides: q token, head; k token,
+ * head; q_out token, head; k_out token, head.  An output may be its input.
+ */
+int svdmlp_rope(const void* q, const void* k, const int64_t* positions, const double* inv_freq, void* q_out,
+                void* k_out, const int64_t* strides /* 8 or NULL */, int64_t T, int64_t Hq, int64_t Hk, int64_t D,
+                int64_t rot, float scale, int32_t dtype, uint32_t flags, void* stream);
+
+/*
+ * svdmlp_rope whose turned keys go to a paged cache, and the values v
+ * (T, Hk, D) with them: token t to row slots[t] % page of page slots[t] / page
+ * of k_cache, v_cache (pages, page, Hk, D).  A slot outside the cache (-1:
+ * a token of padding) leaves the cache as it is.  Slots of one call have to
+ * differ; with a slot twice the row is of neither token for sure.  strides: q
+ * token, head; k token, head; v token, head; q_out token, head; k_cache page,
+ * row, head; v_cache page, row, head.
+ */
+int svdmlp_rope_append(const void* q, const void* k, const void* v, const int64_t* positions, const double* inv_freq,
+                       const int64_t* slots, void* q_out, void* k_cache, void* v_cache,
+                       const int64_t* strides /* 14 or NULL */, int64_t T, int64_t pages, int64_t page, int64_t Hq,
+                       int64_t Hk, int64_t D, int64_t rot, float scale, int32_t dtype, uint32_t flags, void* stream);
+
+/*
+ * Attention of B packed sequences onto themselves: out = softmax(scale q k^T) v
+ * within rows cu_seqlens[b] .. cu_seqlens[b + 1] (int32, B + 1; NULL: one
+ * sequence of all T rows), each token seeing its whole sequence or, with
+ * SVDMLP_CAUSAL, the tokens up to itself.  Keys that a row does not see have no
+ * part in it whatever they hold.  Rows of no sequence are left as they were.
+ * D up to 256, head size, strides and addresses whole 16-byte pieces.  strides:
+ * token and head of q, k, v, out.
+ */
+int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out,
+                            const int64_t* strides /* 8 or NULL */, int64_t T, int64_t B, int64_t Hq, int64_t Hk,
+                            int64_t D, float scale, int32_t dtype, uint32_t flags, void* stream);
+
+/*
+ * Attention of n (1 to 64) new tokens of each of B sequences onto a paged cache
+ * that holds lengths[b] tokens, the new ones last among them.  Token i sees all
+ * keys before the new ones, and new key j if tree[b][i][j] (bytes) is nonzero
+ * or, with tree NULL, if j <= i.  Key x of sequence b is row x % page of page
+ * block_table[b][x / page] (int32, width pages a sequence); a page outside the
+ * cache holds no keys.  A token without keys gets zeros (a sequence of length 0
+ * too).  D as svdmlp_prompt_attention.  strides: q sequence, token, head;
+ * k_cache page, row, head; v_cache page, row, head; out sequence, token, head;
+ * block_table sequence; tree sequence, token.  The workspace
+ * (svdmlp_cache_attention_workspace_bytes; may be 0) holds the partial sums of long contexts and needs no clearing.
+ */
+size_t svdmlp_cache_attention_workspace_bytes(int64_t B, int64_t n, int64_t page, int64_t width, int64_t Hq,
+                                              int64_t Hk, int64_t D, int32_t dtype);
+int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                           const int32_t* lengths, const uint8_t* tree, void* out,
+                           const int64_t* strides /* 15 or NULL */, int64_t B, int64_t n, int64_t pages, int64_t page,
+                           int64_t width, int64_t Hq, int64_t Hk, int64_t D, float scale, int32_t dtype,
+                           void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * The sum after a block and the norm before the next:
+ *   b = branch, or post_w * branch / sqrt(mean(branch^2) + eps) with post_w
+ *   r = x + scale * gate * b      (gate (T, d), or (d) with row stride 0, or NULL)
+ *   n = norm_w * r / sqrt(mean(r^2) + eps), of r before its rounding
+ * x, branch (T, d); branch NULL: r = x.  r_out or n_out may be NULL, and may be
+ * x, branch or (row by row) the gate.  Gains fp32, d up to 32768.  strides: rows
+ * of x, branch, gate, r_out, n_out.
+ */
+int svdmlp_residual_norm(const void* x, const void* branch, const float* post_w, const void* gate,
+                         const float* norm_w, void* r_out, void* n_out, const int64_t* strides /* 5 or NULL */,
+                         int64_t T, int64_t d, float scale, float eps, int32_t dtype, void* stream);
 
 /*
  * Per-stage GPU timing (no counterpart in the reference, whose timing is host

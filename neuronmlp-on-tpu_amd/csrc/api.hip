@@ -30,11 +30,14 @@
 //                                    split-K sums use fp32 atomics
 // Every buffer, including the workspace that holds the rank-r intermediates,
 // h and the split-K slices, is owned by the caller.
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 
 #include <algorithm>
 #include <array>
+#include <cmath>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -45,6 +48,7 @@
 #include "dispatch.hpp"
 #include "decode_gemv.hpp"
 #include "decode_layer.hpp"
+#include "decoder.hpp"
 #include "gemm_big.hpp"
 #include "gemm_f8f8.hpp"
 #include "stream.hpp"
@@ -106,13 +110,17 @@ enum Stage : int {
   ST_QUANT,
   ST_D_XU_F8,
   ST_GU_XUV_DUAL,
+  ST_ROPE,
+  ST_PROMPT_ATTENTION,
+  ST_CACHE_ATTENTION,
+  ST_RESIDUAL_NORM,
   ST_COUNT
 };
 const char* const kStageNames[ST_COUNT] = {
     "zero_fill",        "gate_up_xu",       "gate_up_xuv_swiglu", "down_xu",           "down_xuv",
     "decode_gate_up_xu", "decode_gate_up_xuv", "decode_down_xu",   "decode_down_xuv", "finalize",
     "gate_up_xuv_g",    "decode_layer",       "decode_gemv_layer",  "decode_layer_contracted", "quant_h_e4m3", "down_xu_fp8",
-    "gate_up_xuv_dual"
+    "gate_up_xuv_dual", "rope", "prompt_attention", "cache_attention", "residual_norm"
 };
 
 struct Profiler {
@@ -2516,6 +2524,196 @@ int svdmlp_svd_mlp_ranks(const void* x, const void* ug, const void* vg, const vo
                          int32_t w_dtype, uint32_t flags, void* workspace, size_t ws_bytes, void* stream) {
   return svd_mlp_run(x, ug, vg, uu, vu, ud, vd, scales, ld_in, y, T, d, ff, r_g, r_u, r_d, act_dtype, w_dtype, flags,
                      workspace, ws_bytes, stream, nullptr);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// The operators around the MLP block (decoder.hpp).
+// ---------------------------------------------------------------------------
+namespace {
+
+// Compute units of the current device (256 where there is none to ask).
+int device_cus() {
+  return cached_per_device(DC_CUS, [] {
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+      return 256;
+    return cus > 0 ? cus : 256;
+  });
+}
+
+int act_size(int32_t dtype) { return dtype == SVDMLP_BF16 ? 2 : dtype == SVDMLP_F32 ? 4 : 0; }
+
+bool pieces16(std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> elements, int es) {
+  for (const void* p : ptrs)
+    if (((uintptr_t)p & 15u) != 0) return false;
+  for (int64_t e : elements)
+    if (e * es % 16 != 0) return false;
+  return true;
+}
+
+int check_heads(const char* what, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int32_t dtype, int64_t max_d) {
+  if (!act_size(dtype)) return fail("%s: dtype must be bf16 or fp32, got %d", what, (int)dtype);
+  if (T <= 0 || Hq <= 0 || Hk <= 0 || D <= 0) return fail("%s: sizes must be positive", what);
+  if (Hq % Hk != 0) return fail("%s: %lld query heads are no multiple of %lld key/value heads", what, (long long)Hq, (long long)Hk);
+  if (D > max_d) return fail("%s: head size %lld is over %lld", what, (long long)D, (long long)max_d);
+  if (T > 0x7fffffff / Hq || Hq > 65536) return fail("%s: too many rows", what);
+  return SVDMLP_OK;
+}
+
+int rope_call(const char* what, RopeParams& p, int64_t Hq, int64_t Hk, int64_t D, int64_t rot, float scale,
+              int32_t dtype, uint32_t flags, void* stream) {
+  int rc = check_heads(what, p.T, Hq, Hk, D, dtype, 1024);
+  if (rc) return rc;
+  if (!p.q || !p.k || !p.pos || !p.inv_freq || !p.qo || !p.ko) return fail("%s: null pointer", what);
+  if (rot <= 0 || rot % 2 || rot > D) return fail("%s: %lld turned values of a head of %lld (an even number up to it)", what, (long long)rot, (long long)D);
+  if (flags & ~SVDMLP_ROPE_INTERLEAVED) return fail("%s: unsupported flags 0x%x", what, flags);
+  if (!std::isfinite(scale)) return fail("%s: scale must be finite", what);
+  p.Hq = (int)Hq;
+  p.Hk = (int)Hk;
+  p.D = (int)D;
+  p.rot = (int)rot;
+  p.scale = scale;
+  p.interleaved = (flags & SVDMLP_ROPE_INTERLEAVED) != 0;
+  const int es = act_size(dtype);
+  const bool vec = pieces16({p.q, p.k, p.v, p.qo, p.ko, p.vo},
+                            {D, p.interleaved ? rot : rot / 2, rot, p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h, p.qo_t,
+                             p.qo_h, p.ko_p, p.ko_t, p.ko_h, p.vo_p, p.vo_t, p.vo_h}, es);
+  StageScope s(ST_ROPE, (hipStream_t)stream);
+  return check(launch_rope(p, dtype == SVDMLP_BF16, vec, (hipStream_t)stream), what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int svdmlp_rope(const void* q, const void* k, const int64_t* positions, const double* inv_freq, void* q_out,
+                void* k_out, const int64_t* strides, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t rot,
+                float scale, int32_t dtype, uint32_t flags, void* stream) {
+  RopeParams p = {};
+  p.q = q;
+  p.k = k;
+  p.pos = positions;
+  p.inv_freq = inv_freq;
+  p.qo = q_out;
+  p.ko = k_out;
+  p.T = T;
+  const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hq * D, D, Hk * D, D};
+  const int64_t* s = strides ? strides : dense;
+  p.q_t = s[0], p.q_h = s[1], p.k_t = s[2], p.k_h = s[3], p.qo_t = s[4], p.qo_h = s[5], p.ko_t = s[6], p.ko_h = s[7];
+  return rope_call("rope", p, Hq, Hk, D, rot, scale, dtype, flags, stream);
+}
+
+int svdmlp_rope_append(const void* q, const void* k, const void* v, const int64_t* positions, const double* inv_freq,
+                       const int64_t* slots, void* q_out, void* k_cache, void* v_cache, const int64_t* strides,
+                       int64_t T, int64_t pages, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t rot,
+                       float scale, int32_t dtype, uint32_t flags, void* stream) {
+  if (!v || !slots || !v_cache) return fail("rope_append: null pointer");
+  if (pages <= 0 || page <= 0 || page > 0x7fffffff || pages > INT64_MAX / page) return fail("rope_append: pages and page size must be positive");
+  RopeParams p = {};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.pos = positions;
+  p.inv_freq = inv_freq;
+  p.slots = slots;
+  p.qo = q_out;
+  p.ko = k_cache;
+  p.vo = v_cache;
+  p.T = T;
+  p.pages = pages;
+  p.page = (int)page;
+  const int64_t dense[14] = {Hq * D, D, Hk * D, D, Hk * D, D, Hq * D, D, page * Hk * D, Hk * D, D, page * Hk * D, Hk * D, D};
+  const int64_t* s = strides ? strides : dense;
+  p.q_t = s[0], p.q_h = s[1], p.k_t = s[2], p.k_h = s[3], p.v_t = s[4], p.v_h = s[5], p.qo_t = s[6], p.qo_h = s[7];
+  p.ko_p = s[8], p.ko_t = s[9], p.ko_h = s[10], p.vo_p = s[11], p.vo_t = s[12], p.vo_h = s[13];
+  return rope_call("rope_append", p, Hq, Hk, D, rot, scale, dtype, flags, stream);
+}
+
+int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out,
+                            const int64_t* strides, int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D,
+                            float scale, int32_t dtype, uint32_t flags, void* stream) {
+  int rc = check_heads("prompt_attention", T, Hq, Hk, D, dtype, 256);
+  if (rc) return rc;
+  if (!q || !k || !v || !out) return fail("prompt_attention: null pointer");
+  if (B <= 0 || (!cu_seqlens && B != 1)) return fail("prompt_attention: %lld sequences need their bounds", (long long)B);
+  if (B > 0x7fffffff / Hk / 2 || T > (0x7fffffff - 1024) / 2 / Hq) return fail("prompt_attention: too many rows");
+  if (flags & ~SVDMLP_CAUSAL) return fail("prompt_attention: unsupported flags 0x%x", flags);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail("prompt_attention: scale must be positive and finite");
+  const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hk * D, D, Hq * D, D};
+  const int64_t* s = strides ? strides : dense;
+  const int es = act_size(dtype);
+  if (!pieces16({q, k, v, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]}, es))
+    return fail("prompt_attention: the head size, strides and addresses must be whole 16-byte pieces");
+  PromptParams p = {q, k, v, out, cu_seqlens, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], (int)T, (int)B, (int)Hq,
+                    (int)Hk, (int)D, scale * 1.44269504088896340736f, (flags & SVDMLP_CAUSAL) != 0};
+  StageScope sc(ST_PROMPT_ATTENTION, (hipStream_t)stream);
+  return check(launch_prompt_attention(p, dtype == SVDMLP_BF16, (hipStream_t)stream), "prompt_attention");
+}
+
+size_t svdmlp_cache_attention_workspace_bytes(int64_t B, int64_t n, int64_t page, int64_t width, int64_t Hq, int64_t Hk,
+                                              int64_t D, int32_t dtype) {
+  if (!act_size(dtype) || B <= 0 || B > 0x7fffffff / 64 || n <= 0 || n > 64 || Hq <= 0 || Hq > 65536 || Hk <= 0 || Hq % Hk || D <= 0 || D > 256 ||
+      page <= 0 || width <= 0 || page > 0x7fffff00 / width)
+    return 0;
+  int splits, chunk;
+  plan_cache_attention((int)B, (int)n, (int)Hq, (int)Hk, (int)D, dtype == SVDMLP_BF16, (int)page, page * width, device_cus(), &splits, &chunk);
+  return (size_t)cache_part_floats((int)B, (int)n, (int)Hq, (int)D, splits) * 4;
+}
+
+int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                           const int32_t* lengths, const uint8_t* tree, void* out, const int64_t* strides,
+                           int64_t B, int64_t n, int64_t pages, int64_t page, int64_t width, int64_t Hq, int64_t Hk,
+                           int64_t D, float scale, int32_t dtype, void* workspace, size_t ws_bytes, void* stream) {
+  if (B <= 0 || n <= 0) return fail("cache_attention: sizes must be positive");
+  if (n > 64) return fail("cache_attention: at most 64 new tokens a sequence, got %lld", (long long)n);
+  int rc = check_heads("cache_attention", B > 0x7fffffff / 64 ? INT64_MAX : B * n, Hq, Hk, D, dtype, 256);
+  if (rc) return rc;
+  if (!q || !k_cache || !v_cache || !block_table || !lengths || !out) return fail("cache_attention: null pointer");
+  if (pages <= 0 || page <= 0 || width <= 0 || page > 0x7fffff00 / width)
+    return fail("cache_attention: pages, page size and the table's width must be positive, with less than 2^31 tokens a sequence");
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail("cache_attention: scale must be positive and finite");
+  const int64_t dense[15] = {n * Hq * D, Hq * D, D, page * Hk * D, Hk * D, D, page * Hk * D, Hk * D, D,
+                             n * Hq * D, Hq * D, D, width, n * n, n};
+  const int64_t* s = strides ? strides : dense;
+  const int es = act_size(dtype);
+  if (!pieces16({q, k_cache, v_cache, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10], s[11]}, es))
+    return fail("cache_attention: the head size, strides and addresses must be whole 16-byte pieces");
+  CacheParams p = {};
+  p.q = q, p.kc = k_cache, p.vc = v_cache, p.table = block_table, p.lengths = lengths, p.tree = tree, p.out = out;
+  p.q_b = s[0], p.q_t = s[1], p.q_h = s[2], p.k_p = s[3], p.k_t = s[4], p.k_h = s[5], p.v_p = s[6], p.v_t = s[7], p.v_h = s[8];
+  p.o_b = s[9], p.o_t = s[10], p.o_h = s[11], p.table_b = s[12], p.tree_b = s[13], p.tree_q = s[14];
+  p.pages = pages, p.page = (int)page, p.width = (int)width;
+  p.B = (int)B, p.n = (int)n, p.Hq = (int)Hq, p.Hk = (int)Hk, p.D = (int)D;
+  p.c = scale * 1.44269504088896340736f;
+  plan_cache_attention(p.B, p.n, p.Hq, p.Hk, p.D, dtype == SVDMLP_BF16, p.page, page * width, device_cus(), &p.splits, &p.chunk);
+  const size_t need = (size_t)cache_part_floats(p.B, p.n, p.Hq, p.D, p.splits) * 4;
+  if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15u)))
+    return fail("cache_attention: workspace too small: %zu bytes needed, 16-byte aligned, got %zu", need, ws_bytes);
+  p.part = static_cast<float*>(workspace);
+  StageScope sc(ST_CACHE_ATTENTION, (hipStream_t)stream);
+  return check(launch_cache_attention(p, dtype == SVDMLP_BF16, (hipStream_t)stream), "cache_attention");
+}
+
+int svdmlp_residual_norm(const void* x, const void* branch, const float* post_w, const void* gate,
+                         const float* norm_w, void* r_out, void* n_out, const int64_t* strides, int64_t T, int64_t d,
+                         float scale, float eps, int32_t dtype, void* stream) {
+  const int es = act_size(dtype);
+  if (!es) return fail("residual_norm: dtype must be bf16 or fp32, got %d", (int)dtype);
+  if (T <= 0 || d <= 0 || T > 0x7fffffff) return fail("residual_norm: sizes must be positive");
+  if (d > kResidualNormMaxD) return fail("residual_norm: rows of %lld values, at most %d", (long long)d, kResidualNormMaxD);
+  if (!x || (!r_out && !n_out) || (n_out && !norm_w)) return fail("residual_norm: null pointer");
+  if (!branch && (post_w || gate)) return fail("residual_norm: a post norm or gate needs a branch");
+  if (!(eps > 0.f) || !std::isfinite(eps)) return fail("residual_norm: eps must be positive");
+  if (!std::isfinite(scale)) return fail("residual_norm: scale must be finite");
+  const int64_t dense[5] = {d, d, d, d, d};
+  const int64_t* s = strides ? strides : dense;
+  ResidualNormParams p = {x, branch, post_w, gate, n_out ? norm_w : nullptr, r_out, n_out, s[0], s[1], s[2], s[3], s[4],
+                          T, (int)d, scale, eps};
+  const bool vec = pieces16({x, branch, post_w, gate, norm_w, r_out, n_out}, {d, s[0], s[1], s[2], s[3], s[4]}, es);
+  StageScope sc(ST_RESIDUAL_NORM, (hipStream_t)stream);
+  return check(launch_residual_norm(p, dtype == SVDMLP_BF16, vec, (hipStream_t)stream), "residual_norm");
 }
 
 }  // extern "C"

@@ -1,0 +1,84 @@
+// Parameters and launchers of the operators around the MLP block of a decoder
+// layer: rotary positions (rope.hip), attention over packed prompts
+// (prompt_attention.hip), attention over a paged cache (cache_attention.hip),
+// and the residual sum with the norms on both sides of a block (norm.hip).
+// Strides are in elements; the last dimension of every tensor is contiguous.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace svdmlp {
+
+struct RopeParams {
+  const void* q;  // (T, Hq, D)
+  const void* k;  // (T, Hk, D)
+  const void* v;  // (T, Hk, D), append only
+  const int64_t* pos;      // (T)
+  const double* inv_freq;  // (rot / 2)
+  void* qo;  // (T, Hq, D)
+  void* ko;  // (T, Hk, D), or the key cache (pages, page, Hk, D)
+  void* vo;  // the value cache, append only
+  const int64_t* slots;  // (T): page * page_size + row; null: ko is (T, Hk, D)
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;
+  int64_t qo_t, qo_h;
+  int64_t ko_p, ko_t, ko_h, vo_p, vo_t, vo_h;  // page, token and head strides of the outputs (page: append only)
+  int64_t T, pages;
+  int page, Hq, Hk, D, rot;
+  float scale;  // on cos and sin
+  int interleaved;
+};
+hipError_t launch_rope(const RopeParams& p, bool bf16, bool vec, hipStream_t st);
+
+struct ResidualNormParams {
+  const void* x;       // (T, d) the residual stream
+  const void* branch;  // (T, d) the block's output, or null
+  const float* post;   // (d) gains of the norm of the branch, or null
+  const void* gate;    // (T, d) or (d) (g_t = 0), or null
+  const float* weight; // (d) gains of the norm of r, or null
+  void* r;             // (T, d), or null
+  void* n;             // (T, d), or null
+  int64_t x_t, b_t, g_t, r_t, n_t;
+  int64_t T;
+  int d;
+  float scale, eps;
+};
+constexpr int kResidualNormMaxD = 32768;
+hipError_t launch_residual_norm(const ResidualNormParams& p, bool bf16, bool vec, hipStream_t st);
+
+struct PromptParams {
+  const void *q, *k, *v;  // (T, Hq, D), (T, Hk, D) twice
+  void* out;              // (T, Hq, D)
+  const int* cu;          // (B + 1) first row of each sequence and the end of the last; null: one sequence of T rows
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h;
+  int T, B, Hq, Hk, D;
+  float c;  // softmax scale * log2(e)
+  int causal;
+};
+hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, hipStream_t st);
+
+struct CacheParams {
+  const void* q;          // (B, n, Hq, D)
+  const void *kc, *vc;    // (pages, page, Hk, D)
+  const int* table;       // (B, width) pages of each sequence in order
+  const int* lengths;     // (B) tokens held, the n new ones among them
+  const uint8_t* tree;    // (B, n, n) or (n, n) (tree_b = 0) bytes, or null: a chain
+  void* out;              // (B, n, Hq, D)
+  float* part;            // split partials (cache_attention.hip), or null with splits == 1
+  int64_t q_b, q_t, q_h, k_p, k_t, k_h, v_p, v_t, v_h, o_b, o_t, o_h, table_b, tree_b, tree_q;
+  int64_t pages;
+  int page, width, B, n, Hq, Hk, D;
+  int splits, chunk;  // keys are cut into chunks of `chunk` (a multiple of the key tile), one a block
+  float c;
+};
+// Splits of a call: how many chunks of how many keys cover the table's
+// `capacity` keys.
+void plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, int page, int64_t capacity, int cus,
+                          int* splits, int* chunk);
+// Floats of one (sequence, split, query, head) partial: D sums, the maximum and the sum of weights.
+inline int64_t cache_part_floats(int B, int n, int Hq, int D, int splits) {
+  return splits > 1 ? (int64_t)B * n * Hq * splits * (D + 2) : 0;
+}
+hipError_t launch_cache_attention(const CacheParams& p, bool bf16, hipStream_t st);
+
+}  // namespace svdmlp

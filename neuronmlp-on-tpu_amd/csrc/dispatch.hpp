@@ -115,7 +115,7 @@ hipError_t launch_quant_rows_e4m3(const uint16_t* h, int64_t ldh, uint8_t* q, in
 // A per-device constant (a persistent kernel's grid size) computed once per
 // device and slot: the lookups behind it (device attributes, occupancy) cost
 // host time on every decode call otherwise.
-enum DeviceConst : int { DC_DL1 = 0, DC_DL2, DC_DL4, DC_DL8, DC_DL_CONTRACT, DC_GV1, DC_GV2, DC_COUNT };
+enum DeviceConst : int { DC_DL1 = 0, DC_DL2, DC_DL4, DC_DL8, DC_DL_CONTRACT, DC_GV1, DC_GV2, DC_CUS, DC_COUNT };
 template <class F>
 inline int cached_per_device(int slot, F compute) {
   static std::atomic<int> cache[64][DC_COUNT];  // value + 1; 0 = not yet computed

@@ -1,0 +1,283 @@
+// Attention of packed sequences onto themselves, O = softmax(c Q K^T + mask) V,
+// causal or not; query head h reads key/value head h / (Hq / Hk).
+//
+// A block takes 128 * QG rows of one key/value head and sequence (row = token *
+// G + head of the group: the group's heads share every key and value that the
+// block loads) and walks the keys in tiles through LDS, one pass, with the
+// running maximum and sum.
+#include <math.h>
+
+#include "attn.hpp"
+#include "decoder.hpp"
+
+namespace svdmlp {
+
+namespace {
+
+template <bool BF16_, int DP_, int QG_>
+struct PromptCfg {
+  static constexpr bool BF16 = BF16_;
+  static constexpr int DP = DP_;  // head elements held (D rounded up)
+  static constexpr int QG = QG_;  // 32-row groups a wave
+  static constexpr int ES = BF16 ? 2 : 4;
+  static constexpr int RB = DP * ES;         // bytes of a key row in LDS
+  static constexpr int PIECES = RB / 16;
+  static constexpr int STEPS = RB / 32;      // 32-byte steps of the head
+  static constexpr int KB = BF16 && DP < 256 ? 64 : 32;  // keys a tile
+  static constexpr int BM = 128 * QG;        // rows a block
+  static constexpr int TILE = KB * RB;
+};
+
+template <class C>
+__global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
+  constexpr bool BF16 = C::BF16;
+  constexpr int ES = C::ES, RB = C::RB, QG = C::QG, KB = C::KB, DB = C::DP / 32;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * C::TILE];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
+  const int G = p.Hq / p.Hk;
+
+  // The block's sequence and row tile: tiles are numbered sequence by
+  // sequence, the last rows (the most keys of a causal call) first.
+  const int hk = blockIdx.x % p.Hk;
+  int tile = blockIdx.x / p.Hk;
+  int start = 0, len = p.T;
+  if (p.cu) {
+    len = -1;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const int b = b0 + lane;
+      int s = 0, n = 0;
+      if (b < p.B) {
+        s = min(max(p.cu[b], 0), p.T);
+        n = min(max(p.cu[b + 1], s), p.T) - s;
+      }
+      const int tiles = (int)(((int64_t)n * G + C::BM - 1) / C::BM);
+      int before = tiles;  // inclusive prefix sum
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(before, o);
+        if (lane >= o) before += v;
+      }
+      const uint64_t hit = __ballot(tile < before);
+      if (hit) {
+        const int i = __builtin_ctzll(hit);
+        tile -= __shfl(before - tiles, i);
+        start = __shfl(s, i);
+        len = __shfl(n, i);
+        break;
+      }
+      tile -= __shfl(before, 63);
+    }
+    if (len < 0) return;  // the grid covers the most tiles that B sequences of T rows can have
+  }
+  const int rows = len * G;
+  const int tiles = (rows + C::BM - 1) / C::BM;
+  if (tile >= tiles) return;
+  const int row0 = (tiles - 1 - tile) * C::BM;
+  const int tok_last = min(len - 1, (row0 + C::BM - 1) / G);
+  const int tok_first = row0 / G;
+  const int nkeys = p.causal ? tok_last + 1 : len;
+
+  // Q: lane half h holds the 16-byte piece 2 s + h of its row at step s.
+  u32x4 qf[QG][C::STEPS];
+  int tok[QG];
+  const int npieces = p.D * ES / 16;
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = row0 + (wave * QG + g) * 32 + col;
+    const bool in = r < rows;
+    tok[g] = in ? r / G : 0;
+    const char* qp = static_cast<const char*>(p.q) +
+                     ((int64_t)(start + tok[g]) * p.q_t + (int64_t)(hk * G + (in ? r - tok[g] * G : 0)) * p.q_h) * ES;
+#pragma unroll
+    for (int s = 0; s < C::STEPS; ++s) {
+      const int c = 2 * s + half;
+      qf[g][s] = in && c < npieces ? *reinterpret_cast<const u32x4*>(qp + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+
+  f32x16 o[QG][DB];
+  RowState st[QG];
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    st[g] = {-INFINITY, 0.f};
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[g][d][i] = 0.f;
+  }
+  const char* const kbase = static_cast<const char*>(p.k) + ((int64_t)start * p.k_t + (int64_t)hk * p.k_h) * ES;
+  const char* const vbase = static_cast<const char*>(p.v) + ((int64_t)start * p.v_t + (int64_t)hk * p.v_h) * ES;
+  const attn_lds lk = (attn_lds)lds, lv = lk + C::TILE;
+  const TileLane<RB, BF16> at(lane);
+  uint32_t bad = 0;
+
+  for (int k0 = 0; k0 < nkeys; k0 += KB) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < KB * C::PIECES / 256; ++j) {
+      const int i = threadIdx.x + 256 * j, row = i / C::PIECES, c = i % C::PIECES;
+      u32x4 kv = {0u, 0u, 0u, 0u}, vv = {0u, 0u, 0u, 0u};
+      if (k0 + row < nkeys && c < npieces) {
+        kv = *reinterpret_cast<const u32x4*>(kbase + (int64_t)(k0 + row) * p.k_t * ES + 16 * c);
+        vv = *reinterpret_cast<const u32x4*>(vbase + (int64_t)(k0 + row) * p.v_t * ES + 16 * c);
+      }
+      *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(lk + row * RB + ((c ^ k_swz<RB>(row)) << 4)) = kv;
+      *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(lv + row * RB + ((c ^ v_swz<RB, BF16>(row)) << 4)) = vv;
+    }
+    __syncthreads();
+    const bool masked = p.causal && k0 + KB - 1 > tok_first;  // not every row sees every key
+    const bool edge = masked || k0 + KB > nkeys;
+#pragma unroll
+    for (int u = 0; u < KB / 32; ++u) {
+      const int ku = k0 + 32 * u;
+      if (ku >= nkeys) break;
+      f32x16 s[QG];
+#pragma unroll
+      for (int g = 0; g < QG; ++g)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[g][i] = 0.f;
+#pragma unroll
+      for (int t = 0; t < C::STEPS; ++t) {
+        const u32x4 kf = at.key(lk + 32 * u * RB, t);
+#pragma unroll
+        for (int g = 0; g < QG; ++g) s[g] = attn_mfma<BF16>(kf, qf[g][t], s[g]);
+      }
+      float pf[QG][16];
+#pragma unroll
+      for (int g = 0; g < QG; ++g) {
+        if (edge) {
+          const int last = p.causal ? min(tok[g], nkeys - 1) : nkeys - 1;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = ku + 8 * (i >> 2) + 4 * half + (i & 3);
+            s[g][i] = key <= last ? s[g][i] : -INFINITY;
+          }
+        }
+        float mx = s[g][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[g][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32)) * p.c;
+        if (__any(mx > st[g].m + kSlack)) {
+          const float m = fmaxf(st[g].m, mx);
+          const float a = m == -INFINITY ? 1.f : exp2f(st[g].m - m);
+          st[g].m = m;
+          st[g].l *= a;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[g][d][i] *= a;
+        }
+        const float m = st[g].m == -INFINITY ? 0.f : st[g].m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          pf[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], p.c, -m));
+          st[g].l += pf[g][i];
+        }
+      }
+      if constexpr (BF16) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {  // 16 keys each
+          u32x4 pb[QG];
+#pragma unroll
+          for (int g = 0; g < QG; ++g)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) pb[g][w] = pack_bf16x2(pf[g][8 * t + 2 * w], pf[g][8 * t + 2 * w + 1]);
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            u32x4 vf = at.values(lv + 32 * u * RB, t, d);
+            if (masked)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) vf[w] = scrub<true>(vf[w], bad);
+#pragma unroll
+            for (int g = 0; g < QG; ++g) o[g][d] = attn_mfma<true>(vf, pb[g], o[g][d]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            uint32_t w = at.value(lv + 32 * u * RB, i, d);
+            if (masked) w = scrub<false>(w, bad);
+#pragma unroll
+            for (int g = 0; g < QG; ++g)
+              o[g][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w), pf[g][i], o[g][d], 0, 0, 0);
+          }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const float l = st[g].l + __shfl_xor(st[g].l, 32);
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[g][d][i] *= inv;
+  }
+  // Infinities and NaN among the values of the masked tiles were taken as
+  // zeros, for the rows that do not see them; the rows that do get them here.
+  if (__any(bad != 0)) {
+    for (int key = (tok_first + 1) / KB * KB; key < nkeys; ++key) {
+      const char* const vp = vbase + (int64_t)key * p.v_t * ES;
+      uint32_t see[QG];
+#pragma unroll
+      for (int g = 0; g < QG; ++g) see[g] = key <= tok[g] ? 0xffffffffu : 0u;
+      int D = p.D;
+      asm volatile("" : "+s"(D));  // its comparisons stay in the loop: hoisted, they spill
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
+          const uint32_t w = e >= D ? 0u : BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(vp)[e] << 16 : reinterpret_cast<const uint32_t*>(vp)[e];
+          const uint32_t mask = not_finite<false>(w);
+#pragma unroll
+          for (int g = 0; g < QG; ++g) o[g][d][i] += __uint_as_float(w & mask & see[g]);
+        }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = row0 + (wave * QG + g) * 32 + col;
+    if (r >= rows) continue;
+    char* op = static_cast<char*>(p.out) +
+               ((int64_t)(start + tok[g]) * p.o_t + (int64_t)(hk * G + (r - tok[g] * G)) * p.o_h) * ES;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int e = 32 * d + 8 * b + 4 * half;
+        if (e >= p.D) continue;
+        if constexpr (BF16)
+          *reinterpret_cast<u32x2*>(op + e * 2) = u32x2{pack_bf16x2(o[g][d][4 * b], o[g][d][4 * b + 1]), pack_bf16x2(o[g][d][4 * b + 2], o[g][d][4 * b + 3])};
+        else
+          *reinterpret_cast<f32x4*>(op + e * 4) = f32x4{o[g][d][4 * b], o[g][d][4 * b + 1], o[g][d][4 * b + 2], o[g][d][4 * b + 3]};
+      }
+  }
+}
+
+template <bool BF16, int DP, int QG>
+hipError_t run(const PromptParams& p, hipStream_t st) {
+  using C = PromptCfg<BF16, DP, QG>;
+  // A sequence's last tile may be short: at most one more tile a sequence.
+  const int64_t tiles = (int64_t)p.T * (p.Hq / p.Hk) / C::BM + p.B;
+  hipLaunchKernelGGL((prompt_kernel<C>), dim3((unsigned)(tiles * p.Hk)), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, hipStream_t st) {
+  if (p.T <= 0) return hipSuccess;
+  if (bf16) {
+    if (p.D <= 64) return run<true, 64, 1>(p, st);
+    if (p.D <= 128) return run<true, 128, 1>(p, st);
+    return run<true, 256, 1>(p, st);
+  }
+  if (p.D <= 64) return run<false, 64, 1>(p, st);
+  if (p.D <= 128) return run<false, 128, 1>(p, st);
+  return run<false, 256, 1>(p, st);
+}
+
+}  // namespace svdmlp

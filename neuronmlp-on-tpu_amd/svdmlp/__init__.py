@@ -4,6 +4,10 @@ Host package over libsvdmlp.so (hand-written HIP kernels for gfx950):
 
 * :mod:`svdmlp.ops`     -- kernels/reference.py operator API
   (``fused_gate_up``, ``fused_xuv``, ``svd_mlp``) on ROCm tensors.
+* :mod:`svdmlp.decoder` -- the operators around the MLP block of a decoder
+  layer: ``rope`` / ``rope_append``, ``prompt_attention``,
+  ``cache_attention`` (decode and drafted trees on a paged cache) and
+  ``residual_norm``.
 * :mod:`svdmlp.compat`  -- the test_speedup.py launcher API
   (``fused_mlp_up_T``, ``fused_three_mm_XTUV``, ``svd_mlp_with_fused_kernel``,
   ``nki_mm``, ``get_fused_*_params`` ...).
@@ -23,6 +27,14 @@ Host package over libsvdmlp.so (hand-written HIP kernels for gfx950):
 """
 
 from ._lib import SvdMlpError, load, version, workspace_bytes  # noqa: F401
+from .decoder import (  # noqa: F401
+    cache_attention,
+    prompt_attention,
+    residual_norm,
+    rope,
+    rope_append,
+    rope_frequencies,
+)
 from .ops import (  # noqa: F401
     QuantizedFactor,
     clear_workspace_cache,

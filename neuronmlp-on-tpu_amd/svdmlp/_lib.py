@@ -26,6 +26,8 @@ SVDMLP_OUT_T = 0x4
 SVDMLP_X_T = 0x8
 SVDMLP_CONTRACT = 0x10
 SVDMLP_FP8_ACT = 0x20
+SVDMLP_ROPE_INTERLEAVED = 0x1
+SVDMLP_CAUSAL = 0x1
 SVDMLP_OK = 0
 SVDMLP_EINVAL = -1
 SVDMLP_EHIP = -2
@@ -47,6 +49,12 @@ EXPORTED = (
     "svdmlp_svd_mlp_block_ranks",
     "svdmlp_svd_mlp_noalloc",
     "svdmlp_noalloc_status",
+    "svdmlp_rope",
+    "svdmlp_rope_append",
+    "svdmlp_prompt_attention",
+    "svdmlp_cache_attention_workspace_bytes",
+    "svdmlp_cache_attention",
+    "svdmlp_residual_norm",
     "svdmlp_profile_enable",
     "svdmlp_profile_read",
     "svdmlp_stage_name",
@@ -102,6 +110,19 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.svdmlp_svd_mlp_noalloc.argtypes = [_vp] * 7 + [_vp, _vp, _vp] + [_i64] * 5 + [_i32, _i32, _u32, _vp]
     lib.svdmlp_noalloc_status.restype = ctypes.c_int
     lib.svdmlp_noalloc_status.argtypes = [_i32, _i64, _vp]
+    f32 = ctypes.c_float
+    lib.svdmlp_rope.restype = ctypes.c_int
+    lib.svdmlp_rope.argtypes = [_vp] * 7 + [_i64] * 5 + [f32, _i32, _u32, _vp]
+    lib.svdmlp_rope_append.restype = ctypes.c_int
+    lib.svdmlp_rope_append.argtypes = [_vp] * 10 + [_i64] * 7 + [f32, _i32, _u32, _vp]
+    lib.svdmlp_prompt_attention.restype = ctypes.c_int
+    lib.svdmlp_prompt_attention.argtypes = [_vp] * 6 + [_i64] * 5 + [f32, _i32, _u32, _vp]
+    lib.svdmlp_cache_attention_workspace_bytes.restype = _sz
+    lib.svdmlp_cache_attention_workspace_bytes.argtypes = [_i64] * 7 + [_i32]
+    lib.svdmlp_cache_attention.restype = ctypes.c_int
+    lib.svdmlp_cache_attention.argtypes = [_vp] * 8 + [_i64] * 8 + [f32, _i32, _vp, _sz, _vp]
+    lib.svdmlp_residual_norm.restype = ctypes.c_int
+    lib.svdmlp_residual_norm.argtypes = [_vp] * 8 + [_i64] * 2 + [f32, f32, _i32, _vp]
     lib.svdmlp_profile_enable.restype = ctypes.c_int
     lib.svdmlp_profile_enable.argtypes = [ctypes.c_int]
     lib.svdmlp_profile_read.restype = ctypes.c_int
