@@ -14,6 +14,53 @@ namespace svdmlp {
 
 namespace {
 
+// The rows of a block: sequence rows start .. start + len of the tensors, of
+// key/value head hk, its rows row0 ...
+struct RowTile {
+  int start, len, hk, row0;
+};
+
+// The block's sequence and row tile; false: none.  Tiles of BM rows are numbered
+// sequence by sequence, a sequence's last rows (the most keys of a causal call)
+// first.  The grid covers the most tiles that B sequences of T rows can have.
+__device__ __forceinline__ bool find_rows(const PromptParams& p, int G, int BM, int lane, RowTile& rt) {
+  rt.hk = blockIdx.x % p.Hk;
+  int tile = blockIdx.x / p.Hk;
+  rt.start = 0;
+  rt.len = p.T;
+  if (p.cu) {
+    rt.len = -1;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const int b = b0 + lane;
+      int s = 0, n = 0;
+      if (b < p.B) {
+        s = min(max(p.cu[b], 0), p.T);
+        n = min(max(p.cu[b + 1], s), p.T) - s;
+      }
+      const int tiles = (int)(((int64_t)n * G + BM - 1) / BM);
+      int before = tiles;  // inclusive prefix sum
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(before, o);
+        if (lane >= o) before += v;
+      }
+      const uint64_t hit = __ballot(tile < before);
+      if (hit) {
+        const int i = __builtin_ctzll(hit);
+        tile -= __builtin_amdgcn_readlane(before - tiles, i);
+        rt.start = __builtin_amdgcn_readlane(s, i);
+        rt.len = __builtin_amdgcn_readlane(n, i);
+        break;
+      }
+      tile -= __builtin_amdgcn_readlane(before, 63);
+    }
+    if (rt.len < 0) return false;
+  }
+  const int tiles = (rt.len * G + BM - 1) / BM;
+  if (tile >= tiles) return false;
+  rt.row0 = (tiles - 1 - tile) * BM;
+  return true;
+}
+
 template <bool BF16_, int DP_, int QG_>
 struct PromptCfg {
   static constexpr bool BF16 = BF16_;
@@ -36,42 +83,9 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
   const int G = p.Hq / p.Hk;
 
-  // The block's sequence and row tile: tiles are numbered sequence by
-  // sequence, the last rows (the most keys of a causal call) first.
-  const int hk = blockIdx.x % p.Hk;
-  int tile = blockIdx.x / p.Hk;
-  int start = 0, len = p.T;
-  if (p.cu) {
-    len = -1;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      const int b = b0 + lane;
-      int s = 0, n = 0;
-      if (b < p.B) {
-        s = min(max(p.cu[b], 0), p.T);
-        n = min(max(p.cu[b + 1], s), p.T) - s;
-      }
-      const int tiles = (int)(((int64_t)n * G + C::BM - 1) / C::BM);
-      int before = tiles;  // inclusive prefix sum
-      for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(before, o);
-        if (lane >= o) before += v;
-      }
-      const uint64_t hit = __ballot(tile < before);
-      if (hit) {
-        const int i = __builtin_ctzll(hit);
-        tile -= __shfl(before - tiles, i);
-        start = __shfl(s, i);
-        len = __shfl(n, i);
-        break;
-      }
-      tile -= __shfl(before, 63);
-    }
-    if (len < 0) return;  // the grid covers the most tiles that B sequences of T rows can have
-  }
-  const int rows = len * G;
-  const int tiles = (rows + C::BM - 1) / C::BM;
-  if (tile >= tiles) return;
-  const int row0 = (tiles - 1 - tile) * C::BM;
+  RowTile where;
+  if (!find_rows(p, G, C::BM, lane, where)) return;
+  const int hk = where.hk, start = where.start, len = where.len, row0 = where.row0, rows = len * G;
   const int tok_last = min(len - 1, (row0 + C::BM - 1) / G);
   const int tok_first = row0 / G;
   const int nkeys = p.causal ? tok_last + 1 : len;
@@ -209,7 +223,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
 #pragma unroll
   for (int g = 0; g < QG; ++g) {
     const float l = st[g].l + __shfl_xor(st[g].l, 32);
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
+    const float inv = inverse_sum(l);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -257,6 +271,279 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
   }
 }
 
+// The bf16 kernel for many rows: 4 waves of 64 rows, whose walk over the keys
+// that every row of the block sees is pipelined in units of 32 keys.  A step
+// does three things that do not wait for each other,
+//     S(u + 1) = K(u + 1) Q^T        matrix unit
+//     P(u) = exp2(c S(u) - m)        vector unit
+//     O += V(u - 1)^T P(u - 1)^T     matrix unit
+// so that neither unit waits for the other, with one wave a SIMD.  64 rows a wave
+// halve the LDS reads a product (one piece of K or V feeds two MFMAs).  Tiles of
+// 64 keys come straight to LDS, two ahead, in four stages: the second product
+// still reads tile t - 1 while tile t + 2 arrives.  Keys that only some rows see
+// (the diagonal) and the last, short tile follow in a plain loop.
+template <int DP_>
+struct PipeCfg {
+  static constexpr int DP = DP_, QG = 2, RB = DP * 2, PIECES = RB / 16, STEPS = RB / 32, KB = 64, BM = 256, NS = 4;
+  static constexpr int TILE = KB * RB, STAGE = 2 * TILE, UNIT = 32 * RB;
+  static constexpr int LOADS = TILE / 4096;  // 1 KB loads a wave and tile, of keys and of values
+  static constexpr int RPL = 64 / PIECES;    // rows a load
+};
+
+__device__ __forceinline__ float lane_max(const f32x16& s) {
+  float m = fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) m = fmaxf(fmaxf(m, s[i]), s[i + 1]);
+  return m;
+}
+
+template <class C>
+__global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
+  constexpr int RB = C::RB, QG = C::QG, KB = C::KB, DB = C::DP / 32;
+  __shared__ __attribute__((aligned(1024))) char lds[C::NS * C::STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+  const int G = p.Hq / p.Hk;
+  RowTile rt;
+  if (!find_rows(p, G, C::BM, lane, rt)) return;
+  const int row0 = rt.row0, rows = rt.len * G;
+  const int tok_last = min(rt.len - 1, (row0 + C::BM - 1) / G), tok_first = row0 / G;
+  const int nkeys = p.causal ? tok_last + 1 : rt.len;
+  const int shared = p.causal ? tok_first + 1 : rt.len;  // keys that every row sees
+  const int tiles = (nkeys + KB - 1) / KB, full = shared / KB;
+  const int npieces = p.D / 8;
+
+  const attn_lds base = (attn_lds)lds;
+  const char* const kb = static_cast<const char*>(p.k) + ((int64_t)rt.start * p.k_t + (int64_t)rt.hk * p.k_h) * 2;
+  const char* const vb = static_cast<const char*>(p.v) + ((int64_t)rt.start * p.v_t + (int64_t)rt.hk * p.v_h) * 2;
+  // This wave's loads of a tile: rows wave * LOADS * RPL .. of keys and values.
+  auto issue = [&](int t) {
+    const uint32_t at = (uint32_t)(uintptr_t)(base + (t % C::NS) * C::STAGE) + wave * C::LOADS * 1024;
+    const int last = nkeys - 1 - t * KB;  // rows behind the last key repeat it: they are masked
+    const char* const kt = kb + (int64_t)t * KB * p.k_t * 2;
+    const char* const vt = vb + (int64_t)t * KB * p.v_t * 2;
+#pragma unroll
+    for (int j = 0; j < C::LOADS; ++j) {
+      const int row = (wave * C::LOADS + j) * C::RPL + lane / C::PIECES, c = lane % C::PIECES, r = min(row, last);
+      const int ck = c ^ k_swz<RB>(row), cv = c ^ v_swz<RB, true>(row);
+      if (ck < npieces) load_lds16(kt + (int64_t)r * p.k_t * 2 + 16 * ck, at + j * 1024);
+      if (cv < npieces) load_lds16(vt + (int64_t)r * p.v_t * 2 + 16 * cv, at + C::TILE + j * 1024);
+    }
+  };
+  // Zeros where a head is shorter than its place (never loaded), and in the
+  // last stage's values, which the first step multiplies by zero weights.
+  if (p.D < C::DP) {
+    for (int i = threadIdx.x; i < C::NS * C::STAGE / 16; i += 256) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(base + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+  } else {
+    for (int i = threadIdx.x; i < C::UNIT / 16; i += 256)
+      *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(base + (C::NS - 1) * C::STAGE + C::TILE + C::UNIT + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+  }
+
+  u32x4 qf[QG][C::STEPS];
+  int tok[QG];
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = min(row0 + (wave * QG + g) * 32 + col, rows - 1);  // rows behind the last repeat it, and are not stored
+    tok[g] = r / G;
+    const char* qp = static_cast<const char*>(p.q) + ((int64_t)(rt.start + tok[g]) * p.q_t + (int64_t)(rt.hk * G + r - tok[g] * G) * p.q_h) * 2;
+#pragma unroll
+    for (int s = 0; s < C::STEPS; ++s) {
+      const int c = 2 * s + half;
+      qf[g][s] = c < npieces ? *reinterpret_cast<const u32x4*>(qp + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  issue(0);
+  if (tiles > 1) issue(1);
+
+  f32x16 o[QG][DB];
+  float m[QG], l[QG];
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[g][d][i] = 0.f;
+  }
+  const TileLane<RB, true> at(lane);
+  uint32_t bad = 0;
+
+  // S = K Q^T of the 32 keys at kt.
+  auto scores = [&](attn_lds kt, f32x16 (&s)[QG]) {
+#pragma unroll
+    for (int t = 0; t < C::STEPS; ++t) {
+      const u32x4 kf = at.key(kt, t);
+#pragma unroll
+      for (int g = 0; g < QG; ++g) {
+        if (t == 0) s[g] = f32x16{};
+        s[g] = attn_mfma<true>(kf, qf[g][t], s[g]);
+      }
+    }
+  };
+  // O += V^T P^T of the 32 keys at vt.
+  auto values = [&](attn_lds vt, const u32x4 (&pb)[QG][2], bool masked) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        u32x4 vf = at.values(vt, t, d);
+        if (masked)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) vf[w] = scrub<true>(vf[w], bad);
+#pragma unroll
+        for (int g = 0; g < QG; ++g) o[g][d] = attn_mfma<true>(vf, pb[g][t], o[g][d]);
+      }
+  };
+  // Where a score passes the reference by over kSlack: the new reference, and
+  // what sums so far are to be multiplied by.
+  auto reference = [&](const f32x16 (&s)[QG], float (&scale)[QG]) -> bool {
+    float mx[QG];
+    bool over = false;
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+      mx[g] = lane_max(s[g]) * p.c;
+      over |= mx[g] > m[g] + kSlack;
+    }
+    if (!__any(over)) return false;
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+      const float n = fmaxf(m[g], fmaxf(mx[g], __shfl_xor(mx[g], 32)));
+      scale[g] = n == -INFINITY ? 1.f : exp2f(m[g] - n);
+      m[g] = n;
+      l[g] *= scale[g];
+    }
+    return true;
+  };
+  auto weights = [&](const f32x16 (&s)[QG], u32x4 (&pb)[QG][2]) {
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+      const float ref = m[g] == -INFINITY ? 0.f : m[g];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float a = __builtin_amdgcn_exp2f(fmaf(s[g][8 * t + 2 * w], p.c, -ref));
+          const float b = __builtin_amdgcn_exp2f(fmaf(s[g][8 * t + 2 * w + 1], p.c, -ref));
+          l[g] += a + b;
+          pb[g][t][w] = pack_bf16x2(a, b);
+        }
+    }
+  };
+  auto rescale = [&](const float (&scale)[QG]) {
+#pragma unroll
+    for (int g = 0; g < QG; ++g)
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[g][d][i] *= scale[g];
+  };
+  // Tile t + 1 has arrived for every wave, and every wave is done with tile t - 1's keys and t - 2's values.
+  auto arrive = [&](int t) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 2 < tiles) issue(t + 2);
+  };
+
+  int t = 0;
+  if (full > 0) {
+    f32x16 s0[QG], s1[QG];
+    u32x4 p0[QG][2], p1[QG][2];
+    float scale[QG];
+#pragma unroll
+    for (int g = 0; g < QG; ++g) p1[g][0] = p1[g][1] = u32x4{0u, 0u, 0u, 0u};
+    arrive(0);
+    scores(base, s0);
+    for (;;) {
+      const attn_lds cur = base + (t % C::NS) * C::STAGE, before = base + ((t + C::NS - 1) % C::NS) * C::STAGE,
+                     next = base + ((t + 1) % C::NS) * C::STAGE;
+      {
+        const bool moved = reference(s0, scale);
+        scores(cur + C::UNIT, s1);
+        weights(s0, p0);
+        values(before + C::TILE + C::UNIT, p1, false);
+        if (moved) rescale(scale);
+      }
+      {
+        const bool moved = reference(s1, scale);
+        scores(next, s0);
+        weights(s1, p1);
+        values(cur + C::TILE, p0, false);
+        if (moved) rescale(scale);
+      }
+      if (++t == full) break;
+      arrive(t);
+    }
+    values(base + ((t - 1) % C::NS) * C::STAGE + C::TILE + C::UNIT, p1, false);
+  }
+  for (; t < tiles; ++t) {
+    arrive(t);
+    const attn_lds cur = base + (t % C::NS) * C::STAGE;
+#pragma unroll 1
+    for (int u = 0; u < 2; ++u) {
+      const int k0 = t * KB + 32 * u;
+      const int seen = p.causal ? min((row0 + (wave + 1) * QG * 32 - 1) / G, nkeys - 1) : nkeys - 1;  // the wave's last key
+      if (k0 > seen) break;
+      f32x16 s[QG];
+      u32x4 pb[QG][2];
+      float scale[QG];
+      scores(cur + u * C::UNIT, s);
+#pragma unroll
+      for (int g = 0; g < QG; ++g) {
+        const int last = p.causal ? tok[g] : nkeys - 1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[g][i] = k0 + 8 * (i >> 2) + 4 * half + (i & 3) <= last ? s[g][i] : -INFINITY;
+      }
+      if (reference(s, scale)) rescale(scale);
+      weights(s, pb);
+      values(cur + C::TILE + u * C::UNIT, pb, true);
+    }
+  }
+
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const float inv = inverse_sum(l[g] + __shfl_xor(l[g], 32));
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[g][d][i] *= inv;
+  }
+  // Infinities and NaN among the values of the plain loop were taken as
+  // zeros, for the rows that do not see them; the rows that do get them here.
+  if (__any(bad != 0)) {
+    for (int key = full * KB; key < nkeys; ++key) {
+      const uint16_t* const vp = reinterpret_cast<const uint16_t*>(vb + (int64_t)key * p.v_t * 2);
+      uint32_t see[QG];
+#pragma unroll
+      for (int g = 0; g < QG; ++g) see[g] = !p.causal || key <= tok[g] ? 0xffffffffu : 0u;
+      int D = p.D;
+      asm volatile("" : "+s"(D));  // its comparisons stay in the loop: hoisted, they spill
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
+          const uint32_t w = e >= D ? 0u : (uint32_t)vp[e] << 16, mask = not_finite<false>(w);
+#pragma unroll
+          for (int g = 0; g < QG; ++g) o[g][d][i] += __uint_as_float(w & mask & see[g]);
+        }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = row0 + (wave * QG + g) * 32 + col;
+    if (r >= rows) continue;
+    const int64_t op = (int64_t)(rt.start + tok[g]) * p.o_t + (int64_t)(rt.hk * G + (r - tok[g] * G)) * p.o_h;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int e = 32 * d + 8 * b + 4 * half;
+        if (e < p.D) store4<true>(p.out, op + e, f32x4{o[g][d][4 * b], o[g][d][4 * b + 1], o[g][d][4 * b + 2], o[g][d][4 * b + 3]});
+      }
+  }
+}
+
 template <bool BF16, int DP, int QG>
 hipError_t run(const PromptParams& p, hipStream_t st) {
   using C = PromptCfg<BF16, DP, QG>;
@@ -266,11 +553,20 @@ hipError_t run(const PromptParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int DP>
+hipError_t run_pipe(const PromptParams& p, hipStream_t st) {
+  using C = PipeCfg<DP>;
+  const int64_t tiles = (int64_t)p.T * (p.Hq / p.Hk) / C::BM + p.B;
+  hipLaunchKernelGGL((prompt_pipe_kernel<C>), dim3((unsigned)(tiles * p.Hk)), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, hipStream_t st) {
   if (p.T <= 0) return hipSuccess;
   if (bf16) {
+    if (p.D <= 128 && (int64_t)p.T * p.Hq >= 256 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
     if (p.D <= 64) return run<true, 64, 1>(p, st);
     if (p.D <= 128) return run<true, 128, 1>(p, st);
     return run<true, 256, 1>(p, st);

@@ -228,27 +228,42 @@ def test_prompt_attention(gpu, dtype, causal, lens, H, K, D):
         assert torch.equal(got, svdmlp.prompt_attention(qg, kg, vg, causal=causal))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,H,K,D", [([2100], 32, 8, 128), ([1500, 1, 0, 640], 64, 8, 64), ([1030, 63, 65, 1027], 32, 4, 96), ([4097], 16, 16, 64),
+                                        ([900, 1300], 32, 1, 80), ([2113], 40, 8, 128)])
+def test_prompt_attention_many_rows(gpu, lens, H, K, D, causal):
+    g = _gen(sum(lens) + H)
+    (q, k, v), dev = _qkv(g, sum(lens), H, K, D, BF, gpu)
+    got = svdmlp.prompt_attention(*dev, _cu(lens, gpu), causal=causal).cpu()
+    heads = [0, H // 2 + 1, H - 1]
+    kv = [h // (H // K) for h in heads]
+    out, tol = _prompt_ref(q[:, heads], k[:, kv], v[:, kv], lens, causal, 1 / math.sqrt(D))
+    _close(got[:, heads], out, tol)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_prompt_attention_large_scores_and_scale(gpu, dtype):
     """Scores that grow along the keys by hundreds of powers of two (every tile moves the running maximum) and a scale of one's own."""
     g = _gen(3)
-    T, H, K, D = 400, 4, 2, 64
-    q, k, v = (_randn(g, T, n, D, dtype=dtype) for n in (H, K, K))
-    q = q.abs()
-    k = (k.abs() * torch.linspace(0.0, 4.0, T)[:, None, None]).to(dtype)
-    for causal, scale in ((True, 1.0), (False, 0.37)):
-        out, tol = _prompt_ref(q, k, v, [T], causal, scale)
-        _close(svdmlp.prompt_attention(*(t.to(gpu) for t in (q, k, v)), causal=causal, scale=scale), out, tol)
+    for T, H, K, D in ((400, 4, 2, 64), (700, 96, 2, 128)):
+        q, k, v = (_randn(g, T, n, D, dtype=dtype) for n in (H, K, K))
+        q = q.abs()
+        k = (k.abs() * torch.linspace(0.0, 4.0, T)[:, None, None]).to(dtype)
+        heads = [0, H - 1]
+        for causal, scale in ((True, 1.0), (False, 0.37)):
+            got = svdmlp.prompt_attention(*(t.to(gpu) for t in (q, k, v)), causal=causal, scale=scale)
+            out, tol = _prompt_ref(q[:, heads], k[:, [0, K - 1]], v[:, [0, K - 1]], [T], causal, scale)
+            _close(got[:, heads], out, tol)
 
 
-@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("H,K,D", [(4, 2, 64), (4, 2, 128), (4, 2, 256), (256, 1, 64), (256, 2, 128)])
 @pytest.mark.parametrize("dtype", [BF, F32])
-def test_prompt_attention_hidden_keys_have_no_part(gpu, dtype, D):
+def test_prompt_attention_hidden_keys_have_no_part(gpu, dtype, H, K, D):
     """Infinities and NaN in later tokens, other sequences and rows of no
     sequence; rows of no sequence stay as they were.  A value that a token does
     see reaches it."""
     g = _gen(11)
-    lens, first, H, K = [150, 90], 3, 4, 2
+    lens, first = [150, 90], 3
     T = 260
     q, k, v = (_randn(g, T, n, D, dtype=dtype) for n in (H, K, K))
     out, tol = _prompt_ref(q, k, v, lens, True, 1 / math.sqrt(D), first)
@@ -274,12 +289,13 @@ def test_prompt_attention_hidden_keys_have_no_part(gpu, dtype, D):
 def test_prompt_attention_full_sees_every_value(gpu):
     """Without a causal mask an infinity reaches every token of its sequence, in its column alone."""
     g = _gen(12)
-    q, k, v = (_randn(g, 70, 2, 64) for _ in range(3))
-    v[69, 0, 3] = math.inf
-    got = svdmlp.prompt_attention(*(t.to(gpu) for t in (q, k, v)), causal=False).cpu()
-    assert (got[:, 0, 3] == math.inf).all()
-    got[:, 0, 3] = 0
-    assert torch.isfinite(got.float()).all()
+    for T, H in ((70, 2), (1030, 64)):
+        q, k, v = (_randn(g, T, H, 64) for _ in range(3))
+        v[T - 1, 0, 3], v[5, 1, 4] = math.inf, -math.inf
+        got = svdmlp.prompt_attention(*(t.to(gpu) for t in (q, k, v)), causal=False).cpu()
+        assert (got[:, 0, 3] == math.inf).all() and (got[:, 1, 4] == -math.inf).all()
+        got[:, 0, 3] = got[:, 1, 4] = 0
+        assert torch.isfinite(got.float()).all()
 
 
 def test_prompt_attention_bounds_outside_the_rows(gpu):
