@@ -7,6 +7,8 @@
 // running maximum and sum.
 #include <math.h>
 
+#include <algorithm>
+
 #include "attn.hpp"
 #include "decoder.hpp"
 
@@ -277,17 +279,24 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
 //     S(u + 1) = K(u + 1) Q^T        matrix unit
 //     P(u) = exp2(c S(u) - m)        vector unit
 //     O += V(u - 1)^T P(u - 1)^T     matrix unit
-// so that neither unit waits for the other, with one wave a SIMD.  64 rows a wave
-// halve the LDS reads a product (one piece of K or V feeds two MFMAs).  Tiles of
-// 64 keys come straight to LDS, two ahead, in four stages: the second product
-// still reads tile t - 1 while tile t + 2 arrives.  Keys that only some rows see
-// (the diagonal) and the last, short tile follow in a plain loop.
+// so that with one wave a SIMD neither unit waits for the other.  Its order is
+// laid down in the source: a slot is one MFMA (32 cycles) and what fits beside
+// it, one or two weights and an LDS read of a piece needed some slots later.
+// 64 rows a wave halve the LDS reads a product (one piece of K or V feeds two
+// MFMAs).  Tiles of 64 keys come straight to LDS, two ahead, in four stages:
+// the second product still reads tile t - 1 while tile t + 2 arrives; the loop is
+// unrolled over the stages, whose offsets are then constants.  Keys that only
+// some rows see (the diagonal) and the last, short tile follow in a plain loop.
 template <int DP_>
 struct PipeCfg {
   static constexpr int DP = DP_, QG = 2, RB = DP * 2, PIECES = RB / 16, STEPS = RB / 32, KB = 64, BM = 256, NS = 4;
-  static constexpr int TILE = KB * RB, STAGE = 2 * TILE, UNIT = 32 * RB;
+  static constexpr int TILE = KB * RB, STAGE = 2 * TILE, UNIT = 32 * RB, DB = DP / 32;
   static constexpr int LOADS = TILE / 4096;  // 1 KB loads a wave and tile, of keys and of values
   static constexpr int RPL = 64 / PIECES;    // rows a load
+  static constexpr int FRAGS = STEPS + 2 * DB, SLOTS = QG * FRAGS;  // LDS pieces and MFMAs a step
+  static constexpr int AHEAD = 4;                                   // pieces read before they are needed
+  static constexpr int PER = 16 * QG / SLOTS;                       // weights a slot
+  static_assert(FRAGS % AHEAD == 0 && PER * SLOTS == 16 * QG, "slots");
 };
 
 __device__ __forceinline__ float lane_max(const f32x16& s) {
@@ -295,6 +304,13 @@ __device__ __forceinline__ float lane_max(const f32x16& s) {
 #pragma unroll
   for (int i = 2; i < 16; i += 2) m = fmaxf(fmaxf(m, s[i]), s[i + 1]);
   return m;
+}
+
+typedef __bf16 bf16x2_dot __attribute__((ext_vector_type(2)));
+
+// acc + both bf16 values of w.
+__device__ __forceinline__ float add_pair(uint32_t w, float acc) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_dot, w), __builtin_bit_cast(bf16x2_dot, 0x3f803f80u), acc, false);
 }
 
 template <class C>
@@ -426,8 +442,8 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
         for (int w = 0; w < 4; ++w) {
           const float a = __builtin_amdgcn_exp2f(fmaf(s[g][8 * t + 2 * w], p.c, -ref));
           const float b = __builtin_amdgcn_exp2f(fmaf(s[g][8 * t + 2 * w + 1], p.c, -ref));
-          l[g] += a + b;
           pb[g][t][w] = pack_bf16x2(a, b);
+          l[g] = add_pair(pb[g][t][w], l[g]);
         }
     }
   };
@@ -441,39 +457,118 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   };
   // Tile t + 1 has arrived for every wave, and every wave is done with tile t - 1's keys and t - 2's values.
   auto arrive = [&](int t) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     if (t + 2 < tiles) issue(t + 2);
   };
 
   int t = 0;
   if (full > 0) {
     f32x16 s0[QG], s1[QG];
-    u32x4 p0[QG][2], p1[QG][2];
-    float scale[QG];
+    u32x4 p0[QG][2], p1[QG][2], frag[C::AHEAD];
+    float scale[QG], over[QG];  // over: the score beyond which the reference moves
+    bool moved = false;
 #pragma unroll
     for (int g = 0; g < QG; ++g) p1[g][0] = p1[g][1] = u32x4{0u, 0u, 0u, 0u};
+    // Places in the stages whose offsets do not fit an instruction (64 KB).
+    constexpr int NEAR = std::min(C::NS, 65536 / C::STAGE);
+    TileLane<RB, true> at2 = at;
+    if constexpr (NEAR < C::NS) {
+#pragma unroll
+      for (int i = 0; i < TileLane<RB, true>::KN; ++i) {
+        at2.k[i] += NEAR * C::STAGE;
+        asm volatile("" : "+v"(at2.k[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < TileLane<RB, true>::VN; ++i) {
+        at2.v[i] += NEAR * C::STAGE;
+        asm volatile("" : "+v"(at2.v[i]));
+      }
+    }
+    // Piece f of the step at unit U of the tile in stage S: K of the unit after
+    // it, then V of the unit before it.
+    auto read = [&](auto S_, auto U_, int f) {
+      constexpr int S = decltype(S_)::value, U = decltype(U_)::value;
+      if (f < C::STEPS) {
+        constexpr int st = U ? (S + 1) % C::NS : S;
+        frag[f % C::AHEAD] = (st < NEAR ? at : at2).key(base + st % NEAR * C::STAGE + (U ? 0 : C::UNIT), f);
+      } else {
+        constexpr int st = U ? S : (S + C::NS - 1) % C::NS;
+        frag[f % C::AHEAD] = (st < NEAR ? at : at2).values(base + st % NEAR * C::STAGE + C::TILE + (U ? 0 : C::UNIT),
+                                                          (f - C::STEPS) / DB, (f - C::STEPS) % DB);
+      }
+    };
+    auto step = [&](auto S_, auto U_, f32x16 (&sc)[QG], f32x16 (&sn)[QG], u32x4 (&pc)[QG][2], const u32x4 (&pp)[QG][2]) {
+      constexpr int S = decltype(S_)::value, U = decltype(U_)::value;
+      float hold = 0.f;
+#pragma unroll
+      for (int n = 0; n < C::SLOTS; ++n) {
+        const int f = n / QG, g = n % QG;
+        __builtin_amdgcn_sched_barrier(0);
+        if (f < C::STEPS) {
+          if (f == 0) sn[g] = f32x16{};
+          sn[g] = attn_mfma<true>(frag[f % C::AHEAD], qf[g][f], sn[g]);
+        } else {
+          const int v = f - C::STEPS;
+          o[g][v % DB] = attn_mfma<true>(frag[f % C::AHEAD], pp[g][v / DB], o[g][v % DB]);
+        }
+        if (g == QG - 1) {  // the piece's last product: its registers take the one AHEAD of it
+          if (f + C::AHEAD < C::FRAGS) read(S_, U_, f + C::AHEAD);
+          else read(std::integral_constant<int, U ? (S + 1) % C::NS : S>{}, std::integral_constant<int, 1 - U>{}, f + C::AHEAD - C::FRAGS);
+        }
+        // Weights PER n ..; the empty asm keeps them in their slot.
+#pragma unroll
+        for (int q = 0; q < C::PER; ++q) {
+          const int i = n * C::PER + q, wg = i / 16, wi = i % 16;
+          const float e = __builtin_amdgcn_exp2f(fmaf(sc[wg][wi], p.c, -m[wg]));
+          if (i % 2 == 0) {
+            hold = e;
+            asm volatile("" : "+v"(hold));
+          } else {
+            uint32_t both = pack_bf16x2(hold, e);
+            l[wg] = add_pair(both, l[wg]);
+            asm volatile("" : "+v"(both), "+v"(l[wg]));
+            pc[wg][wi / 8][wi % 8 / 2] = both;
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      bool any = moved;
+#pragma unroll
+      for (int g = 0; g < QG; ++g) any |= lane_max(sn[g]) > over[g];
+      if (__any(any)) {  // rare: a reference moves, or has moved
+        if (moved) rescale(scale);
+        // behind the last unit here come keys that not every row sees, or none
+        moved = (U == 0 || t + 1 < full) && reference(sn, scale);
+#pragma unroll
+        for (int g = 0; g < QG; ++g) over[g] = (m[g] + kSlack) / p.c;
+      }
+    };
     arrive(0);
     scores(base, s0);
-    for (;;) {
-      const attn_lds cur = base + (t % C::NS) * C::STAGE, before = base + ((t + C::NS - 1) % C::NS) * C::STAGE,
-                     next = base + ((t + 1) % C::NS) * C::STAGE;
-      {
-        const bool moved = reference(s0, scale);
-        scores(cur + C::UNIT, s1);
-        weights(s0, p0);
-        values(before + C::TILE + C::UNIT, p1, false);
-        if (moved) rescale(scale);
-      }
-      {
-        const bool moved = reference(s1, scale);
-        scores(next, s0);
-        weights(s1, p1);
-        values(cur + C::TILE, p0, false);
-        if (moved) rescale(scale);
-      }
-      if (++t == full) break;
-      arrive(t);
+    if (reference(s0, scale)) {}  // nothing has been summed yet
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+      if (m[g] == -INFINITY) m[g] = -1e30f;  // no finite score yet: a finite reference that any will move
+      over[g] = (m[g] + kSlack) / p.c;
     }
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+#pragma unroll
+    for (int f = 0; f < C::AHEAD; ++f) read(I0{}, I0{}, f);
+#define SVDMLP_PIPE_TILE(S)                 \
+  step(S{}, I0{}, s0, s1, p0, p1);          \
+  step(S{}, I1{}, s1, s0, p1, p0);          \
+  if (++t == full) break;                   \
+  arrive(t);
+    for (;;) {
+      SVDMLP_PIPE_TILE(I0)
+      SVDMLP_PIPE_TILE(I1)
+      SVDMLP_PIPE_TILE(I2)
+      SVDMLP_PIPE_TILE(I3)
+    }
+#undef SVDMLP_PIPE_TILE
     values(base + ((t - 1) % C::NS) * C::STAGE + C::TILE + C::UNIT, p1, false);
   }
   for (; t < tiles; ++t) {

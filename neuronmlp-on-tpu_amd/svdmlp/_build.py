@@ -50,6 +50,11 @@ HIPCC_FLAGS = [
     f"-I{CSRC}",
 ]
 
+# Flags of single translation units.  prompt_attention: results of MFMAs in
+# vector registers where they fit (by itself the compiler puts them all into
+# accumulation registers, from which the softmax would copy every score).
+UNIT_FLAGS = {"prompt_attention": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+
 
 def _hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
@@ -109,7 +114,7 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
 
     def compile_one(pair):
         src, obj = pair
-        cmd = [hipcc, *HIPCC_FLAGS, REMARK_FLAG, "-fno-caret-diagnostics", "-c", str(src), "-o", str(obj)]
+        cmd = [hipcc, *HIPCC_FLAGS, *UNIT_FLAGS.get(src.stem, []), REMARK_FLAG, "-fno-caret-diagnostics", "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         return resources(_run(cmd))
