@@ -2545,6 +2545,13 @@ int device_cus() {
 
 int act_size(int32_t dtype) { return dtype == SVDMLP_BF16 ? 2 : dtype == SVDMLP_F32 ? 4 : 0; }
 
+// Strides of the attention entry points: not negative.
+bool no_negative(const int64_t* s, int n) {
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0) return false;
+  return true;
+}
+
 bool pieces16(std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> elements, int es) {
   for (const void* p : ptrs)
     if (((uintptr_t)p & 15u) != 0) return false;
@@ -2644,6 +2651,7 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
   const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hk * D, D, Hq * D, D};
   const int64_t* s = strides ? strides : dense;
   const int es = act_size(dtype);
+  if (!no_negative(s, 8)) return fail("prompt_attention: strides must not be negative");
   if (!pieces16({q, k, v, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]}, es))
     return fail("prompt_attention: the head size, strides and addresses must be whole 16-byte pieces");
   PromptParams p = {q, k, v, out, cu_seqlens, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], (int)T, (int)B, (int)Hq,
@@ -2678,6 +2686,7 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
                              n * Hq * D, Hq * D, D, width, n * n, n};
   const int64_t* s = strides ? strides : dense;
   const int es = act_size(dtype);
+  if (!no_negative(s, 15)) return fail("cache_attention: strides must not be negative");
   if (!pieces16({q, k_cache, v_cache, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10], s[11]}, es))
     return fail("cache_attention: the head size, strides and addresses must be whole 16-byte pieces");
   CacheParams p = {};

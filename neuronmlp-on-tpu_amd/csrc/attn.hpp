@@ -141,6 +141,16 @@ __device__ __forceinline__ void load_lds16(const void* p, uint32_t base) {
                : "s"((uint32_t)__builtin_amdgcn_readfirstlane((int)base)), "v"(p)
                : "memory");
 }
+// The same from a base that all lanes share and an offset of each.
+__device__ __forceinline__ void load_lds16(const void* p, uint32_t offset, uint32_t base) {
+  const uint64_t a = (uint64_t)p;
+  const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"((uint32_t)__builtin_amdgcn_readfirstlane((int)base)), "v"(offset), "s"(u)
+               : "memory");
+}
 // Until at most N of the wave's loads are on their way.
 template <int N>
 __device__ __forceinline__ void wait_loads() {

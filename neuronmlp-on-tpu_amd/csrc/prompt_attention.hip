@@ -283,9 +283,9 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
 // laid down in the source: a slot is one MFMA (32 cycles) and what fits beside
 // it, one or two weights and an LDS read of a piece needed some slots later.
 // 64 rows a wave halve the LDS reads a product (one piece of K or V feeds two
-// MFMAs).  Tiles of 64 keys come straight to LDS, two ahead, in four stages:
-// the second product still reads tile t - 1 while tile t + 2 arrives; the loop is
-// unrolled over the stages, whose offsets are then constants.  Keys that only
+// MFMAs).  Tiles of 64 keys come straight to LDS, the keys three and the
+// values two tiles ahead, in four stages each; the loop is unrolled over the
+// stages, whose offsets are then constants.  Keys that only
 // some rows see (the diagonal) and the last, short tile follow in a plain loop.
 template <int DP_>
 struct PipeCfg {
@@ -331,18 +331,51 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   const attn_lds base = (attn_lds)lds;
   const char* const kb = static_cast<const char*>(p.k) + ((int64_t)rt.start * p.k_t + (int64_t)rt.hk * p.k_h) * 2;
   const char* const vb = static_cast<const char*>(p.v) + ((int64_t)rt.start * p.v_t + (int64_t)rt.hk * p.v_h) * 2;
-  // This wave's loads of a tile: rows wave * LOADS * RPL .. of keys and values.
-  auto issue = [&](int t) {
-    const uint32_t at = (uint32_t)(uintptr_t)(base + (t % C::NS) * C::STAGE) + wave * C::LOADS * 1024;
-    const int last = nkeys - 1 - t * KB;  // rows behind the last key repeat it: they are masked
-    const char* const kt = kb + (int64_t)t * KB * p.k_t * 2;
-    const char* const vt = vb + (int64_t)t * KB * p.v_t * 2;
+  // This wave's loads of a tile: rows wave * LOADS * RPL .. of keys (of tile tk)
+  // and of values (of tile tv).  In whole tiles a lane's offsets are the same
+  // every time; in the last one rows behind the last key repeat it (masked).
+  uint32_t koff[C::LOADS], voff;
+  const int lrow = wave * C::LOADS * C::RPL + lane / C::PIECES, lc = lane % C::PIECES;
+  bool kin[C::LOADS];
+  const int vc = lc ^ v_swz<RB, true>(lrow);
 #pragma unroll
-    for (int j = 0; j < C::LOADS; ++j) {
-      const int row = (wave * C::LOADS + j) * C::RPL + lane / C::PIECES, c = lane % C::PIECES, r = min(row, last);
-      const int ck = c ^ k_swz<RB>(row), cv = c ^ v_swz<RB, true>(row);
-      if (ck < npieces) load_lds16(kt + (int64_t)r * p.k_t * 2 + 16 * ck, at + j * 1024);
-      if (cv < npieces) load_lds16(vt + (int64_t)r * p.v_t * 2 + 16 * cv, at + C::TILE + j * 1024);
+  for (int j = 0; j < C::LOADS; ++j) {
+    const int row = lrow + j * C::RPL, c = lc ^ k_swz<RB>(row);
+    koff[j] = (uint32_t)(row * (int)p.k_t * 2 + 16 * c);
+    kin[j] = c < npieces;
+  }
+  voff = (uint32_t)(lrow * (int)p.v_t * 2 + 16 * vc);
+  const bool vin = vc < npieces;
+  auto issue_keys = [&](int t) {
+    if (t >= tiles) return;
+    const uint32_t at = (uint32_t)(uintptr_t)(base + (t % C::NS) * C::STAGE) + wave * C::LOADS * 1024;
+    const char* const kt = kb + (int64_t)t * KB * p.k_t * 2;
+    if ((t + 1) * KB <= nkeys) {
+#pragma unroll
+      for (int j = 0; j < C::LOADS; ++j)
+        if (kin[j]) load_lds16(kt, koff[j], at + j * 1024);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::LOADS; ++j) {
+        const int row = lrow + j * C::RPL, r = min(row, nkeys - 1 - t * KB);
+        if (kin[j]) load_lds16(kt, (uint32_t)(r * (int)p.k_t * 2 + 16 * (lc ^ k_swz<RB>(row))), at + j * 1024);
+      }
+    }
+  };
+  auto issue_values = [&](int t) {
+    if (t >= tiles) return;
+    const uint32_t at = (uint32_t)(uintptr_t)(base + (t % C::NS) * C::STAGE) + C::TILE + wave * C::LOADS * 1024;
+    const char* const vt = vb + (int64_t)t * KB * p.v_t * 2;
+    if ((t + 1) * KB <= nkeys) {
+#pragma unroll
+      for (int j = 0; j < C::LOADS; ++j)
+        if (vin) load_lds16(vt + (int64_t)j * C::RPL * p.v_t * 2, voff, at + j * 1024);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::LOADS; ++j) {
+        const int r = min(lrow + j * C::RPL, nkeys - 1 - t * KB);
+        if (vin) load_lds16(vt, (uint32_t)(r * (int)p.v_t * 2 + 16 * vc), at + j * 1024);
+      }
     }
   };
   // Zeros where a head is shorter than its place (never loaded), and in the
@@ -369,8 +402,11 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  issue(0);
-  if (tiles > 1) issue(1);
+  issue_keys(0);
+  issue_keys(1);
+  issue_values(0);
+  issue_keys(2);
+  issue_values(1);
 
   f32x16 o[QG][DB];
   float m[QG], l[QG];
@@ -455,10 +491,16 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[g][d][i] *= scale[g];
   };
-  // Tile t + 1 has arrived for every wave, and every wave is done with tile t - 1's keys and t - 2's values.
+  // Before tile t: the keys of tile t + 1 and the values of tile t are there for
+  // every wave (they were asked for two tiles ago; what was asked for one tile
+  // ago may still be on its way), and every wave is done with the keys of tile
+  // t - 1 and the values of tile t - 2, whose places are filled again.
   auto arrive = [&](int t) {
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 2 < tiles) issue(t + 2);
+    if (t + 2 < tiles) wait_loads<2 * C::LOADS>();
+    else wait_loads<0>();
+    asm volatile("s_barrier" ::: "memory");
+    issue_keys(t + 3);
+    issue_values(t + 2);
   };
 
   int t = 0;
@@ -499,7 +541,8 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
     };
     auto step = [&](auto S_, auto U_, f32x16 (&sc)[QG], f32x16 (&sn)[QG], u32x4 (&pc)[QG][2], const u32x4 (&pp)[QG][2]) {
       constexpr int S = decltype(S_)::value, U = decltype(U_)::value;
-      float hold = 0.f;
+      constexpr int MPS = C::SLOTS >= 32 ? 2 : 4;  // maxima a slot, in the last 8 or 4
+      float hold = 0.f, mx[QG] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int n = 0; n < C::SLOTS; ++n) {
         const int f = n / QG, g = n % QG;
@@ -514,6 +557,14 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
         if (g == QG - 1) {  // the piece's last product: its registers take the one AHEAD of it
           if (f + C::AHEAD < C::FRAGS) read(S_, U_, f + C::AHEAD);
           else read(std::integral_constant<int, U ? (S + 1) % C::NS : S>{}, std::integral_constant<int, 1 - U>{}, f + C::AHEAD - C::FRAGS);
+        }
+        // The maximum of the new scores, once they are complete.
+        if (n >= C::SLOTS - 16 * QG / 2 / MPS) {
+#pragma unroll
+          for (int q = 0; q < MPS; ++q) {
+            const int i = (n - (C::SLOTS - 16 * QG / 2 / MPS)) * MPS + q, wg = i / 8, wi = 2 * (i % 8);
+            mx[wg] = fmaxf(fmaxf(mx[wg], sn[wg][wi]), sn[wg][wi + 1]);
+          }
         }
         // Weights PER n ..; the empty asm keeps them in their slot.
 #pragma unroll
@@ -534,7 +585,7 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
       __builtin_amdgcn_sched_barrier(0);
       bool any = moved;
 #pragma unroll
-      for (int g = 0; g < QG; ++g) any |= lane_max(sn[g]) > over[g];
+      for (int g = 0; g < QG; ++g) any |= mx[g] > over[g];
       if (__any(any)) {  // rare: a reference moves, or has moved
         if (moved) rescale(scale);
         // behind the last unit here come keys that not every row sees, or none
@@ -661,7 +712,8 @@ hipError_t run_pipe(const PromptParams& p, hipStream_t st) {
 hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, hipStream_t st) {
   if (p.T <= 0) return hipSuccess;
   if (bf16) {
-    if (p.D <= 128 && (int64_t)p.T * p.Hq >= 256 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
+    const bool near = p.k_t < 1 << 24 && p.v_t < 1 << 24;  // a tile's offsets fit 32 bits
+    if (p.D <= 128 && near && (int64_t)p.T * p.Hq >= 256 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
     if (p.D <= 64) return run<true, 64, 1>(p, st);
     if (p.D <= 128) return run<true, 128, 1>(p, st);
     return run<true, 256, 1>(p, st);
