@@ -148,6 +148,8 @@ def _mapped_hip_runtimes() -> set[str]:
 def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     """Load (once) and return the library; raises RuntimeError if unavailable."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -26,46 +26,74 @@ import math
 import torch
 
 from . import _lib
-from .ops import _ACT_CODES, _on_device, _stream
+from .ops import _ACT_CODES
+
+# A call at decode shapes takes a few microseconds on the GPU, so the host's
+# part is kept short: sizes, types and devices are compared in line (a tensor's
+# attribute costs ~0.06 us), what only unusual arguments need (strides that
+# overlap, shared memory) is looked at only for them, and the stream is asked
+# for without an object around it (0.1 us, 2 us with).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_BF16 = torch.bfloat16
 
 
-def _check(name: str, dtype: torch.dtype, *tensors) -> torch.device:
-    """All tensors on one GPU; those of the activation's type; none that asks for a gradient."""
-    if dtype not in _ACT_CODES:
-        raise TypeError("supported dtypes are bfloat16 and float32")
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise ValueError(f"{name} runs on a ROCm GPU; got tensors on {dev}")
-    grad = torch.is_grad_enabled()
+def _refuse_device(name: str, *tensors) -> None:
+    """Raises for tensors that are not all on one GPU."""
     for t in tensors:
-        if t.device != dev:
-            raise ValueError("all inputs must be on the same device")
-        if grad and t.requires_grad:
+        if t is not None and not t.is_cuda:
+            raise ValueError(f"{name} runs on a ROCm GPU; got tensors on {t.device}" if t is tensors[0]
+                             else "all inputs must be on the same device")
+    raise ValueError("all inputs must be on the same device")
+
+
+def _refuse_dtype(*dtypes) -> None:
+    if any(d != dtypes[0] for d in dtypes):
+        raise TypeError("all inputs must have the same dtype")
+    raise TypeError("supported dtypes are bfloat16 and float32")
+
+
+def _refuse_grad(name: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.requires_grad:
             raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), or on detached tensors")
-    return dev
 
 
-def _same_dtype(x, *tensors) -> None:
-    for t in tensors:
-        if t.dtype != x.dtype:
-            raise TypeError("all inputs must have the same dtype")
+def _launch(index: int, fn, *args) -> None:
+    """fn(*args, stream) on device `index`, its status checked."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself where the kernels can read it in place (last dimension
     contiguous, rows in whole 16-byte pieces), else a contiguous copy."""
-    es = t.element_size()
-    if t.stride(-1) != 1 and t.shape[-1] != 1 or t.data_ptr() % 16 or any(s * es % 16 for s in t.stride()[:-1]):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
+    step = 8 if t.dtype is _BF16 else 4
+    st = t.stride()
+    if st[-1] == 1 and not t.data_ptr() % 16:
+        for s in st[:-1]:
+            if s % step:
+                break
+        else:
+            return t
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _last(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 else t.contiguous()
 
 
 def _writable(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> None:
     """An output: of the shape, type and device, its elements all apart."""
     if tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must be a {tuple(shape)} tensor of {like.dtype} on {like.device}")
+    if t.is_contiguous():
+        return
     reach = 0
     for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if stride <= reach:
@@ -76,8 +104,8 @@ def _writable(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> None:
 
 
 def _aligned(name: str, t: torch.Tensor) -> None:
-    es = t.element_size()
-    if t.data_ptr() % 16 or any(s * es % 16 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+    step = 8 if t.dtype is _BF16 else 4
+    if t.data_ptr() % 16 or any(s % step for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
         raise ValueError(f"rows of {name} must be 16-byte aligned")
 
 
@@ -109,18 +137,18 @@ def _apart(name: str, out: torch.Tensor, *tensors, own=()) -> None:
             raise ValueError(f"{name} must not overlap the inputs")
 
 
-def _index(name: str, t: torch.Tensor, shape, dtype, dev) -> torch.Tensor:
+def _index(name: str, t: torch.Tensor, shape, dtype, device) -> torch.Tensor:
+    """An index tensor as the kernels take it: t itself, or a copy of the type and layout."""
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be an int32 or int64 tensor")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != dev:
+    if t.get_device() != device:
         raise ValueError("all inputs must be on the same device")
-    return t.to(dtype).contiguous()
+    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
-def _heads(q, k, *more) -> tuple[int, int, int, int]:
-    """(T, Hq, Hk, D) of q (T, Hq, D) and k, v ... (T, Hk, D)."""
+def _refuse_heads(q, k, *more) -> None:
     for t in (q, k, *more):
         if t.dim() != 3:
             raise ValueError(f"expected (tokens, heads, head size), got {tuple(t.shape)}")
@@ -129,13 +157,14 @@ def _heads(q, k, *more) -> tuple[int, int, int, int]:
     for t in (k, *more):
         if tuple(t.shape) != (T, Hk, D):
             raise ValueError(f"keys and values must have shape {(T, Hk, D)}, got {tuple(t.shape)}")
-    if min(Hq, Hk, D) <= 0 or Hq % Hk:
-        raise ValueError(f"{Hq} query heads are no multiple of {Hk} key/value heads")
-    return T, Hq, Hk, D
+    raise ValueError(f"{Hq} query heads are no multiple of {Hk} key/value heads")
 
 
-def _strides(*values):
-    return (ctypes.c_int64 * len(values))(*values)
+_Strides5 = ctypes.c_int64 * 5
+_Strides8 = ctypes.c_int64 * 8
+_Strides14 = ctypes.c_int64 * 14
+_Strides15 = ctypes.c_int64 * 15
+_address = ctypes.addressof
 
 
 # ---------------------------------------------------------------------------
@@ -198,23 +227,31 @@ def rope_frequencies(rot: int, theta: float = 10000.0, *, scaling: dict | None =
     return freq.to(device) if device is not None else freq, scale
 
 
-def _rope_args(name, q, k, more, positions, inv_freq, scale):
-    T, Hq, Hk, D = _heads(q, k, *more)
-    _same_dtype(q, k, *more)
-    dev = _check(name, q.dtype, q, k, *more)
-    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or inv_freq.device != dev:
+def _rope_args(name, q, k, v, positions, inv_freq, scale):
+    """The checks that rope and rope_append share (v None: rope); (T, Hq, Hk, D, device index, rot, positions, inv_freq)."""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks[0] != qs[0] or ks[2] != qs[2] or not ks[1] or not qs[2] or not qs[1] or qs[1] % ks[1] or (
+            v is not None and v.shape != ks):
+        _refuse_heads(q, k, *(() if v is None else (v,)))
+    T, Hq, D = qs
+    dtype, index = q.dtype, q.get_device()
+    if k.dtype != dtype or dtype not in _ACT_CODES or (v is not None and v.dtype != dtype):
+        _refuse_dtype(dtype, k.dtype, *(() if v is None else (v.dtype,)))
+    if index < 0 or k.get_device() != index or (v is not None and v.get_device() != index):
+        _refuse_device(name, q, k, v)
+    if torch.is_grad_enabled():
+        _refuse_grad(name, q, k, v)
+    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or inv_freq.get_device() != index:
         raise ValueError("inv_freq must be a 1-D floating point tensor on the inputs' device")
     rot = 2 * inv_freq.shape[0]
     if not 0 < rot <= D:
         raise ValueError(f"{rot} turned values (two a frequency) of a head of {D}")
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
-    positions = _index("positions", positions, (T,), torch.int64, dev)
-    return T, Hq, Hk, D, dev, rot, positions, inv_freq.to(torch.float64).contiguous()
-
-
-def _last(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    positions = _index("positions", positions, (T,), torch.int64, index)
+    if inv_freq.dtype is not torch.float64 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(torch.float64).contiguous()
+    return T, Hq, ks[1], D, index, rot, positions, inv_freq
 
 
 def rope(q, k, positions, inv_freq, *, interleaved: bool = False, scale: float = 1.0,
@@ -225,9 +262,9 @@ def rope(q, k, positions, inv_freq, *, interleaved: bool = False, scale: float =
     head is copied.  ``scale`` multiplies cos and sin (see
     :func:`rope_frequencies`).  q (T, Hq, D), k (T, Hk, D), positions (T,).
     ``out``: the pair of tensors to write, which may be q and k themselves."""
-    T, Hq, Hk, D, dev, rot, positions, inv_freq = _rope_args("rope", q, k, (), positions, inv_freq, scale)
+    T, Hq, Hk, D, index, rot, positions, inv_freq = _rope_args("rope", q, k, None, positions, inv_freq, scale)
     if out is None:
-        qo, ko = torch.empty((T, Hq, D), dtype=q.dtype, device=dev), torch.empty((T, Hk, D), dtype=q.dtype, device=dev)
+        qo, ko = q.new_empty((T, Hq, D)), q.new_empty((T, Hk, D))
     else:
         qo, ko = out
         _writable("out[0]", qo, (T, Hq, D), q)
@@ -237,20 +274,16 @@ def rope(q, k, positions, inv_freq, *, interleaved: bool = False, scale: float =
     if T == 0:
         return qo, ko
     q, k = _last(q), _last(k)
-    lib = _lib.load()
-    st = _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), qo.stride(0), qo.stride(1), ko.stride(0), ko.stride(1))
-    _lib.check(_on_device(dev, lambda: lib.svdmlp_rope(
-        q.data_ptr(), k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), qo.data_ptr(), ko.data_ptr(),
-        ctypes.addressof(st), T, Hq, Hk, D, rot, scale, _ACT_CODES[q.dtype],
-        _lib.SVDMLP_ROPE_INTERLEAVED if interleaved else 0, _stream(dev))))
+    st = _Strides8(*q.stride()[:2], *k.stride()[:2], *qo.stride()[:2], *ko.stride()[:2])
+    _launch(index, _lib.load().svdmlp_rope, q.data_ptr(), k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+            qo.data_ptr(), ko.data_ptr(), _address(st), T, Hq, Hk, D, rot, scale, _ACT_CODES[q.dtype], 1 if interleaved else 0)
     return qo, ko
 
 
-def _cache(k_cache, v_cache, q, Hk, D):
+def _refuse_caches(k_cache, v_cache, Hk, D) -> None:
     for c in (k_cache, v_cache):
         if c.dim() != 4 or tuple(c.shape[2:]) != (Hk, D) or c.shape[:2] != k_cache.shape[:2] or min(c.shape[:2]) <= 0:
             raise ValueError(f"caches must have shape (pages, page size, {Hk}, {D}), got {tuple(c.shape)}")
-    return int(k_cache.shape[0]), int(k_cache.shape[1])
 
 
 def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interleaved: bool = False,
@@ -260,30 +293,37 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interl
     ``slots[t] // page size`` of the caches (pages, page size, Hk, D).  A token
     whose slot lies outside the cache (-1: padding) is not written.  The slots of
     one call have to differ from each other."""
-    T, Hq, Hk, D, dev, rot, positions, inv_freq = _rope_args("rope_append", q, k, (v,), positions, inv_freq, scale)
-    _same_dtype(q, k_cache, v_cache)
-    _check("rope_append", q.dtype, q, k_cache, v_cache)
-    pages, page = _cache(k_cache, v_cache, q, Hk, D)
-    _writable("k_cache", k_cache, k_cache.shape, q)
-    _writable("v_cache", v_cache, v_cache.shape, q)
-    _apart("k_cache", k_cache, v_cache, q, k, v)
-    _apart("v_cache", v_cache, q, k, v)
-    slots = _index("slots", slots, (T,), torch.int64, dev)
+    T, Hq, Hk, D, index, rot, positions, inv_freq = _rope_args("rope_append", q, k, v, positions, inv_freq, scale)
+    cs = k_cache.shape
+    if len(cs) != 4 or v_cache.shape != cs or cs[2] != Hk or cs[3] != D or not cs[0] or not cs[1]:
+        _refuse_caches(k_cache, v_cache, Hk, D)
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        _refuse_dtype(q.dtype, k_cache.dtype, v_cache.dtype)
+    if k_cache.get_device() != index or v_cache.get_device() != index:
+        _refuse_device("rope_append", q, k_cache, v_cache)
+    if torch.is_grad_enabled():
+        _refuse_grad("rope_append", k_cache, v_cache)
+    _writable("k_cache", k_cache, cs, q)
+    _writable("v_cache", v_cache, cs, q)
+    kb, vb = k_cache.untyped_storage().data_ptr(), v_cache.untyped_storage().data_ptr()
+    inputs = {t.untyped_storage().data_ptr() for t in (q, k, v)}
+    if kb == vb or kb in inputs or vb in inputs:  # of one storage: perhaps of the same memory
+        _apart("k_cache", k_cache, v_cache, q, k, v)
+        _apart("v_cache", v_cache, q, k, v)
+    slots = _index("slots", slots, (T,), torch.int64, index)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        out = q.new_empty((T, Hq, D))
     else:
         _writable("out", out, (T, Hq, D), q)
         _apart("out", out, q, k, v, k_cache, v_cache, own=(q,))
     if T == 0:
         return out
     q, k, v = _last(q), _last(k), _last(v)
-    lib = _lib.load()
-    st = _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1),
-                  *k_cache.stride()[:3], *v_cache.stride()[:3])
-    _lib.check(_on_device(dev, lambda: lib.svdmlp_rope_append(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(),
-        out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ctypes.addressof(st), T, pages, page, Hq, Hk, D, rot, scale,
-        _ACT_CODES[q.dtype], _lib.SVDMLP_ROPE_INTERLEAVED if interleaved else 0, _stream(dev))))
+    st = _Strides14(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3],
+                    *v_cache.stride()[:3])
+    _launch(index, _lib.load().svdmlp_rope_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
+            inv_freq.data_ptr(), slots.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _address(st), T,
+            cs[0], cs[1], Hq, Hk, D, rot, scale, _ACT_CODES[q.dtype], 1 if interleaved else 0)
     return out
 
 
@@ -299,7 +339,7 @@ def _attention_scale(scale, D: int) -> float:
 
 
 def _head_size(D: int, dtype: torch.dtype) -> None:
-    step = 16 // torch.empty(0, dtype=dtype).element_size()
+    step = 8 if dtype is _BF16 else 4
     if D > 256 or D % step:
         raise ValueError(f"head sizes are multiples of {step} up to 256 for {dtype}, got {D}")
 
@@ -312,19 +352,28 @@ def prompt_attention(q, k, v, cu_seqlens=None, *, causal: bool = True, scale: fl
     own, else its whole sequence.  ``scale`` defaults to 1/sqrt(D).  Query head
     h reads key/value head h // (Hq // Hk).  Head sizes are multiples of 8 (bf16)
     or 4 (fp32) up to 256.  Rows behind the last sequence are not written."""
-    T, Hq, Hk, D = _heads(q, k, v)
-    _same_dtype(q, k, v)
-    dev = _check("prompt_attention", q.dtype, q, k, v)
-    _head_size(D, q.dtype)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks[0] != qs[0] or ks[2] != qs[2] or not ks[1] or not qs[2] or not qs[1] or qs[1] % ks[1] or v.shape != ks:
+        _refuse_heads(q, k, v)
+    T, Hq, D = qs
+    dtype, index = q.dtype, q.get_device()
+    if k.dtype != dtype or v.dtype != dtype or dtype not in _ACT_CODES:
+        _refuse_dtype(dtype, k.dtype, v.dtype)
+    if index < 0 or k.get_device() != index or v.get_device() != index:
+        _refuse_device("prompt_attention", q, k, v)
+    if torch.is_grad_enabled():
+        _refuse_grad("prompt_attention", q, k, v)
+    _head_size(D, dtype)
     scale = _attention_scale(scale, D)
-    B = 1
+    B, cu = 1, None
     if cu_seqlens is not None:
         if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
             raise ValueError("cu_seqlens must hold the first row of each sequence and the end of the last")
-        B = int(cu_seqlens.shape[0]) - 1
-        cu_seqlens = _index("cu_seqlens", cu_seqlens, (B + 1,), torch.int32, dev)
+        B = cu_seqlens.shape[0] - 1
+        cu_seqlens = _index("cu_seqlens", cu_seqlens, (B + 1,), torch.int32, index)
+        cu = cu_seqlens.data_ptr()
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        out = q.new_empty((T, Hq, D))
     else:
         _writable("out", out, (T, Hq, D), q)
         _aligned("out", out)
@@ -332,12 +381,9 @@ def prompt_attention(q, k, v, cu_seqlens=None, *, causal: bool = True, scale: fl
     if T == 0:
         return out
     q, k, v = _rows(q), _rows(k), _rows(v)
-    lib = _lib.load()
-    st = _strides(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1))
-    _lib.check(_on_device(dev, lambda: lib.svdmlp_prompt_attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(), out.data_ptr(),
-        ctypes.addressof(st), T, B, Hq, Hk, D, scale, _ACT_CODES[q.dtype], _lib.SVDMLP_CAUSAL if causal else 0,
-        _stream(dev))))
+    st = _Strides8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2])
+    _launch(index, _lib.load().svdmlp_prompt_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu, out.data_ptr(),
+            _address(st), T, B, Hq, ks[1], D, scale, _ACT_CODES[dtype], 1 if causal else 0)
     return out
 
 
@@ -351,44 +397,49 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
     ((n, n) or (B, n, n) bool) names; without a tree, those up to itself.  n = 1 is
     the decode step.  A token without keys (length 0, or an empty row of a tree
     without context) gets zeros.  Pages outside the cache hold no keys."""
-    if q.dim() != 4:
-        raise ValueError(f"expected q (sequences, new tokens, heads, head size), got {tuple(q.shape)}")
-    B, n, Hq, D = q.shape
-    if k_cache.dim() != 4:
-        raise ValueError(f"caches must have shape (pages, page size, kv heads, {D}), got {tuple(k_cache.shape)}")
-    Hk = int(k_cache.shape[2])
-    pages, page = _cache(k_cache, v_cache, q, Hk, D)
-    if min(Hq, Hk, D) <= 0 or Hq % Hk:
+    qs, cs = q.shape, k_cache.shape
+    if len(qs) != 4:
+        raise ValueError(f"expected q (sequences, new tokens, heads, head size), got {tuple(qs)}")
+    B, n, Hq, D = qs
+    if len(cs) != 4 or v_cache.shape != cs or cs[3] != D or not cs[0] or not cs[1]:
+        _refuse_caches(k_cache, v_cache, cs[2] if len(cs) == 4 else "kv heads", D)
+    pages, page, Hk, _ = cs
+    if not Hq or not Hk or not D or Hq % Hk:
         raise ValueError(f"{Hq} query heads are no multiple of {Hk} key/value heads")
     if not 1 <= n <= 64:
         raise ValueError(f"1 to 64 new tokens a sequence, got {n}")
-    _same_dtype(q, k_cache, v_cache)
-    dev = _check("cache_attention", q.dtype, q, k_cache, v_cache)
-    _head_size(D, q.dtype)
+    dtype, index = q.dtype, q.get_device()
+    if k_cache.dtype != dtype or v_cache.dtype != dtype or dtype not in _ACT_CODES:
+        _refuse_dtype(dtype, k_cache.dtype, v_cache.dtype)
+    if index < 0 or k_cache.get_device() != index or v_cache.get_device() != index:
+        _refuse_device("cache_attention", q, k_cache, v_cache)
+    if torch.is_grad_enabled():
+        _refuse_grad("cache_attention", q, k_cache, v_cache)
+    _head_size(D, dtype)
     scale = _attention_scale(scale, D)
     if block_table.dim() != 2 or block_table.shape[1] == 0:
         raise ValueError("block_table must have shape (sequences, pages of the longest)")
-    width = int(block_table.shape[1])
-    if block_table.stride(1) != 1 or block_table.dtype != torch.int32:
-        block_table = _index("block_table", block_table, (B, width), torch.int32, dev)
-    elif block_table.shape[0] != B or block_table.device != dev:
-        raise ValueError(f"block_table must have shape ({B}, pages of the longest) on {dev}")
-    lengths = _index("lengths", lengths, (B,), torch.int32, dev)
-    tree_ptr = tree_b = tree_q = 0
+    width = block_table.shape[1]
+    if block_table.stride(1) != 1 or block_table.dtype is not torch.int32:
+        block_table = _index("block_table", block_table, (B, width), torch.int32, index)
+    elif block_table.shape[0] != B or block_table.get_device() != index:
+        raise ValueError(f"block_table must have shape ({B}, pages of the longest) on {q.device}")
+    lengths = _index("lengths", lengths, (B,), torch.int32, index)
+    tree_ptr, tree_b, tree_q = None, 0, 0
     if tree is not None:
         if tree.dtype not in (torch.bool, torch.uint8) or tuple(tree.shape) not in ((n, n), (B, n, n)):
             raise ValueError(f"tree must be a bool tensor ({n}, {n}) or ({B}, {n}, {n}), got {tree.dtype} {tuple(tree.shape)}")
-        if tree.device != dev:
+        if tree.get_device() != index:
             raise ValueError("all inputs must be on the same device")
         if n > 1 and tree.stride(-1) != 1:
             tree = tree.contiguous()
         tree_ptr, tree_b, tree_q = tree.data_ptr(), tree.stride(0) if tree.dim() == 3 else 0, tree.stride(-2)
     for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.stride(-1) != 1:
+        if c.stride(3) != 1:
             raise ValueError(f"the last dimension of {name} must be contiguous")
         _aligned(name, c)
     if out is None:
-        out = torch.empty((B, n, Hq, D), dtype=q.dtype, device=dev)
+        out = q.new_empty((B, n, Hq, D))
     else:
         _writable("out", out, (B, n, Hq, D), q)
         _aligned("out", out)
@@ -397,33 +448,44 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
         return out
     q = _rows(q)
     lib = _lib.load()
-    st = _strides(*q.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3], *out.stride()[:3], block_table.stride(0),
-                  tree_b, tree_q)
-
-    def call():
-        # the partial sums of long contexts: of the call alone, from torch's
-        # allocator (of a graph's own pool under capture)
-        nbytes = int(lib.svdmlp_cache_attention_workspace_bytes(B, n, page, width, Hq, Hk, D, _ACT_CODES[q.dtype]))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        return lib.svdmlp_cache_attention(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), tree_ptr or None,
-            out.data_ptr(), ctypes.addressof(st), B, n, pages, page, width, Hq, Hk, D, scale, _ACT_CODES[q.dtype],
-            None if ws is None else ws.data_ptr(), nbytes, _stream(dev))
-
-    _lib.check(_on_device(dev, call))
+    st = _Strides15(*q.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3], *out.stride()[:3], block_table.stride(0),
+                    tree_b, tree_q)
+    # the partial sums of long contexts: of the call alone, from torch's
+    # allocator (of a graph's own pool under capture)
+    code = _ACT_CODES[dtype]
+    nbytes, ws = _part_bytes(lib, index, B, n, page, width, Hq, Hk, D, code), None
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+            lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
+            None if ws is None else ws.data_ptr(), nbytes)
     return out
+
+
+_PART_BYTES: dict = {}
+
+
+def _part_bytes(lib, index, *sizes) -> int:
+    """svdmlp_cache_attention_workspace_bytes of the sizes on device `index` (it depends on the sizes and its CUs alone)."""
+    key = (index, *sizes)
+    n = _PART_BYTES.get(key)
+    if n is None:
+        with torch.cuda.device(index):
+            n = int(lib.svdmlp_cache_attention_workspace_bytes(*sizes))
+        if len(_PART_BYTES) > 4096:
+            _PART_BYTES.clear()
+        _PART_BYTES[key] = n
+    return n
 
 
 # ---------------------------------------------------------------------------
 # Residual sum and norms
 # ---------------------------------------------------------------------------
 
-def _gain(name, w, d, dev):
-    if w is None:
-        return None
-    if w.dim() != 1 or w.shape[0] != d or w.device != dev or not w.is_floating_point():
+def _gain(name, w, d, index):
+    if w.dim() != 1 or w.shape[0] != d or w.get_device() != index or not w.is_floating_point():
         raise ValueError(f"{name} must be a ({d},) tensor on x.device")
-    return w.to(torch.float32).contiguous()
+    return w if w.dtype is torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
 
 
 def residual_norm(x, branch, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-5,
@@ -439,50 +501,65 @@ def residual_norm(x, branch, weight, *, post_weight=None, gate=None, scale: floa
     itself (the norm before a model's first block); weight None: n is None (the
     sum after its last).  d up to 32768.  ``out``: (r, n) to write, either may be
     None; they may be x and branch themselves."""
-    if x.dim() != 2 or min(x.shape) <= 0:
-        raise ValueError(f"expected a nonempty 2D array, got {tuple(x.shape)}")
-    T, d = x.shape
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 2 or not shape[0] or not shape[1]:
+        raise ValueError(f"expected a nonempty 2D array, got {tuple(shape)}")
+    T, d = shape
     if branch is None and (post_weight is not None or gate is not None or weight is None):
         raise ValueError("without a branch there is only a norm of x")
-    tensors = [t for t in (branch, gate) if t is not None]
-    _same_dtype(x, *tensors)
-    dev = _check("residual_norm", x.dtype, x, *tensors, *(w for w in (weight, post_weight) if w is not None))
-    if branch is not None and branch.shape != x.shape:
-        raise ValueError(f"branch must have x's shape {tuple(x.shape)}, got {tuple(branch.shape)}")
+    if dtype not in _ACT_CODES or (branch is not None and branch.dtype != dtype) or (gate is not None and gate.dtype != dtype):
+        _refuse_dtype(dtype, *(t.dtype for t in (branch, gate) if t is not None))
+    index = x.get_device()
+    if index < 0 or (branch is not None and branch.get_device() != index) or (gate is not None and gate.get_device() != index):
+        _refuse_device("residual_norm", x, branch, gate)
+    if torch.is_grad_enabled():
+        _refuse_grad("residual_norm", x, branch, gate, weight, post_weight)
+    if branch is not None and branch.shape != shape:
+        raise ValueError(f"branch must have x's shape {tuple(shape)}, got {tuple(branch.shape)}")
     if gate is not None and tuple(gate.shape) not in ((d,), (T, d)):
         raise ValueError(f"gate must have shape ({d},) or ({T}, {d}), got {tuple(gate.shape)}")
     if d > 32768:
         raise ValueError(f"rows of {d} values, at most 32768")
-    eps, scale = float(eps), float(scale)
     if not (eps > 0 and math.isfinite(eps)):
         raise ValueError(f"eps must be positive, got {eps}")
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
-    w, pw = _gain("weight", weight, d, dev), _gain("post_weight", post_weight, d, dev)
-    x0 = x
-    x = _last(x)
-    branch = None if branch is None else _last(branch)
-    gate = None if gate is None else _last(gate)
-    r, n = (None, None) if out is None else out
-    for name, t in (("out[0]", r), ("out[1]", n)):
-        if t is not None:
-            _writable(name, t, (T, d), x)
-            inputs = [a for a in (x, branch, gate) if a is not None]
-            _apart(name, t, *inputs, own=[a for a in inputs if a.dim() == 2])
-    if r is not None and n is not None:
-        _apart("out[0]", r, n)
+    w = pw = wp = pwp = bp = gp = rp = n_p = None
+    bs = gs = rs = ns = 0
+    if weight is not None:
+        w = _gain("weight", weight, d, index)
+        wp = w.data_ptr()
+    if post_weight is not None:
+        pw = _gain("post_weight", post_weight, d, index)
+        pwp = pw.data_ptr()
+    x0, x = x, _last(x)
+    if branch is not None:
+        branch = _last(branch)
+        bp, bs = branch.data_ptr(), branch.stride(0)
+    if gate is not None:
+        gate = _last(gate)
+        gp, gs = gate.data_ptr(), gate.stride(0) if gate.dim() == 2 else 0
+    r = n = None
+    if out is not None:
+        r, n = out
+        inputs = [a for a in (x, branch, gate) if a is not None]
+        for name, t in (("out[0]", r), ("out[1]", n)):
+            if t is not None:
+                _writable(name, t, (T, d), x)
+                _apart(name, t, *inputs, own=[a for a in inputs if a.dim() == 2])
+        if r is not None and n is not None:
+            _apart("out[0]", r, n)
     if branch is not None and r is None:
-        r = torch.empty((T, d), dtype=x.dtype, device=dev)
-    if w is not None and n is None:
-        n = torch.empty((T, d), dtype=x.dtype, device=dev)
-    elif w is None:
+        r = x.new_empty((T, d))
+    if w is None:
         n = None
-    lib = _lib.load()
-    st = _strides(x.stride(0), branch.stride(0) if branch is not None else 0,
-                  gate.stride(0) if gate is not None and gate.dim() == 2 else 0,
-                  r.stride(0) if r is not None else 0, n.stride(0) if n is not None else 0)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _lib.check(_on_device(dev, lambda: lib.svdmlp_residual_norm(
-        x.data_ptr(), ptr(branch), ptr(pw), ptr(gate), ptr(w), ptr(r), ptr(n), ctypes.addressof(st), T, d, scale, eps,
-        _ACT_CODES[x.dtype], _stream(dev))))
+    elif n is None:
+        n = x.new_empty((T, d))
+    if r is not None:
+        rp, rs = r.data_ptr(), r.stride(0)
+    if n is not None:
+        n_p, ns = n.data_ptr(), n.stride(0)
+    st = _Strides5(x.stride(0), bs, gs, rs, ns)
+    _launch(index, _lib.load().svdmlp_residual_norm, x.data_ptr(), bp, pwp, gp, wp, rp, n_p, _address(st), T, d, scale, eps,
+            _ACT_CODES[dtype])
     return (x0 if r is None else r), n
