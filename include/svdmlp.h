@@ -347,20 +347,24 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
  * that holds lengths[b] tokens, the new ones last among them.  Token i sees all
  * keys before the new ones, and new key j if tree[b][i][j] (bytes) is nonzero
  * or, with tree NULL, if j <= i.  Key x of sequence b is row x % page of page
- * block_table[b][x / page] (int32, width pages a sequence); a page outside the
+ * block_table[b][x / page] (int32, width pages a sequence, at most 65536); a page outside the
  * cache holds no keys.  A token without keys gets zeros (a sequence of length 0
  * too).  D as svdmlp_prompt_attention.  strides: q sequence, token, head;
  * k_cache page, row, head; v_cache page, row, head; out sequence, token, head;
  * block_table sequence; tree sequence, token.  The workspace
- * (svdmlp_cache_attention_workspace_bytes; may be 0) holds the partial sums of long contexts and needs no clearing.
+ * (svdmlp_cache_attention_workspace_bytes; may be 0) holds the partial sums of
+ * long contexts and needs no clearing.  With one go `counters` int32 counters
+ * (*counters of svdmlp_cache_attention_workspace_bytes, if not NULL), zero
+ * before the call, which leaves them zero: calls in flight at the same time
+ * (other streams, graphs) need workspaces and counters of their own.
  */
 size_t svdmlp_cache_attention_workspace_bytes(int64_t B, int64_t n, int64_t page, int64_t width, int64_t Hq,
-                                              int64_t Hk, int64_t D, int32_t dtype);
+                                              int64_t Hk, int64_t D, int32_t dtype, int64_t* counters);
 int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                            const int32_t* lengths, const uint8_t* tree, void* out,
                            const int64_t* strides /* 15 or NULL */, int64_t B, int64_t n, int64_t pages, int64_t page,
                            int64_t width, int64_t Hq, int64_t Hk, int64_t D, float scale, int32_t dtype,
-                           void* workspace, size_t ws_bytes, void* stream);
+                           void* workspace, size_t ws_bytes, int32_t* counters, int64_t n_counters, void* stream);
 
 /*
  * The sum after a block and the norm before the next:

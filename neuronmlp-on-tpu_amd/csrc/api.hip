@@ -2661,19 +2661,22 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
 }
 
 size_t svdmlp_cache_attention_workspace_bytes(int64_t B, int64_t n, int64_t page, int64_t width, int64_t Hq, int64_t Hk,
-                                              int64_t D, int32_t dtype) {
-  if (!act_size(dtype) || B <= 0 || B > 0x7fffffff / 64 || n <= 0 || n > 64 || Hq <= 0 || Hq > 65536 || Hk <= 0 || Hq % Hk || D <= 0 || D > 256 ||
-      page <= 0 || width <= 0 || page > 0x7fffff00 / width)
+                                              int64_t D, int32_t dtype, int64_t* counters) {
+  if (counters) *counters = 0;
+  if (!act_size(dtype) || B <= 0 || B > 0x7fffffff / 64 || n <= 0 || n > 64 || Hq <= 0 || Hq > 65536 || Hk <= 0 || Hq % Hk ||
+      D <= 0 || D > 256 || page <= 0 || width <= 0 || width > kCachePagesMost || page > 0x7fffff00 / width)
     return 0;
-  int splits, chunk;
-  plan_cache_attention((int)B, (int)n, (int)Hq, (int)Hk, (int)D, dtype == SVDMLP_BF16, (int)page, page * width, device_cus(), &splits, &chunk);
-  return (size_t)cache_part_floats((int)B, (int)n, (int)Hq, (int)D, splits) * 4;
+  const CachePlan plan = plan_cache_attention((int)B, (int)n, (int)Hq, (int)Hk, (int)D, dtype == SVDMLP_BF16, (int)page,
+                                              page * width, device_cus());
+  if (counters && plan.splits > 1) *counters = B * Hk * plan.rtiles;
+  return (size_t)cache_part_floats((int)B, (int)n, (int)Hq, (int)D, plan.splits) * 4;
 }
 
 int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                            const int32_t* lengths, const uint8_t* tree, void* out, const int64_t* strides,
                            int64_t B, int64_t n, int64_t pages, int64_t page, int64_t width, int64_t Hq, int64_t Hk,
-                           int64_t D, float scale, int32_t dtype, void* workspace, size_t ws_bytes, void* stream) {
+                           int64_t D, float scale, int32_t dtype, void* workspace, size_t ws_bytes, int32_t* counters,
+                           int64_t n_counters, void* stream) {
   if (B <= 0 || n <= 0) return fail("cache_attention: sizes must be positive");
   if (n > 64) return fail("cache_attention: at most 64 new tokens a sequence, got %lld", (long long)n);
   int rc = check_heads("cache_attention", B > 0x7fffffff / 64 ? INT64_MAX : B * n, Hq, Hk, D, dtype, 256);
@@ -2681,6 +2684,7 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   if (!q || !k_cache || !v_cache || !block_table || !lengths || !out) return fail("cache_attention: null pointer");
   if (pages <= 0 || page <= 0 || width <= 0 || page > 0x7fffff00 / width)
     return fail("cache_attention: pages, page size and the table's width must be positive, with less than 2^31 tokens a sequence");
+  if (width > kCachePagesMost) return fail("cache_attention: %lld pages a sequence, at most %lld", (long long)width, (long long)kCachePagesMost);
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail("cache_attention: scale must be positive and finite");
   const int64_t dense[15] = {n * Hq * D, Hq * D, D, page * Hk * D, Hk * D, D, page * Hk * D, Hk * D, D,
                              n * Hq * D, Hq * D, D, width, n * n, n};
@@ -2689,6 +2693,7 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   if (!no_negative(s, 15)) return fail("cache_attention: strides must not be negative");
   if (!pieces16({q, k_cache, v_cache, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10], s[11]}, es))
     return fail("cache_attention: the head size, strides and addresses must be whole 16-byte pieces");
+  if (s[4] > 1 << 24 || s[7] > 1 << 24) return fail("cache_attention: rows of the cache are more than 2^24 elements apart");
   CacheParams p = {};
   p.q = q, p.kc = k_cache, p.vc = v_cache, p.table = block_table, p.lengths = lengths, p.tree = tree, p.out = out;
   p.q_b = s[0], p.q_t = s[1], p.q_h = s[2], p.k_p = s[3], p.k_t = s[4], p.k_h = s[5], p.v_p = s[6], p.v_t = s[7], p.v_h = s[8];
@@ -2696,13 +2701,18 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   p.pages = pages, p.page = (int)page, p.width = (int)width;
   p.B = (int)B, p.n = (int)n, p.Hq = (int)Hq, p.Hk = (int)Hk, p.D = (int)D;
   p.c = scale * 1.44269504088896340736f;
-  plan_cache_attention(p.B, p.n, p.Hq, p.Hk, p.D, dtype == SVDMLP_BF16, p.page, page * width, device_cus(), &p.splits, &p.chunk);
+  const CachePlan plan = plan_cache_attention(p.B, p.n, p.Hq, p.Hk, p.D, dtype == SVDMLP_BF16, p.page, page * width, device_cus());
+  p.splits = plan.splits, p.chunk = plan.chunk;
   const size_t need = (size_t)cache_part_floats(p.B, p.n, p.Hq, p.D, p.splits) * 4;
   if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15u)))
     return fail("cache_attention: workspace too small: %zu bytes needed, 16-byte aligned, got %zu", need, ws_bytes);
+  const int64_t nc = B * Hk * plan.rtiles;
+  if (need && (!counters || n_counters < nc || ((uintptr_t)counters & 3u)))
+    return fail("cache_attention: %lld counters needed, got %lld", (long long)nc, (long long)(counters ? n_counters : 0));
   p.part = static_cast<float*>(workspace);
+  p.counters = counters;
   StageScope sc(ST_CACHE_ATTENTION, (hipStream_t)stream);
-  return check(launch_cache_attention(p, dtype == SVDMLP_BF16, (hipStream_t)stream), "cache_attention");
+  return check(launch_cache_attention(p, dtype == SVDMLP_BF16, plan.waves, (hipStream_t)stream), "cache_attention");
 }
 
 int svdmlp_residual_norm(const void* x, const void* branch, const float* post_w, const void* gate,

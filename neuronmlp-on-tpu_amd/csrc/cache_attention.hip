@@ -4,12 +4,15 @@
 // itself).  n = 1 is the decode step.
 //
 // Bound by the cache's bytes, read once for all heads of a group and all new
-// tokens (up to 32 * QG rows).  Nothing is shared between waves: each of a
-// block's waves takes every NW-th tile of 32 keys of the block's chunk through
-// LDS of its own (direct loads, the next tile's in flight while one is
-// computed), with no barrier in the loop, and their sums meet at the end.
-// A long context is cut into chunks, one a block; a second launch joins their
-// partial sums in the chunks' order (no atomics: the same bits every time).
+// tokens (up to 32 * QG rows).  Nothing is shared between waves: each takes tiles
+// of 32 keys of its block's chunk through LDS of its own (direct loads, the next
+// tile's in flight while one is computed), with no barrier in the loop.  Where
+// there is work for every wave of the card, a block is one wave, and four of
+// them share a CU, one's start and end hidden behind the others' loads; where
+// there is not, a block's four waves share a chunk, and their sums meet in LDS.
+// A long context is cut into chunks, one a block; the last block of a
+// (sequence, head, row tile) to arrive joins the chunks' partial sums, in the
+// chunks' order (the same bits every time).
 #include <math.h>
 
 #include <algorithm>
@@ -21,9 +24,10 @@ namespace svdmlp {
 
 namespace {
 
+constexpr int kSplitsMost = 64;   // chunks of a sequence
 constexpr int kPagesMost = 1024;  // whole pages of a chunk: their numbers lie in LDS
 
-template <bool BF16_, int DP_, int QG_>
+template <bool BF16_, int DP_, int QG_, int NW_>
 struct CacheCfg {
   static constexpr bool BF16 = BF16_;
   static constexpr int DP = DP_, QG = QG_;
@@ -31,17 +35,34 @@ struct CacheCfg {
   static constexpr int RB = DP * ES;
   static constexpr int PIECES = RB / 16;
   static constexpr int STEPS = RB / 32;
-  static constexpr int NW = RB <= 256 ? 4 : RB == 512 ? 2 : 1;  // waves: two stages of two tiles each in 160 KB
+  static constexpr int NW = NW_;  // waves a block
   static constexpr int TILE = 32 * RB;
   static constexpr int STAGE = 2 * TILE;  // keys, values
   static constexpr int ROWS = 32 * QG;
   static constexpr int RPI = 64 / PIECES;        // rows a load
   static constexpr int LOADS = 32 / RPI;         // loads a tile, of keys and of values
   static_assert(2 * STAGE >= ROWS * DP * 4, "a wave's sums fit its stages");
+  static_assert(NW * 2 * STAGE >= ROWS * kSplitsMost * 4, "the chunks' weights fit too");
 };
 
 // 16 bytes of zeros that lanes without a key load.
 __device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
+
+// Lane j's v, the same for all lanes (j a constant).
+__device__ __forceinline__ int64_t lane64(int64_t v, int j) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, j) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), j) << 32);
+}
+
+// Partial sums cross blocks, and so XCDs with an L2 each, by device-scope
+// accesses (past the L2), without any cache maintenance: fences that write back
+// and drop the L2 for every block made a call of 4096 blocks twice as long.
+__device__ __forceinline__ void store_device(float* p, f32x2 v) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 load_device(const float* p) {
+  return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float*>(p)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
 
 __device__ __forceinline__ int held(const CacheParams& p, int b) {
   const int64_t cap = (int64_t)p.width * p.page;
@@ -76,7 +97,8 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   const int b = id % p.B, split = id / p.B;
   const int len = held(p, b);
   const int kbeg = split * p.chunk, kend = min(len, kbeg + p.chunk);
-  if (kbeg >= kend && p.splits > 1) return;  // the join knows from the length
+  const int used = max(1, (int)(((int64_t)len + p.chunk - 1) / p.chunk));  // chunks that hold keys; the first always answers
+  if (split >= used) return;
   const int context = len - p.n;             // keys that every row sees
 
   // The chunk's pages, and the queries.
@@ -147,23 +169,48 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     const int pg = ku + row < kend ? ids[i] : -1;
     return pg >= 0 && pg < p.pages ? pg : -1;
   };
+  // A lane's part of a load's addresses: row lane / PIECES of its RPI rows,
+  // piece lane % PIECES, both swizzled; load j adds a constant (the swizzles
+  // pick bits of the row, so that they combine by exclusive or).
+  const int lrow = lane / C::PIECES, lc = lane % C::PIECES;
+  const int kpiece = lc ^ k_swz<RB>(lrow), vpiece = lc ^ v_swz<RB, BF16>(lrow);
+  const uint32_t krow = (uint32_t)(lrow * (int)p.k_t * ES), vrow = (uint32_t)(lrow * (int)p.v_t * ES);
   auto issue = [&](int ku, attn_lds stage) {
     const uint32_t base = (uint32_t)(uintptr_t)stage;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
+    if (p.page_shift >= 0 && ku + 32 <= kend) {
+      // Pages of a power of two that hold whole loads: lane j finds load j's
+      // page, and its address goes to all lanes through scalar registers.
+      const int key = ku + lane % C::LOADS * C::RPI, pg = ids[(key >> p.page_shift) - pg0], in = key & (p.page - 1);
+      if (__all(pg >= 0 && pg < p.pages)) {
+        const int64_t ko = ((int64_t)pg * p.k_p + (int64_t)in * p.k_t) * ES, vo = ((int64_t)pg * p.v_p + (int64_t)in * p.v_t) * ES;
 #pragma unroll
+        for (int j = 0; j < C::LOADS; ++j) {
+          const int ck = kpiece ^ k_swz<RB>(j * C::RPI), cv = vpiece ^ v_swz<RB, BF16>(j * C::RPI);
+          const char* const kp = kb + lane64(ko, j);
+          const char* const vp = vb + lane64(vo, j);
+          if (ck < npieces) load_lds16(kp, krow + 16 * ck, base + j * 1024);
+          if (cv < npieces) load_lds16(vp, vrow + 16 * cv, base + C::TILE + j * 1024);
+        }
+        return;
+      }
+    }
+#pragma unroll 2
     for (int j = 0; j < C::LOADS; ++j) {
-      const int row = j * C::RPI + lane / C::PIECES, c = lane % C::PIECES;
+      const int row = j * C::RPI + lrow;
       int in;
       const int pg = place(ku, row, &in);
-      const int ck = c ^ k_swz<RB>(row), cv = c ^ v_swz<RB, BF16>(row);
+      const int ck = lc ^ k_swz<RB>(row), cv = lc ^ v_swz<RB, BF16>(row);
       const char* kp = kb + ((int64_t)pg * p.k_p + (int64_t)in * p.k_t) * ES + 16 * ck;
       const char* vp = vb + ((int64_t)pg * p.v_p + (int64_t)in * p.v_t) * ES + 16 * cv;
-      kp = pg >= 0 && ck < npieces ? kp : reinterpret_cast<const char*>(&kZeroPiece);
-      vp = pg >= 0 && cv < npieces ? vp : reinterpret_cast<const char*>(&kZeroPiece);
-      load_lds16(kp, base + j * 1024);
-      load_lds16(vp, base + C::TILE + j * 1024);
+      kp = pg >= 0 ? kp : reinterpret_cast<const char*>(&kZeroPiece);
+      vp = pg >= 0 ? vp : reinterpret_cast<const char*>(&kZeroPiece);
+      if (ck < npieces) load_lds16(kp, base + j * 1024);
+      if (cv < npieces) load_lds16(vp, base + C::TILE + j * 1024);
     }
   };
+  if (p.D < C::DP)  // pieces behind the head's end: never loaded, zeros
+    for (int i = lane; i < 2 * C::STAGE / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
 
   int ku = kbeg + 32 * wave;
   attn_lds cur = mine, nxt = mine + C::STAGE;
@@ -329,64 +376,75 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
       v += *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>((attn_lds)lds + w * 2 * C::STAGE + (rr * OP + (piece ^ (rr & OM))) * 16);
     }
     const int t = r / G, h = hk * G + r - t * G;
-    if (p.splits == 1) {
+    if (used == 1) {
       v *= inverse_sum(l);
       store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
     } else {
       const int64_t row = (((int64_t)b * p.n + t) * p.Hq + h) * p.splits + split;
-      *reinterpret_cast<f32x4*>(p.part + row * p.D + 4 * piece) = v;
-      if (piece == 0) *reinterpret_cast<f32x2*>(p.part + total * p.splits * p.D + 2 * row) = f32x2{m, l};
+      store_device(p.part + row * p.D + 4 * piece, f32x2{v.x, v.y});
+      store_device(p.part + row * p.D + 4 * piece + 2, f32x2{v.z, v.w});
+      if (piece == 0) store_device(p.part + total * p.splits * p.D + 2 * row, f32x2{m, l});
     }
   }
+  if (used == 1) return;
+
+  // The last block to get here joins the chunks.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums are out
+  __syncthreads();
+  int* const counter = p.counters + ((int64_t)b * p.Hk + hk) * rtiles + rt;
+  int last = 0;
+  if (threadIdx.x == 0) {
+    last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == used - 1;
+    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // as the next call finds it
+    stats[0][0][0] = last ? 1.f : 0.f;
+  }
+  __syncthreads();
+  if (stats[0][0][0] == 0.f) return;
+  SVDMLP_ATTN_LDS float* const weight = (SVDMLP_ATTN_LDS float*)(attn_lds)lds;  // [row][kSplitsMost]
+  const int nrows = min(C::ROWS, rows - rt * C::ROWS);
+  const float* const ml = p.part + total * p.splits * p.D;
+  auto part_row = [&](int rr) -> int64_t {
+    const int r = rt * C::ROWS + rr, t = r / G;
+    return (((int64_t)b * p.n + t) * p.Hq + hk * G + r - t * G) * p.splits;
+  };
+  // A wave takes a row: its lanes the chunks' maxima and sums.
+  for (int rr = wave; rr < nrows; rr += NW) {
+    const f32x2 v = lane < used ? load_device(ml + 2 * (part_row(rr) + lane)) : f32x2{-INFINITY, 0.f};
+    float m = v.x;
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float a = v.x == -INFINITY ? 1.f : exp2f(v.x - m);
+    float l = v.y * a;
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    weight[rr * kSplitsMost + lane] = a * inverse_sum(l);
+  }
+  __syncthreads();
+  const int dp = p.D / 4;
+  for (int i = threadIdx.x; i < nrows * dp; i += 64 * NW) {
+    const int rr = i / dp, piece = i - rr * dp;
+    const int64_t row = part_row(rr);
+    const float* const part = p.part + row * p.D + 4 * piece;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < used; ++s) {
+      const f32x2 a = load_device(part + (int64_t)s * p.D), c = load_device(part + (int64_t)s * p.D + 2);
+      v += f32x4{a.x, a.y, c.x, c.y} * weight[rr * kSplitsMost + s];
+    }
+    const int r = rt * C::ROWS + rr, t = r / G, h = hk * G + r - t * G;
+    store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
+  }
 }
 
-// Joins the chunks' partial sums: `per` groups of LPR lanes share a row, each
-// takes every per-th chunk, and the first adds the groups' sums in order.
-template <bool BF16, int LPR>
-__global__ __launch_bounds__(256) void cache_join_kernel(CacheParams p, int per) {
-  constexpr int GROUPS = 256 / LPR;
-  __shared__ f32x4 sums[GROUPS][LPR];
-  const int group = threadIdx.x / LPR, piece = threadIdx.x % LPR, sub = group % per;
-  const int64_t total = (int64_t)p.B * p.n * p.Hq;
-  const int64_t row = (int64_t)blockIdx.x * (GROUPS / per) + group / per;
-  const bool in = row < total && 4 * piece < p.D;
-  const int64_t bt = row / p.Hq;
-  const int h = (int)(row - bt * p.Hq), b = (int)(bt / p.n), t = (int)(bt - (int64_t)b * p.n);
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  if (in) {
-    const int used = min(p.splits, (int)(((int64_t)held(p, b) + p.chunk - 1) / p.chunk));
-    const float* const part = p.part + row * p.splits * p.D + 4 * piece;
-    const f32x2* const ml = reinterpret_cast<const f32x2*>(p.part + total * p.splits * p.D) + row * p.splits;
-    float m = -INFINITY;
-    for (int s = 0; s < used; ++s) m = fmaxf(m, ml[s].x);
-    for (int s = 0; s < used; ++s) l += ml[s].y * (ml[s].x == -INFINITY ? 1.f : exp2f(ml[s].x - m));
-    for (int s = sub; s < used; s += per)
-      v += *reinterpret_cast<const f32x4*>(part + (int64_t)s * p.D) * (ml[s].x == -INFINITY ? 1.f : exp2f(ml[s].x - m));
-  }
-  if (per > 1) {
-    sums[group][piece] = v;
-    __syncthreads();
-    if (sub) return;
-    for (int g = 1; g < per; ++g) v += sums[group + g][piece];
-  }
-  if (in) store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v * inverse_sum(l));
-}
-
-template <bool BF16, int DP, int QG>
+template <bool BF16, int DP, int QG, int NW>
 hipError_t run(const CacheParams& p, hipStream_t st) {
-  using C = CacheCfg<BF16, DP, QG>;
+  using C = CacheCfg<BF16, DP, QG, NW>;
   const int64_t rtiles = ((int64_t)p.n * (p.Hq / p.Hk) + C::ROWS - 1) / C::ROWS;
   const int64_t blocks = rtiles * p.Hk * p.B * p.splits;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((cache_kernel<C>), dim3((unsigned)blocks), dim3(64 * C::NW), 0, st, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  constexpr int LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
-  int per = 1;
-  while (per < 256 / LPR && per < p.splits) per *= 2;
-  const int64_t total = (int64_t)p.B * p.n * p.Hq, rpb = 256 / LPR / per;
-  hipLaunchKernelGGL((cache_join_kernel<BF16, LPR>), dim3((unsigned)((total + rpb - 1) / rpb)), dim3(256), 0, st, p, per);
+  CacheParams q = p;
+  q.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (p.page == 1 << s && p.page >= C::RPI) q.page_shift = s;
+  hipLaunchKernelGGL((cache_kernel<C>), dim3((unsigned)blocks), dim3(64 * NW), 0, st, q);
   return hipGetLastError();
 }
 
@@ -397,28 +455,39 @@ int row_groups(int n, int Hq, int Hk, int D, bool bf16) {
 
 }  // namespace
 
-void plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, int page, int64_t capacity, int cus,
-                          int* splits, int* chunk) {
+CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, int page, int64_t capacity, int cus) {
+  CachePlan plan;
   const int64_t rows = (int64_t)n * (Hq / Hk), rt = 32 * row_groups(n, Hq, Hk, D, bf16);
-  const int64_t base = (int64_t)B * Hk * ((rows + rt - 1) / rt);
-  int64_t want = std::max<int64_t>(1, 16 * cus / base);
-  int64_t c = ((capacity + want - 1) / want + 127) / 128 * 128;
-  c = std::min(c, std::max<int64_t>(128, (int64_t)kPagesMost * page / 128 * 128));
-  *chunk = (int)std::min<int64_t>(c, 0x7fffff80);
-  *splits = (int)((capacity + *chunk - 1) / *chunk);
+  plan.rtiles = (int)((rows + rt - 1) / rt);
+  const int64_t base = (int64_t)B * Hk * plan.rtiles;
+  const int waves = D * (bf16 ? 2 : 4) <= 256 ? 4 : D * (bf16 ? 2 : 4) <= 512 ? 2 : 1;  // that a CU's LDS holds
+  // One wave a block, of chunks of `solo` keys, where those give every wave of
+  // the card one; else a block of all the waves a CU holds, of chunks that
+  // give every CU one.  A chunk's partial sums are written and read: `solo`
+  // keeps them to an eighth of the chunk's keys and values.
+  const int64_t solo = std::max<int64_t>(512, 16 * std::min(rows, rt));
+  plan.waves = base * ((capacity + solo - 1) / solo) >= (int64_t)waves * cus ? 1 : waves;
+  int64_t c = solo;
+  if (plan.waves > 1 || waves == 1) c = capacity * base / cus;
+  c = std::max<int64_t>(c, (capacity + kSplitsMost - 1) / kSplitsMost);
+  c = std::max<int64_t>(128, (c + 127) / 128 * 128);
+  c = std::min(c, (int64_t)kPagesMost * page / 128 * 128);
+  plan.chunk = (int)std::min<int64_t>(c, 0x7fffff80);
+  plan.splits = (int)((capacity + plan.chunk - 1) / plan.chunk);
+  return plan;
 }
 
-hipError_t launch_cache_attention(const CacheParams& p, bool bf16, hipStream_t st) {
+hipError_t launch_cache_attention(const CacheParams& p, bool bf16, int waves, hipStream_t st) {
   if (p.B <= 0 || p.n <= 0) return hipSuccess;
-  const bool two = row_groups(p.n, p.Hq, p.Hk, p.D, bf16) == 2;
+  const bool two = row_groups(p.n, p.Hq, p.Hk, p.D, bf16) == 2, one = waves == 1;
   if (bf16) {
-    if (p.D <= 64) return two ? run<true, 64, 2>(p, st) : run<true, 64, 1>(p, st);
-    if (p.D <= 128) return two ? run<true, 128, 2>(p, st) : run<true, 128, 1>(p, st);
-    return run<true, 256, 1>(p, st);
+    if (p.D <= 64) return two ? (one ? run<true, 64, 2, 1>(p, st) : run<true, 64, 2, 4>(p, st)) : (one ? run<true, 64, 1, 1>(p, st) : run<true, 64, 1, 4>(p, st));
+    if (p.D <= 128) return two ? (one ? run<true, 128, 2, 1>(p, st) : run<true, 128, 2, 4>(p, st)) : (one ? run<true, 128, 1, 1>(p, st) : run<true, 128, 1, 4>(p, st));
+    return one ? run<true, 256, 1, 1>(p, st) : run<true, 256, 1, 2>(p, st);
   }
-  if (p.D <= 64) return two ? run<false, 64, 2>(p, st) : run<false, 64, 1>(p, st);
-  if (p.D <= 128) return run<false, 128, 1>(p, st);
-  return run<false, 256, 1>(p, st);
+  if (p.D <= 64) return two ? (one ? run<false, 64, 2, 1>(p, st) : run<false, 64, 2, 4>(p, st)) : (one ? run<false, 64, 1, 1>(p, st) : run<false, 64, 1, 4>(p, st));
+  if (p.D <= 128) return one ? run<false, 128, 1, 1>(p, st) : run<false, 128, 1, 2>(p, st);
+  return run<false, 256, 1, 1>(p, st);
 }
 
 }  // namespace svdmlp

@@ -64,21 +64,27 @@ struct CacheParams {
   const int* lengths;     // (B) tokens held, the n new ones among them
   const uint8_t* tree;    // (B, n, n) or (n, n) (tree_b = 0) bytes, or null: a chain
   void* out;              // (B, n, Hq, D)
-  float* part;            // split partials (cache_attention.hip), or null with splits == 1
+  float* part;            // split partials, or null with splits == 1
+  int* counters;          // one a (sequence, key/value head, row tile), zero before and after; null with splits == 1
   int64_t q_b, q_t, q_h, k_p, k_t, k_h, v_p, v_t, v_h, o_b, o_t, o_h, table_b, tree_b, tree_q;
   int64_t pages;
   int page, width, B, n, Hq, Hk, D;
+  int page_shift;     // log2 of a page that is a power of two and holds whole loads, else -1 (set by the launcher)
   int splits, chunk;  // keys are cut into chunks of `chunk` (a multiple of the key tile), one a block
   float c;
 };
-// Splits of a call: how many chunks of how many keys cover the table's
-// `capacity` keys.
-void plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, int page, int64_t capacity, int cus,
-                          int* splits, int* chunk);
-// Floats of one (sequence, split, query, head) partial: D sums, the maximum and the sum of weights.
+// How a call is cut: `splits` chunks of `chunk` keys cover the table's
+// `capacity`, a block of `waves` waves each; rtiles row tiles a sequence and head.
+constexpr int64_t kCachePagesMost = 65536;  // pages of a sequence: 64 chunks of 1024
+struct CachePlan {
+  int splits, chunk, waves, rtiles;
+};
+CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, int page, int64_t capacity, int cus);
+// Floats of the partial sums: D sums, the maximum and the sum of weights of
+// every (sequence, token, head, split).
 inline int64_t cache_part_floats(int B, int n, int Hq, int D, int splits) {
   return splits > 1 ? (int64_t)B * n * Hq * splits * (D + 2) : 0;
 }
-hipError_t launch_cache_attention(const CacheParams& p, bool bf16, hipStream_t st);
+hipError_t launch_cache_attention(const CacheParams& p, bool bf16, int waves, hipStream_t st);
 
 }  // namespace svdmlp

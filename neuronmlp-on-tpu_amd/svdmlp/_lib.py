@@ -118,9 +118,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.svdmlp_prompt_attention.restype = ctypes.c_int
     lib.svdmlp_prompt_attention.argtypes = [_vp] * 6 + [_i64] * 5 + [f32, _i32, _u32, _vp]
     lib.svdmlp_cache_attention_workspace_bytes.restype = _sz
-    lib.svdmlp_cache_attention_workspace_bytes.argtypes = [_i64] * 7 + [_i32]
+    lib.svdmlp_cache_attention_workspace_bytes.argtypes = [_i64] * 7 + [_i32, ctypes.POINTER(_i64)]
     lib.svdmlp_cache_attention.restype = ctypes.c_int
-    lib.svdmlp_cache_attention.argtypes = [_vp] * 8 + [_i64] * 8 + [f32, _i32, _vp, _sz, _vp]
+    lib.svdmlp_cache_attention.argtypes = [_vp] * 8 + [_i64] * 8 + [f32, _i32, _vp, _sz, _vp, _i64, _vp]
     lib.svdmlp_residual_norm.restype = ctypes.c_int
     lib.svdmlp_residual_norm.argtypes = [_vp] * 8 + [_i64] * 2 + [f32, f32, _i32, _vp]
     lib.svdmlp_profile_enable.restype = ctypes.c_int

@@ -450,32 +450,49 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
     lib = _lib.load()
     st = _Strides15(*q.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3], *out.stride()[:3], block_table.stride(0),
                     tree_b, tree_q)
-    # the partial sums of long contexts: of the call alone, from torch's
-    # allocator (of a graph's own pool under capture)
     code = _ACT_CODES[dtype]
-    nbytes, ws = _part_bytes(lib, index, B, n, page, width, Hq, Hk, D, code), None
-    if nbytes:
+    ws, ws_ptr, counters_ptr = None, None, None
+    nbytes, counters = _partials(lib, index, B, n, page, width, Hq, Hk, D, code)
+    if nbytes:  # the partial sums of long contexts: of the call alone, from torch's allocator
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws_ptr, counters_ptr = ws.data_ptr(), _counters(index, counters).data_ptr()
     _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
             lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
-            None if ws is None else ws.data_ptr(), nbytes)
+            ws_ptr, nbytes, counters_ptr, counters)
     return out
 
 
-_PART_BYTES: dict = {}
+_PARTIALS: dict = {}
 
 
-def _part_bytes(lib, index, *sizes) -> int:
-    """svdmlp_cache_attention_workspace_bytes of the sizes on device `index` (it depends on the sizes and its CUs alone)."""
+def _partials(lib, index, *sizes) -> tuple[int, int]:
+    """Workspace bytes and counters of a call's sizes on device `index` (they depend on the sizes and its CUs alone)."""
     key = (index, *sizes)
-    n = _PART_BYTES.get(key)
-    if n is None:
+    plan = _PARTIALS.get(key)
+    if plan is None:
+        counters = ctypes.c_int64(0)
         with torch.cuda.device(index):
-            n = int(lib.svdmlp_cache_attention_workspace_bytes(*sizes))
-        if len(_PART_BYTES) > 4096:
-            _PART_BYTES.clear()
-        _PART_BYTES[key] = n
-    return n
+            nbytes = int(lib.svdmlp_cache_attention_workspace_bytes(*sizes, ctypes.byref(counters)))
+        if len(_PARTIALS) > 4096:
+            _PARTIALS.clear()
+        plan = _PARTIALS[key] = (nbytes, counters.value)
+    return plan
+
+
+# The counters of cache_attention, one tensor of zeros a (device, stream): every
+# call leaves them zero for the next on its stream.  A captured call gets its
+# own, cleared by the graph.
+_COUNTERS: dict = {}
+
+
+def _counters(index: int, n: int) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(n, dtype=torch.int32, device=f"cuda:{index}")
+    key = (index, _raw_stream(index))
+    held = _COUNTERS.get(key)
+    if held is None or held.numel() < n:
+        held = _COUNTERS[key] = torch.zeros(max(n, 4096), dtype=torch.int32, device=f"cuda:{index}")
+    return held
 
 
 # ---------------------------------------------------------------------------

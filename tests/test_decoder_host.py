@@ -61,16 +61,17 @@ def test_prompt_attention_refusals(lib, kw, msg):
     assert msg in lib.svdmlp_last_error()
 
 
-def _cache(lib, B=2, n=1, pages=4, page=16, width=2, Hq=4, Hk=2, D=16, scale=0.25, dtype=1, table=P, ws=None, nbytes=0):
-    return lib.svdmlp_cache_attention(P, P, P, table, P, None, P, None, B, n, pages, page, width, Hq, Hk, D, scale, dtype, ws, nbytes, None)
+def _cache(lib, B=2, n=1, pages=4, page=16, width=2, Hq=4, Hk=2, D=16, scale=0.25, dtype=1, table=P, ws=None, nbytes=0, counters=None, n_counters=0):
+    return lib.svdmlp_cache_attention(P, P, P, table, P, None, P, None, B, n, pages, page, width, Hq, Hk, D, scale, dtype, ws, nbytes, counters, n_counters, None)
 
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(B=0), b"positive"), (dict(n=0), b"positive"), (dict(n=65), b"at most 64"), (dict(width=0), b"positive"),
-    (dict(page=1 << 20, width=1 << 20), b"2^31"), (dict(pages=0), b"positive"), (dict(D=320), b"head size"),
+    (dict(page=1 << 20, width=1 << 20), b"2^31"), (dict(pages=0), b"positive"), (dict(page=1, width=65537), b"at most 65536"), (dict(D=320), b"head size"),
     (dict(table=None), b"null"), (dict(scale=-1.0), b"scale"), (dict(B=1 << 40), b"too many"),
     (dict(width=4096), b"workspace too small"),  # a long context's partial sums need one
     (dict(width=4096, ws=ctypes.c_void_p(264), nbytes=1 << 30), b"workspace too small"),
+    (dict(width=4096, ws=P, nbytes=1 << 30), b"counters needed"), (dict(width=4096, ws=P, nbytes=1 << 30, counters=P, n_counters=3), b"counters needed"),
 ])
 def test_cache_attention_refusals(lib, kw, msg):
     assert _cache(lib, **kw) == BAD
@@ -78,11 +79,17 @@ def test_cache_attention_refusals(lib, kw, msg):
 
 
 def test_cache_attention_workspace(lib):
-    f = lib.svdmlp_cache_attention_workspace_bytes
-    assert f(1, 1, 16, 0, 32, 8, 128, 1) == 0
-    assert f(1, 1, 16, 10, 32, 7, 128, 1) == 0
-    assert f(1, 1, 16, 1, 32, 8, 128, 1) == 0        # one chunk: no partial sums
-    assert f(1, 1, 16, 1 << 13, 32, 8, 128, 1) > 0
+    counters = ctypes.c_int64(-1)
+
+    def f(*sizes):
+        return lib.svdmlp_cache_attention_workspace_bytes(*sizes, 1, ctypes.byref(counters))
+
+    assert f(1, 1, 16, 0, 32, 8, 128) == 0 and counters.value == 0
+    assert f(1, 1, 16, 10, 32, 7, 128) == 0 and counters.value == 0
+    assert f(1, 1, 16, 1, 32, 8, 128) == 0 and counters.value == 0  # one chunk: no partial sums
+    assert f(1, 1, 16, 1 << 13, 32, 8, 128) > 0 and counters.value == 8
+    assert f(3, 16, 16, 1 << 13, 64, 8, 128) > 0 and counters.value == 3 * 8 * 2  # 128 rows a head: two tiles
+    assert lib.svdmlp_cache_attention_workspace_bytes(1, 1, 16, 1 << 13, 32, 8, 128, 1, None) > 0
 
 
 def test_residual_norm_refusals(lib):

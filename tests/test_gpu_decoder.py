@@ -430,6 +430,29 @@ def test_cache_attention(gpu, dtype, lens, n, H, K, D, page, tree):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("dtype,B,n,H,K,D,page,most", [
+    (BF, 40, 1, 8, 2, 64, 16, 4000), (BF, 70, 1, 16, 8, 128, 16, 1500), (BF, 24, 9, 32, 8, 128, 32, 2500), (BF, 33, 3, 8, 8, 256, 64, 900),
+    (F32, 64, 1, 8, 4, 64, 16, 2100), (F32, 40, 4, 8, 8, 128, 3, 700), (BF, 90, 20, 8, 4, 64, 128, 1800), (F32, 9, 2, 8, 8, 256, 16, 3000),
+    (BF, 1, 1, 8, 1, 128, 1, 60000), (BF, 2, 17, 8, 8, 96, 8, 20000)])
+def test_cache_attention_many_keys(gpu, dtype, B, n, H, K, D, page, most):
+    """Long caches and many sequences: chunks of every kind, joined by the last block; the counters end where they began."""
+    g = _gen(B + most)
+    lens = [most, 0, n - 1, n][:B] + [int(x) for x in torch.randint(1, most, (max(B - 4, 0),), generator=g)]
+    table, pages = _pages(g, lens, page)
+    q = _randn(g, B, n, H, D, dtype=dtype)
+    kc, vc = _randn(g, pages, page, K, D, dtype=dtype), _randn(g, pages, page, K, D, dtype=dtype)
+    tree = _random_tree(g, B, n) if n > 1 else None
+    some = sorted({0, 1 % B, 2 % B, 3 % B, B - 1, B // 2})
+    out, tol = _cache_ref(q[some], kc, vc, table[some], [lens[b] for b in some], None if tree is None else tree[some], 1 / math.sqrt(D))
+    args = [t.to(gpu) for t in (q, kc, vc, table)]
+    ln, tg = torch.tensor(lens, device=gpu), None if tree is None else tree.to(gpu)
+    got = svdmlp.cache_attention(*args, ln, tree=tg)
+    _close(got[some], out, tol)
+    for _ in range(3):
+        assert torch.equal(got, svdmlp.cache_attention(*args, ln, tree=tg))
+    assert all(int(c.abs().max()) == 0 for c in decoder._COUNTERS.values())
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_cache_attention_hidden_drafts_have_no_part(gpu, dtype):
     """Infinities and NaN in a draft reach its descendants alone; a token whose row of the tree is empty sees the context, or nothing."""
