@@ -2704,6 +2704,7 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   const CachePlan plan = plan_cache_attention(p.B, p.n, p.Hq, p.Hk, p.D, dtype == SVDMLP_BF16, p.page, page * width, device_cus());
   p.splits = plan.splits, p.chunk = plan.chunk;
   const size_t need = (size_t)cache_part_floats(p.B, p.n, p.Hq, p.D, p.splits) * 4;
+  if ((int64_t)n * Hq * plan.splits * D * 4 > 0x7fffffff) return fail("cache_attention: too many rows");
   if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15u)))
     return fail("cache_attention: workspace too small: %zu bytes needed, 16-byte aligned, got %zu", need, ws_bytes);
   const int64_t nc = B * Hk * plan.rtiles;

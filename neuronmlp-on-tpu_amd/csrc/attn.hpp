@@ -158,6 +158,13 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+typedef __bf16 bf16x2_dot __attribute__((ext_vector_type(2)));
+
+// acc + both bf16 values of w.
+__device__ __forceinline__ float add_pair(uint32_t w, float acc) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_dot, w), __builtin_bit_cast(bf16x2_dot, 0x3f803f80u), acc, false);
+}
+
 // 1 / l; a row without keys gives zeros, NaN stays.
 __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
 

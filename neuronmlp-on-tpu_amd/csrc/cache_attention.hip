@@ -54,14 +54,15 @@ __device__ __forceinline__ int64_t lane64(int64_t v, int j) {
                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), j) << 32);
 }
 
-// Partial sums cross blocks, and so XCDs with an L2 each, by device-scope
-// accesses (past the L2), without any cache maintenance: fences that write back
-// and drop the L2 for every block made a call of 4096 blocks twice as long.
-__device__ __forceinline__ void store_device(float* p, f32x2 v) {
-  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x2 load_device(const float* p) {
-  return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<uint64_t*>(const_cast<float*>(p)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+// Partial sums cross blocks, and so XCDs with an L2 each, by device-scope (sc1)
+// accesses past the L2, without any cache maintenance: fences that write back
+// and drop the L2 for every block made a call of 4096 blocks 325 us instead of
+// 137.  Offsets are in bytes from a sequence's part.
+constexpr int kDevice = 16;  // the sc1 bit of a buffer access
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_of(const CacheParams& p, int b, int floats) {
+  const int64_t rows = (int64_t)p.n * p.Hq * p.splits;
+  float* const base = p.part + (floats == 2 ? (int64_t)p.B * rows * p.D : 0) + (int64_t)b * rows * floats;
+  return __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)(rows * floats * 4), 0x00020000);
 }
 
 __device__ __forceinline__ int held(const CacheParams& p, int b) {
@@ -212,50 +213,53 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   if (p.D < C::DP)  // pieces behind the head's end: never loaded, zeros
     for (int i = lane; i < 2 * C::STAGE / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
 
-  int ku = kbeg + 32 * wave;
-  attn_lds cur = mine, nxt = mine + C::STAGE;
-  if (ku < kend) issue(ku, cur);
-  for (; ku < kend; ku += 32 * NW) {
-    if (ku + 32 * NW < kend) {
-      issue(ku + 32 * NW, nxt);
-      wait_loads<(2 * C::LOADS < 63 ? 2 * C::LOADS : 63)>();
-    } else {
-      wait_loads<0>();
-    }
-    const attn_lds lk = cur, lv = cur + C::TILE;
-    const bool masked = ku + 31 >= context;
-    int in;
-    const uint32_t there = (uint32_t)__ballot(place(ku, col, &in) >= 0);  // keys that lie in a page of the cache
+  // One tile: S = K Q^T, the weights, O += V^T P^T.  Pieces are read from LDS
+  // kAhead products before they are needed, the first of V behind the weights
+  // (a read takes as long as two products, and one wave a SIMD hides nothing).
+  constexpr int kAhead = RB < 1024 ? 4 : 2, VF = BF16 ? 2 * DB : 16 * DB;  // VF: pieces of V
+  static_assert(C::STEPS >= kAhead && VF >= kAhead, "pieces");
+  auto unit = [&](auto masked_, attn_lds stage, int ku, uint32_t there) {
+    constexpr bool masked = decltype(masked_)::value;
+    const attn_lds lk = stage, lv = stage + C::TILE;
+    u32x4 kf[kAhead], vf[kAhead];
+    auto read_value = [&](int f) {
+      if constexpr (BF16) vf[f % kAhead] = at.values(lv, f / DB, f % DB);
+      else vf[f % kAhead].x = at.value(lv, f / DB, f % DB);
+    };
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) kf[t] = at.key(lk, t);
     f32x16 s[QG];
 #pragma unroll
-    for (int g = 0; g < QG; ++g)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[g][i] = 0.f;
+    for (int g = 0; g < QG; ++g) s[g] = f32x16{};
 #pragma unroll
     for (int t = 0; t < C::STEPS; ++t) {
-      const u32x4 kf = at.key(lk, t);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < QG; ++g) {
         if constexpr (!QREG) {
           const int c = 2 * t + half;
           qf[g][0] = c < npieces ? *reinterpret_cast<const u32x4*>(qptr[g] + 16 * c) : u32x4{0u, 0u, 0u, 0u};
         }
-        s[g] = attn_mfma<BF16>(kf, qf[g][QREG ? t : 0], s[g]);
+        s[g] = attn_mfma<BF16>(kf[t % kAhead], qf[g][QREG ? t : 0], s[g]);
       }
+      if (t + kAhead < C::STEPS) kf[t % kAhead] = at.key(lk, t + kAhead);
+      else read_value(t + kAhead - C::STEPS);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 pb[QG][2];
 #pragma unroll
     for (int g = 0; g < QG; ++g) {
-      if (masked || there != 0xffffffffu) {
+      if constexpr (masked) {
         const uint32_t see = (there & seen32(row_sees[g], ku - context)) >> (4 * half);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[g][i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[g][i] : -INFINITY;
       }
-      float mx = s[g][0];
+      float mx = fmaxf(s[g][0], s[g][1]);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[g][i]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32)) * p.c;
+      for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[g][i]), s[g][i + 1]);
+      mx *= p.c;
       if (__any(mx > st[g].m + kSlack)) {
-        const float m = fmaxf(st[g].m, mx);
+        const float m = fmaxf(st[g].m, fmaxf(mx, __shfl_xor(mx, 32)));
         const float a = m == -INFINITY ? 1.f : exp2f(st[g].m - m);
         st[g].m = m;
         st[g].l *= a;
@@ -266,41 +270,51 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
       }
       const float m = st[g].m == -INFINITY ? 0.f : st[g].m;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], p.c, -m));
-        st[g].l += s[g][i];
+      for (int i = 0; i < 16; ++i) s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], p.c, -m));
+      if constexpr (BF16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          pb[g][i / 4][i % 4] = pack_bf16x2(s[g][2 * i], s[g][2 * i + 1]);
+          st[g].l = add_pair(pb[g][i / 4][i % 4], st[g].l);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[g].l += s[g][i];
       }
     }
-    if constexpr (BF16) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        u32x4 pb[QG];
+    for (int f = 0; f < VF; ++f) {
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 v = vf[f % kAhead];
+      if constexpr (masked) {
 #pragma unroll
-        for (int g = 0; g < QG; ++g)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) pb[g][w] = pack_bf16x2(s[g][8 * t + 2 * w], s[g][8 * t + 2 * w + 1]);
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          u32x4 vf = at.values(lv, t, d);
-          if (masked)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) vf[w] = scrub<true>(vf[w], bad);
-#pragma unroll
-          for (int g = 0; g < QG; ++g) o[g][d] = attn_mfma<true>(vf, pb[g], o[g][d]);
-        }
+        for (int w = 0; w < (BF16 ? 4 : 1); ++w) v[w] = scrub<BF16>(v[w], bad);
       }
+#pragma unroll
+      for (int g = 0; g < QG; ++g) {
+        if constexpr (BF16) o[g][f % DB] = attn_mfma<true>(v, pb[g][f / DB], o[g][f % DB]);
+        else o[g][f % DB] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v.x), s[g][f / DB], o[g][f % DB], 0, 0, 0);
+      }
+      if (f + kAhead < VF) read_value(f + kAhead);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  int ku = kbeg + 32 * wave;
+  attn_lds cur = mine, nxt = mine + C::STAGE;
+  if (ku < kend) issue(ku, cur);
+  for (; ku < kend; ku += 32 * NW) {
+    if (ku + 32 * NW < kend) {
+      issue(ku + 32 * NW, nxt);
+      wait_loads<(2 * C::LOADS < 63 ? 2 * C::LOADS : 63)>();
     } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          uint32_t w = at.value(lv, i, d);
-          if (masked) w = scrub<false>(w, bad);
-#pragma unroll
-          for (int g = 0; g < QG; ++g)
-            o[g][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w), s[g][i], o[g][d], 0, 0, 0);
-        }
+      wait_loads<0>();
     }
+    const bool masked = ku + 31 >= context;
+    int in;
+    const uint32_t there = (uint32_t)__ballot(place(ku, col, &in) >= 0);  // keys that lie in a page of the cache
+    if (masked || there != 0xffffffffu) unit(std::true_type{}, cur, ku, there);
+    else unit(std::false_type{}, cur, ku, there);
     const attn_lds swap = cur;
     cur = nxt;
     nxt = swap;
@@ -361,7 +375,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     }
   }
   __syncthreads();
-  const int64_t total = (int64_t)p.B * p.n * p.Hq;
+  const __amdgpu_buffer_rsrc_t sums = part_of(p, b, p.D), ml = part_of(p, b, 2);
   for (int i = threadIdx.x; i < C::ROWS * OP; i += 64 * NW) {
     const int rr = i / OP, piece = i % OP, r = rt * C::ROWS + rr;
     if (r >= rows || 4 * piece >= p.D) continue;
@@ -380,10 +394,9 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
       v *= inverse_sum(l);
       store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
     } else {
-      const int64_t row = (((int64_t)b * p.n + t) * p.Hq + h) * p.splits + split;
-      store_device(p.part + row * p.D + 4 * piece, f32x2{v.x, v.y});
-      store_device(p.part + row * p.D + 4 * piece + 2, f32x2{v.z, v.w});
-      if (piece == 0) store_device(p.part + total * p.splits * p.D + 2 * row, f32x2{m, l});
+      const int row = (t * p.Hq + h) * p.splits + split;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), sums, (row * p.D + 4 * piece) * 4, 0, kDevice);
+      if (piece == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, ml, row * 8, 0, kDevice);
     }
   }
   if (used == 1) return;
@@ -402,14 +415,14 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   if (stats[0][0][0] == 0.f) return;
   SVDMLP_ATTN_LDS float* const weight = (SVDMLP_ATTN_LDS float*)(attn_lds)lds;  // [row][kSplitsMost]
   const int nrows = min(C::ROWS, rows - rt * C::ROWS);
-  const float* const ml = p.part + total * p.splits * p.D;
-  auto part_row = [&](int rr) -> int64_t {
+  auto part_row = [&](int rr) -> int {
     const int r = rt * C::ROWS + rr, t = r / G;
-    return (((int64_t)b * p.n + t) * p.Hq + hk * G + r - t * G) * p.splits;
+    return (t * p.Hq + hk * G + r - t * G) * p.splits;
   };
   // A wave takes a row: its lanes the chunks' maxima and sums.
   for (int rr = wave; rr < nrows; rr += NW) {
-    const f32x2 v = lane < used ? load_device(ml + 2 * (part_row(rr) + lane)) : f32x2{-INFINITY, 0.f};
+    f32x2 v = {-INFINITY, 0.f};
+    if (lane < used) v = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, (part_row(rr) + lane) * 8, 0, kDevice));
     float m = v.x;
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const float a = v.x == -INFINITY ? 1.f : exp2f(v.x - m);
@@ -421,14 +434,11 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   const int dp = p.D / 4;
   for (int i = threadIdx.x; i < nrows * dp; i += 64 * NW) {
     const int rr = i / dp, piece = i - rr * dp;
-    const int64_t row = part_row(rr);
-    const float* const part = p.part + row * p.D + 4 * piece;
+    const int at0 = (part_row(rr) * p.D + 4 * piece) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int s = 0; s < used; ++s) {
-      const f32x2 a = load_device(part + (int64_t)s * p.D), c = load_device(part + (int64_t)s * p.D + 2);
-      v += f32x4{a.x, a.y, c.x, c.y} * weight[rr * kSplitsMost + s];
-    }
+    for (int s = 0; s < used; ++s)
+      v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sums, at0 + s * p.D * 4, 0, kDevice)) * weight[rr * kSplitsMost + s];
     const int r = rt * C::ROWS + rr, t = r / G, h = hk * G + r - t * G;
     store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
   }
@@ -461,14 +471,15 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   plan.rtiles = (int)((rows + rt - 1) / rt);
   const int64_t base = (int64_t)B * Hk * plan.rtiles;
   const int waves = D * (bf16 ? 2 : 4) <= 256 ? 4 : D * (bf16 ? 2 : 4) <= 512 ? 2 : 1;  // that a CU's LDS holds
-  // One wave a block, of chunks of `solo` keys, where those give every wave of
-  // the card one; else a block of all the waves a CU holds, of chunks that
-  // give every CU one.  A chunk's partial sums are written and read: `solo`
-  // keeps them to an eighth of the chunk's keys and values.
-  const int64_t solo = std::max<int64_t>(512, 16 * std::min(rows, rt));
-  plan.waves = base * ((capacity + solo - 1) / solo) >= (int64_t)waves * cus ? 1 : waves;
-  int64_t c = solo;
-  if (plan.waves > 1 || waves == 1) c = capacity * base / cus;
+  // One wave a block, of chunks of 512 keys, where those give every wave of the
+  // card one.  Else, and where a wave has 64 rows (whose partial sums, written
+  // and read, would be an eighth of such a chunk's keys and values), a block of
+  // all the waves a CU holds, of chunks that give every CU one; or three, of
+  // different lengths, if the chunks stay long.
+  constexpr int64_t kSolo = 512;
+  plan.waves = rt == 32 && base * ((capacity + kSolo - 1) / kSolo) >= (int64_t)waves * cus ? 1 : waves;
+  int64_t c = kSolo;
+  if (plan.waves > 1 || waves == 1) c = std::max(capacity * base / cus / 3, std::min<int64_t>(1024, capacity * base / cus));
   c = std::max<int64_t>(c, (capacity + kSplitsMost - 1) / kSplitsMost);
   c = std::max<int64_t>(128, (c + 127) / 128 * 128);
   c = std::min(c, (int64_t)kPagesMost * page / 128 * 128);

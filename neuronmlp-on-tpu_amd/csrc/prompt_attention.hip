@@ -306,13 +306,6 @@ __device__ __forceinline__ float lane_max(const f32x16& s) {
   return m;
 }
 
-typedef __bf16 bf16x2_dot __attribute__((ext_vector_type(2)));
-
-// acc + both bf16 values of w.
-__device__ __forceinline__ float add_pair(uint32_t w, float acc) {
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_dot, w), __builtin_bit_cast(bf16x2_dot, 0x3f803f80u), acc, false);
-}
-
 template <class C>
 __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   constexpr int RB = C::RB, QG = C::QG, KB = C::KB, DB = C::DP / 32;

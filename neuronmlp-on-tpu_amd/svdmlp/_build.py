@@ -50,10 +50,10 @@ HIPCC_FLAGS = [
     f"-I{CSRC}",
 ]
 
-# Flags of single translation units.  prompt_attention: results of MFMAs in
-# vector registers where they fit (by itself the compiler puts them all into
+# Flags of single translation units.  Attention: results of MFMAs in vector
+# registers where they fit (by itself the compiler puts them all into
 # accumulation registers, from which the softmax would copy every score).
-UNIT_FLAGS = {"prompt_attention": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+UNIT_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("prompt_attention", "cache_attention")}
 
 
 def _hipcc() -> str:
