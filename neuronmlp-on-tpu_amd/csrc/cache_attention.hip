@@ -25,6 +25,7 @@ namespace svdmlp {
 namespace {
 
 constexpr int kSplitsMost = 64;   // chunks of a sequence
+constexpr int kJoin = 16;         // chunks' sums in flight when they are joined
 constexpr int kPagesMost = 1024;  // whole pages of a chunk: their numbers lie in LDS
 
 template <bool BF16_, int DP_, int QG_, int NW_>
@@ -174,26 +175,40 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   // piece lane % PIECES, both swizzled; load j adds a constant (the swizzles
   // pick bits of the row, so that they combine by exclusive or).
   const int lrow = lane / C::PIECES, lc = lane % C::PIECES;
-  const int kpiece = lc ^ k_swz<RB>(lrow), vpiece = lc ^ v_swz<RB, BF16>(lrow);
+  const int kpiece0 = lc ^ k_swz<RB>(lrow), vpiece0 = lc ^ v_swz<RB, BF16>(lrow);
   const uint32_t krow = (uint32_t)(lrow * (int)p.k_t * ES), vrow = (uint32_t)(lrow * (int)p.v_t * ES);
-  auto issue = [&](int ku, attn_lds stage) {
+  const bool alike = p.page_shift >= 0 && p.k_p == p.v_p && p.k_t == p.v_t;
+  // Loads of the tile at key ku; true: all 32 keys are there.
+  auto issue = [&](int ku, attn_lds stage) -> bool {
     const uint32_t base = (uint32_t)(uintptr_t)stage;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
-    if (p.page_shift >= 0 && ku + 32 <= kend) {
-      // Pages of a power of two that hold whole loads: lane j finds load j's
-      // page, and its address goes to all lanes through scalar registers.
+    int kpiece = kpiece0, vpiece = vpiece0;
+    // where registers are short, the loads' offsets are computed each time
+    if constexpr (QG == 2 || RB >= 512) asm volatile("" : "+v"(kpiece), "+v"(vpiece));
+    if (alike && ku + 32 <= kend) {
+      // Pages of a power of two that hold whole loads, both caches laid out
+      // alike: lane j finds load j's page, and the place of its rows goes to
+      // all lanes through scalar registers.
       const int key = ku + lane % C::LOADS * C::RPI, pg = ids[(key >> p.page_shift) - pg0], in = key & (p.page - 1);
       if (__all(pg >= 0 && pg < p.pages)) {
-        const int64_t ko = ((int64_t)pg * p.k_p + (int64_t)in * p.k_t) * ES, vo = ((int64_t)pg * p.v_p + (int64_t)in * p.v_t) * ES;
+        const int64_t off = ((int64_t)pg * p.k_p + (int64_t)in * p.k_t) * ES;
+        if (p.D == C::DP) {
 #pragma unroll
-        for (int j = 0; j < C::LOADS; ++j) {
-          const int ck = kpiece ^ k_swz<RB>(j * C::RPI), cv = vpiece ^ v_swz<RB, BF16>(j * C::RPI);
-          const char* const kp = kb + lane64(ko, j);
-          const char* const vp = vb + lane64(vo, j);
-          if (ck < npieces) load_lds16(kp, krow + 16 * ck, base + j * 1024);
-          if (cv < npieces) load_lds16(vp, vrow + 16 * cv, base + C::TILE + j * 1024);
+          for (int j = 0; j < C::LOADS; ++j) {
+            const int64_t at = lane64(off, j);
+            load_lds16(kb + at, krow + 16 * (kpiece ^ k_swz<RB>(j * C::RPI)), base + j * 1024);
+            load_lds16(vb + at, vrow + 16 * (vpiece ^ v_swz<RB, BF16>(j * C::RPI)), base + C::TILE + j * 1024);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < C::LOADS; ++j) {
+            const int ck = kpiece ^ k_swz<RB>(j * C::RPI), cv = vpiece ^ v_swz<RB, BF16>(j * C::RPI);
+            const int64_t at = lane64(off, j);
+            if (ck < npieces) load_lds16(kb + at, krow + 16 * ck, base + j * 1024);
+            if (cv < npieces) load_lds16(vb + at, vrow + 16 * cv, base + C::TILE + j * 1024);
+          }
         }
-        return;
+        return true;
       }
     }
 #pragma unroll 2
@@ -209,6 +224,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
       if (ck < npieces) load_lds16(kp, base + j * 1024);
       if (cv < npieces) load_lds16(vp, base + C::TILE + j * 1024);
     }
+    return false;
   };
   if (p.D < C::DP)  // pieces behind the head's end: never loaded, zeros
     for (int i = lane; i < 2 * C::STAGE / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
@@ -302,19 +318,24 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
 
   int ku = kbeg + 32 * wave;
   attn_lds cur = mine, nxt = mine + C::STAGE;
-  if (ku < kend) issue(ku, cur);
+  bool whole = false;
+  if (ku < kend) whole = issue(ku, cur);
   for (; ku < kend; ku += 32 * NW) {
+    bool next_whole = false;
     if (ku + 32 * NW < kend) {
-      issue(ku + 32 * NW, nxt);
+      next_whole = issue(ku + 32 * NW, nxt);
       wait_loads<(2 * C::LOADS < 63 ? 2 * C::LOADS : 63)>();
     } else {
       wait_loads<0>();
     }
-    const bool masked = ku + 31 >= context;
     int in;
-    const uint32_t there = (uint32_t)__ballot(place(ku, col, &in) >= 0);  // keys that lie in a page of the cache
-    if (masked || there != 0xffffffffu) unit(std::true_type{}, cur, ku, there);
-    else unit(std::false_type{}, cur, ku, there);
+    if constexpr (RB < 1024) {
+      if (whole && ku + 31 < context) unit(std::false_type{}, cur, ku, 0xffffffffu);
+      else unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
+    } else {  // one copy of the code: two do not fit the registers
+      unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
+    }
+    whole = next_whole;
     const attn_lds swap = cur;
     cur = nxt;
     nxt = swap;
@@ -428,7 +449,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     const float a = v.x == -INFINITY ? 1.f : exp2f(v.x - m);
     float l = v.y * a;
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-    weight[rr * kSplitsMost + lane] = a * inverse_sum(l);
+    weight[rr * kSplitsMost + lane] = lane < used ? a * inverse_sum(l) : 0.f;
   }
   __syncthreads();
   const int dp = p.D / 4;
@@ -436,9 +457,14 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     const int rr = i / dp, piece = i - rr * dp;
     const int at0 = (part_row(rr) * p.D + 4 * piece) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s < used; ++s)
-      v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sums, at0 + s * p.D * 4, 0, kDevice)) * weight[rr * kSplitsMost + s];
+    for (int s0 = 0; s0 < used; s0 += kJoin) {  // kJoin loads in flight; behind the last chunk zeros
+      u32x4 x[kJoin];
+#pragma unroll
+      for (int s = 0; s < kJoin; ++s)
+        x[s] = __builtin_amdgcn_raw_buffer_load_b128(sums, s0 + s < used ? (uint32_t)(at0 + (s0 + s) * p.D * 4) : 0x80000000u, 0, kDevice);
+#pragma unroll
+      for (int s = 0; s < kJoin; ++s) v += __builtin_bit_cast(f32x4, x[s]) * weight[rr * kSplitsMost + min(s0 + s, kSplitsMost - 1)];
+    }
     const int r = rt * C::ROWS + rr, t = r / G, h = hk * G + r - t * G;
     store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
   }
@@ -492,11 +518,11 @@ hipError_t launch_cache_attention(const CacheParams& p, bool bf16, int waves, hi
   if (p.B <= 0 || p.n <= 0) return hipSuccess;
   const bool two = row_groups(p.n, p.Hq, p.Hk, p.D, bf16) == 2, one = waves == 1;
   if (bf16) {
-    if (p.D <= 64) return two ? (one ? run<true, 64, 2, 1>(p, st) : run<true, 64, 2, 4>(p, st)) : (one ? run<true, 64, 1, 1>(p, st) : run<true, 64, 1, 4>(p, st));
-    if (p.D <= 128) return two ? (one ? run<true, 128, 2, 1>(p, st) : run<true, 128, 2, 4>(p, st)) : (one ? run<true, 128, 1, 1>(p, st) : run<true, 128, 1, 4>(p, st));
+    if (p.D <= 64) return two ? run<true, 64, 2, 4>(p, st) : (one ? run<true, 64, 1, 1>(p, st) : run<true, 64, 1, 4>(p, st));
+    if (p.D <= 128) return two ? run<true, 128, 2, 4>(p, st) : (one ? run<true, 128, 1, 1>(p, st) : run<true, 128, 1, 4>(p, st));
     return one ? run<true, 256, 1, 1>(p, st) : run<true, 256, 1, 2>(p, st);
   }
-  if (p.D <= 64) return two ? (one ? run<false, 64, 2, 1>(p, st) : run<false, 64, 2, 4>(p, st)) : (one ? run<false, 64, 1, 1>(p, st) : run<false, 64, 1, 4>(p, st));
+  if (p.D <= 64) return two ? run<false, 64, 2, 4>(p, st) : (one ? run<false, 64, 1, 1>(p, st) : run<false, 64, 1, 4>(p, st));
   if (p.D <= 128) return one ? run<false, 128, 1, 1>(p, st) : run<false, 128, 1, 2>(p, st);
   return run<false, 256, 1, 1>(p, st);
 }
