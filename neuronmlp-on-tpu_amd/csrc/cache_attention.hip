@@ -43,7 +43,6 @@ struct CacheCfg {
   static constexpr int RPI = 64 / PIECES;        // rows a load
   static constexpr int LOADS = 32 / RPI;         // loads a tile, of keys and of values
   static_assert(2 * STAGE >= ROWS * DP * 4, "a wave's sums fit its stages");
-  static_assert(NW * 2 * STAGE >= ROWS * kSplitsMost * 4, "the chunks' weights fit too");
 };
 
 // 16 bytes of zeros that lanes without a key load.
@@ -440,7 +439,26 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     const int r = rt * C::ROWS + rr, t = r / G;
     return (t * p.Hq + hk * G + r - t * G) * p.splits;
   };
-  // A wave takes a row: its lanes the chunks' maxima and sums.
+  // An item: 16 bytes of a row's sums.  Few items are shared by `parts` threads
+  // each, a thread taking every parts-th chunk, kJoin in flight.
+  constexpr int NT = 64 * NW;
+  const int dp = p.D / 4, items = nrows * dp;
+  int parts = 1;
+  while (2 * parts * items <= NT && parts < 8) parts *= 2;
+  const int lanes = NT / parts, part = threadIdx.x / lanes;
+  u32x4 x[kJoin];
+  auto fetch = [&](int item, int k0) {  // behind the last chunk zeros
+    const int rr = item / dp, at0 = (part_row(rr) * p.D + 4 * (item - rr * dp)) * 4;
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      const int s = part + parts * (k0 + k);
+      x[k] = __builtin_amdgcn_raw_buffer_load_b128(sums, s < used ? (uint32_t)(at0 + s * p.D * 4) : 0x80000000u, 0, kDevice);
+    }
+  };
+  int item = threadIdx.x % lanes;
+  if (item < items) fetch(item, 0);
+  // Meanwhile the chunks' weights: a wave takes a row, its lanes the chunks'
+  // maxima and sums.
   for (int rr = wave; rr < nrows; rr += NW) {
     f32x2 v = {-INFINITY, 0.f};
     if (lane < used) v = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, (part_row(rr) + lane) * 8, 0, kDevice));
@@ -452,21 +470,36 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     weight[rr * kSplitsMost + lane] = lane < used ? a * inverse_sum(l) : 0.f;
   }
   __syncthreads();
-  const int dp = p.D / 4;
-  for (int i = threadIdx.x; i < nrows * dp; i += 64 * NW) {
-    const int rr = i / dp, piece = i - rr * dp;
-    const int at0 = (part_row(rr) * p.D + 4 * piece) * 4;
+  auto gather = [&](int item, bool fetched) -> f32x4 {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < used; s0 += kJoin) {  // kJoin loads in flight; behind the last chunk zeros
-      u32x4 x[kJoin];
+    for (int k0 = 0; part + parts * k0 < used; k0 += kJoin) {
+      if (!fetched || k0 > 0) fetch(item, k0);
 #pragma unroll
-      for (int s = 0; s < kJoin; ++s)
-        x[s] = __builtin_amdgcn_raw_buffer_load_b128(sums, s0 + s < used ? (uint32_t)(at0 + (s0 + s) * p.D * 4) : 0x80000000u, 0, kDevice);
-#pragma unroll
-      for (int s = 0; s < kJoin; ++s) v += __builtin_bit_cast(f32x4, x[s]) * weight[rr * kSplitsMost + min(s0 + s, kSplitsMost - 1)];
+      for (int k = 0; k < kJoin; ++k)
+        v += __builtin_bit_cast(f32x4, x[k]) * weight[item / dp * kSplitsMost + min(part + parts * (k0 + k), kSplitsMost - 1)];
     }
-    const int r = rt * C::ROWS + rr, t = r / G, h = hk * G + r - t * G;
-    store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
+    return v;
+  };
+  auto write = [&](int item, f32x4 v) {
+    const int rr = item / dp, r = rt * C::ROWS + rr, t = r / G, h = hk * G + r - t * G;
+    store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * (item - rr * dp), v);
+  };
+  if (parts > 1) {  // one item a thread
+    SVDMLP_ATTN_LDS f32x4* const others = (SVDMLP_ATTN_LDS f32x4*)((attn_lds)lds + C::ROWS * kSplitsMost * 4);
+    static_assert(C::ROWS * kSplitsMost * 4 + NT * 16 <= NW * 2 * C::STAGE, "weights and the parts' sums fit the stages");
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (item < items) v = gather(item, true);
+    others[threadIdx.x] = v;
+    __syncthreads();
+    if (part > 0 || item >= items) return;
+    for (int q = 1; q < parts; ++q) v += others[threadIdx.x + q * lanes];
+    write(item, v);
+    return;
+  }
+  bool fetched = true;
+  for (; item < items; item += NT) {
+    write(item, gather(item, fetched));
+    fetched = false;
   }
 }
 

@@ -26,7 +26,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _ACT_CODES
+from .ops import _ACT_CODES, _PARTIALS_CACHE
 
 # A call at decode shapes takes a few microseconds on the GPU, so the host's
 # part is kept short: sizes, types and devices are compared in line (a tensor's
@@ -434,10 +434,13 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
         if n > 1 and tree.stride(-1) != 1:
             tree = tree.contiguous()
         tree_ptr, tree_b, tree_q = tree.data_ptr(), tree.stride(0) if tree.dim() == 3 else 0, tree.stride(-2)
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.stride(3) != 1:
-            raise ValueError(f"the last dimension of {name} must be contiguous")
-        _aligned(name, c)
+    kst, vst, step = k_cache.stride(), v_cache.stride(), 8 if dtype is _BF16 else 4
+    if (kst[3] != 1 or vst[3] != 1 or kst[0] % step or kst[1] % step or kst[2] % step or vst[0] % step or vst[1] % step
+            or vst[2] % step or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16):
+        for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if c.stride(3) != 1:
+                raise ValueError(f"the last dimension of {name} must be contiguous")
+            _aligned(name, c)
     if out is None:
         out = q.new_empty((B, n, Hq, D))
     else:
@@ -448,50 +451,53 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
         return out
     q = _rows(q)
     lib = _lib.load()
-    st = _Strides15(*q.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3], *out.stride()[:3], block_table.stride(0),
-                    tree_b, tree_q)
+    qst, ost = q.stride(), out.stride()
+    st = _Strides15(qst[0], qst[1], qst[2], kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], ost[0], ost[1], ost[2],
+                    block_table.stride(0), tree_b, tree_q)
     code = _ACT_CODES[dtype]
-    ws, ws_ptr, counters_ptr = None, None, None
-    nbytes, counters = _partials(lib, index, B, n, page, width, Hq, Hk, D, code)
-    if nbytes:  # the partial sums of long contexts: of the call alone, from torch's allocator
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        ws_ptr, counters_ptr = ws.data_ptr(), _counters(index, counters).data_ptr()
-    _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-            lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
-            ws_ptr, nbytes, counters_ptr, counters)
+    nbytes, counters = _sizes(lib, index, B, n, page, width, Hq, Hk, D, code)
+    if nbytes:
+        held = _partials(index, nbytes, counters)
+        _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
+                held[0].data_ptr(), nbytes, held[1].data_ptr(), counters)
+    else:
+        _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
+                None, 0, None, 0)
     return out
 
 
-_PARTIALS: dict = {}
+_SIZES: dict = {}
 
 
-def _partials(lib, index, *sizes) -> tuple[int, int]:
+def _sizes(lib, index, *sizes) -> tuple[int, int]:
     """Workspace bytes and counters of a call's sizes on device `index` (they depend on the sizes and its CUs alone)."""
     key = (index, *sizes)
-    plan = _PARTIALS.get(key)
+    plan = _SIZES.get(key)
     if plan is None:
         counters = ctypes.c_int64(0)
         with torch.cuda.device(index):
             nbytes = int(lib.svdmlp_cache_attention_workspace_bytes(*sizes, ctypes.byref(counters)))
-        if len(_PARTIALS) > 4096:
-            _PARTIALS.clear()
-        plan = _PARTIALS[key] = (nbytes, counters.value)
+        if len(_SIZES) > 4096:
+            _SIZES.clear()
+        plan = _SIZES[key] = (nbytes, counters.value)
     return plan
 
 
-# The counters of cache_attention, one tensor of zeros a (device, stream): every
-# call leaves them zero for the next on its stream.  A captured call gets its
-# own, cleared by the graph.
-_COUNTERS: dict = {}
-
-
-def _counters(index: int, n: int) -> torch.Tensor:
+def _partials(index: int, nbytes: int, counters: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Room for partial sums and zeroed counters.  One pair a (device, stream),
+    grown on demand and kept until :func:`svdmlp.clear_workspace_cache`: every
+    call leaves the counters zero for the next on its stream.  A captured call
+    gets its own from the graph's pool, its counters cleared by the graph."""
+    device = f"cuda:{index}"
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.int32, device=f"cuda:{index}")
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), torch.zeros(counters, dtype=torch.int32, device=device)
     key = (index, _raw_stream(index))
-    held = _COUNTERS.get(key)
-    if held is None or held.numel() < n:
-        held = _COUNTERS[key] = torch.zeros(max(n, 4096), dtype=torch.int32, device=f"cuda:{index}")
+    held = _PARTIALS_CACHE.get(key)
+    if held is None or held[0].numel() < nbytes or held[1].numel() < counters:
+        held = _PARTIALS_CACHE[key] = (torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device),
+                                       torch.zeros(max(counters, 4096), dtype=torch.int32, device=device))
     return held
 
 

@@ -222,10 +222,16 @@ def _shared_workspace(dev, T, d, ff, r, w_code) -> torch.Tensor:
     return ws
 
 
+# What cache_attention (decoder.py) keeps a (device, stream): zeroed counters
+# and room for partial sums.
+_PARTIALS_CACHE: dict = {}
+
+
 def clear_workspace_cache() -> None:
     """Release the workspaces kept for calls that pass none (allocated again
     on the next such call)."""
     _WS_CACHE.clear()
+    _PARTIALS_CACHE.clear()
 
 
 # ---------------------------------------------------------------------------

@@ -450,7 +450,7 @@ def test_cache_attention_many_keys(gpu, dtype, B, n, H, K, D, page, most):
     _close(got[some], out, tol)
     for _ in range(3):
         assert torch.equal(got, svdmlp.cache_attention(*args, ln, tree=tg))
-    assert all(int(c.abs().max()) == 0 for c in decoder._COUNTERS.values())
+    assert all(int(c.abs().max()) == 0 for _, c in decoder._PARTIALS_CACHE.values())
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
