@@ -375,10 +375,17 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   // last stage's values, which the first step multiplies by zero weights.
   if (p.D < C::DP) {
     for (int i = threadIdx.x; i < C::NS * C::STAGE / 16; i += 256) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(base + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
   } else {
     for (int i = threadIdx.x; i < C::UNIT / 16; i += 256)
       *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(base + (C::NS - 1) * C::STAGE + C::TILE + C::UNIT + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before the first barrier
   }
+  issue_keys(0);
+  issue_keys(1);
+  issue_values(0);
+  issue_keys(2);
+  issue_values(1);
 
   u32x4 qf[QG][C::STEPS];
   int tok[QG];
@@ -393,14 +400,6 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
       qf[g][s] = c < npieces ? *reinterpret_cast<const u32x4*>(qp + 16 * c) : u32x4{0u, 0u, 0u, 0u};
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  issue_keys(0);
-  issue_keys(1);
-  issue_values(0);
-  issue_keys(2);
-  issue_values(1);
-
   f32x16 o[QG][DB];
   float m[QG], l[QG];
 #pragma unroll
@@ -415,31 +414,39 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   const TileLane<RB, true> at(lane);
   uint32_t bad = 0;
 
-  // S = K Q^T of the 32 keys at kt.
-  auto scores = [&](attn_lds kt, f32x16 (&s)[QG]) {
+  // S = K Q^T of the 32 keys at kt; the first pieces of V at vt are read behind
+  // it (an LDS read takes as long as two products, and one wave a SIMD hides none).
+  u32x4 piece[C::AHEAD];
+  auto scores = [&](attn_lds kt, attn_lds vt, f32x16 (&s)[QG]) {
+#pragma unroll
+    for (int t = 0; t < C::AHEAD; ++t) piece[t] = at.key(kt, t);
 #pragma unroll
     for (int t = 0; t < C::STEPS; ++t) {
-      const u32x4 kf = at.key(kt, t);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < QG; ++g) {
         if (t == 0) s[g] = f32x16{};
-        s[g] = attn_mfma<true>(kf, qf[g][t], s[g]);
+        s[g] = attn_mfma<true>(piece[t % C::AHEAD], qf[g][t], s[g]);
       }
+      const int n = t + C::AHEAD;
+      piece[t % C::AHEAD] = n < C::STEPS ? at.key(kt, n) : at.values(vt, (n - C::STEPS) / DB, (n - C::STEPS) % DB);
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
-  // O += V^T P^T of the 32 keys at vt.
+  // O += V^T P^T of the 32 keys at vt, whose first pieces are read.
   auto values = [&](attn_lds vt, const u32x4 (&pb)[QG][2], bool masked) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int f = 0; f < 2 * DB; ++f) {
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 vf = piece[f % C::AHEAD];
+      if (masked)
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        u32x4 vf = at.values(vt, t, d);
-        if (masked)
+        for (int w = 0; w < 4; ++w) vf[w] = scrub<true>(vf[w], bad);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) vf[w] = scrub<true>(vf[w], bad);
-#pragma unroll
-        for (int g = 0; g < QG; ++g) o[g][d] = attn_mfma<true>(vf, pb[g][t], o[g][d]);
-      }
+      for (int g = 0; g < QG; ++g) o[g][f % DB] = attn_mfma<true>(vf, pb[g][f / DB], o[g][f % DB]);
+      if (f + C::AHEAD < 2 * DB) piece[f % C::AHEAD] = at.values(vt, (f + C::AHEAD) / DB, (f + C::AHEAD) % DB);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
   // Where a score passes the reference by over kSlack: the new reference, and
   // what sums so far are to be multiplied by.
@@ -588,7 +595,7 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
       }
     };
     arrive(0);
-    scores(base, s0);
+    scores(base, base, s0);
     if (reference(s0, scale)) {}  // nothing has been summed yet
 #pragma unroll
     for (int g = 0; g < QG; ++g) {
@@ -613,7 +620,10 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
       SVDMLP_PIPE_TILE(I3)
     }
 #undef SVDMLP_PIPE_TILE
-    values(base + ((t - 1) % C::NS) * C::STAGE + C::TILE + C::UNIT, p1, false);
+    const attn_lds last = base + ((t - 1) % C::NS) * C::STAGE + C::TILE + C::UNIT;
+#pragma unroll
+    for (int f = 0; f < C::AHEAD; ++f) piece[f] = at.values(last, f / DB, f % DB);
+    values(last, p1, false);
   }
   for (; t < tiles; ++t) {
     arrive(t);
@@ -626,16 +636,17 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
       f32x16 s[QG];
       u32x4 pb[QG][2];
       float scale[QG];
-      scores(cur + u * C::UNIT, s);
+      const attn_lds vt = cur + C::TILE + u * C::UNIT;
+      scores(cur + u * C::UNIT, vt, s);
 #pragma unroll
       for (int g = 0; g < QG; ++g) {
-        const int last = p.causal ? tok[g] : nkeys - 1;
+        const int last = (p.causal ? tok[g] : nkeys - 1) - k0 - 4 * half;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[g][i] = k0 + 8 * (i >> 2) + 4 * half + (i & 3) <= last ? s[g][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[g][i] = 8 * (i >> 2) + (i & 3) <= last ? s[g][i] : -INFINITY;
       }
       if (reference(s, scale)) rescale(scale);
       weights(s, pb);
-      values(cur + C::TILE + u * C::UNIT, pb, true);
+      values(vt, pb, true);
     }
   }
 
