@@ -2652,6 +2652,7 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
   const int64_t* s = strides ? strides : dense;
   const int es = act_size(dtype);
   if (!no_negative(s, 8)) return fail("prompt_attention: strides must not be negative");
+  if (s[2] > kTokenStrideMost || s[4] > kTokenStrideMost) return fail("prompt_attention: keys or values are more than %lld elements apart", (long long)kTokenStrideMost);
   if (!pieces16({q, k, v, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]}, es))
     return fail("prompt_attention: the head size, strides and addresses must be whole 16-byte pieces");
   PromptParams p = {q, k, v, out, cu_seqlens, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], (int)T, (int)B, (int)Hq,
@@ -2693,7 +2694,7 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   if (!no_negative(s, 15)) return fail("cache_attention: strides must not be negative");
   if (!pieces16({q, k_cache, v_cache, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10], s[11]}, es))
     return fail("cache_attention: the head size, strides and addresses must be whole 16-byte pieces");
-  if (s[4] > 1 << 24 || s[7] > 1 << 24) return fail("cache_attention: rows of the cache are more than 2^24 elements apart");
+  if (s[4] > kTokenStrideMost || s[7] > kTokenStrideMost) return fail("cache_attention: rows of the cache are more than %lld elements apart", (long long)kTokenStrideMost);
   CacheParams p = {};
   p.q = q, p.kc = k_cache, p.vc = v_cache, p.table = block_table, p.lengths = lengths, p.tree = tree, p.out = out;
   p.q_b = s[0], p.q_t = s[1], p.q_h = s[2], p.k_p = s[3], p.k_t = s[4], p.k_h = s[5], p.v_p = s[6], p.v_t = s[7], p.v_h = s[8];

@@ -133,6 +133,53 @@ struct RowState {
 // so that weights stay below 2^8 and sums far from overflow.
 constexpr float kSlack = 8.0f;
 
+// The rows of a block: sequence rows start .. start + len of the tensors, of
+// key/value head hk, its rows row0 ...
+struct RowTile {
+  int start, len, hk, row0;
+};
+
+// The block's sequence and row tile; false: none.  Tiles of BM rows are numbered
+// sequence by sequence, a sequence's last rows (the most keys of a causal call)
+// first.  The grid covers the most tiles that B sequences of T rows can have.
+__device__ __forceinline__ bool find_rows(const int* cu, int T, int B, int Hk, int G, int BM, int lane, RowTile& rt) {
+  rt.hk = blockIdx.x % Hk;
+  int tile = blockIdx.x / Hk;
+  rt.start = 0;
+  rt.len = T;
+  if (cu) {
+    rt.len = -1;
+    for (int b0 = 0; b0 < B; b0 += 64) {
+      const int b = b0 + lane;
+      int s = 0, n = 0;
+      if (b < B) {
+        s = min(max(cu[b], 0), T);
+        n = min(max(cu[b + 1], s), T) - s;
+      }
+      const int tiles = (int)(((int64_t)n * G + BM - 1) / BM);
+      int before = tiles;  // inclusive prefix sum
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(before, o);
+        if (lane >= o) before += v;
+      }
+      const uint64_t hit = __ballot(tile < before);
+      if (hit) {
+        const int i = __builtin_ctzll(hit);
+        tile -= __builtin_amdgcn_readlane(before - tiles, i);
+        rt.start = __builtin_amdgcn_readlane(s, i);
+        rt.len = __builtin_amdgcn_readlane(n, i);
+        break;
+      }
+      tile -= __builtin_amdgcn_readlane(before, 63);
+    }
+    if (rt.len < 0) return false;
+  }
+  const int tiles = (rt.len * G + BM - 1) / BM;
+  if (tile >= tiles) return false;
+  rt.row0 = (tiles - 1 - tile) * BM;
+  return true;
+}
+
 // 16 bytes a lane from global memory straight to LDS, lane i's to base + 16 i.
 // The compiler does not know of the load: wait_loads before the tile is read.
 __device__ __forceinline__ void load_lds16(const void* p, uint32_t base) {

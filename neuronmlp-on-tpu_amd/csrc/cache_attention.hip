@@ -13,495 +13,13 @@
 // A long context is cut into chunks, one a block; the last block of a
 // (sequence, head, row tile) to arrive joins the chunks' partial sums, in the
 // chunks' order (the same bits every time).
-#include <math.h>
-
 #include <algorithm>
 
-#include "attn.hpp"
-#include "decoder.hpp"
+#include "wave_attention.hpp"
 
 namespace svdmlp {
 
 namespace {
-
-constexpr int kSplitsMost = 64;   // chunks of a sequence
-constexpr int kJoin = 16;         // chunks' sums in flight when they are joined
-constexpr int kPagesMost = 1024;  // whole pages of a chunk: their numbers lie in LDS
-
-template <bool BF16_, int DP_, int QG_, int NW_>
-struct CacheCfg {
-  static constexpr bool BF16 = BF16_;
-  static constexpr int DP = DP_, QG = QG_;
-  static constexpr int ES = BF16 ? 2 : 4;
-  static constexpr int RB = DP * ES;
-  static constexpr int PIECES = RB / 16;
-  static constexpr int STEPS = RB / 32;
-  static constexpr int NW = NW_;  // waves a block
-  static constexpr int TILE = 32 * RB;
-  static constexpr int STAGE = 2 * TILE;  // keys, values
-  static constexpr int ROWS = 32 * QG;
-  static constexpr int RPI = 64 / PIECES;        // rows a load
-  static constexpr int LOADS = 32 / RPI;         // loads a tile, of keys and of values
-  static_assert(2 * STAGE >= ROWS * DP * 4, "a wave's sums fit its stages");
-};
-
-// 16 bytes of zeros that lanes without a key load.
-__device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
-
-// Lane j's v, the same for all lanes (j a constant).
-__device__ __forceinline__ int64_t lane64(int64_t v, int j) {
-  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, j) |
-                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), j) << 32);
-}
-
-// Partial sums cross blocks, and so XCDs with an L2 each, by device-scope (sc1)
-// accesses past the L2, without any cache maintenance: fences that write back
-// and drop the L2 for every block made a call of 4096 blocks 325 us instead of
-// 137.  Offsets are in bytes from a sequence's part.
-constexpr int kDevice = 16;  // the sc1 bit of a buffer access
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_of(const CacheParams& p, int b, int floats) {
-  const int64_t rows = (int64_t)p.n * p.Hq * p.splits;
-  float* const base = p.part + (floats == 2 ? (int64_t)p.B * rows * p.D : 0) + (int64_t)b * rows * floats;
-  return __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)(rows * floats * 4), 0x00020000);
-}
-
-__device__ __forceinline__ int held(const CacheParams& p, int b) {
-  const int64_t cap = (int64_t)p.width * p.page;
-  return (int)min((int64_t)max(p.lengths[b], 0), cap);
-}
-
-// Which of the 32 keys from `draft` keys after the context on a token sees,
-// whose row of the tree is `row`: all of the context.
-__device__ __forceinline__ uint32_t seen32(uint64_t row, int draft) {
-  if (draft >= 64) return 0;
-  if (draft >= 0) return (uint32_t)(row >> draft);
-  if (draft <= -32) return 0xffffffffu;
-  return (uint32_t)(row << -draft) | ((1u << -draft) - 1u);
-}
-
-template <class C>
-__global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
-  constexpr bool BF16 = C::BF16;
-  constexpr int ES = C::ES, RB = C::RB, QG = C::QG, DB = C::DP / 32, NW = C::NW;
-  __shared__ __attribute__((aligned(1024))) char lds[NW * 2 * C::STAGE];
-  __shared__ float stats[NW][C::ROWS][2];
-  __shared__ int ids[kPagesMost + 2];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-  const int G = p.Hq / p.Hk;
-  const int rows = p.n * G;
-  const int rtiles = (rows + C::ROWS - 1) / C::ROWS;
-  int id = blockIdx.x;
-  const int hk = id % p.Hk;
-  id /= p.Hk;
-  const int rt = id % rtiles;
-  id /= rtiles;
-  const int b = id % p.B, split = id / p.B;
-  const int len = held(p, b);
-  const int kbeg = split * p.chunk, kend = min(len, kbeg + p.chunk);
-  const int used = max(1, (int)(((int64_t)len + p.chunk - 1) / p.chunk));  // chunks that hold keys; the first always answers
-  if (split >= used) return;
-  const int context = len - p.n;             // keys that every row sees
-
-  // The chunk's pages, and the queries.
-  const int pg0 = kbeg / p.page;
-  const int npages = min(p.width - pg0, (int)min((int64_t)p.chunk + p.page - 1, (int64_t)kPagesMost * p.page) / p.page + 1);
-  for (int i = threadIdx.x; i < npages; i += 64 * NW) ids[i] = p.table[(int64_t)b * p.table_b + pg0 + i];
-  // Heads of over 128 elements leave no registers for Q: its pieces are read
-  // again (from the caches) for every tile.
-  constexpr bool QREG = C::DP < 256;
-  u32x4 qf[QG][QREG ? C::STEPS : 1];
-  const char* qptr[QG];
-  int qi[QG];  // which of the new tokens
-  const int npieces = p.D * ES / 16;
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int r = min(rt * C::ROWS + 32 * g + col, rows - 1);  // rows behind the last repeat it, and are not stored
-    qi[g] = r / G;
-    qptr[g] = static_cast<const char*>(p.q) + ((int64_t)b * p.q_b + (int64_t)qi[g] * p.q_t + (int64_t)(hk * G + r - qi[g] * G) * p.q_h) * ES;
-    if constexpr (QREG)
-#pragma unroll
-      for (int s = 0; s < C::STEPS; ++s) {
-        const int c = 2 * s + half;
-        qf[g][s] = c < npieces ? *reinterpret_cast<const u32x4*>(qptr[g] + 16 * c) : u32x4{0u, 0u, 0u, 0u};
-      }
-  }
-  // Each row's 64 bits of the tree, where the chunk reaches the new tokens: a
-  // lane reads one byte of a token's row, and a ballot gathers them.
-  uint64_t row_sees[QG];
-#pragma unroll
-  for (int g = 0; g < QG; ++g) row_sees[g] = (2ull << qi[g]) - 1;  // a chain (token 63: all)
-  if (p.tree && kend > context) {
-    const uint8_t* const tree = p.tree + (int64_t)b * p.tree_b;
-    const int first = rt * C::ROWS / G, last = min(rt * C::ROWS + C::ROWS - 1, rows - 1) / G;
-    for (int t = first; t <= last; ++t) {
-      const uint64_t bits = __ballot(tree[(int64_t)t * p.tree_q + min(lane, p.n - 1)] != 0);
-#pragma unroll
-      for (int g = 0; g < QG; ++g) row_sees[g] = qi[g] == t ? bits : row_sees[g];
-    }
-  }
-  f32x16 o[QG][DB];
-  RowState st[QG];
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    st[g] = {-INFINITY, 0.f};
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[g][d][i] = 0.f;
-  }
-  // The loop's loads are counted (wait_loads): none of the above may be among them.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-
-  const attn_lds mine = (attn_lds)lds + wave * 2 * C::STAGE;
-  const char* const kb = static_cast<const char*>(p.kc) + (int64_t)hk * p.k_h * ES;
-  const char* const vb = static_cast<const char*>(p.vc) + (int64_t)hk * p.v_h * ES;
-  const TileLane<RB, BF16> at(lane);
-  const float per_page = 1.0f / (float)p.page;
-  uint32_t bad = 0;
-
-  // The row (page, place in it) of key ku + row; -1: of none.
-  auto place = [&](int ku, int row, int* in) -> int {
-    const int first = ku / p.page, x = ku - first * p.page + row;
-    // x < page + 32: one division of small numbers, exact in 32 bits
-    const int q = p.page >= 32 ? (x >= p.page) : (int)(((float)x + 0.5f) * per_page);
-    *in = x - q * p.page;
-    const int i = first + q - pg0;
-    const int pg = ku + row < kend ? ids[i] : -1;
-    return pg >= 0 && pg < p.pages ? pg : -1;
-  };
-  // A lane's part of a load's addresses: row lane / PIECES of its RPI rows,
-  // piece lane % PIECES, both swizzled; load j adds a constant (the swizzles
-  // pick bits of the row, so that they combine by exclusive or).
-  const int lrow = lane / C::PIECES, lc = lane % C::PIECES;
-  const int kpiece0 = lc ^ k_swz<RB>(lrow), vpiece0 = lc ^ v_swz<RB, BF16>(lrow);
-  const uint32_t krow = (uint32_t)(lrow * (int)p.k_t * ES), vrow = (uint32_t)(lrow * (int)p.v_t * ES);
-  const bool alike = p.page_shift >= 0 && p.k_p == p.v_p && p.k_t == p.v_t;
-  // Loads of the tile at key ku; true: all 32 keys are there.
-  auto issue = [&](int ku, attn_lds stage) -> bool {
-    const uint32_t base = (uint32_t)(uintptr_t)stage;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
-    int kpiece = kpiece0, vpiece = vpiece0;
-    // where registers are short, the loads' offsets are computed each time
-    if constexpr (QG == 2 || RB >= 512) asm volatile("" : "+v"(kpiece), "+v"(vpiece));
-    if (alike && ku + 32 <= kend) {
-      // Pages of a power of two that hold whole loads, both caches laid out
-      // alike: lane j finds load j's page, and the place of its rows goes to
-      // all lanes through scalar registers.
-      const int key = ku + lane % C::LOADS * C::RPI, pg = ids[(key >> p.page_shift) - pg0], in = key & (p.page - 1);
-      if (__all(pg >= 0 && pg < p.pages)) {
-        const int64_t off = ((int64_t)pg * p.k_p + (int64_t)in * p.k_t) * ES;
-        if (p.D == C::DP) {
-#pragma unroll
-          for (int j = 0; j < C::LOADS; ++j) {
-            const int64_t at = lane64(off, j);
-            load_lds16(kb + at, krow + 16 * (kpiece ^ k_swz<RB>(j * C::RPI)), base + j * 1024);
-            load_lds16(vb + at, vrow + 16 * (vpiece ^ v_swz<RB, BF16>(j * C::RPI)), base + C::TILE + j * 1024);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < C::LOADS; ++j) {
-            const int ck = kpiece ^ k_swz<RB>(j * C::RPI), cv = vpiece ^ v_swz<RB, BF16>(j * C::RPI);
-            const int64_t at = lane64(off, j);
-            if (ck < npieces) load_lds16(kb + at, krow + 16 * ck, base + j * 1024);
-            if (cv < npieces) load_lds16(vb + at, vrow + 16 * cv, base + C::TILE + j * 1024);
-          }
-        }
-        return true;
-      }
-    }
-#pragma unroll 2
-    for (int j = 0; j < C::LOADS; ++j) {
-      const int row = j * C::RPI + lrow;
-      int in;
-      const int pg = place(ku, row, &in);
-      const int ck = lc ^ k_swz<RB>(row), cv = lc ^ v_swz<RB, BF16>(row);
-      const char* kp = kb + ((int64_t)pg * p.k_p + (int64_t)in * p.k_t) * ES + 16 * ck;
-      const char* vp = vb + ((int64_t)pg * p.v_p + (int64_t)in * p.v_t) * ES + 16 * cv;
-      kp = pg >= 0 ? kp : reinterpret_cast<const char*>(&kZeroPiece);
-      vp = pg >= 0 ? vp : reinterpret_cast<const char*>(&kZeroPiece);
-      if (ck < npieces) load_lds16(kp, base + j * 1024);
-      if (cv < npieces) load_lds16(vp, base + C::TILE + j * 1024);
-    }
-    return false;
-  };
-  if (p.D < C::DP)  // pieces behind the head's end: never loaded, zeros
-    for (int i = lane; i < 2 * C::STAGE / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
-
-  // One tile: S = K Q^T, the weights, O += V^T P^T.  Pieces are read from LDS
-  // kAhead products before they are needed, the first of V behind the weights
-  // (a read takes as long as two products, and one wave a SIMD hides nothing).
-  constexpr int kAhead = RB < 1024 ? 4 : 2, VF = BF16 ? 2 * DB : 16 * DB;  // VF: pieces of V
-  static_assert(C::STEPS >= kAhead && VF >= kAhead, "pieces");
-  auto unit = [&](auto masked_, attn_lds stage, int ku, uint32_t there) {
-    constexpr bool masked = decltype(masked_)::value;
-    const attn_lds lk = stage, lv = stage + C::TILE;
-    u32x4 kf[kAhead], vf[kAhead];
-    auto read_value = [&](int f) {
-      if constexpr (BF16) vf[f % kAhead] = at.values(lv, f / DB, f % DB);
-      else vf[f % kAhead].x = at.value(lv, f / DB, f % DB);
-    };
-#pragma unroll
-    for (int t = 0; t < kAhead; ++t) kf[t] = at.key(lk, t);
-    f32x16 s[QG];
-#pragma unroll
-    for (int g = 0; g < QG; ++g) s[g] = f32x16{};
-#pragma unroll
-    for (int t = 0; t < C::STEPS; ++t) {
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int g = 0; g < QG; ++g) {
-        if constexpr (!QREG) {
-          const int c = 2 * t + half;
-          qf[g][0] = c < npieces ? *reinterpret_cast<const u32x4*>(qptr[g] + 16 * c) : u32x4{0u, 0u, 0u, 0u};
-        }
-        s[g] = attn_mfma<BF16>(kf[t % kAhead], qf[g][QREG ? t : 0], s[g]);
-      }
-      if (t + kAhead < C::STEPS) kf[t % kAhead] = at.key(lk, t + kAhead);
-      else read_value(t + kAhead - C::STEPS);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    u32x4 pb[QG][2];
-#pragma unroll
-    for (int g = 0; g < QG; ++g) {
-      if constexpr (masked) {
-        const uint32_t see = (there & seen32(row_sees[g], ku - context)) >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[g][i] = see >> (8 * (i >> 2) + (i & 3)) & 1u ? s[g][i] : -INFINITY;
-      }
-      float mx = fmaxf(s[g][0], s[g][1]);
-#pragma unroll
-      for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, s[g][i]), s[g][i + 1]);
-      mx *= p.c;
-      if (__any(mx > st[g].m + kSlack)) {
-        const float m = fmaxf(st[g].m, fmaxf(mx, __shfl_xor(mx, 32)));
-        const float a = m == -INFINITY ? 1.f : exp2f(st[g].m - m);
-        st[g].m = m;
-        st[g].l *= a;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[g][d][i] *= a;
-      }
-      const float m = st[g].m == -INFINITY ? 0.f : st[g].m;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], p.c, -m));
-      if constexpr (BF16) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          pb[g][i / 4][i % 4] = pack_bf16x2(s[g][2 * i], s[g][2 * i + 1]);
-          st[g].l = add_pair(pb[g][i / 4][i % 4], st[g].l);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[g].l += s[g][i];
-      }
-    }
-#pragma unroll
-    for (int f = 0; f < VF; ++f) {
-      __builtin_amdgcn_sched_barrier(0);
-      u32x4 v = vf[f % kAhead];
-      if constexpr (masked) {
-#pragma unroll
-        for (int w = 0; w < (BF16 ? 4 : 1); ++w) v[w] = scrub<BF16>(v[w], bad);
-      }
-#pragma unroll
-      for (int g = 0; g < QG; ++g) {
-        if constexpr (BF16) o[g][f % DB] = attn_mfma<true>(v, pb[g][f / DB], o[g][f % DB]);
-        else o[g][f % DB] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v.x), s[g][f / DB], o[g][f % DB], 0, 0, 0);
-      }
-      if (f + kAhead < VF) read_value(f + kAhead);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-
-  int ku = kbeg + 32 * wave;
-  attn_lds cur = mine, nxt = mine + C::STAGE;
-  bool whole = false;
-  if (ku < kend) whole = issue(ku, cur);
-  for (; ku < kend; ku += 32 * NW) {
-    bool next_whole = false;
-    if (ku + 32 * NW < kend) {
-      next_whole = issue(ku + 32 * NW, nxt);
-      wait_loads<(2 * C::LOADS < 63 ? 2 * C::LOADS : 63)>();
-    } else {
-      wait_loads<0>();
-    }
-    int in;
-    if constexpr (RB < 1024) {
-      if (whole && ku + 31 < context) unit(std::false_type{}, cur, ku, 0xffffffffu);
-      else unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
-    } else {  // one copy of the code: two do not fit the registers
-      unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
-    }
-    whole = next_whole;
-    const attn_lds swap = cur;
-    cur = nxt;
-    nxt = swap;
-  }
-
-  // Each wave's sums, scaled to the block's maximum, in its own LDS; then all
-  // threads add the waves' in order.  Row r's 16-byte pieces are spread by r.
-  constexpr int OP = C::DP / 4;  // pieces of a row of sums
-  constexpr int OM = OP < 32 ? OP - 1 : 31;
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const float l = st[g].l + __shfl_xor(st[g].l, 32);
-    if (half == 0) {
-      stats[wave][32 * g + col][0] = st[g].m;
-      stats[wave][32 * g + col][1] = l;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][32 * g + col][0]);
-    const float a = st[g].m == -INFINITY ? 1.f : exp2f(st[g].m - m);
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int piece = 8 * d + 2 * q + half;
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = o[g][d][4 * q + e] * a;
-        *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>(mine + ((32 * g + col) * OP + (piece ^ (col & OM))) * 16) = v;
-      }
-  }
-  // Infinities and NaN among the values of the masked tiles were taken as
-  // zeros, for the rows that do not see them; the rows that do get them here.
-  if (__any(bad != 0)) {
-    for (int kt = kbeg + 32 * wave; kt < kend; kt += 32 * NW) {
-      if (kt + 31 < context) continue;
-      for (int key = kt; key < min(kt + 32, kend); ++key) {
-        int in;
-        const int pg = place(key, 0, &in);
-        if (pg < 0) continue;
-        const char* const vp = vb + ((int64_t)pg * p.v_p + (int64_t)in * p.v_t) * ES;
-        for (int e = 0; e < p.D; ++e) {
-          const uint32_t w = BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(vp)[e] << 16 : reinterpret_cast<const uint32_t*>(vp)[e];
-          if (not_finite<false>(w) && half == 0)
-#pragma unroll
-            for (int g = 0; g < QG; ++g)
-              if (seen32(row_sees[g], key - context) & 1u) {
-                SVDMLP_ATTN_LDS float* const sum =
-                    (SVDMLP_ATTN_LDS float*)(mine + ((32 * g + col) * OP + ((e >> 2) ^ (col & OM))) * 16) + (e & 3);
-                *sum += __uint_as_float(w);
-              }
-        }
-      }
-    }
-  }
-  __syncthreads();
-  const __amdgpu_buffer_rsrc_t sums = part_of(p, b, p.D), ml = part_of(p, b, 2);
-  for (int i = threadIdx.x; i < C::ROWS * OP; i += 64 * NW) {
-    const int rr = i / OP, piece = i % OP, r = rt * C::ROWS + rr;
-    if (r >= rows || 4 * piece >= p.D) continue;
-    float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][rr][0]);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = stats[w][rr][0];
-      l += mw == -INFINITY ? stats[w][rr][1] : stats[w][rr][1] * exp2f(mw - m);
-      v += *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>((attn_lds)lds + w * 2 * C::STAGE + (rr * OP + (piece ^ (rr & OM))) * 16);
-    }
-    const int t = r / G, h = hk * G + r - t * G;
-    if (used == 1) {
-      v *= inverse_sum(l);
-      store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
-    } else {
-      const int row = (t * p.Hq + h) * p.splits + split;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), sums, (row * p.D + 4 * piece) * 4, 0, kDevice);
-      if (piece == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, ml, row * 8, 0, kDevice);
-    }
-  }
-  if (used == 1) return;
-
-  // The last block to get here joins the chunks.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums are out
-  __syncthreads();
-  int* const counter = p.counters + ((int64_t)b * p.Hk + hk) * rtiles + rt;
-  int last = 0;
-  if (threadIdx.x == 0) {
-    last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == used - 1;
-    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // as the next call finds it
-    stats[0][0][0] = last ? 1.f : 0.f;
-  }
-  __syncthreads();
-  if (stats[0][0][0] == 0.f) return;
-  SVDMLP_ATTN_LDS float* const weight = (SVDMLP_ATTN_LDS float*)(attn_lds)lds;  // [row][kSplitsMost]
-  const int nrows = min(C::ROWS, rows - rt * C::ROWS);
-  auto part_row = [&](int rr) -> int {
-    const int r = rt * C::ROWS + rr, t = r / G;
-    return (t * p.Hq + hk * G + r - t * G) * p.splits;
-  };
-  // An item: 16 bytes of a row's sums.  Few items are shared by `parts` threads
-  // each, a thread taking every parts-th chunk, kJoin in flight.
-  constexpr int NT = 64 * NW;
-  const int dp = p.D / 4, items = nrows * dp;
-  int parts = 1;
-  while (2 * parts * items <= NT && parts < 8) parts *= 2;
-  const int lanes = NT / parts, part = threadIdx.x / lanes;
-  u32x4 x[kJoin];
-  auto fetch = [&](int item, int k0) {  // behind the last chunk zeros
-    const int rr = item / dp, at0 = (part_row(rr) * p.D + 4 * (item - rr * dp)) * 4;
-#pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      const int s = part + parts * (k0 + k);
-      x[k] = __builtin_amdgcn_raw_buffer_load_b128(sums, s < used ? (uint32_t)(at0 + s * p.D * 4) : 0x80000000u, 0, kDevice);
-    }
-  };
-  int item = threadIdx.x % lanes;
-  if (item < items) fetch(item, 0);
-  // Meanwhile the chunks' weights: a wave takes a row, its lanes the chunks'
-  // maxima and sums.
-  for (int rr = wave; rr < nrows; rr += NW) {
-    f32x2 v = {-INFINITY, 0.f};
-    if (lane < used) v = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, (part_row(rr) + lane) * 8, 0, kDevice));
-    float m = v.x;
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const float a = v.x == -INFINITY ? 1.f : exp2f(v.x - m);
-    float l = v.y * a;
-    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-    weight[rr * kSplitsMost + lane] = lane < used ? a * inverse_sum(l) : 0.f;
-  }
-  __syncthreads();
-  auto gather = [&](int item, bool fetched) -> f32x4 {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; part + parts * k0 < used; k0 += kJoin) {
-      if (!fetched || k0 > 0) fetch(item, k0);
-#pragma unroll
-      for (int k = 0; k < kJoin; ++k)
-        v += __builtin_bit_cast(f32x4, x[k]) * weight[item / dp * kSplitsMost + min(part + parts * (k0 + k), kSplitsMost - 1)];
-    }
-    return v;
-  };
-  auto write = [&](int item, f32x4 v) {
-    const int rr = item / dp, r = rt * C::ROWS + rr, t = r / G, h = hk * G + r - t * G;
-    store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 4 * (item - rr * dp), v);
-  };
-  if (parts > 1) {  // one item a thread
-    SVDMLP_ATTN_LDS f32x4* const others = (SVDMLP_ATTN_LDS f32x4*)((attn_lds)lds + C::ROWS * kSplitsMost * 4);
-    static_assert(C::ROWS * kSplitsMost * 4 + NT * 16 <= NW * 2 * C::STAGE, "weights and the parts' sums fit the stages");
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (item < items) v = gather(item, true);
-    others[threadIdx.x] = v;
-    __syncthreads();
-    if (part > 0 || item >= items) return;
-    for (int q = 1; q < parts; ++q) v += others[threadIdx.x + q * lanes];
-    write(item, v);
-    return;
-  }
-  bool fetched = true;
-  for (; item < items; item += NT) {
-    write(item, gather(item, fetched));
-    fetched = false;
-  }
-}
 
 template <bool BF16, int DP, int QG, int NW>
 hipError_t run(const CacheParams& p, hipStream_t st) {

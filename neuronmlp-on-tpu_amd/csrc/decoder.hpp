@@ -70,11 +70,14 @@ struct CacheParams {
   int64_t pages;
   int page, width, B, n, Hq, Hk, D;
   int page_shift;     // log2 of a page that is a power of two and holds whole loads, else -1 (set by the launcher)
+  const int* cu;      // prompts only (wave_attention.hpp): their bounds, rows and mask; n, table, lengths unused
+  int T, causal;
   int splits, chunk;  // keys are cut into chunks of `chunk` (a multiple of the key tile), one a block
   float c;
 };
 // How a call is cut: `splits` chunks of `chunk` keys cover the table's
 // `capacity`, a block of `waves` waves each; rtiles row tiles a sequence and head.
+constexpr int64_t kTokenStrideMost = 1 << 23;  // a 64-row tile's byte offsets fit 31 bits, in both types
 constexpr int64_t kCachePagesMost = 65536;  // pages of a sequence: 64 chunks of 1024
 struct CachePlan {
   int splits, chunk, waves, rtiles;

@@ -9,59 +9,11 @@
 
 #include <algorithm>
 
-#include "attn.hpp"
-#include "decoder.hpp"
+#include "wave_attention.hpp"
 
 namespace svdmlp {
 
 namespace {
-
-// The rows of a block: sequence rows start .. start + len of the tensors, of
-// key/value head hk, its rows row0 ...
-struct RowTile {
-  int start, len, hk, row0;
-};
-
-// The block's sequence and row tile; false: none.  Tiles of BM rows are numbered
-// sequence by sequence, a sequence's last rows (the most keys of a causal call)
-// first.  The grid covers the most tiles that B sequences of T rows can have.
-__device__ __forceinline__ bool find_rows(const PromptParams& p, int G, int BM, int lane, RowTile& rt) {
-  rt.hk = blockIdx.x % p.Hk;
-  int tile = blockIdx.x / p.Hk;
-  rt.start = 0;
-  rt.len = p.T;
-  if (p.cu) {
-    rt.len = -1;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      const int b = b0 + lane;
-      int s = 0, n = 0;
-      if (b < p.B) {
-        s = min(max(p.cu[b], 0), p.T);
-        n = min(max(p.cu[b + 1], s), p.T) - s;
-      }
-      const int tiles = (int)(((int64_t)n * G + BM - 1) / BM);
-      int before = tiles;  // inclusive prefix sum
-      for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(before, o);
-        if (lane >= o) before += v;
-      }
-      const uint64_t hit = __ballot(tile < before);
-      if (hit) {
-        const int i = __builtin_ctzll(hit);
-        tile -= __builtin_amdgcn_readlane(before - tiles, i);
-        rt.start = __builtin_amdgcn_readlane(s, i);
-        rt.len = __builtin_amdgcn_readlane(n, i);
-        break;
-      }
-      tile -= __builtin_amdgcn_readlane(before, 63);
-    }
-    if (rt.len < 0) return false;
-  }
-  const int tiles = (rt.len * G + BM - 1) / BM;
-  if (tile >= tiles) return false;
-  rt.row0 = (tiles - 1 - tile) * BM;
-  return true;
-}
 
 template <bool BF16_, int DP_, int QG_>
 struct PromptCfg {
@@ -86,7 +38,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
   const int G = p.Hq / p.Hk;
 
   RowTile where;
-  if (!find_rows(p, G, C::BM, lane, where)) return;
+  if (!find_rows(p.cu, p.T, p.B, p.Hk, G, C::BM, lane, where)) return;
   const int hk = where.hk, start = where.start, len = where.len, row0 = where.row0, rows = len * G;
   const int tok_last = min(len - 1, (row0 + C::BM - 1) / G);
   const int tok_first = row0 / G;
@@ -313,7 +265,7 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
   const int G = p.Hq / p.Hk;
   RowTile rt;
-  if (!find_rows(p, G, C::BM, lane, rt)) return;
+  if (!find_rows(p.cu, p.T, p.B, p.Hk, G, C::BM, lane, rt)) return;
   const int row0 = rt.row0, rows = rt.len * G;
   const int tok_last = min(rt.len - 1, (row0 + C::BM - 1) / G), tok_first = row0 / G;
   const int nkeys = p.causal ? tok_last + 1 : rt.len;
@@ -711,20 +663,37 @@ hipError_t run_pipe(const PromptParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <bool BF16, int DP, int QG, int NW>
+hipError_t run_wave(const PromptParams& p, hipStream_t st) {
+  using C = CacheCfg<BF16, DP, QG, NW, true>;
+  CacheParams w = {};
+  w.q = p.q, w.kc = p.k, w.vc = p.v, w.out = p.out, w.cu = p.cu;
+  w.q_t = p.q_t, w.q_h = p.q_h, w.k_t = p.k_t, w.k_h = p.k_h, w.v_t = p.v_t, w.v_h = p.v_h, w.o_t = p.o_t, w.o_h = p.o_h;
+  w.T = p.T, w.B = p.B, w.Hq = p.Hq, w.Hk = p.Hk, w.D = p.D, w.causal = p.causal, w.splits = 1, w.c = p.c;
+  const int64_t tiles = (int64_t)p.T * (p.Hq / p.Hk) / C::ROWS + p.B;
+  if (tiles * p.Hk > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((cache_kernel<C>), dim3((unsigned)(tiles * p.Hk)), dim3(64 * NW), 0, st, w);
+  return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, hipStream_t st) {
   if (p.T <= 0) return hipSuccess;
-  if (bf16) {
-    const bool near = p.k_t < 1 << 24 && p.v_t < 1 << 24;  // a tile's offsets fit 32 bits
-    if (p.D <= 128 && near && (int64_t)p.T * p.Hq >= 256 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
-    if (p.D <= 64) return run<true, 64, 1>(p, st);
-    if (p.D <= 128) return run<true, 128, 1>(p, st);
-    return run<true, 256, 1>(p, st);
+  const int64_t rows = (int64_t)p.T * p.Hq;
+  if (bf16 && p.D <= 128) {
+    // 256-row blocks where they give half the CUs work, else 64-row ones that
+    // share the keys among their waves.
+    if (rows >= 128 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
+    return p.D <= 64 ? run_wave<true, 64, 2, 4>(p, st) : run_wave<true, 128, 2, 4>(p, st);
   }
-  if (p.D <= 64) return run<false, 64, 1>(p, st);
-  if (p.D <= 128) return run<false, 128, 1>(p, st);
-  return run<false, 256, 1>(p, st);
+  if (!bf16 && p.D <= 64) return run_wave<false, 64, 2, 4>(p, st);
+  if (rows < 128 * 256) {
+    if (bf16) return run_wave<true, 256, 1, 2>(p, st);
+    return p.D <= 128 ? run_wave<false, 128, 1, 2>(p, st) : run_wave<false, 256, 1, 1>(p, st);
+  }
+  if (bf16) return run<true, 256, 1>(p, st);
+  return p.D <= 128 ? run<false, 128, 1>(p, st) : run<false, 256, 1>(p, st);
 }
 
 }  // namespace svdmlp

@@ -381,6 +381,8 @@ def prompt_attention(q, k, v, cu_seqlens=None, *, causal: bool = True, scale: fl
     if T == 0:
         return out
     q, k, v = _rows(q), _rows(k), _rows(v)
+    if k.stride(0) > 1 << 23 or v.stride(0) > 1 << 23:  # farther apart than the kernels' offsets reach
+        k, v = k.contiguous(), v.contiguous()
     st = _Strides8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2])
     _launch(index, _lib.load().svdmlp_prompt_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu, out.data_ptr(),
             _address(st), T, B, Hq, ks[1], D, scale, _ACT_CODES[dtype], 1 if causal else 0)

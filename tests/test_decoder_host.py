@@ -54,7 +54,8 @@ def _prompt(lib, T=4, B=1, Hq=4, Hk=2, D=16, scale=0.25, dtype=1, flags=1, cu=No
     (dict(T=0), b"positive"), (dict(Hk=3), b"no multiple"), (dict(D=264), b"head size"), (dict(D=12), b"16-byte"),
     (dict(B=2), b"bounds"), (dict(B=0), b"bounds"), (dict(scale=0.0), b"scale"), (dict(scale=math.nan), b"scale"),
     (dict(flags=4), b"flags"), (dict(out=ctypes.c_void_p(264)), b"16-byte"), (dict(out=None), b"null"),
-    (dict(strides=_strides(64, 16, 32, 16, 32, 16, 64, 12)), b"16-byte"), (dict(T=1 << 31), b"too many"), (dict(dtype=2), b"dtype"),
+    (dict(strides=_strides(64, 16, 32, 16, 32, 16, 64, 12)), b"16-byte"), (dict(strides=_strides(64, 16, -32, 16, 32, 16, 64, 16)), b"negative"),
+    (dict(strides=_strides(64, 16, 32, 16, 1 << 24, 16, 64, 16)), b"apart"), (dict(T=1 << 31), b"too many"), (dict(dtype=2), b"dtype"),
 ])
 def test_prompt_attention_refusals(lib, kw, msg):
     assert _prompt(lib, **kw) == BAD

@@ -478,6 +478,23 @@ def test_cache_attention_hidden_drafts_have_no_part(gpu, dtype):
     assert (got[1, 3] == 0).all()  # no context, an empty row
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D,B", [(64, 1), (128, 1), (256, 1), (128, 300)])
+def test_cache_attention_context_values_reach_every_token(gpu, dtype, D, B):
+    """An infinity among the context's values is in every row's result, in its column alone."""
+    g = _gen(25)
+    n, H, K, page, most = 3, 4, 2, 16, 600
+    lens = [most] * B
+    table, pages = _pages(g, lens, page)
+    q, kc, vc = _randn(g, B, n, H, D, dtype=dtype), _randn(g, pages, page, K, D, dtype=dtype), _randn(g, pages, page, K, D, dtype=dtype)
+    vc[table[0, 2].item(), 5, 0, 7], vc[table[0, 20].item(), 0, 1, 9] = math.inf, -math.inf
+    vc[table[0, most // page].item(), most % page - n - 1, 1, 3] = math.inf  # the last of the context
+    got = svdmlp.cache_attention(*(t.to(gpu) for t in (q, kc, vc, table)), torch.tensor(lens, device=gpu)).cpu()
+    assert (got[0, :, :H // K, 7] == math.inf).all() and (got[0, :, H // K:, 9] == -math.inf).all() and (got[0, :, H // K:, 3] == math.inf).all()
+    got[0, :, :H // K, 7] = got[0, :, H // K:, 9] = got[0, :, H // K:, 3] = 0
+    assert torch.isfinite(got.float()).all()
+
+
 def test_cache_attention_broken_tables(gpu):
     """Pages outside the cache hold no keys, lengths beyond the table are cut, negative ones empty."""
     g = _gen(22)
