@@ -55,7 +55,7 @@ struct PromptParams {
   float c;  // softmax scale * log2(e)
   int causal;
 };
-hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, hipStream_t st);
+hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, int cus, hipStream_t st);
 
 struct CacheParams {
   const void* q;          // (B, n, Hq, D)

@@ -1,10 +1,11 @@
 // Attention of packed sequences onto themselves, O = softmax(c Q K^T + mask) V,
 // causal or not; query head h reads key/value head h / (Hq / Hk).
 //
-// A block takes 128 * QG rows of one key/value head and sequence (row = token *
-// G + head of the group: the group's heads share every key and value that the
-// block loads) and walks the keys in tiles through LDS, one pass, with the
-// running maximum and sum.
+// A block takes some rows of one key/value head and sequence (row = token * G +
+// head of the group: the group's heads share every key and value that the block
+// loads) and walks the keys in tiles through LDS, one pass, with the running
+// maximum and sum.  Three kernels: prompt_pipe_kernel (bf16, heads up to 128, many
+// rows), the one of wave_attention.hpp (few rows), prompt_kernel (the others).
 #include <math.h>
 
 #include <algorithm>
@@ -78,20 +79,29 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
   const TileLane<RB, BF16> at(lane);
   uint32_t bad = 0;
 
+  // The next tile's pieces wait in registers while one is computed.
+  constexpr int PER = KB * C::PIECES / 256;
+  u32x4 kv[PER], vv[PER];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = threadIdx.x + 256 * j, row = i / C::PIECES, c = i % C::PIECES;
+      const bool in = k0 + row < nkeys && c < npieces;
+      kv[j] = in ? *reinterpret_cast<const u32x4*>(kbase + (int64_t)(k0 + row) * p.k_t * ES + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+      vv[j] = in ? *reinterpret_cast<const u32x4*>(vbase + (int64_t)(k0 + row) * p.v_t * ES + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  fetch(0);
   for (int k0 = 0; k0 < nkeys; k0 += KB) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < KB * C::PIECES / 256; ++j) {
+    for (int j = 0; j < PER; ++j) {
       const int i = threadIdx.x + 256 * j, row = i / C::PIECES, c = i % C::PIECES;
-      u32x4 kv = {0u, 0u, 0u, 0u}, vv = {0u, 0u, 0u, 0u};
-      if (k0 + row < nkeys && c < npieces) {
-        kv = *reinterpret_cast<const u32x4*>(kbase + (int64_t)(k0 + row) * p.k_t * ES + 16 * c);
-        vv = *reinterpret_cast<const u32x4*>(vbase + (int64_t)(k0 + row) * p.v_t * ES + 16 * c);
-      }
-      *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(lk + row * RB + ((c ^ k_swz<RB>(row)) << 4)) = kv;
-      *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(lv + row * RB + ((c ^ v_swz<RB, BF16>(row)) << 4)) = vv;
+      *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(lk + row * RB + ((c ^ k_swz<RB>(row)) << 4)) = kv[j];
+      *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(lv + row * RB + ((c ^ v_swz<RB, BF16>(row)) << 4)) = vv[j];
     }
     __syncthreads();
+    if (k0 + KB < nkeys) fetch(k0 + KB);
     const bool masked = p.causal && k0 + KB - 1 > tok_first;  // not every row sees every key
     const bool edge = masked || k0 + KB > nkeys;
 #pragma unroll
@@ -678,22 +688,25 @@ hipError_t run_wave(const PromptParams& p, hipStream_t st) {
 
 }  // namespace
 
-hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, hipStream_t st) {
+hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, int cus, hipStream_t st) {
   if (p.T <= 0) return hipSuccess;
-  const int64_t rows = (int64_t)p.T * p.Hq;
+  const int64_t rows = (int64_t)p.T * p.Hq, few = rows / 32;
   if (bf16 && p.D <= 128) {
-    // 256-row blocks where they give half the CUs work, else 64-row ones that
-    // share the keys among their waves.
-    if (rows >= 128 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
-    return p.D <= 64 ? run_wave<true, 64, 2, 4>(p, st) : run_wave<true, 128, 2, 4>(p, st);
+    // 256-row blocks where they give almost half the CUs work (32 heads of 128,
+    // 768 / 1000 tokens: 29 / 35 us, 29 / 37 in 64-row blocks that share the
+    // keys among their waves, 512 tokens 22 / 18).  Below, 64 rows a block, or 32
+    // while a round of blocks holds them all (256 tokens: 14.0 / 9.4 us, 512 of
+    // 24 heads 17.1 / 20.1); with heads of 64 two blocks share a CU.
+    if (rows >= (int64_t)cus * 7 / 16 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
+    if (p.D <= 64) return few <= 2 * cus ? run_wave<true, 64, 1, 4>(p, st) : run_wave<true, 64, 2, 4>(p, st);
+    return few <= cus ? run_wave<true, 128, 1, 4>(p, st) : run_wave<true, 128, 2, 4>(p, st);
   }
-  if (!bf16 && p.D <= 64) return run_wave<false, 64, 2, 4>(p, st);
-  if (rows < 128 * 256) {
-    if (bf16) return run_wave<true, 256, 1, 2>(p, st);
-    return p.D <= 128 ? run_wave<false, 128, 1, 2>(p, st) : run_wave<false, 256, 1, 1>(p, st);
-  }
-  if (bf16) return run<true, 256, 1>(p, st);
-  return p.D <= 128 ? run<false, 128, 1>(p, st) : run<false, 256, 1>(p, st);
+  // fp32: its products take so long that 32 rows a block pay up to two rounds
+  // (16 heads of 64, 1001 / 2001 tokens: 35 / 108 us, in 64-row blocks 46 / 94).
+  if (!bf16 && p.D <= 64) return few <= 2 * cus ? run_wave<false, 64, 1, 4>(p, st) : run_wave<false, 64, 2, 4>(p, st);
+  // 32 heads of 128, 500 / 1000 tokens: 62 / 201 us, in 128-row blocks 81 / 163.
+  if (!bf16 && p.D <= 128) return rows < (int64_t)cus * 80 ? run_wave<false, 128, 1, 2>(p, st) : run<false, 128, 1>(p, st);
+  return bf16 ? run<true, 256, 1>(p, st) : run<false, 256, 1>(p, st);
 }
 
 }  // namespace svdmlp
