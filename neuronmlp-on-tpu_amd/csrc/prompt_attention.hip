@@ -5,7 +5,8 @@
 // head of the group: the group's heads share every key and value that the block
 // loads) and walks the keys in tiles through LDS, one pass, with the running
 // maximum and sum.  Three kernels: prompt_pipe_kernel (bf16, heads up to 128, many
-// rows), the one of wave_attention.hpp (few rows), prompt_kernel (the others).
+// rows), the one of wave_attention.hpp (few rows, fp32), prompt_kernel (heads up
+// to 256).
 #include <math.h>
 
 #include <algorithm>
@@ -673,9 +674,12 @@ hipError_t run_pipe(const PromptParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
+// One tile in LDS a wave, so that two blocks share a CU and hide each other's
+// loads, starts and ends: with two tiles and one block a CU 512 tokens of 32
+// heads took 18 us instead of 13; 64-row blocks of two tiles 18 too.
 template <bool BF16, int DP, int QG, int NW>
 hipError_t run_wave(const PromptParams& p, hipStream_t st) {
-  using C = CacheCfg<BF16, DP, QG, NW, true>;
+  using C = CacheCfg<BF16, DP, QG, NW, true, 1>;
   CacheParams w = {};
   w.q = p.q, w.kc = p.k, w.vc = p.v, w.out = p.out, w.cu = p.cu;
   w.q_t = p.q_t, w.q_h = p.q_h, w.k_t = p.k_t, w.k_h = p.k_h, w.v_t = p.v_t, w.v_h = p.v_h, w.o_t = p.o_t, w.o_h = p.o_h;
@@ -690,22 +694,15 @@ hipError_t run_wave(const PromptParams& p, hipStream_t st) {
 
 hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, int cus, hipStream_t st) {
   if (p.T <= 0) return hipSuccess;
-  const int64_t rows = (int64_t)p.T * p.Hq, few = rows / 32;
-  if (bf16 && p.D <= 128) {
-    // 256-row blocks where they give almost half the CUs work (32 heads of 128,
-    // 768 / 1000 tokens: 29 / 35 us, 29 / 37 in 64-row blocks that share the
-    // keys among their waves, 512 tokens 22 / 18).  Below, 64 rows a block, or 32
-    // while a round of blocks holds them all (256 tokens: 14.0 / 9.4 us, 512 of
-    // 24 heads 17.1 / 20.1); with heads of 64 two blocks share a CU.
-    if (rows >= (int64_t)cus * 7 / 16 * 256) return p.D <= 64 ? run_pipe<64>(p, st) : run_pipe<128>(p, st);
-    if (p.D <= 64) return few <= 2 * cus ? run_wave<true, 64, 1, 4>(p, st) : run_wave<true, 64, 2, 4>(p, st);
-    return few <= cus ? run_wave<true, 128, 1, 4>(p, st) : run_wave<true, 128, 2, 4>(p, st);
-  }
-  // fp32: its products take so long that 32 rows a block pay up to two rounds
-  // (16 heads of 64, 1001 / 2001 tokens: 35 / 108 us, in 64-row blocks 46 / 94).
-  if (!bf16 && p.D <= 64) return few <= 2 * cus ? run_wave<false, 64, 1, 4>(p, st) : run_wave<false, 64, 2, 4>(p, st);
-  // 32 heads of 128, 500 / 1000 tokens: 62 / 201 us, in 128-row blocks 81 / 163.
-  if (!bf16 && p.D <= 128) return rows < (int64_t)cus * 80 ? run_wave<false, 128, 1, 2>(p, st) : run<false, 128, 1>(p, st);
+  const int64_t rows = (int64_t)p.T * p.Hq;
+  // Many rows of bf16: 256-row blocks; else 32-row ones whose waves share the
+  // keys.  32 heads of 128, 1000 / 1300 / 2048 tokens: 34 / 42 / 61 us in the
+  // former, 32 / 44 / 77 in the latter (17 packed prompts of 8191 tokens 97 /
+  // 190); 16 heads of 64, 2048 / 4096 / 8192 tokens: 45 / 81 / 185, 24 / 66 / 238.
+  if (bf16 && p.D <= 64) return rows >= (int64_t)cus * 384 ? run_pipe<64>(p, st) : run_wave<true, 64, 1, 4>(p, st);
+  if (bf16 && p.D <= 128) return rows >= (int64_t)cus * 144 ? run_pipe<128>(p, st) : run_wave<true, 128, 1, 4>(p, st);
+  if (!bf16 && p.D <= 64) return run_wave<false, 64, 1, 4>(p, st);
+  if (!bf16 && p.D <= 128) return run_wave<false, 128, 1, 2>(p, st);
   return bf16 ? run<true, 256, 1>(p, st) : run<false, 256, 1>(p, st);
 }
 

@@ -19,7 +19,7 @@ constexpr int kSplitsMost = 64;   // chunks of a sequence
 constexpr int kJoin = 16;         // chunks' sums in flight when they are joined
 constexpr int kPagesMost = 1024;  // whole pages of a chunk: their numbers lie in LDS
 
-template <bool BF16_, int DP_, int QG_, int NW_, bool PROMPT_ = false>
+template <bool BF16_, int DP_, int QG_, int NW_, bool PROMPT_ = false, int STAGES_ = 2>
 struct CacheCfg {
   static constexpr bool PROMPT = PROMPT_;  // packed prompts in place of a paged cache
   static constexpr bool BF16 = BF16_;
@@ -29,12 +29,13 @@ struct CacheCfg {
   static constexpr int PIECES = RB / 16;
   static constexpr int STEPS = RB / 32;
   static constexpr int NW = NW_;  // waves a block
+  static constexpr int STAGES = STAGES_;  // tiles in LDS a wave: 1 where another block of the CU hides its loads
   static constexpr int TILE = 32 * RB;
   static constexpr int STAGE = 2 * TILE;  // keys, values
   static constexpr int ROWS = 32 * QG;
   static constexpr int RPI = 64 / PIECES;        // rows a load
   static constexpr int LOADS = 32 / RPI;         // loads a tile, of keys and of values
-  static_assert(2 * STAGE >= ROWS * DP * 4, "a wave's sums fit its stages");
+  static_assert(STAGES * STAGE >= ROWS * DP * 4, "a wave's sums fit its stages");
 };
 
 // 16 bytes of zeros that lanes without a key load.
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   constexpr bool BF16 = C::BF16;
   constexpr bool PROMPT = C::PROMPT;
   constexpr int ES = C::ES, RB = C::RB, QG = C::QG, DB = C::DP / 32, NW = C::NW;
-  __shared__ __attribute__((aligned(1024))) char lds[NW * 2 * C::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds[NW * C::STAGES * C::STAGE];
   __shared__ float stats[NW][C::ROWS][2];
   __shared__ int ids[PROMPT ? 1 : kPagesMost + 2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 
-  const attn_lds mine = (attn_lds)lds + wave * 2 * C::STAGE;
+  const attn_lds mine = (attn_lds)lds + wave * C::STAGES * C::STAGE;
   const char* const kb = static_cast<const char*>(p.kc) + ((int64_t)start * p.k_t + (int64_t)hk * p.k_h) * ES;
   const char* const vb = static_cast<const char*>(p.vc) + ((int64_t)start * p.v_t + (int64_t)hk * p.v_h) * ES;
   // Key `key - context` of the tokens that not all see: whether row group g's lane does.
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     return false;
   };
   if (p.D < C::DP)  // pieces behind the head's end: never loaded, zeros
-    for (int i = lane; i < 2 * C::STAGE / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+    for (int i = lane; i < C::STAGES * C::STAGE / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
 
   // One tile: S = K Q^T, the weights, O += V^T P^T.  Pieces are read from LDS
   // kAhead products before they are needed, the first of V behind the weights
@@ -354,12 +355,15 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   };
 
   int ku = kbeg + 32 * wave;
-  attn_lds cur = mine, nxt = mine + C::STAGE;
+  attn_lds cur = mine, nxt = mine + (C::STAGES - 1) * C::STAGE;
   bool whole = false;
-  if (ku < kend) whole = issue(ku, cur);
+  if (C::STAGES > 1 && ku < kend) whole = issue(ku, cur);
   for (; ku < kend; ku += 32 * NW) {
     bool next_whole = false;
-    if (ku + 32 * NW < kend) {
+    if constexpr (C::STAGES == 1) {
+      whole = issue(ku, cur);
+      wait_loads<0>();
+    } else if (ku + 32 * NW < kend) {
       next_whole = issue(ku + 32 * NW, nxt);
       wait_loads<(2 * C::LOADS < 63 ? 2 * C::LOADS : 63)>();
     } else {
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     for (int w = 0; w < NW; ++w) {
       const float mw = stats[w][rr][0];
       l += mw == -INFINITY ? stats[w][rr][1] : stats[w][rr][1] * exp2f(mw - m);
-      v += *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>((attn_lds)lds + w * 2 * C::STAGE + (rr * OP + (piece ^ (rr & OM))) * 16);
+      v += *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>((attn_lds)lds + w * C::STAGES * C::STAGE + (rr * OP + (piece ^ (rr & OM))) * 16);
     }
     const int t = r / G, h = hk * G + r - t * G;
     if (PROMPT || used == 1) {
@@ -524,7 +528,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   };
   if (parts > 1) {  // one item a thread
     SVDMLP_ATTN_LDS f32x4* const others = (SVDMLP_ATTN_LDS f32x4*)((attn_lds)lds + C::ROWS * kSplitsMost * 4);
-    static_assert(C::ROWS * kSplitsMost * 4 + NT * 16 <= NW * 2 * C::STAGE, "weights and the parts' sums fit the stages");
+    static_assert(C::ROWS * kSplitsMost * 4 + NT * 16 <= NW * C::STAGES * C::STAGE || PROMPT, "weights and the parts' sums fit the stages");
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (item < items) v = gather(item, true);
     others[threadIdx.x] = v;
