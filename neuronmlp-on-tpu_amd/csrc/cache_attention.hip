@@ -23,7 +23,11 @@ namespace {
 
 template <bool BF16, int DP, int QG, int NW>
 hipError_t run(const CacheParams& p, hipStream_t st) {
-  using C = CacheCfg<BF16, DP, QG, NW>;
+  // One tile in LDS a wave where its sums fit it: twice as many waves a CU, whose
+  // loads and products overlap (64 sequences 127 -> 121 us; one sequence, whose
+  // 264 blocks then run in one round, 18 -> 14).
+  constexpr int RB = DP * (BF16 ? 2 : 4);
+  using C = CacheCfg<BF16, DP, QG, NW, false, QG == 1 && RB >= 256 ? 1 : 2>;
   const int64_t rtiles = ((int64_t)p.n * (p.Hq / p.Hk) + C::ROWS - 1) / C::ROWS;
   const int64_t blocks = rtiles * p.Hk * p.B * p.splits;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
@@ -47,14 +51,14 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   const int64_t rows = (int64_t)n * (Hq / Hk), rt = 32 * row_groups(n, Hq, Hk, D, bf16);
   plan.rtiles = (int)((rows + rt - 1) / rt);
   const int64_t base = (int64_t)B * Hk * plan.rtiles;
-  const int waves = D * (bf16 ? 2 : 4) <= 256 ? 4 : D * (bf16 ? 2 : 4) <= 512 ? 2 : 1;  // that a CU's LDS holds
-  // One wave a block, of chunks of 512 keys, where those give every wave of the
-  // card one.  Else, and where a wave has 64 rows (whose partial sums, written
-  // and read, would be an eighth of such a chunk's keys and values), a block of
-  // all the waves a CU holds, of chunks that give every CU one; or three, of
-  // different lengths, if the chunks stay long.
-  constexpr int64_t kSolo = 512;
-  plan.waves = rt == 32 && base * ((capacity + kSolo - 1) / kSolo) >= (int64_t)waves * cus ? 1 : waves;
+  const int row = D * (bf16 ? 2 : 4), waves = row <= 256 ? 4 : row <= 512 ? 2 : 1;  // of a block that shares a chunk
+  // One wave a block, of chunks of 256 keys, where those give every SIMD one.
+  // Else, and where a wave has 64 rows (whose partial sums, written and read,
+  // would be a quarter of such a chunk's keys and values), blocks that share a
+  // chunk, of chunks that give every CU one; or three, of different lengths, if
+  // the chunks stay long.
+  constexpr int64_t kSolo = 256;
+  plan.waves = rt == 32 && base * ((capacity + kSolo - 1) / kSolo) >= 4 * (int64_t)cus ? 1 : waves;
   int64_t c = kSolo;
   if (plan.waves > 1 || waves == 1) c = std::max(capacity * base / cus / 3, std::min<int64_t>(1024, capacity * base / cus));
   c = std::max<int64_t>(c, (capacity + kSplitsMost - 1) / kSplitsMost);
