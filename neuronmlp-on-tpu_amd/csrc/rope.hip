@@ -88,11 +88,16 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
   const int turned = VEC ? (p.interleaved ? p.rot / E : half / E) : half;
   const int units = turned + (VEC ? (p.D - p.rot) / E : p.D - p.rot);
   const int total = heads * units;
+  // i / d as a product with d's reciprocal, exact below 2^16 (a head's units
+  // and a block's are that few for all but giant calls)
+  const bool small = TOK * total < 65536;
+  const uint32_t mtotal = small ? 0xffffffffu / (uint32_t)total + 1 : 0, munits = small ? 0xffffffffu / (uint32_t)units + 1 : 0;
+  auto quotient = [&](int i, int d, uint32_t m) -> int { return d == 1 ? i : small ? (int)__umulhi((uint32_t)i, m) : i / d; };
   for (int i = threadIdx.x; i < TOK * total; i += 256) {
-    const int tt = i / total, rest = i - tt * total;
+    const int tt = TOK == 1 ? 0 : quotient(i, total, mtotal), rest = i - tt * total;
     const int64_t t = t0 + tt;
     if (t >= p.T) break;
-    const int hh = rest / units, u = rest - hh * units;
+    const int hh = quotient(rest, units, munits), u = rest - hh * units;
     const char* src;
     char* dst;
     bool plain = false;
@@ -176,9 +181,9 @@ hipError_t launch_rope(const RopeParams& p, bool bf16, bool vec, hipStream_t st)
   if (p.T <= 0) return hipSuccess;
   auto go = [&](auto b, auto v) {
     constexpr bool B = decltype(b)::value, V = decltype(v)::value;
-    // One token a block while that leaves CUs idle, else four: their cosines
-    // keep all 256 threads busy at 128 turned values.
-    if (p.T < 1024)
+    // One token a block while eight a CU do not fill the card, else four: their
+    // cosines keep all 256 threads busy at 128 turned values.
+    if (p.T < 4096)
       hipLaunchKernelGGL((rope_kernel<B, V, 1>), dim3((unsigned)p.T), dim3(256), p.rot * 4, st, p);
     else
       hipLaunchKernelGGL((rope_kernel<B, V, 4>), dim3((unsigned)((p.T + 3) / 4)), dim3(256), 4 * p.rot * 4, st, p);
