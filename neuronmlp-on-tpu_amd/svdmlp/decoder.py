@@ -303,27 +303,36 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interl
         _refuse_device("rope_append", q, k_cache, v_cache)
     if torch.is_grad_enabled():
         _refuse_grad("rope_append", k_cache, v_cache)
-    _writable("k_cache", k_cache, cs, q)
-    _writable("v_cache", v_cache, cs, q)
-    kb, vb = k_cache.untyped_storage().data_ptr(), v_cache.untyped_storage().data_ptr()
-    inputs = {t.untyped_storage().data_ptr() for t in (q, k, v)}
-    if kb == vb or kb in inputs or vb in inputs:  # of one storage: perhaps of the same memory
-        _apart("k_cache", k_cache, v_cache, q, k, v)
-        _apart("v_cache", v_cache, q, k, v)
+    if not k_cache.is_contiguous():
+        _writable("k_cache", k_cache, cs, q)
+    if not v_cache.is_contiguous():
+        _writable("v_cache", v_cache, cs, q)
     slots = _index("slots", slots, (T,), torch.int64, index)
-    if out is None:
-        out = q.new_empty((T, Hq, D))
-    else:
+    if out is not None:
         _writable("out", out, (T, Hq, D), q)
         _apart("out", out, q, k, v, k_cache, v_cache, own=(q,))
     if T == 0:
-        return out
+        return q.new_empty((0, Hq, D)) if out is None else out
     q, k, v = _last(q), _last(k), _last(v)
-    st = _Strides14(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3],
-                    *v_cache.stride()[:3])
-    _launch(index, _lib.load().svdmlp_rope_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
-            inv_freq.data_ptr(), slots.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _address(st), T,
-            cs[0], cs[1], Hq, Hk, D, rot, scale, _ACT_CODES[q.dtype], 1 if interleaved else 0)
+    a, b, c, kc, vc = q.stride(), k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    qp, kp, vp, kcp, vcp = q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    # The caches apart from each other and the inputs: by their first and last
+    # bytes, exactly where those meet.
+    es, n0, n1, n2 = 2 if q.dtype is _BF16 else 4, cs[0] - 1, cs[1] - 1, Hk - 1
+    kce, vce = kcp + es * (n0 * kc[0] + n1 * kc[1] + n2 * kc[2] + D), vcp + es * (n0 * vc[0] + n1 * vc[1] + n2 * vc[2] + D)
+    low = min(qp, kp, vp)
+    high = max(qp + es * (a[0] * (T - 1) + a[1] * (Hq - 1) + D), kp + es * (b[0] * (T - 1) + b[1] * n2 + D),
+               vp + es * (c[0] * (T - 1) + c[1] * n2 + D))
+    if (kcp < vce and vcp < kce) or (low < kce and kcp < high) or (low < vce and vcp < high):
+        _apart("k_cache", k_cache, v_cache, q, k, v)
+        _apart("v_cache", v_cache, q, k, v)
+    if out is None:
+        out = q.new_empty((T, Hq, D))
+    o = out.stride()
+    st = _Strides14(a[0], a[1], b[0], b[1], c[0], c[1], o[0], o[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2])
+    _launch(index, _lib.load().svdmlp_rope_append, qp, kp, vp, positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(),
+            out.data_ptr(), kcp, vcp, _address(st), T, cs[0], cs[1], Hq, Hk, D, rot, scale, _ACT_CODES[q.dtype],
+            1 if interleaved else 0)
     return out
 
 
@@ -537,7 +546,8 @@ def residual_norm(x, branch, weight, *, post_weight=None, gate=None, scale: floa
     index = x.get_device()
     if index < 0 or (branch is not None and branch.get_device() != index) or (gate is not None and gate.get_device() != index):
         _refuse_device("residual_norm", x, branch, gate)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (x.requires_grad or (branch is not None and branch.requires_grad) or gate is not None
+                                    or post_weight is not None or (weight is not None and weight.requires_grad)):
         _refuse_grad("residual_norm", x, branch, gate, weight, post_weight)
     if branch is not None and branch.shape != shape:
         raise ValueError(f"branch must have x's shape {tuple(shape)}, got {tuple(branch.shape)}")

@@ -774,3 +774,17 @@ def test_decoder_layer_prefill_and_decode(gpu):
 def test_entry_points_are_exported():
     for name in ("rope", "rope_append", "prompt_attention", "cache_attention", "residual_norm", "rope_frequencies"):
         assert getattr(svdmlp, name) is getattr(decoder, name)
+
+
+def test_rope_append_refuses_shared_memory(gpu):
+    """Caches that are each other, or that hold the inputs; halves of one pool, and inputs beside a cache in one buffer, are fine."""
+    pos, f = torch.arange(4, device=gpu), torch.ones(4, dtype=torch.float64, device=gpu)
+    pool = torch.zeros(8, 2, 16, 1, 8, device=gpu)
+    q, k = torch.randn(4, 2, 8, device=gpu), torch.randn(4, 1, 8, device=gpu)
+    svdmlp.rope_append(q, k, k, pos, f, pool[:, 0], pool[:, 1], pos)
+    assert torch.equal(pool[0, 1, :4], k)
+    for kc, vc, kk in ((pool[:, 0], pool[:, 0], k), (pool[:4, 0], pool[2:6, 0], k), (pool[:, 0], pool[:, 1], pool[0, 0, :4])):
+        with pytest.raises(ValueError, match="overlap"):
+            svdmlp.rope_append(q, kk, k, pos, f, kc, vc, pos)
+    with pytest.raises(ValueError, match="overlap"):
+        svdmlp.rope_append(q, k, k, pos, f, pool[:, 0], pool[:, 1], pos, out=pool.view(-1)[:64].view(4, 2, 8))
