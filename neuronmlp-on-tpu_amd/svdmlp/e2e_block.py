@@ -13,8 +13,13 @@ X ~ 0.02 N(0, 1)).  The arms differ only in how the SVD MLP runs:
   ``nki_matmul_fully_optimized_`` arm, on the vendor library);
 * ``dense_block`` (``--dense-arm``, not in the reference's report): the
   dense SwiGLU (``compat.nki_baseline``) on weights rebuilt as U.V.
+* ``decoder_block`` and ``decoder_step`` (``--decoder-arm``, not in the
+  reference's report): the layers as a served model runs them, causal and with
+  rotary positions, all but the projections in the library's kernels
+  (:mod:`svdmlp.decoder`): a prompt of S tokens that fills a paged cache, and
+  one more token onto it.
 
-Attention is the same in all arms and is not the subject of the comparison:
+Attention is the same in the other arms and is not the subject of the comparison:
 torch's scaled_dot_product_attention, restricted to its flash and
 memory-efficient kernels (non-causal, as ``jax.nn.dot_product_attention`` is
 called at bench/e2e_block.py:222), with the KV heads repeated per group.
@@ -158,6 +163,71 @@ def dense_block(x, w, dense, num_heads: int, num_kv_heads: int):
     return x + compat.nki_baseline(rmsnorm(x, w["norm2_w"]), *dense)
 
 
+class DecoderModel:
+    """The layers of ``weights`` as a served model runs them, on the library's
+    kernels: q, k, v from one product, rotary positions, a paged cache a layer,
+    causal attention, the SVD MLP, and each residual sum with the norm after it.
+
+    ``prompt(x)`` runs one sequence and fills the caches; ``step(x, position)``
+    runs one token at ``position``, whose keys and values go into the caches, onto
+    what they hold before it.  ``capacity``: tokens the caches can hold."""
+
+    PAGE = 64
+
+    def __init__(self, weights, num_heads: int, num_kv_heads: int, capacity: int, theta: float = 500000.0, workspace=None):
+        import torch
+
+        from . import decoder
+
+        self.weights, self.workspace = weights, workspace
+        self.heads = (num_heads, num_kv_heads, num_kv_heads)
+        H, like = weights[0]["wq"].shape[0], weights[0]["wq"]
+        self.head_dim = H // num_heads
+        pages = -(-capacity // self.PAGE)
+        self.qkv = [torch.cat([w["wq"], w["wk"], w["wv"]], dim=1) for w in weights]
+        self.gains = [(w["norm1_w"].float(), w["norm2_w"].float()) for w in weights]
+        self.caches = [like.new_zeros((2, pages, self.PAGE, num_kv_heads, self.head_dim)) for _ in weights]
+        # one sequence: its pages lie in order, so a prompt's keys are the cache's first rows
+        self.table = torch.arange(pages, dtype=torch.int32, device=like.device)[None]
+        self.places = torch.arange(pages * self.PAGE, device=like.device)
+        self.lengths = torch.arange(pages * self.PAGE + 1, dtype=torch.int32, device=like.device)
+        self.inv_freq, self.rope_scale = decoder.rope_frequencies(self.head_dim, theta, device=like.device)
+
+    def prompt(self, x):
+        from . import decoder
+
+        rows = x.shape[0]
+
+        def attend(q, cache):
+            k, v = cache.flatten(1, 2)[:, :rows]
+            return decoder.prompt_attention(q, k, v)
+
+        return self._layers(x, 0, attend)
+
+    def step(self, x, position: int):
+        from . import decoder
+
+        lengths = self.lengths[position + 1:position + 2]
+        return self._layers(x, position, lambda q, cache: decoder.cache_attention(q[None], cache[0], cache[1], self.table, lengths)[0])
+
+    def _layers(self, x, first: int, attend):
+        from . import decoder, ops
+
+        T = x.shape[0]
+        if first + T > self.places.shape[0]:
+            raise ValueError(f"positions up to {first + T - 1} of caches for {self.places.shape[0]} tokens")
+        at = self.places[first:first + T]
+        _, n = decoder.residual_norm(x, None, self.gains[0][0], eps=RMS_EPS)
+        for i, w in enumerate(self.weights):
+            q, k, v = (n @ self.qkv[i]).view(T, -1, self.head_dim).split(self.heads, dim=1)
+            cache = self.caches[i]
+            q = decoder.rope_append(q, k, v, at, self.inv_freq, cache[0], cache[1], at, scale=self.rope_scale)
+            x, n = decoder.residual_norm(x, attend(q, cache).reshape(T, -1) @ w["wo"], self.gains[i][1], eps=RMS_EPS)
+            y = ops.svd_mlp(n, w["ug"], w["vg"], w["uu"], w["vu"], w["ud"], w["vd"], workspace=self.workspace)
+            x, n = decoder.residual_norm(x, y, self.gains[i + 1][0] if i + 1 < len(self.weights) else None, eps=RMS_EPS)
+        return x
+
+
 def _stats(samples) -> dict:
     """The latency keys of bench/e2e_block.py:281-302."""
     samples = sorted(samples)
@@ -245,6 +315,13 @@ def bench_model(S: int, cfg: dict, args) -> dict:
         rec["dense_block"] = _time_model(torch, dense_model, x, args.warmup, args.repeats)
         rec["speedup_fused_vs_dense"] = rec["dense_block"]["latency_ms_avg"] / fused_stats["latency_ms_avg"]
         del dense
+    if getattr(args, "decoder_arm", False):
+        model = DecoderModel(weights, n_heads, kv_heads, S + 1, workspace=workspace)
+        want = model.prompt(x)[-1:].float()
+        got = model.step(x[-1:], S - 1).float()  # the last token again, by the other attention
+        rec["decoder_step_vs_block_relative_l2"] = float(torch.linalg.norm(got - want) / torch.clamp(torch.linalg.norm(want), min=1e-12))
+        rec["decoder_block"] = _time_model(torch, model.prompt, x, args.warmup, args.repeats)
+        rec["decoder_step"] = _time_model(torch, lambda x: model.step(x, S), x[:1].contiguous(), args.warmup, args.repeats)
     del weights
     return rec
 
@@ -263,6 +340,8 @@ def _parser() -> argparse.ArgumentParser:
     p.add_argument("--seed", type=int, default=42)
     p.add_argument("--output", type=str, default=None, help="Write full JSON report to this path")
     p.add_argument("--dense-arm", action="store_true", help="also time the dense SwiGLU block (weights rebuilt as U.V)")
+    p.add_argument("--decoder-arm", action="store_true",
+                   help="also time the causal decoder with rotary positions and a paged cache: a prompt, and one more token")
     return p
 
 

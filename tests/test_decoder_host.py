@@ -170,3 +170,10 @@ def test_rope_frequencies():
 def test_rope_frequencies_refusals(args):
     with pytest.raises(ValueError):
         svdmlp.rope_frequencies(**args)
+
+
+def test_e2e_parser_has_the_decoder_arm():
+    from svdmlp import e2e_block
+
+    assert e2e_block._parser().parse_args([]).decoder_arm is False
+    assert e2e_block._parser().parse_args(["--decoder-arm"]).decoder_arm is True

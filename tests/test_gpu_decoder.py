@@ -788,3 +788,95 @@ def test_rope_append_refuses_shared_memory(gpu):
             svdmlp.rope_append(q, kk, k, pos, f, kc, vc, pos)
     with pytest.raises(ValueError, match="overlap"):
         svdmlp.rope_append(q, k, k, pos, f, pool[:, 0], pool[:, 1], pos, out=pool.view(-1)[:64].view(4, 2, 8))
+
+
+def _cpu_decoder(x, weights, heads, kv_heads, theta):
+    """The decoder's layers in 64 bits: causal, rotary positions of halves, no rounding in between."""
+    x = x.double()
+    T, H = x.shape
+    D = H // heads
+    angle = torch.arange(T, dtype=torch.float64)[:, None] * theta ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))
+    cos, sin = angle.cos()[:, None], angle.sin()[:, None]
+
+    def norm(t, w):
+        return t / (t.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w
+
+    def turn(t):
+        a, b = t[..., :D // 2], t[..., D // 2:]
+        return torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+
+    for w in weights:
+        w = {k: v.double().cpu() for k, v in w.items()}
+        n = norm(x, w["norm1_w"])
+        q, k, v = (turn((n @ w["wq"]).view(T, heads, D)), turn((n @ w["wk"]).view(T, kv_heads, D)), (n @ w["wv"]).view(T, kv_heads, D))
+        k, v = k.repeat_interleave(heads // kv_heads, 1), v.repeat_interleave(heads // kv_heads, 1)
+        s = torch.einsum("thd,uhd->htu", q, k) / math.sqrt(D)
+        s = s.masked_fill(torch.ones(T, T).triu(1).bool(), -math.inf).softmax(-1)
+        x = x + torch.einsum("htu,uhd->thd", s, v).reshape(T, H) @ w["wo"]
+        n = norm(x, w["norm2_w"])
+        h = torch.nn.functional.silu(n @ w["ug"] @ w["vg"]) * (n @ w["uu"] @ w["vu"])
+        x = x + h @ w["ud"] @ w["vd"]
+    return x
+
+
+def test_decoder_model_prompt_and_steps(gpu):
+    """The served model's layers against the same in 64 bits: a prompt, then tokens one by one over a page's end.
+
+    Tolerance: per layer some 12 tensors are rounded to bf16 (half a step, at most 2^-8 of a value, 2^-9.8 rms), each of a
+    branch that is at most the sum's size, twice over in the worst case: 2 layers * 12 * 2^-9.8 < 0.03 if all errors
+    added up, 0.006 as independent ones; 0.02 lies between.
+    """
+    from svdmlp import e2e_block
+
+    H, I, R, heads, kv = 512, 1024, 256, 8, 2
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(5)
+    weights = [e2e_block.make_layer_weights(gen, gpu, H, I, R, heads, kv, torch.bfloat16) for _ in range(2)]
+    x = (torch.randn((70, H), generator=gen, device=gpu) * 0.02).to(torch.bfloat16)
+    want = _cpu_decoder(x.cpu(), weights, heads, kv, 500000.0)
+    model = e2e_block.DecoderModel(weights, heads, kv, 70)
+    got = [model.prompt(x[:61])] + [model.step(x[t:t + 1], t) for t in range(61, 70)]
+    for a, b in ((got[0], want[:61]), *((g, want[t:t + 1]) for t, g in zip(range(61, 70), got[1:]))):
+        a = a.double().cpu()
+        assert float((a - b).norm() / b.norm()) < 0.02
+    with pytest.raises(ValueError, match="positions"):
+        model.step(x[:1], 128)
+
+
+def test_decoder_step_captured(gpu):
+    """The served model's step as one graph, replayed after its caches and input changed."""
+    from svdmlp import e2e_block
+
+    gen = torch.Generator(device=gpu)
+    gen.manual_seed(6)
+    weights = [e2e_block.make_layer_weights(gen, gpu, 512, 1024, 256, 8, 2, torch.bfloat16) for _ in range(2)]
+    x = (torch.randn((40, 512), generator=gen, device=gpu) * 0.02).to(torch.bfloat16)
+    model = e2e_block.DecoderModel(weights, 8, 2, 64)
+    model.prompt(x[:39])
+    inp = x[39:].clone()
+    model.step(inp, 39)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = model.step(inp, 39)
+    for seed in range(3):
+        other = x.roll(seed + 1, 0)
+        model.prompt(other[:39])
+        inp.copy_(other[39:])
+        want = model.step(inp, 39).clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_e2e_record_of_the_decoder_arm(gpu):
+    import argparse
+
+    from svdmlp import e2e_block
+
+    args = argparse.Namespace(layers=2, model_path=None, compress_ratio=0.8, warmup=1, repeats=2, seed=3, dense_arm=False, decoder_arm=True)
+    rec = e2e_block.bench_model(64, dict(hidden=512, intermediate=1024, heads=8, kv_heads=2, layers=2), args)
+    assert rec["decoder_step_vs_block_relative_l2"] < 0.02  # as above
+    for arm in ("decoder_block", "decoder_step"):
+        assert rec[arm]["iterations"] == 2 and 0 < rec[arm]["latency_ms_min"] <= rec[arm]["latency_ms_max"]
