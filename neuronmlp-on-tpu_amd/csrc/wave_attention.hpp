@@ -354,14 +354,18 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     __builtin_amdgcn_sched_barrier(0);
   };
 
+  // Whole tiles that every row sees, up to the first that is not; then the
+  // others, masked.  Two loops: in one, the sums of 64 rows were copied between
+  // the files of registers for each tile (380 moves).
   int ku = kbeg + 32 * wave;
   attn_lds cur = mine, nxt = mine + (C::STAGES - 1) * C::STAGE;
   bool whole = false;
   if (C::STAGES > 1 && ku < kend) whole = issue(ku, cur);
-  for (; ku < kend; ku += 32 * NW) {
+  // Loads of the tile at ku and, with two stages, the next one's; returns with the first there.
+  auto advance = [&]() -> bool {
     bool next_whole = false;
     if constexpr (C::STAGES == 1) {
-      whole = issue(ku, cur);
+      next_whole = issue(ku, cur);
       wait_loads<0>();
     } else if (ku + 32 * NW < kend) {
       next_whole = issue(ku + 32 * NW, nxt);
@@ -369,17 +373,28 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     } else {
       wait_loads<0>();
     }
-    int in;
-    if constexpr (RB < 1024) {
-      if (whole && ku + 31 < context) unit(std::false_type{}, cur, ku, 0xffffffffu);
-      else unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
-    } else {  // one copy of the code: two do not fit the registers
-      unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
-    }
-    whole = next_whole;
-    const attn_lds swap = cur;
+    return next_whole;
+  };
+  auto swap = [&] {
+    const attn_lds t = cur;
     cur = nxt;
-    nxt = swap;
+    nxt = t;
+  };
+  if constexpr (RB < 1024)  // (else two copies of a tile's code do not fit the registers)
+    for (; ku + 31 < context && ku + 31 < kend; ku += 32 * NW) {
+      if (C::STAGES > 1 && !whole) break;
+      const bool next_whole = advance();
+      if (C::STAGES == 1 && !next_whole) break;  // loaded again below
+      unit(std::false_type{}, cur, ku, 0xffffffffu);
+      whole = next_whole;
+      swap();
+    }
+  const int masked_from = ku;
+  for (; ku < kend; ku += 32 * NW) {
+    advance();
+    int in;
+    unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
+    swap();
   }
 
   // Each wave's sums, scaled to the block's maximum, in its own LDS; then all
@@ -415,15 +430,20 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   // Infinities and NaN among the values of the masked tiles were taken as
   // zeros, for the rows that do not see them; the rows that do get them here.
   if (__any(bad != 0)) {
-    for (int kt = kbeg + 32 * wave; kt < kend; kt += 32 * NW) {
-      if (RB < 1024 && kt + 31 < context) continue;  // (rows of 1 KB: every tile was taken as masked)
+    for (int kt = masked_from; kt < kend; kt += 32 * NW)
       for (int key = kt; key < min(kt + 32, kend); ++key) {
         int in;
         const int pg = place(key, 0, &in);
         if (pg < 0) continue;
         const char* const vp = vb + ((int64_t)pg * v_p + (int64_t)in * p.v_t) * ES;
+        auto value = [&](int e) -> uint32_t {
+          return BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(vp)[e] << 16 : reinterpret_cast<const uint32_t*>(vp)[e];
+        };
+        bool any = false;
+        for (int e = lane; e < p.D; e += 64) any |= not_finite<false>(value(e));
+        if (!__any(any)) continue;
         for (int e = 0; e < p.D; ++e) {
-          const uint32_t w = BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(vp)[e] << 16 : reinterpret_cast<const uint32_t*>(vp)[e];
+          const uint32_t w = value(e);
           if (not_finite<false>(w) && half == 0)
 #pragma unroll
             for (int g = 0; g < QG; ++g)
@@ -434,7 +454,6 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
               }
         }
       }
-    }
   }
   __syncthreads();
   const __amdgpu_buffer_rsrc_t sums = part_of(p, b, PROMPT ? 0 : p.D), ml = part_of(p, b, PROMPT ? 0 : 2);

@@ -495,6 +495,25 @@ def test_cache_attention_context_values_reach_every_token(gpu, dtype, D, B):
     assert torch.isfinite(got.float()).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D,B,n", [(64, 1, 3), (128, 1, 3), (64, 1, 40), (128, 1, 40), (256, 1, 3), (128, 300, 3)])
+@pytest.mark.parametrize("page,lost", [(48, False), (16, True)])
+def test_cache_attention_context_values_of_any_page(gpu, dtype, D, B, n, page, lost):
+    """The same where tiles are not loaded whole: pages of no power of two, and a page outside the cache among the others."""
+    g = _gen(26)
+    H, K, most = 4, 2, 600
+    table, pages = _pages(g, [most] * B, page)
+    q, kc, vc = _randn(g, B, n, H, D, dtype=dtype), _randn(g, pages, page, K, D, dtype=dtype), _randn(g, pages, page, K, D, dtype=dtype)
+    for key, head, e, x in ((37, 0, 7, math.inf), (321, 1, 9, -math.inf), (400, 1, 3, math.nan)):
+        vc[table[0, key // page].item(), key % page, head, e] = x
+    if lost:
+        table[:, 10] = pages + 5
+    got = svdmlp.cache_attention(*(t.to(gpu) for t in (q, kc, vc, table)), torch.tensor([most] * B, device=gpu)).cpu()
+    assert (got[0, :, :H // K, 7] == math.inf).all() and (got[0, :, H // K:, 9] == -math.inf).all() and torch.isnan(got[0, :, H // K:, 3]).all()
+    got[0, :, :H // K, 7] = got[0, :, H // K:, 9] = got[0, :, H // K:, 3] = 0
+    assert torch.isfinite(got.float()).all()
+
+
 def test_cache_attention_broken_tables(gpu):
     """Pages outside the cache hold no keys, lengths beyond the table are cut, negative ones empty."""
     g = _gen(22)
