@@ -2669,8 +2669,8 @@ size_t svdmlp_cache_attention_workspace_bytes(int64_t B, int64_t n, int64_t page
     return 0;
   const CachePlan plan = plan_cache_attention((int)B, (int)n, (int)Hq, (int)Hk, (int)D, dtype == SVDMLP_BF16, (int)page,
                                               page * width, device_cus());
-  if (counters && plan.splits > 1) *counters = B * Hk * plan.rtiles;
-  return (size_t)cache_part_floats((int)B, (int)n, (int)Hq, (int)D, plan.splits) * 4;
+  if (counters) *counters = cache_counters(plan, (int)B, (int)Hk);
+  return (size_t)cache_part_floats(plan, (int)n, (int)Hq, (int)D) * 4;
 }
 
 int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -2703,18 +2703,18 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   p.B = (int)B, p.n = (int)n, p.Hq = (int)Hq, p.Hk = (int)Hk, p.D = (int)D;
   p.c = scale * 1.44269504088896340736f;
   const CachePlan plan = plan_cache_attention(p.B, p.n, p.Hq, p.Hk, p.D, dtype == SVDMLP_BF16, p.page, page * width, device_cus());
-  p.splits = plan.splits, p.chunk = plan.chunk;
-  const size_t need = (size_t)cache_part_floats(p.B, p.n, p.Hq, p.D, p.splits) * 4;
+  p.splits = plan.splits, p.chunk = plan.chunk, p.chunk_most = plan.chunk_most, p.chunks = plan.chunks, p.slots = plan.slots;
+  const size_t need = (size_t)cache_part_floats(plan, p.n, p.Hq, p.D) * 4;
   if ((int64_t)n * Hq * plan.splits * D * 4 > 0x7fffffff) return fail("cache_attention: too many rows");
   if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15u)))
     return fail("cache_attention: workspace too small: %zu bytes needed, 16-byte aligned, got %zu", need, ws_bytes);
-  const int64_t nc = B * Hk * plan.rtiles;
-  if (need && (!counters || n_counters < nc || ((uintptr_t)counters & 3u)))
+  const int64_t nc = cache_counters(plan, p.B, p.Hk);
+  if (nc && (!counters || n_counters < nc || ((uintptr_t)counters & 3u)))
     return fail("cache_attention: %lld counters needed, got %lld", (long long)nc, (long long)(counters ? n_counters : 0));
   p.part = static_cast<float*>(workspace);
   p.counters = counters;
   StageScope sc(ST_CACHE_ATTENTION, (hipStream_t)stream);
-  return check(launch_cache_attention(p, dtype == SVDMLP_BF16, plan.waves, (hipStream_t)stream), "cache_attention");
+  return check(launch_cache_attention(p, dtype == SVDMLP_BF16, plan, (hipStream_t)stream), "cache_attention");
 }
 
 int svdmlp_residual_norm(const void* x, const void* branch, const float* post_w, const void* gate,

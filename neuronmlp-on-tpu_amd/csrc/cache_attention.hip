@@ -21,34 +21,40 @@ namespace svdmlp {
 
 namespace {
 
-template <bool BF16, int DP, int QG, int NW>
+template <bool BF16, int DP, int QG, int NW, bool SHARE = false>
 hipError_t run(const CacheParams& p, hipStream_t st) {
   // One tile in LDS a wave where its sums fit it: twice as many waves a CU, whose
   // loads and products overlap (64 sequences 127 -> 121 us; one sequence, whose
   // 264 blocks then run in one round, 18 -> 14).
   constexpr int RB = DP * (BF16 ? 2 : 4);
-  using C = CacheCfg<BF16, DP, QG, NW, false, QG == 1 && RB >= 256 ? 1 : 2>;
+  using C = CacheCfg<BF16, DP, QG, NW, false, SHARE ? 65536 / (64 * RB) : QG == 1 && RB >= 256 ? 1 : 2, SHARE>;
   const int64_t rtiles = ((int64_t)p.n * (p.Hq / p.Hk) + C::ROWS - 1) / C::ROWS;
-  const int64_t blocks = rtiles * p.Hk * p.B * p.splits;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  const int64_t blocks = rtiles * p.Hk * p.chunks;
+  if (blocks > 0x7fffffff || (int64_t)p.B * p.n * p.Hq > 0x7fffffff) return hipErrorInvalidValue;
   CacheParams q = p;
   q.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (p.page == 1 << s && p.page >= C::RPI) q.page_shift = s;
   hipLaunchKernelGGL((cache_kernel<C>), dim3((unsigned)blocks), dim3(64 * NW), 0, st, q);
+  if (SHARE && p.splits > 1) {
+    const int64_t rows = (int64_t)p.B * p.n * p.Hq;
+    hipLaunchKernelGGL((cache_join_kernel<BF16>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, (int)rtiles);
+  }
   return hipGetLastError();
 }
 
-// 64 rows a wave where there are more than 32 and their sums fit the registers.
-int row_groups(int n, int Hq, int Hk, int D, bool bf16) {
-  return (int64_t)n * (Hq / Hk) > 32 && D <= (bf16 ? 128 : 64) ? 2 : 1;
+// Rows a block: 64 a wave where there are more than 32, and a tile shared by
+// four waves of 32 rows where there are more than 64, as far as their sums fit.
+int block_rows(int n, int Hq, int Hk, int D, bool bf16) {
+  const int64_t rows = (int64_t)n * (Hq / Hk);
+  return rows <= 32 || D > (bf16 ? 128 : 64) ? 32 : rows <= 64 ? 64 : 128;
 }
 
 }  // namespace
 
 CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, int page, int64_t capacity, int cus) {
   CachePlan plan;
-  const int64_t rows = (int64_t)n * (Hq / Hk), rt = 32 * row_groups(n, Hq, Hk, D, bf16);
+  const int64_t rows = (int64_t)n * (Hq / Hk), rt = block_rows(n, Hq, Hk, D, bf16);
   plan.rtiles = (int)((rows + rt - 1) / rt);
   const int64_t base = (int64_t)B * Hk * plan.rtiles;
   const int row = D * (bf16 ? 2 : 4), waves = row <= 256 ? 4 : row <= 512 ? 2 : 1;  // of a block that shares a chunk
@@ -61,17 +67,30 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   plan.waves = rt == 32 && base * ((capacity + kSolo - 1) / kSolo) >= 4 * (int64_t)cus ? 1 : waves;
   int64_t c = kSolo;
   if (plan.waves > 1 || waves == 1) c = std::max(capacity * base / cus / 3, std::min<int64_t>(1024, capacity * base / cus));
+  if (rt == 128) c = 512;  // at least: as many as the lengths ask for (shared_chunk)
   c = std::max<int64_t>(c, (capacity + kSplitsMost - 1) / kSplitsMost);
   c = std::max<int64_t>(128, (c + 127) / 128 * 128);
   c = std::min(c, (int64_t)kPagesMost * page / 128 * 128);
   plan.chunk = (int)std::min<int64_t>(c, 0x7fffff80);
   plan.splits = (int)((capacity + plan.chunk - 1) / plan.chunk);
+  plan.shared = rt == 128;
+  plan.slots = 2 * cus;
+  plan.chunk_most = (int)std::min((int64_t)kPagesMost * page, (int64_t)0x7fffff80);
+  plan.chunks = B * plan.splits;
+  if (plan.shared && plan.splits > 1) {  // at most total / chunk + B
+    const int64_t most = std::max(plan.slots / ((int64_t)Hk * plan.rtiles), (B * capacity + plan.chunk_most - 1) / plan.chunk_most);
+    plan.chunks = (int)std::min(B + most, (int64_t)plan.chunks);
+  }
   return plan;
 }
 
-hipError_t launch_cache_attention(const CacheParams& p, bool bf16, int waves, hipStream_t st) {
+hipError_t launch_cache_attention(const CacheParams& p, bool bf16, const CachePlan& plan, hipStream_t st) {
   if (p.B <= 0 || p.n <= 0) return hipSuccess;
-  const bool two = row_groups(p.n, p.Hq, p.Hk, p.D, bf16) == 2, one = waves == 1;
+  const bool two = block_rows(p.n, p.Hq, p.Hk, p.D, bf16) == 64, one = plan.waves == 1;
+  if (plan.shared) {
+    if (!bf16) return run<false, 64, 1, 4, true>(p, st);
+    return p.D <= 64 ? run<true, 64, 1, 4, true>(p, st) : run<true, 128, 1, 4, true>(p, st);
+  }
   if (bf16) {
     if (p.D <= 64) return two ? run<true, 64, 2, 4>(p, st) : (one ? run<true, 64, 1, 1>(p, st) : run<true, 64, 1, 4>(p, st));
     if (p.D <= 128) return two ? run<true, 128, 2, 4>(p, st) : (one ? run<true, 128, 1, 1>(p, st) : run<true, 128, 1, 4>(p, st));

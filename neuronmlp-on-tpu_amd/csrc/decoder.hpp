@@ -73,21 +73,30 @@ struct CacheParams {
   const int* cu;      // prompts only (wave_attention.hpp): their bounds, rows and mask; n, table, lengths unused
   int T, causal;
   int splits, chunk;  // keys are cut into chunks of `chunk` (a multiple of the key tile), one a block
+  int chunk_most, chunks;  // shared tiles: the kernel's choice lies in chunk .. chunk_most; chunks in all, at most
+  int slots;               // and the blocks that run at once
   float c;
 };
 // How a call is cut: `splits` chunks of `chunk` keys cover the table's
 // `capacity`, a block of `waves` waves each; rtiles row tiles a sequence and head.
 constexpr int64_t kTokenStrideMost = 1 << 23;  // a 64-row tile's byte offsets fit 31 bits, in both types
 constexpr int64_t kCachePagesMost = 65536;  // pages of a sequence: 64 chunks of 1024
+// Blocks of 128 rows (plan.shared) choose their chunk on the device, from the
+// lengths: `chunk` to chunk_most keys, `chunks` of them in all.
 struct CachePlan {
-  int splits, chunk, waves, rtiles;
+  int splits, chunk, waves, rtiles, chunk_most, chunks, slots;
+  bool shared;
 };
 CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, int page, int64_t capacity, int cus);
 // Floats of the partial sums: D sums, the maximum and the sum of weights of
-// every (sequence, token, head, split).
-inline int64_t cache_part_floats(int B, int n, int Hq, int D, int splits) {
-  return splits > 1 ? (int64_t)B * n * Hq * splits * (D + 2) : 0;
+// every (token, head) of every chunk.
+inline int64_t cache_part_floats(const CachePlan& plan, int n, int Hq, int D) {
+  return plan.splits > 1 ? (int64_t)plan.chunks * n * Hq * (D + 2) : 0;
 }
-hipError_t launch_cache_attention(const CacheParams& p, bool bf16, int waves, hipStream_t st);
+// Counters: one a (sequence, key/value head, row tile) whose last block joins the chunks.
+inline int64_t cache_counters(const CachePlan& plan, int B, int Hk) {
+  return plan.splits > 1 && !plan.shared ? (int64_t)B * Hk * plan.rtiles : 0;
+}
+hipError_t launch_cache_attention(const CacheParams& p, bool bf16, const CachePlan& plan, hipStream_t st);
 
 }  // namespace svdmlp

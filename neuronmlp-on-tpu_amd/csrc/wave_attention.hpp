@@ -19,7 +19,7 @@ constexpr int kSplitsMost = 64;   // chunks of a sequence
 constexpr int kJoin = 16;         // chunks' sums in flight when they are joined
 constexpr int kPagesMost = 1024;  // whole pages of a chunk: their numbers lie in LDS
 
-template <bool BF16_, int DP_, int QG_, int NW_, bool PROMPT_ = false, int STAGES_ = 2>
+template <bool BF16_, int DP_, int QG_, int NW_, bool PROMPT_ = false, int STAGES_ = 2, bool SHARE_ = false>
 struct CacheCfg {
   static constexpr bool PROMPT = PROMPT_;  // packed prompts in place of a paged cache
   static constexpr bool BF16 = BF16_;
@@ -32,10 +32,14 @@ struct CacheCfg {
   static constexpr int STAGES = STAGES_;  // tiles in LDS a wave: 1 where another block of the CU hides its loads
   static constexpr int TILE = 32 * RB;
   static constexpr int STAGE = 2 * TILE;  // keys, values
-  static constexpr int ROWS = 32 * QG;
+  static constexpr bool SHARE = SHARE_;  // every wave takes every tile, for 32 rows of its own; all load them
+  static constexpr int WROWS = 32 * QG, ROWS = SHARE ? NW * WROWS : WROWS;  // rows of a wave, of a block
   static constexpr int RPI = 64 / PIECES;        // rows a load
   static constexpr int LOADS = 32 / RPI;         // loads a tile, of keys and of values
-  static_assert(STAGES * STAGE >= ROWS * DP * 4, "a wave's sums fit its stages");
+  static constexpr int MINE = SHARE ? LOADS / NW : LOADS;  // of them a wave's
+  static constexpr int LDS = (SHARE ? 1 : NW) * STAGES * STAGE;
+  static_assert(LDS / NW >= WROWS * DP * 4, "a wave's sums fit its part of LDS");
+  static_assert(!SHARE || (LOADS % NW == 0 && STAGES > 2 && !PROMPT), "shared tiles");
 };
 
 // 16 bytes of zeros that lanes without a key load.
@@ -63,6 +67,21 @@ __device__ __forceinline__ int held(const CacheParams& p, int b) {
   return (int)min((int64_t)max(p.lengths[b], 0), cap);
 }
 
+// Keys of a chunk of blocks that share their tiles: as many chunks as blocks run
+// at once, over all sequences, heads and row tiles.  (From the table's width
+// instead, sequences of unequal lengths left half the card idle.)
+__device__ __forceinline__ int shared_chunk(const CacheParams& p, int rtiles, int lane) {
+  if (p.splits == 1) return p.chunk;
+  int64_t total = 0;
+  for (int b = lane; b < p.B; b += 64) total += held(p, b);
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+  const int64_t want = (total * p.Hk * rtiles / p.slots + 127) / 128 * 128;
+  return __builtin_amdgcn_readfirstlane((int)min(max(want, (int64_t)p.chunk), (int64_t)p.chunk_most));
+}
+__device__ __forceinline__ int chunks_of(int len, int chunk) {  // the first always answers
+  return max(1, (int)(((int64_t)len + chunk - 1) / chunk));
+}
+
 // Which of the 32 keys from `draft` keys after the context on a token sees,
 // whose row of the tree is `row`: all of the context.
 __device__ __forceinline__ uint32_t seen32(uint64_t row, int draft) {
@@ -81,16 +100,16 @@ __device__ __forceinline__ uint32_t upto32(int last, int ku) {
 template <class C>
 __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   constexpr bool BF16 = C::BF16;
-  constexpr bool PROMPT = C::PROMPT;
+  constexpr bool PROMPT = C::PROMPT, SHARE = C::SHARE;
   constexpr int ES = C::ES, RB = C::RB, QG = C::QG, DB = C::DP / 32, NW = C::NW;
-  __shared__ __attribute__((aligned(1024))) char lds[NW * C::STAGES * C::STAGE];
-  __shared__ float stats[NW][C::ROWS][2];
+  __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+  __shared__ float stats[NW][C::WROWS][2];
   __shared__ int ids[PROMPT ? 1 : kPagesMost + 2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
   const int G = p.Hq / p.Hk;
   // The block's rows (r0 .. of `rows`, sequence rows start ..), keys kbeg ..
   // kend, of which those before `context` are seen by every row.
-  int rows, rtiles = 1, rt = 0, hk, b = 0, split = 0, used = 1, r0, start = 0, kbeg = 0, kend, context, pg0 = 0;
+  int rows, rtiles = 1, rt = 0, hk, b = 0, split = 0, used = 1, r0, start = 0, kbeg = 0, kend, context, pg0 = 0, chunk = 0, at_chunk = 0;
   if constexpr (PROMPT) {
     RowTile where;
     if (!find_rows(p.cu, p.T, p.B, p.Hk, G, C::ROWS, lane, where)) return;
@@ -105,19 +124,45 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     id /= p.Hk;
     rt = id % rtiles;
     id /= rtiles;
-    b = id % p.B, split = id / p.B;
+    chunk = p.chunk;
+    if (SHARE && p.splits > 1) {
+      // Chunk `id` of all sequences' in order.
+      chunk = shared_chunk(p, rtiles, lane);
+      int left = id;
+      b = -1;
+      for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int n = b0 + lane < p.B ? chunks_of(held(p, b0 + lane), chunk) : 0;
+        int upto = n;
+        for (int o = 1; o < 64; o <<= 1) {
+          const int v = __shfl_up(upto, o);
+          if (lane >= o) upto += v;
+        }
+        const uint64_t hit = __ballot(left < upto);
+        if (hit) {
+          const int i = __builtin_ctzll(hit);
+          b = b0 + i, split = left - __builtin_amdgcn_readlane(upto - n, i);
+          break;
+        }
+        left -= __builtin_amdgcn_readlane(upto, 63);
+      }
+      if (b < 0) return;
+    } else {
+      b = id % p.B, split = id / p.B;
+    }
+    at_chunk = id;
     const int len = held(p, b);
     r0 = rt * C::ROWS;
-    kbeg = split * p.chunk, kend = min(len, kbeg + p.chunk);
-    used = max(1, (int)(((int64_t)len + p.chunk - 1) / p.chunk));  // chunks that hold keys; the first always answers
+    kbeg = split * chunk, kend = min(len, kbeg + chunk);
+    used = chunks_of(len, chunk);
     if (split >= used) return;
     context = len - p.n;
     // The chunk's pages.
     pg0 = kbeg / p.page;
-    const int npages = min(p.width - pg0, (int)min((int64_t)p.chunk + p.page - 1, (int64_t)kPagesMost * p.page) / p.page + 1);
+    const int npages = min(p.width - pg0, (int)min((int64_t)chunk + p.page - 1, (int64_t)kPagesMost * p.page) / p.page + 1);
     for (int i = threadIdx.x; i < npages; i += 64 * NW) ids[i] = p.table[(int64_t)b * p.table_b + pg0 + i];
   }
 
+  const int w0 = r0 + (SHARE ? wave * C::WROWS : 0);  // the wave's first row
   // Heads of over 128 elements leave no registers for Q: its pieces are read
   // again (from the caches) for every tile.
   constexpr bool QREG = C::DP < 256;
@@ -127,7 +172,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   const int npieces = p.D * ES / 16;
 #pragma unroll
   for (int g = 0; g < QG; ++g) {
-    const int r = min(r0 + 32 * g + col, rows - 1);  // rows behind the last repeat it, and are not stored
+    const int r = min(w0 + 32 * g + col, rows - 1);  // rows behind the last repeat it, and are not stored
     qi[g] = r / G;
     qptr[g] = static_cast<const char*>(p.q) + ((int64_t)b * p.q_b + (int64_t)(start + qi[g]) * p.q_t + (int64_t)(hk * G + r - qi[g] * G) * p.q_h) * ES;
     if constexpr (QREG)
@@ -144,7 +189,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   for (int g = 0; g < QG; ++g) row_sees[g] = (2ull << qi[g]) - 1;  // a chain (token 63: all)
   if (!PROMPT && p.tree && kend > context) {
     const uint8_t* const tree = p.tree + (int64_t)b * p.tree_b;
-    const int first = r0 / G, last = min(r0 + C::ROWS - 1, rows - 1) / G;
+    const int first = min(w0, rows - 1) / G, last = min(w0 + C::WROWS - 1, rows - 1) / G;
     for (int t = first; t <= last; ++t) {
       const uint64_t bits = __ballot(tree[(int64_t)t * p.tree_q + min(lane, p.n - 1)] != 0);
 #pragma unroll
@@ -165,7 +210,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 
-  const attn_lds mine = (attn_lds)lds + wave * C::STAGES * C::STAGE;
+  const attn_lds mine = (attn_lds)lds + wave * (C::LDS / NW);
   const char* const kb = static_cast<const char*>(p.kc) + ((int64_t)start * p.k_t + (int64_t)hk * p.k_h) * ES;
   const char* const vb = static_cast<const char*>(p.vc) + ((int64_t)start * p.v_t + (int64_t)hk * p.v_h) * ES;
   // Key `key - context` of the tokens that not all see: whether row group g's lane does.
@@ -201,6 +246,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   const uint32_t krow = (uint32_t)(lrow * (int)p.k_t * ES), vrow = (uint32_t)(lrow * (int)p.v_t * ES);
   const bool alike = p.page_shift >= 0 && p.k_p == p.v_p && p.k_t == p.v_t;
   // Loads of the tile at key ku; true: all 32 keys are there.
+  const int j0 = SHARE ? wave * C::MINE : 0;  // the first load of this wave
   auto issue = [&](int ku, attn_lds stage) -> bool {
     const uint32_t base = (uint32_t)(uintptr_t)stage;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
@@ -229,14 +275,16 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
         const int64_t off = ((int64_t)pg * p.k_p + (int64_t)in * p.k_t) * ES;
         if (p.D == C::DP) {
 #pragma unroll
-          for (int j = 0; j < C::LOADS; ++j) {
+          for (int i = 0; i < C::MINE; ++i) {
+            const int j = j0 + i;
             const int64_t at = lane64(off, j);
             load_lds16(kb + at, krow + 16 * (kpiece ^ k_swz<RB>(j * C::RPI)), base + j * 1024);
             load_lds16(vb + at, vrow + 16 * (vpiece ^ v_swz<RB, BF16>(j * C::RPI)), base + C::TILE + j * 1024);
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < C::LOADS; ++j) {
+          for (int i = 0; i < C::MINE; ++i) {
+            const int j = j0 + i;
             const int ck = kpiece ^ k_swz<RB>(j * C::RPI), cv = vpiece ^ v_swz<RB, BF16>(j * C::RPI);
             const int64_t at = lane64(off, j);
             if (ck < npieces) load_lds16(kb + at, krow + 16 * ck, base + j * 1024);
@@ -247,8 +295,8 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
       }
     }
 #pragma unroll 2
-    for (int j = 0; j < C::LOADS; ++j) {
-      const int row = j * C::RPI + lrow;
+    for (int i = 0; i < C::MINE; ++i) {
+      const int j = j0 + i, row = j * C::RPI + lrow;
       int in;
       const int pg = place(ku, row, &in);
       const int ck = lc ^ k_swz<RB>(row), cv = lc ^ v_swz<RB, BF16>(row);
@@ -261,8 +309,10 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     }
     return false;
   };
-  if (p.D < C::DP)  // pieces behind the head's end: never loaded, zeros
-    for (int i = lane; i < C::STAGES * C::STAGE / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+  if (p.D < C::DP) {  // pieces behind the head's end: never loaded, zeros
+    for (int i = lane; i < C::LDS / NW / 16; i += 64) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(mine + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+    if constexpr (SHARE) __syncthreads();
+  }
 
   // One tile: S = K Q^T, the weights, O += V^T P^T.  Pieces are read from LDS
   // kAhead products before they are needed, the first of V behind the weights
@@ -357,18 +407,42 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   // Whole tiles that every row sees, up to the first that is not; then the
   // others, masked.  Two loops: in one, the sums of 64 rows were copied between
   // the files of registers for each tile (380 moves).
-  int ku = kbeg + 32 * wave;
-  attn_lds cur = mine, nxt = mine + (C::STAGES - 1) * C::STAGE;
+  constexpr int STEP = SHARE ? 32 : 32 * NW;  // from a tile of the wave to its next
+  int ku = kbeg + (SHARE ? 0 : 32 * wave);
   bool whole = false;
-  if (C::STAGES > 1 && ku < kend) whole = issue(ku, cur);
-  // Loads of the tile at ku and, with two stages, the next one's; returns with the first there.
+  attn_lds cur = mine, nxt = mine + (C::STAGES - 1) * C::STAGE;
+  int issued = 0;       // SHARE: tiles whose loads are on their way or done,
+  uint32_t wholes = 0;  // and which of the last 32 are whole
+  auto issue_next = [&] {
+    const int at = kbeg + 32 * issued;
+    if (at >= kend) return;
+    const uint32_t bit = 1u << (issued & 31);
+    wholes = issue(at, (attn_lds)lds + issued % C::STAGES * C::STAGE) ? wholes | bit : wholes & ~bit;
+    ++issued;
+  };
+  if constexpr (SHARE) {
+    for (int i = 0; i < C::STAGES - 1; ++i) issue_next();
+    whole = wholes & 1;
+  } else if (C::STAGES > 1 && ku < kend) {
+    whole = issue(ku, cur);
+  }
+  // Loads of tiles ahead; returns with the one at ku there, as `cur`.  The value: whether the next is whole.
   auto advance = [&]() -> bool {
     bool next_whole = false;
-    if constexpr (C::STAGES == 1) {
+    if constexpr (SHARE) {
+      const int t = (ku - kbeg) / 32;
+      if (issued - t == C::STAGES - 1) wait_loads<(C::STAGES - 2) * 2 * C::MINE>();
+      else wait_loads<0>();
+      // Every wave's part of tile t is there, and every wave is done with tile t - 1, whose place is filled again.
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      issue_next();
+      cur = (attn_lds)lds + t % C::STAGES * C::STAGE;
+      next_whole = wholes >> ((t + 1) & 31) & 1;
+    } else if constexpr (C::STAGES == 1) {
       next_whole = issue(ku, cur);
       wait_loads<0>();
-    } else if (ku + 32 * NW < kend) {
-      next_whole = issue(ku + 32 * NW, nxt);
+    } else if (ku + STEP < kend) {
+      next_whole = issue(ku + STEP, nxt);
       wait_loads<(2 * C::LOADS < 63 ? 2 * C::LOADS : 63)>();
     } else {
       wait_loads<0>();
@@ -381,20 +455,20 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     nxt = t;
   };
   if constexpr (RB < 1024)  // (else two copies of a tile's code do not fit the registers)
-    for (; ku + 31 < context && ku + 31 < kend; ku += 32 * NW) {
+    for (; ku + 31 < context && ku + 31 < kend; ku += STEP) {
       if (C::STAGES > 1 && !whole) break;
       const bool next_whole = advance();
       if (C::STAGES == 1 && !next_whole) break;  // loaded again below
       unit(std::false_type{}, cur, ku, 0xffffffffu);
       whole = next_whole;
-      swap();
+      if constexpr (!SHARE) swap();
     }
   const int masked_from = ku;
-  for (; ku < kend; ku += 32 * NW) {
+  for (; ku < kend; ku += STEP) {
     advance();
     int in;
     unit(std::true_type{}, cur, ku, (uint32_t)__ballot(place(ku, col, &in) >= 0));
-    swap();
+    if constexpr (!SHARE) swap();
   }
 
   // Each wave's sums, scaled to the block's maximum, in its own LDS; then all
@@ -412,9 +486,10 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   __syncthreads();
 #pragma unroll
   for (int g = 0; g < QG; ++g) {
-    float m = -INFINITY;
+    float m = SHARE ? st[g].m : -INFINITY;
+    if constexpr (!SHARE)
 #pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][32 * g + col][0]);
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][32 * g + col][0]);
     const float a = st[g].m == -INFINITY ? 1.f : exp2f(st[g].m - m);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -430,7 +505,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   // Infinities and NaN among the values of the masked tiles were taken as
   // zeros, for the rows that do not see them; the rows that do get them here.
   if (__any(bad != 0)) {
-    for (int kt = masked_from; kt < kend; kt += 32 * NW)
+    for (int kt = masked_from; kt < kend; kt += STEP)
       for (int key = kt; key < min(kt + 32, kend); ++key) {
         int in;
         const int pg = place(key, 0, &in);
@@ -461,26 +536,38 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     const int rr = i / OP, piece = i % OP, r = r0 + rr;
     if (r >= rows || 4 * piece >= p.D) continue;
     float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][rr][0]);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    const int wr = rr % C::WROWS;  // the row in its wave, or in each
+    const attn_lds at = (attn_lds)lds + (wr * OP + (piece ^ (wr & OM))) * 16;
+    if constexpr (SHARE) {
+      const int w = rr / C::WROWS;
+      m = stats[w][wr][0], l = stats[w][wr][1];
+      v = *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>(at + w * (C::LDS / NW));
+    } else {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = stats[w][rr][0];
-      l += mw == -INFINITY ? stats[w][rr][1] : stats[w][rr][1] * exp2f(mw - m);
-      v += *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>((attn_lds)lds + w * C::STAGES * C::STAGE + (rr * OP + (piece ^ (rr & OM))) * 16);
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][wr][0]);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = stats[w][wr][0];
+        l += mw == -INFINITY ? stats[w][wr][1] : stats[w][wr][1] * exp2f(mw - m);
+        v += *reinterpret_cast<SVDMLP_ATTN_LDS f32x4*>(at + w * (C::LDS / NW));
+      }
     }
     const int t = r / G, h = hk * G + r - t * G;
     if (PROMPT || used == 1) {
       v *= inverse_sum(l);
       store4<BF16>(p.out, (int64_t)b * p.o_b + (int64_t)(start + t) * p.o_t + (int64_t)h * p.o_h + 4 * piece, v);
+    } else if (SHARE) {
+      const int64_t row = ((int64_t)at_chunk * p.n + t) * p.Hq + h;
+      *reinterpret_cast<f32x4*>(p.part + row * p.D + 4 * piece) = v;
+      if (piece == 0) *reinterpret_cast<f32x2*>(p.part + (int64_t)p.chunks * p.n * p.Hq * p.D + 2 * row) = f32x2{m, l};
     } else {
       const int row = (t * p.Hq + h) * p.splits + split;
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), sums, (row * p.D + 4 * piece) * 4, 0, kDevice);
       if (piece == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, ml, row * 8, 0, kDevice);
     }
   }
-  if (PROMPT || used == 1) return;
+  if (PROMPT || SHARE || used == 1) return;
 
   // The last block to get here joins the chunks.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums are out
@@ -547,7 +634,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   };
   if (parts > 1) {  // one item a thread
     SVDMLP_ATTN_LDS f32x4* const others = (SVDMLP_ATTN_LDS f32x4*)((attn_lds)lds + C::ROWS * kSplitsMost * 4);
-    static_assert(C::ROWS * kSplitsMost * 4 + NT * 16 <= NW * C::STAGES * C::STAGE || PROMPT, "weights and the parts' sums fit the stages");
+    static_assert(C::ROWS * kSplitsMost * 4 + NT * 16 <= C::LDS || PROMPT, "weights and the parts' sums fit the stages");
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (item < items) v = gather(item, true);
     others[threadIdx.x] = v;
@@ -562,6 +649,46 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     write(item, gather(item, fetched));
     fetched = false;
   }
+}
+
+// The chunks' sums of blocks that share their tiles, joined: a wave a row, a lane
+// two elements.  (Joined by the last block, 128 rows of 8 chunks took 37 us.)
+template <bool BF16>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheParams p, int rtiles) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  const int heads = p.n * p.Hq, b = (int)(row / heads), th = (int)(row - (int64_t)b * heads);
+  if (b >= p.B) return;
+  const int chunk = shared_chunk(p, rtiles, lane), used = chunks_of(held(p, b), chunk);
+  if (used == 1) return;
+  int first = 0;
+  for (int i = lane; i < b; i += 64) first += chunks_of(held(p, i), chunk);
+  for (int o = 32; o > 0; o >>= 1) first += __shfl_xor(first, o);
+  const int64_t at = (int64_t)__builtin_amdgcn_readfirstlane(first) * heads + th;
+  const float* const ml = p.part + (int64_t)p.chunks * heads * p.D + 2 * at;
+  f32x2 v = {-INFINITY, 0.f};
+  if (lane < used) v = *reinterpret_cast<const f32x2*>(ml + (int64_t)lane * heads * 2);
+  float m = v.x;
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float a = v.x == -INFINITY ? 1.f : exp2f(v.x - m);
+  float l = v.y * a;
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  const float weight = lane < used ? a * inverse_sum(l) : 0.f;
+  if (2 * lane >= p.D) return;
+  const float* const sums = p.part + at * p.D + 2 * lane;
+  f32x2 o = {0.f, 0.f};
+  for (int s0 = 0; s0 < used; s0 += 8) {
+    f32x2 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = *reinterpret_cast<const f32x2*>(sums + (int64_t)min(s0 + k, used - 1) * heads * p.D);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (s0 + k < used) o += x[k] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), s0 + k));
+  }
+  const int t = th / p.Hq, h = th - t * p.Hq;
+  const int64_t to = (int64_t)b * p.o_b + (int64_t)t * p.o_t + (int64_t)h * p.o_h + 2 * lane;
+  if constexpr (BF16) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to) = pack_bf16x2(o.x, o.y);
+  else *reinterpret_cast<f32x2*>(static_cast<float*>(p.out) + to) = o;
 }
 
 }  // namespace svdmlp

@@ -89,7 +89,8 @@ def test_cache_attention_workspace(lib):
     assert f(1, 1, 16, 10, 32, 7, 128) == 0 and counters.value == 0
     assert f(1, 1, 16, 1, 32, 8, 128) == 0 and counters.value == 0  # one chunk: no partial sums
     assert f(1, 1, 16, 1 << 13, 32, 8, 128) > 0 and counters.value == 8
-    assert f(3, 16, 16, 1 << 13, 64, 8, 128) > 0 and counters.value == 3 * 8 * 2  # 128 rows a head: two tiles
+    assert f(3, 8, 16, 1 << 13, 64, 8, 128) > 0 and counters.value == 3 * 8  # 64 rows a head: one tile
+    assert f(3, 16, 16, 1 << 13, 64, 8, 128) > 0 and counters.value == 0     # over 64 rows: joined by a kernel of its own
     assert lib.svdmlp_cache_attention_workspace_bytes(1, 1, 16, 1 << 13, 32, 8, 128, 1, None) > 0
 
 

@@ -453,6 +453,26 @@ def test_cache_attention_many_keys(gpu, dtype, B, n, H, K, D, page, most):
     assert all(int(c.abs().max()) == 0 for _, c in decoder._PARTIALS_CACHE.values())
 
 
+@pytest.mark.parametrize("dtype,B,n,H,K,D,page,most", [
+    (BF, 3, 17, 8, 2, 128, 16, 9000), (BF, 70, 9, 8, 1, 64, 64, 1500), (BF, 2, 64, 16, 2, 40, 7, 3000), (F32, 3, 33, 4, 2, 64, 16, 4000),
+    (F32, 67, 17, 4, 1, 24, 32, 700), (BF, 1, 64, 8, 1, 128, 1, 20000), (BF, 2, 65 - 1, 2, 1, 96, 48, 513)])
+def test_cache_attention_many_rows(gpu, dtype, B, n, H, K, D, page, most):
+    """Over 64 rows a head: tiles that four waves share, chunks chosen from the lengths, joined by a kernel of its own."""
+    g = _gen(B + n)
+    lens = [most, 0, n, n - 1][:B] + [int(x) for x in torch.randint(1, most, (max(B - 4, 0),), generator=g)]
+    table, pages = _pages(g, lens, page)
+    q = _randn(g, B, n, H, D, dtype=dtype)
+    kc, vc = _randn(g, pages, page, K, D, dtype=dtype), _randn(g, pages, page, K, D, dtype=dtype)
+    for tree in (None, _random_tree(g, B, n)):
+        some = sorted({0, 1 % B, 2 % B, 3 % B, B - 1, B // 2})
+        out, tol = _cache_ref(q[some], kc, vc, table[some], [lens[b] for b in some], None if tree is None else tree[some], 1 / math.sqrt(D))
+        args = [t.to(gpu) for t in (q, kc, vc, table)]
+        ln, tg = torch.tensor(lens, device=gpu), None if tree is None else tree.to(gpu)
+        got = svdmlp.cache_attention(*args, ln, tree=tg)
+        _close(got[some], out, tol)
+        assert torch.equal(got, svdmlp.cache_attention(*args, ln, tree=tg))
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_cache_attention_hidden_drafts_have_no_part(gpu, dtype):
     """Infinities and NaN in a draft reach its descendants alone; a token whose row of the tree is empty sees the context, or nothing."""
