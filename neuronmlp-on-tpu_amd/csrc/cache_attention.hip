@@ -4,15 +4,21 @@
 // itself).  n = 1 is the decode step.
 //
 // Bound by the cache's bytes, read once for all heads of a group and all new
-// tokens (up to 32 * QG rows).  Nothing is shared between waves: each takes tiles
-// of 32 keys of its block's chunk through LDS of its own (direct loads, the next
-// tile's in flight while one is computed), with no barrier in the loop.  Where
-// there is work for every wave of the card, a block is one wave, and four of
-// them share a CU, one's start and end hidden behind the others' loads; where
-// there is not, a block's four waves share a chunk, and their sums meet in LDS.
-// A long context is cut into chunks, one a block; the last block of a
-// (sequence, head, row tile) to arrive joins the chunks' partial sums, in the
-// chunks' order (the same bits every time).
+// tokens (up to 128 rows).  Up to 32 rows nothing is shared between waves: each
+// takes tiles of 32 keys of its block's chunk through LDS of its own (direct
+// loads), with no barrier in the loop.  Where there is work for every wave of the
+// card, a block is one wave, and eight of them share a CU, one's start and end
+// hidden behind the others' loads; where there is not, a block's four waves share
+// a chunk, and their sums meet in LDS.  Up to 64 rows a wave takes both 32s of
+// its tile.  Over 64, four waves load each tile together and take 32 rows each:
+// a quarter of the loads, three tiles ahead of the one computed.
+// A long context is cut into chunks, one a block; the last block of a (sequence,
+// head, row tile) to arrive joins the chunks' partial sums, in the chunks' order
+// (the same bits every time), or, over 64 rows, a kernel of its own.
+// Heads of 128 in bf16, 8 of keys: one sequence of 4097 tokens 14.3 us (latency:
+// a chunk of 256 keys, then the join); 64 sequences of up to 4096 120.8 us
+// (4.3 TB/s of a copy's 5.2); 16 tokens' trees of 8 sequences of up to 16384, 128
+// rows a head, 95.3 us (3.4 TB/s, the pace of 32-row tiles).
 #include <algorithm>
 
 #include "wave_attention.hpp"
@@ -43,8 +49,11 @@ hipError_t run(const CacheParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Rows a block: 64 a wave where there are more than 32, and a tile shared by
-// four waves of 32 rows where there are more than 64, as far as their sums fit.
+// Rows a block, as far as their sums fit: 64 a wave where there are more than 32,
+// and four waves of 32 that share a tile where there are more than 64 (8 sequences
+// of up to 16384 tokens, 40, 64, 72 and 128 rows: 77.7, 87.6, 119.5 and 124.6 us
+// by 64 a wave, 83.4, 86.1, 85.9 and 100.7 shared; of up to 8000 in fp32, 40, 64
+// and 72 rows: 41.7, 48.8, 67.4 and 52.8, 54.7, 54.9).
 int block_rows(int n, int Hq, int Hk, int D, bool bf16) {
   const int64_t rows = (int64_t)n * (Hq / Hk);
   return rows <= 32 || D > (bf16 ? 128 : 64) ? 32 : rows <= 64 ? 64 : 128;
@@ -62,7 +71,9 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   // Else, and where a wave has 64 rows (whose partial sums, written and read,
   // would be a quarter of such a chunk's keys and values), blocks that share a
   // chunk, of chunks that give every CU one; or three, of different lengths, if
-  // the chunks stay long.
+  // the chunks stay long.  Blocks that share their tiles: two a CU, which is what
+  // fits (trees of 16 over up to 16384 tokens, one, two, three, four a CU: 131,
+  // 95, 115, 109 us).
   constexpr int64_t kSolo = 256;
   plan.waves = rt == 32 && base * ((capacity + kSolo - 1) / kSolo) >= 4 * (int64_t)cus ? 1 : waves;
   int64_t c = kSolo;

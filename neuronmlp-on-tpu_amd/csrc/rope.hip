@@ -11,7 +11,8 @@
 // computed once for all its heads, through LDS.
 //
 // Bound by HBM: every value is read and written once.  A block takes a few
-// tokens, its threads their 16-byte pieces.
+// tokens, its threads their 16-byte pieces.  6007 tokens of 32 + 8 heads of 128
+// in bf16: 23.5 us, 5.2 TB/s, a copy's rate; 16 into a cache: 4.4 us, latency.
 #include "common.hpp"
 #include "decoder.hpp"
 
@@ -181,8 +182,9 @@ hipError_t launch_rope(const RopeParams& p, bool bf16, bool vec, hipStream_t st)
   if (p.T <= 0) return hipSuccess;
   auto go = [&](auto b, auto v) {
     constexpr bool B = decltype(b)::value, V = decltype(v)::value;
-    // One token a block while eight a CU do not fill the card, else four: their
-    // cosines keep all 256 threads busy at 128 turned values.
+    // One token a block while those are few, else four: their cosines keep all
+    // 256 threads busy at 128 turned values (2501 fp32 tokens of 32 heads of 64:
+    // 9.9 us by one, 14.6 by four).
     if (p.T < 4096)
       hipLaunchKernelGGL((rope_kernel<B, V, 1>), dim3((unsigned)p.T), dim3(256), p.rot * 4, st, p);
     else

@@ -1,9 +1,10 @@
-// Attention with nothing shared between waves: the kernel of cache_attention.hip
-// (new tokens onto a paged cache) and, with CacheCfg::PROMPT, of prompts of few
-// rows (prompt_attention.hip).  Each wave takes every NW-th tile of 32 keys through
-// LDS of its own (direct loads, the next tile's in flight while one is computed),
-// with no barrier in the loop; a block's waves share its rows, and their sums
-// meet in LDS at the end.
+// Attention of up to 32 rows a wave (64 with QG = 2): the kernel of
+// cache_attention.hip (new tokens onto a paged cache) and, with CacheCfg::PROMPT,
+// of prompts of few rows (prompt_attention.hip).  Without CacheCfg::SHARE each
+// wave takes every NW-th tile of 32 keys through LDS of its own, with no barrier
+// in the loop; a block's waves share its rows, and their sums meet in LDS at the
+// end.  With it every wave takes every tile, for rows of its own; each loads a
+// part of it, and a barrier a tile keeps them together.
 #pragma once
 
 #include <math.h>
