@@ -354,7 +354,7 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
  * block_table sequence; tree sequence, token.  The workspace
  * (svdmlp_cache_attention_workspace_bytes; may be 0) holds the partial sums of
  * long contexts and needs no clearing.  With one go `counters` int32 counters
- * (*counters of svdmlp_cache_attention_workspace_bytes, if not NULL), zero
+ * (*counters of svdmlp_cache_attention_workspace_bytes, if not NULL; may be 0), zero
  * before the call, which leaves them zero: calls in flight at the same time
  * (other streams, graphs) need workspaces and counters of their own.
  */
