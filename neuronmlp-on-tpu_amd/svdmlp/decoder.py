@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -119,12 +120,27 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     pa, pb = a.data_ptr(), b.data_ptr()
     if pa + _extent(a) <= pb or pb + _extent(b) <= pa:
         return False
+    if a.dim() == b.dim() and a.dtype == b.dtype and all(s == t or m == 1 or n == 1 for s, t, m, n in zip(a.stride(), b.stride(), a.shape, b.shape)):
+        steps = [(s if m > 1 else t, m, n) for s, t, m, n in zip(a.stride(), b.stride(), a.shape, b.shape) if m > 1 or n > 1]
+        steps.sort(reverse=True)
+        if all(s > sum(t * (max(m, n) - 1) for t, m, n in steps[i + 1:]) for i, (s, _, _) in enumerate(steps)):
+            d, rest = divmod(pb - pa, a.element_size())
+            return bool(rest) or _meet(d, steps)
     pitch = a.stride(0) * a.element_size()
     wa, wb = _extent(a, 1), _extent(b, 1)
     if pitch == b.stride(0) * b.element_size() and max(wa, wb) <= pitch:
         d = (pb - pa) % pitch
         return d < wa or d + wb > pitch
     return True
+
+
+def _meet(d: int, steps) -> bool:
+    """Whether an element of a and one of b, `d` elements further on, are the same: d = sum of stride * (index in a - in b),
+    each stride beyond what the smaller ones reach."""
+    if not steps:
+        return d == 0
+    s, m, n = steps[0]
+    return any(-n < i < m and _meet(d - i * s, steps[1:]) for i in (d // s, d // s + 1))
 
 
 def _apart(name: str, out: torch.Tensor, *tensors, own=()) -> None:
@@ -468,10 +484,11 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
     code = _ACT_CODES[dtype]
     nbytes, counters = _sizes(lib, index, B, n, page, width, Hq, Hk, D, code)
     if nbytes:
-        held = _partials(index, nbytes, counters)
-        _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
-                held[0].data_ptr(), nbytes, held[1].data_ptr(), counters)
+        with _partials_lock:  # a call may be two launches: no other thread's between them
+            held = _partials(index, nbytes, counters)
+            _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                    lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
+                    held[0].data_ptr(), nbytes, held[1].data_ptr(), counters)
     else:
         _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
                 lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
@@ -480,6 +497,7 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
 
 
 _SIZES: dict = {}
+_partials_lock = threading.Lock()
 
 
 def _sizes(lib, index, *sizes) -> tuple[int, int]:

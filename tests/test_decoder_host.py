@@ -178,3 +178,21 @@ def test_e2e_parser_has_the_decoder_arm():
 
     assert e2e_block._parser().parse_args([]).decoder_arm is False
     assert e2e_block._parser().parse_args(["--decoder-arm"]).decoder_arm is True
+
+
+def test_overlap_of_views():
+    """Views of one buffer: told apart exactly where their strides are alike."""
+    from svdmlp.decoder import _overlap
+
+    def brute(a, b):
+        cells = lambda t: {t.storage_offset() + o for o in (torch.arange(200).as_strided(t.shape, t.stride(), 0)).flatten().tolist()}
+        return bool(cells(a) & cells(b))
+
+    x = torch.zeros(200)
+    pairs = [(x.view(10, 20)[:, :8], x.view(10, 20)[:, 8:]), (x.view(10, 20)[:, :8], x.view(10, 20)[:, 7:]),
+             (x.view(5, 5, 2, 4)[..., 0, :], x.view(5, 5, 2, 4)[..., 1, :]), (x.view(5, 5, 2, 4)[:3, :, 0], x.view(5, 5, 2, 4)[2:, :, 0]),
+             (x.view(5, 5, 2, 4)[:2, :, 0], x.view(5, 5, 2, 4)[2:, :, 0]), (x.view(5, 40)[:, :12].view(5, 3, 4), x.view(5, 40)[:, 12:20].view(5, 2, 4)),
+             (x.view(5, 40)[:, :12].view(5, 3, 4), x.view(5, 40)[:, 8:16].view(5, 2, 4)), (x[:8].view(1, 2, 4), x[4:12].view(1, 2, 4)),
+             (x.view(4, 2, 25)[:, 0], x.view(4, 2, 25)[:, 1]), (x.view(4, 2, 25)[1:, 0], x.view(4, 2, 25)[:3, 1])]
+    for a, b in pairs:
+        assert _overlap(a, b) == brute(a, b) and _overlap(b, a) == brute(a, b), (a.shape, a.stride(), b.shape, b.storage_offset())

@@ -516,7 +516,7 @@ def test_cache_attention_context_values_reach_every_token(gpu, dtype, D, B):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("D,B,n", [(64, 1, 3), (128, 1, 3), (64, 1, 40), (128, 1, 40), (256, 1, 3), (128, 300, 3)])
+@pytest.mark.parametrize("D,B,n", [(64, 1, 3), (128, 1, 3), (64, 1, 20), (128, 1, 20), (64, 1, 40), (128, 1, 40), (256, 1, 3), (128, 300, 3)])
 @pytest.mark.parametrize("page,lost", [(48, False), (16, True)])
 def test_cache_attention_context_values_of_any_page(gpu, dtype, D, B, n, page, lost):
     """The same where tiles are not loaded whole: pages of no power of two, and a page outside the cache among the others."""
@@ -919,3 +919,42 @@ def test_e2e_record_of_the_decoder_arm(gpu):
     assert rec["decoder_step_vs_block_relative_l2"] < 0.02  # as above
     for arm in ("decoder_block", "decoder_step"):
         assert rec[arm]["iterations"] == 2 and 0 < rec[arm]["latency_ms_min"] <= rec[arm]["latency_ms_max"]
+
+
+def test_cache_attention_two_threads_on_a_stream(gpu):
+    """Two threads' calls on one stream, each of two launches that share the stream's room for partial sums."""
+    import threading
+
+    g = _gen(31)
+    B, n, H, K, D, page = 2, 16, 16, 2, 128, 16
+    sets = []
+    for lens in ([9000, 4000], [500, 7000]):
+        table, pages = _pages(g, lens, page)
+        sets.append([t.to(gpu) for t in (_randn(g, B, n, H, D), _randn(g, pages, page, K, D), _randn(g, pages, page, K, D), table, torch.tensor(lens))])
+    want = [svdmlp.cache_attention(*s) for s in sets]
+    got = [[], []]
+
+    def work(i):
+        for _ in range(40):
+            got[i].append(svdmlp.cache_attention(*sets[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i]) and len(got[0]) == len(got[1]) == 40
+
+
+def test_rope_append_into_interleaved_caches(gpu):
+    """Keys and values of a head side by side, (pages, page, Hk, 2, D): two views of one buffer that share no element."""
+    pos, f = torch.arange(20, device=gpu), torch.ones(4, dtype=torch.float64, device=gpu)
+    pool = torch.zeros(3, 16, 2, 2, 8, device=gpu)
+    q, k, v = torch.randn(20, 4, 8, device=gpu), torch.randn(20, 2, 8, device=gpu), torch.randn(20, 2, 8, device=gpu)
+    svdmlp.rope_append(q, k, v, pos, f, pool[..., 0, :], pool[..., 1, :], pos)
+    _, turned = svdmlp.rope(q, k, pos, f)
+    assert torch.equal(pool.flatten(0, 1)[:20, :, 0], turned) and torch.equal(pool.flatten(0, 1)[:20, :, 1], v)
+    assert (pool.flatten(0, 1)[20:] == 0).all()
+    with pytest.raises(ValueError, match="overlap"):
+        svdmlp.rope_append(q, k, v, pos, f, pool[..., 0, :], pool[..., 0, :], pos)
