@@ -5,8 +5,8 @@
 // head of the group: the group's heads share every key and value that the block
 // loads) and walks the keys in tiles through LDS, one pass, with the running
 // maximum and sum.  Three kernels: prompt_pipe_kernel (bf16, heads up to 128, many
-// rows), the one of wave_attention.hpp (few rows, fp32), prompt_kernel (heads up
-// to 256).
+// rows), the one of wave_attention.hpp (few rows, many short sequences, fp32),
+// prompt_kernel (heads up to 256).
 #include <math.h>
 
 #include <algorithm>
@@ -681,12 +681,12 @@ hipError_t run_pipe(const PromptParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// One tile in LDS a wave, so that two blocks share a CU and hide each other's
+// Without SHARE one tile in LDS a wave, so that two blocks share a CU and hide each other's
 // loads, starts and ends: with two tiles and one block a CU 512 tokens of 32
 // heads took 18 us instead of 13; 64-row blocks of two tiles 18 too.
-template <bool BF16, int DP, int NW>
+template <bool BF16, int DP, int NW, bool SHARE = false>
 hipError_t run_wave(const PromptParams& p, hipStream_t st) {
-  using C = CacheCfg<BF16, DP, 1, NW, true, 1>;
+  using C = CacheCfg<BF16, DP, 1, NW, true, SHARE ? 512 / DP : 1, SHARE>;
   CacheParams w = {};
   w.q = p.q, w.kc = p.k, w.vc = p.v, w.out = p.out, w.cu = p.cu;
   w.q_t = p.q_t, w.q_h = p.q_h, w.k_t = p.k_t, w.k_h = p.k_h, w.v_t = p.v_t, w.v_h = p.v_h, w.o_t = p.o_t, w.o_h = p.o_h;
@@ -707,7 +707,13 @@ hipError_t launch_prompt_attention(const PromptParams& p, bool bf16, int cus, hi
   // former, 32 / 44 / 77 in the latter (17 packed prompts of 8191 tokens 97 /
   // 190); 16 heads of 64, 2048 / 4096 / 8192 tokens: 45 / 81 / 185, 24 / 66 / 238.
   if (bf16 && p.D <= 64) return rows >= (int64_t)cus * 384 ? run_pipe<64>(p, st) : run_wave<true, 64, 4>(p, st);
-  if (bf16 && p.D <= 128) return rows >= (int64_t)cus * 144 ? run_pipe<128>(p, st) : run_wave<true, 128, 4>(p, st);
+  if (bf16 && p.D <= 128) {
+    // Short sequences: 128-row blocks, two a CU, which hide each other's starts
+    // and ends (8192 tokens in sequences of 64 / 128 / 256 / 512: 53 / 58 / 69 / 87
+    // us, by the 256-row blocks 68 / 65 / 76 / 83).
+    if (rows < (int64_t)cus * 144) return run_wave<true, 128, 4>(p, st);
+    return (int64_t)p.T * (p.Hq / p.Hk) < (int64_t)1536 * p.B ? run_wave<true, 128, 4, true>(p, st) : run_pipe<128>(p, st);
+  }
   if (!bf16 && p.D <= 64) return run_wave<false, 64, 4>(p, st);
   if (!bf16 && p.D <= 128) return run_wave<false, 128, 2>(p, st);
   return bf16 ? run<true>(p, st) : run<false>(p, st);

@@ -40,7 +40,7 @@ struct CacheCfg {
   static constexpr int MINE = SHARE ? LOADS / NW : LOADS;  // of them a wave's
   static constexpr int LDS = (SHARE ? 1 : NW) * STAGES * STAGE;
   static_assert(LDS / NW >= WROWS * DP * 4, "a wave's sums fit its part of LDS");
-  static_assert(!SHARE || (LOADS % NW == 0 && STAGES > 2 && !PROMPT), "shared tiles");
+  static_assert(!SHARE || (LOADS % NW == 0 && STAGES > 2), "shared tiles");
 };
 
 // 16 bytes of zeros that lanes without a key load.
@@ -259,8 +259,8 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
         const char* const kt = kb + (int64_t)ku * p.k_t * ES;
         const char* const vt = vb + (int64_t)ku * p.v_t * ES;
 #pragma unroll
-        for (int j = 0; j < C::LOADS; ++j) {
-          const int ck = kpiece ^ k_swz<RB>(j * C::RPI), cv = vpiece ^ v_swz<RB, BF16>(j * C::RPI);
+        for (int i = 0; i < C::MINE; ++i) {
+          const int j = j0 + i, ck = kpiece ^ k_swz<RB>(j * C::RPI), cv = vpiece ^ v_swz<RB, BF16>(j * C::RPI);
           if (ck < npieces) load_lds16(kt + (int64_t)j * C::RPI * p.k_t * ES, krow + 16 * ck, base + j * 1024);
           if (cv < npieces) load_lds16(vt + (int64_t)j * C::RPI * p.v_t * ES, vrow + 16 * cv, base + C::TILE + j * 1024);
         }

@@ -230,7 +230,8 @@ def test_prompt_attention(gpu, dtype, causal, lens, H, K, D):
 
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("lens,H,K,D", [([2100], 32, 8, 128), ([1500, 1, 0, 640], 64, 8, 64), ([1030, 63, 65, 1027], 32, 4, 96), ([4097], 16, 16, 64),
-                                        ([900, 1300], 32, 1, 80), ([2113], 40, 8, 128)])
+                                        ([900, 1300], 32, 1, 80), ([2113], 40, 8, 128), ([1, 0, 129, 31, 33, 300, 77, 128, 400, 201], 32, 8, 128),
+                                        ([33, 250, 64, 2, 391, 460, 7, 193], 32, 4, 96), ([311], 128, 32, 128), ([160, 97], 160, 80, 72)])
 def test_prompt_attention_many_rows(gpu, lens, H, K, D, causal):
     g = _gen(sum(lens) + H)
     (q, k, v), dev = _qkv(g, sum(lens), H, K, D, BF, gpu)
@@ -256,7 +257,7 @@ def test_prompt_attention_large_scores_and_scale(gpu, dtype):
             _close(got[:, heads], out, tol)
 
 
-@pytest.mark.parametrize("H,K,D", [(4, 2, 64), (4, 2, 128), (4, 2, 256), (256, 1, 64), (256, 2, 128)])
+@pytest.mark.parametrize("H,K,D", [(4, 2, 64), (4, 2, 128), (4, 2, 256), (256, 1, 64), (256, 2, 128), (256, 32, 128)])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_prompt_attention_hidden_keys_have_no_part(gpu, dtype, H, K, D):
     """Infinities and NaN in later tokens, other sequences and rows of no
