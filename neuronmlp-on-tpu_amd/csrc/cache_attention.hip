@@ -78,7 +78,13 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   plan.waves = rt == 32 && base * ((capacity + kSolo - 1) / kSolo) >= 4 * (int64_t)cus ? 1 : waves;
   int64_t c = kSolo;
   if (plan.waves > 1 || waves == 1) c = std::max(capacity * base / cus / 3, std::min<int64_t>(1024, capacity * base / cus));
-  if (rt == 128) c = 512;  // at least: as many as the lengths ask for (shared_chunk)
+  // Of few sequences, whose lengths may be any part of the table's width, from
+  // the lengths (shared_chunk), 512 at least; many even out by themselves (heads
+  // of 128, 8 of keys, 16 new tokens; 4 sequences of up to 32768 tokens 75 us from
+  // the lengths, 101 from the width; 8 of 16384 102 and 103, of 8192 48 and 58; 16
+  // of 8192 135 and 116; 64 of 4000 242 and 198).
+  const bool choose = rt == 128 && B <= 64 && base * 4 <= cus;
+  if (rt == 128) c = choose ? 512 : std::max<int64_t>(512, capacity * base / (2 * cus));
   c = std::max<int64_t>(c, (capacity + kSplitsMost - 1) / kSplitsMost);
   c = std::max<int64_t>(128, (c + 127) / 128 * 128);
   c = std::min(c, (int64_t)kPagesMost * page / 128 * 128);
@@ -86,9 +92,11 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   plan.splits = (int)((capacity + plan.chunk - 1) / plan.chunk);
   plan.shared = rt == 128;
   plan.slots = 2 * cus;
-  plan.chunk_most = (int)std::min((int64_t)kPagesMost * page, (int64_t)0x7fffff80);
+  plan.chunk_most = plan.chunk;
   plan.chunks = B * plan.splits;
-  if (plan.shared && plan.splits > 1) {  // at most total / chunk + B
+  if (choose && plan.splits > 1) {
+    plan.chunk_most = (int)std::min((int64_t)kPagesMost * page, (int64_t)0x7fffff80);
+    // at most total / chunk + B
     const int64_t most = std::max(plan.slots / ((int64_t)Hk * plan.rtiles), (B * capacity + plan.chunk_most - 1) / plan.chunk_most);
     plan.chunks = (int)std::min(B + most, (int64_t)plan.chunks);
   }

@@ -82,7 +82,7 @@ struct CacheParams {
 constexpr int64_t kTokenStrideMost = 1 << 23;  // a 64-row tile's byte offsets fit 31 bits, in both types
 constexpr int64_t kCachePagesMost = 65536;  // pages of a sequence: 64 chunks of 1024
 // Blocks of 128 rows (plan.shared) choose their chunk on the device, from the
-// lengths: `chunk` to chunk_most keys, `chunks` of them in all.
+// lengths: `chunk` to chunk_most keys (equal: no choice), `chunks` of them in all.
 struct CachePlan {
   int splits, chunk, waves, rtiles, chunk_most, chunks, slots;
   bool shared;

@@ -72,11 +72,10 @@ __device__ __forceinline__ int held(const CacheParams& p, int b) {
 // at once, over all sequences, heads and row tiles.  (From the table's width
 // instead, sequences of unequal lengths left half the card idle.)
 __device__ __forceinline__ int shared_chunk(const CacheParams& p, int rtiles, int lane) {
-  if (p.splits == 1) return p.chunk;
-  int64_t total = 0;
-  for (int b = lane; b < p.B; b += 64) total += held(p, b);
+  if (p.chunk == p.chunk_most) return p.chunk;
+  int64_t total = lane < p.B ? held(p, lane) : 0;  // (up to 64 sequences)
   for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-  const int64_t want = (total * p.Hk * rtiles / p.slots + 127) / 128 * 128;
+  const int64_t want = ((total * p.Hk * rtiles + p.slots - 1) / p.slots + 127) / 128 * 128;
   return __builtin_amdgcn_readfirstlane((int)min(max(want, (int64_t)p.chunk), (int64_t)p.chunk_most));
 }
 __device__ __forceinline__ int chunks_of(int len, int chunk) {  // the first always answers
@@ -126,31 +125,22 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     rt = id % rtiles;
     id /= rtiles;
     chunk = p.chunk;
-    if (SHARE && p.splits > 1) {
+    if (SHARE && p.chunk < p.chunk_most) {
       // Chunk `id` of all sequences' in order.
       chunk = shared_chunk(p, rtiles, lane);
-      int left = id;
-      b = -1;
-      for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int n = b0 + lane < p.B ? chunks_of(held(p, b0 + lane), chunk) : 0;
-        int upto = n;
-        for (int o = 1; o < 64; o <<= 1) {
-          const int v = __shfl_up(upto, o);
-          if (lane >= o) upto += v;
-        }
-        const uint64_t hit = __ballot(left < upto);
-        if (hit) {
-          const int i = __builtin_ctzll(hit);
-          b = b0 + i, split = left - __builtin_amdgcn_readlane(upto - n, i);
-          break;
-        }
-        left -= __builtin_amdgcn_readlane(upto, 63);
+      const int n = lane < p.B ? chunks_of(held(p, lane), chunk) : 0;
+      int upto = n;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o);
+        if (lane >= o) upto += v;
       }
-      if (b < 0) return;
+      const uint64_t hit = __ballot(id < upto);
+      if (!hit) return;
+      b = __builtin_ctzll(hit), split = id - __builtin_amdgcn_readlane(upto - n, b);
     } else {
       b = id % p.B, split = id / p.B;
     }
-    at_chunk = id;
+    at_chunk = SHARE && p.chunk == p.chunk_most ? b * p.splits + split : id;
     const int len = held(p, b);
     r0 = rt * C::ROWS;
     kbeg = split * chunk, kend = min(len, kbeg + chunk);
@@ -662,9 +652,11 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheParams p, int rtil
   if (b >= p.B) return;
   const int chunk = shared_chunk(p, rtiles, lane), used = chunks_of(held(p, b), chunk);
   if (used == 1) return;
-  int first = 0;
-  for (int i = lane; i < b; i += 64) first += chunks_of(held(p, i), chunk);
-  for (int o = 32; o > 0; o >>= 1) first += __shfl_xor(first, o);
+  int first = b * p.splits;
+  if (p.chunk < p.chunk_most) {
+    first = lane < b ? chunks_of(held(p, lane), chunk) : 0;
+    for (int o = 32; o > 0; o >>= 1) first += __shfl_xor(first, o);
+  }
   const int64_t at = (int64_t)__builtin_amdgcn_readfirstlane(first) * heads + th;
   const float* const ml = p.part + (int64_t)p.chunks * heads * p.D + 2 * at;
   f32x2 v = {-INFINITY, 0.f};

@@ -456,7 +456,8 @@ def test_cache_attention_many_keys(gpu, dtype, B, n, H, K, D, page, most):
 
 @pytest.mark.parametrize("dtype,B,n,H,K,D,page,most", [
     (BF, 3, 17, 8, 2, 128, 16, 9000), (BF, 70, 9, 8, 1, 64, 64, 1500), (BF, 2, 64, 16, 2, 40, 7, 3000), (F32, 3, 33, 4, 2, 64, 16, 4000),
-    (F32, 67, 17, 4, 1, 24, 32, 700), (BF, 1, 64, 8, 1, 128, 1, 20000), (BF, 2, 65 - 1, 2, 1, 96, 48, 513)])
+    (F32, 67, 17, 4, 1, 24, 32, 700), (BF, 1, 64, 8, 1, 128, 1, 20000), (BF, 2, 64, 2, 1, 96, 48, 513),
+    (BF, 300, 9, 8, 1, 32, 16, 1300), (BF, 257, 5, 16, 1, 128, 32, 600)])
 def test_cache_attention_many_rows(gpu, dtype, B, n, H, K, D, page, most):
     """Over 64 rows a head: tiles that four waves share, chunks chosen from the lengths, joined by a kernel of its own."""
     g = _gen(B + n)
@@ -959,3 +960,24 @@ def test_rope_append_into_interleaved_caches(gpu):
     assert (pool.flatten(0, 1)[20:] == 0).all()
     with pytest.raises(ValueError, match="overlap"):
         svdmlp.rope_append(q, k, v, pos, f, pool[..., 0, :], pool[..., 0, :], pos)
+
+
+def test_cache_attention_graph_with_growing_sequences(gpu):
+    """A captured call of many rows, whose chunks follow the lengths: replayed as the sequences grow, with other calls between."""
+    g = _gen(51)
+    B, n, H, K, D, page = 3, 16, 16, 2, 64, 16
+    table, pages = _pages(g, [6000, 5000, 4000], page)
+    q, kc, vc = (t.to(gpu) for t in (_randn(g, B, n, H, D), _randn(g, pages, page, K, D), _randn(g, pages, page, K, D)))
+    table, lens = table.to(gpu), torch.tensor([30, 16, 700], dtype=torch.int32, device=gpu)
+    svdmlp.cache_attention(q, kc, vc, table, lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = svdmlp.cache_attention(q, kc, vc, table, lens)
+    for now in ([30, 16, 700], [6000, 0, 1], [5999, 5000, 4000], [17, 900, 3999]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        out.fill_(3.0)
+        graph.replay()
+        want = svdmlp.cache_attention(q, kc, vc, table, lens)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
