@@ -82,11 +82,13 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   // the lengths (shared_chunk), 512 at least; many even out by themselves (heads
   // of 128, 8 of keys, 16 new tokens; 4 sequences of up to 32768 tokens 75 us from
   // the lengths, 101 from the width; 8 of 16384 102 and 103, of 8192 48 and 58; 16
-  // of 8192 135 and 116; 64 of 4000 242 and 198).
-  const bool choose = rt == 128 && B <= 64 && base * 4 <= cus;
+  // of 8192 135 and 116; 64 of 4000 242 and 198; 8 of 8192, 64 new tokens, 119 and 172).
+  const bool choose = rt == 128 && B <= 64 && (B <= 8 || base * 4 <= cus);
   if (rt == 128) c = choose ? 512 : std::max<int64_t>(512, capacity * base / (2 * cus));
   c = std::max<int64_t>(c, (capacity + kSplitsMost - 1) / kSplitsMost);
-  c = std::max<int64_t>(128, (c + 127) / 128 * 128);
+  // (a single wave of rows of 1 KB: a tile, whose products take 7 us)
+  const int64_t step = waves == 1 ? 32 : 128;
+  c = std::max(step, (c + step - 1) / step * step);
   c = std::min(c, (int64_t)kPagesMost * page / 128 * 128);
   plan.chunk = (int)std::min<int64_t>(c, 0x7fffff80);
   plan.splits = (int)((capacity + plan.chunk - 1) / plan.chunk);

@@ -38,6 +38,8 @@ struct CacheCfg {
   static constexpr int RPI = 64 / PIECES;        // rows a load
   static constexpr int LOADS = 32 / RPI;         // loads a tile, of keys and of values
   static constexpr int MINE = SHARE ? LOADS / NW : LOADS;  // of them a wave's
+  static constexpr bool QREG = DP < 256;  // Q in registers
+  static_assert(QREG || (QG == 1 && !SHARE), "Q in LDS: one copy for the block");
   static constexpr int LDS = (SHARE ? 1 : NW) * STAGES * STAGE;
   static_assert(LDS / NW >= WROWS * DP * 4, "a wave's sums fit its part of LDS");
   static_assert(!SHARE || (LOADS % NW == 0 && STAGES > 2), "shared tiles");
@@ -103,6 +105,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   constexpr bool PROMPT = C::PROMPT, SHARE = C::SHARE;
   constexpr int ES = C::ES, RB = C::RB, QG = C::QG, DB = C::DP / 32, NW = C::NW;
   __shared__ __attribute__((aligned(1024))) char lds[C::LDS];
+  __shared__ __attribute__((aligned(16))) char qlds[C::QREG ? 16 : C::STEPS * 1024];
   __shared__ float stats[NW][C::WROWS][2];
   __shared__ int ids[PROMPT ? 1 : kPagesMost + 2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
@@ -154,23 +157,28 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   }
 
   const int w0 = r0 + (SHARE ? wave * C::WROWS : 0);  // the wave's first row
-  // Heads of over 128 elements leave no registers for Q: its pieces are read
-  // again (from the caches) for every tile.
-  constexpr bool QREG = C::DP < 256;
+  // Heads of over 128 elements leave no registers for Q: its pieces lie in LDS, in
+  // the order of the products.
+  constexpr bool QREG = C::QREG;
   u32x4 qf[QG][QREG ? C::STEPS : 1];
-  const char* qptr[QG];
   int qi[QG];  // which of the sequence's (new) tokens
   const int npieces = p.D * ES / 16;
 #pragma unroll
   for (int g = 0; g < QG; ++g) {
     const int r = min(w0 + 32 * g + col, rows - 1);  // rows behind the last repeat it, and are not stored
     qi[g] = r / G;
-    qptr[g] = static_cast<const char*>(p.q) + ((int64_t)b * p.q_b + (int64_t)(start + qi[g]) * p.q_t + (int64_t)(hk * G + r - qi[g] * G) * p.q_h) * ES;
+    const char* const qptr = static_cast<const char*>(p.q) + ((int64_t)b * p.q_b + (int64_t)(start + qi[g]) * p.q_t + (int64_t)(hk * G + r - qi[g] * G) * p.q_h) * ES;
     if constexpr (QREG)
 #pragma unroll
       for (int s = 0; s < C::STEPS; ++s) {
         const int c = 2 * s + half;
-        qf[g][s] = c < npieces ? *reinterpret_cast<const u32x4*>(qptr[g] + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+        qf[g][s] = c < npieces ? *reinterpret_cast<const u32x4*>(qptr + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+      }
+    else
+      for (int s = wave; s < C::STEPS; s += NW) {
+        const int c = 2 * s + half;
+        *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>((attn_lds)qlds + (s * 64 + lane) * 16) =
+            c < npieces ? *reinterpret_cast<const u32x4*>(qptr + 16 * c) : u32x4{0u, 0u, 0u, 0u};
       }
   }
   // Each row's 64 bits of the tree, where the chunk reaches the new tokens: a
@@ -313,13 +321,17 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
   auto unit = [&](auto masked_, attn_lds stage, int ku, uint32_t there) {
     constexpr bool masked = decltype(masked_)::value;
     const attn_lds lk = stage, lv = stage + C::TILE;
-    u32x4 kf[kAhead], vf[kAhead];
+    u32x4 kf[kAhead], vf[kAhead], qa[kAhead];
+    auto read_query = [&](int t) { return *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>((attn_lds)qlds + (t * 64 + lane) * 16); };
     auto read_value = [&](int f) {
       if constexpr (BF16) vf[f % kAhead] = at.values(lv, f / DB, f % DB);
       else vf[f % kAhead].x = at.value(lv, f / DB, f % DB);
     };
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) kf[t] = at.key(lk, t);
+    for (int t = 0; t < kAhead; ++t) {
+      kf[t] = at.key(lk, t);
+      if constexpr (!QREG) qa[t] = read_query(t);
+    }
     f32x16 s[QG];
 #pragma unroll
     for (int g = 0; g < QG; ++g) s[g] = f32x16{};
@@ -328,14 +340,12 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < QG; ++g) {
-        if constexpr (!QREG) {
-          const int c = 2 * t + half;
-          qf[g][0] = c < npieces ? *reinterpret_cast<const u32x4*>(qptr[g] + 16 * c) : u32x4{0u, 0u, 0u, 0u};
-        }
-        s[g] = attn_mfma<BF16>(kf[t % kAhead], qf[g][QREG ? t : 0], s[g]);
+        s[g] = attn_mfma<BF16>(kf[t % kAhead], QREG ? qf[g][QREG ? t : 0] : qa[t % kAhead], s[g]);
       }
-      if (t + kAhead < C::STEPS) kf[t % kAhead] = at.key(lk, t + kAhead);
-      else read_value(t + kAhead - C::STEPS);
+      if (t + kAhead < C::STEPS) {
+        kf[t % kAhead] = at.key(lk, t + kAhead);
+        if constexpr (!QREG) qa[t % kAhead] = read_query(t + kAhead);
+      } else read_value(t + kAhead - C::STEPS);
     }
     __builtin_amdgcn_sched_barrier(0);
     u32x4 pb[QG][2];
