@@ -336,7 +336,8 @@ int svdmlp_rope_append(const void* q, const void* k, const void* v, const int64_
  * SVDMLP_CAUSAL, the tokens up to itself.  Keys that a row does not see have no
  * part in it whatever they hold.  Rows of no sequence are left as they were.
  * D up to 256, head size, strides and addresses whole 16-byte pieces, keys and
- * values at most 2^23 elements apart.  strides: token and head of q, k, v, out.
+ * values at most 2^23 elements apart; calls of more blocks than a launch can
+ * have (2^24, of 32 to 256 rows) are refused.  strides: token and head of q, k, v, out.
  */
 int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out,
                             const int64_t* strides /* 8 or NULL */, int64_t T, int64_t B, int64_t Hq, int64_t Hk,

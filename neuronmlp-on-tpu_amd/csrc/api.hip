@@ -2658,7 +2658,8 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
   PromptParams p = {q, k, v, out, cu_seqlens, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], (int)T, (int)B, (int)Hq,
                     (int)Hk, (int)D, scale * 1.44269504088896340736f, (flags & SVDMLP_CAUSAL) != 0};
   StageScope sc(ST_PROMPT_ATTENTION, (hipStream_t)stream);
-  return check(launch_prompt_attention(p, dtype == SVDMLP_BF16, device_cus(), (hipStream_t)stream), "prompt_attention");
+  return check(launch_prompt_attention(p, dtype == SVDMLP_BF16, device_cus(), (hipStream_t)stream), "prompt_attention",
+               "too many rows or sequences for one launch");
 }
 
 size_t svdmlp_cache_attention_workspace_bytes(int64_t B, int64_t n, int64_t page, int64_t width, int64_t Hq, int64_t Hk,
@@ -2714,7 +2715,8 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   p.part = static_cast<float*>(workspace);
   p.counters = counters;
   StageScope sc(ST_CACHE_ATTENTION, (hipStream_t)stream);
-  return check(launch_cache_attention(p, dtype == SVDMLP_BF16, plan, (hipStream_t)stream), "cache_attention");
+  return check(launch_cache_attention(p, dtype == SVDMLP_BF16, plan, (hipStream_t)stream), "cache_attention",
+               "too many sequences or chunks for one launch");
 }
 
 int svdmlp_residual_norm(const void* x, const void* branch, const float* post_w, const void* gate,

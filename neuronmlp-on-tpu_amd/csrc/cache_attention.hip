@@ -36,16 +36,15 @@ hipError_t run(const CacheParams& p, hipStream_t st) {
   using C = CacheCfg<BF16, DP, QG, NW, false, SHARE ? 65536 / (64 * RB) : QG == 1 && RB >= 256 ? 1 : 2, SHARE>;
   const int64_t rtiles = ((int64_t)p.n * (p.Hq / p.Hk) + C::ROWS - 1) / C::ROWS;
   const int64_t blocks = rtiles * p.Hk * p.chunks;
-  if (blocks > 0x7fffffff || (int64_t)p.B * p.n * p.Hq > 0x7fffffff) return hipErrorInvalidValue;
+  const int64_t joins = ((int64_t)p.B * p.n * p.Hq + 3) / 4;
+  const bool joined = SHARE && p.splits > 1;  // by a kernel of its own
+  if (!fits_launch(blocks, 64 * NW) || (joined && !fits_launch(joins, 256))) return hipErrorInvalidValue;
   CacheParams q = p;
   q.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (p.page == 1 << s && p.page >= C::RPI) q.page_shift = s;
   hipLaunchKernelGGL((cache_kernel<C>), dim3((unsigned)blocks), dim3(64 * NW), 0, st, q);
-  if (SHARE && p.splits > 1) {
-    const int64_t rows = (int64_t)p.B * p.n * p.Hq;
-    hipLaunchKernelGGL((cache_join_kernel<BF16>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p, (int)rtiles);
-  }
+  if (joined) hipLaunchKernelGGL((cache_join_kernel<BF16>), dim3((unsigned)joins), dim3(256), 0, st, p, (int)rtiles);
   return hipGetLastError();
 }
 

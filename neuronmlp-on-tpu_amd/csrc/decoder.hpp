@@ -10,6 +10,10 @@
 
 namespace svdmlp {
 
+// Whether one launch can have so many blocks: HIP cuts a grid of 2^32 threads or
+// more to its low 32 bits, without an error.
+inline bool fits_launch(int64_t blocks, int threads) { return blocks * threads < (int64_t)1 << 32; }
+
 struct RopeParams {
   const void* q;  // (T, Hq, D)
   const void* k;  // (T, Hk, D)

@@ -669,6 +669,7 @@ hipError_t run(const PromptParams& p, hipStream_t st) {
   using C = PromptCfg<BF16>;
   // A sequence's last tile may be short: at most one more tile a sequence.
   const int64_t tiles = (int64_t)p.T * (p.Hq / p.Hk) / C::BM + p.B;
+  if (!fits_launch(tiles * p.Hk, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((prompt_kernel<C>), dim3((unsigned)(tiles * p.Hk)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
@@ -677,6 +678,7 @@ template <int DP>
 hipError_t run_pipe(const PromptParams& p, hipStream_t st) {
   using C = PipeCfg<DP>;
   const int64_t tiles = (int64_t)p.T * (p.Hq / p.Hk) / C::BM + p.B;
+  if (!fits_launch(tiles * p.Hk, 256)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((prompt_pipe_kernel<C>), dim3((unsigned)(tiles * p.Hk)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
@@ -692,7 +694,7 @@ hipError_t run_wave(const PromptParams& p, hipStream_t st) {
   w.q_t = p.q_t, w.q_h = p.q_h, w.k_t = p.k_t, w.k_h = p.k_h, w.v_t = p.v_t, w.v_h = p.v_h, w.o_t = p.o_t, w.o_h = p.o_h;
   w.T = p.T, w.B = p.B, w.Hq = p.Hq, w.Hk = p.Hk, w.D = p.D, w.causal = p.causal, w.splits = 1, w.c = p.c;
   const int64_t tiles = (int64_t)p.T * (p.Hq / p.Hk) / C::ROWS + p.B;
-  if (tiles * p.Hk > 0x7fffffff) return hipErrorInvalidValue;
+  if (!fits_launch(tiles * p.Hk, 64 * NW)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((cache_kernel<C>), dim3((unsigned)(tiles * p.Hk)), dim3(64 * NW), 0, st, w);
   return hipGetLastError();
 }

@@ -13,6 +13,8 @@
 // Bound by HBM: every value is read and written once.  A block takes a few
 // tokens, its threads their 16-byte pieces.  6007 tokens of 32 + 8 heads of 128
 // in bf16: 23.5 us, 5.2 TB/s, a copy's rate; 16 into a cache: 4.4 us, latency.
+#include <algorithm>
+
 #include "common.hpp"
 #include "decoder.hpp"
 
@@ -185,11 +187,24 @@ hipError_t launch_rope(const RopeParams& p, bool bf16, bool vec, hipStream_t st)
     // One token a block while those are few, else four: their cosines keep all
     // 256 threads busy at 128 turned values (2501 fp32 tokens of 32 heads of 64:
     // 9.9 us by one, 14.6 by four).
-    if (p.T < 4096)
+    if (p.T < 4096) {
       hipLaunchKernelGGL((rope_kernel<B, V, 1>), dim3((unsigned)p.T), dim3(256), p.rot * 4, st, p);
-    else
-      hipLaunchKernelGGL((rope_kernel<B, V, 4>), dim3((unsigned)((p.T + 3) / 4)), dim3(256), 4 * p.rot * 4, st, p);
-    return hipGetLastError();
+      return hipGetLastError();
+    }
+    constexpr int64_t kTokens = 1 << 24;  // a launch
+    static_assert(kTokens / 4 * 256 < (int64_t)1 << 32, "threads of a launch");
+    constexpr int ES = B ? 2 : 4;
+    for (int64_t t = 0; t < p.T; t += kTokens) {
+      RopeParams c = p;
+      c.T = std::min(kTokens, p.T - t);
+      c.q = static_cast<const char*>(p.q) + t * p.q_t * ES, c.k = static_cast<const char*>(p.k) + t * p.k_t * ES;
+      c.qo = static_cast<char*>(p.qo) + t * p.qo_t * ES, c.pos = p.pos + t;
+      if (p.slots) c.v = static_cast<const char*>(p.v) + t * p.v_t * ES, c.slots = p.slots + t;
+      else c.ko = static_cast<char*>(p.ko) + t * p.ko_t * ES;
+      hipLaunchKernelGGL((rope_kernel<B, V, 4>), dim3((unsigned)((c.T + 3) / 4)), dim3(256), 4 * p.rot * 4, st, c);
+      if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
   };
   using T = std::true_type;
   using F = std::false_type;

@@ -1,0 +1,69 @@
+"""The operators around the MLP block where layouts, indices and sizes are
+unusual: dimensions of one element with any stride, indices beyond 32 bits,
+calls of tens of millions of rows, memory shared with what a call reads."""
+
+import math
+
+import pytest
+import torch
+
+import svdmlp
+from svdmlp import decoder
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _randn(seed, *shape, dtype=BF):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g).to(dtype)
+
+
+def _laid_out(t, strides, gpu):
+    """t's values in a tensor of these strides on the GPU."""
+    room = 1 + sum(s * (n - 1) for s, n in zip(strides, t.shape))
+    out = torch.zeros(room, dtype=t.dtype, device=gpu).as_strided(t.shape, strides)
+    return out.copy_(t)
+
+
+@pytest.mark.parametrize("T,d,dtype", [((1 << 24) + 5, 8, BF), ((1 << 23) + 3, 6, F32)])
+def test_residual_norm_of_many_rows(gpu, T, d, dtype):
+    """More rows than one launch can have (2^32 threads): the same bits as of the rows alone."""
+    x = torch.randn((T, d), device=gpu, dtype=F32).to(dtype)
+    b, gate, w = x.flip(0), torch.randn((T, d), device=gpu).to(dtype), torch.rand(d, device=gpu)
+    r, n = svdmlp.residual_norm(x, b, w, gate=gate, scale=0.5)
+    for at in (0, (1 << 21) - 3, (1 << 22) - 2, (1 << 23) - 4, T - 7):
+        s = slice(at, at + 7)
+        r1, n1 = svdmlp.residual_norm(x[s], b[s], w, gate=gate[s], scale=0.5)
+        assert torch.equal(r[s], r1) and torch.equal(n[s], n1)
+
+
+def test_rope_of_many_tokens(gpu):
+    T = (1 << 26) + 9
+    q, k = torch.randn((T, 1, 2), device=gpu, dtype=BF), torch.randn((T, 1, 2), device=gpu, dtype=BF)
+    pos, f = torch.arange(T, device=gpu), torch.ones(1, dtype=torch.float64, device=gpu)
+    oq, ok = svdmlp.rope(q, k, pos, f)
+    kc, vc = torch.zeros((T, 1, 1, 2), device=gpu, dtype=BF), torch.zeros((T, 1, 1, 2), device=gpu, dtype=BF)
+    aq = svdmlp.rope_append(q, k, q, pos, f, kc, vc, pos)
+    assert torch.equal(aq, oq) and torch.equal(kc[:, 0], ok) and torch.equal(vc[:, 0], q)
+    for at in (0, (1 << 24) - 3, (1 << 25) - 3, (1 << 26) - 3, T - 7):
+        s = slice(at, at + 7)
+        q1, k1 = svdmlp.rope(q[s], k[s], pos[s], f)
+        assert torch.equal(oq[s], q1) and torch.equal(ok[s], k1)
+
+
+def test_attention_of_more_blocks_than_a_launch_has(gpu):
+    """Refused, not cut."""
+    q = torch.zeros((1, 1, 64), dtype=BF, device=gpu)
+    cu = torch.ones((1 << 24) + 2, dtype=torch.int32, device=gpu)
+    cu[0] = 0
+    with pytest.raises(ValueError, match="one launch"):
+        svdmlp.prompt_attention(q, q, q, cu)
+    assert torch.equal(svdmlp.prompt_attention(q, q, q, cu[:1 << 20]), q)
+    many = torch.zeros((1, 1, 1, 64), dtype=BF, device=gpu).expand((1 << 22) + 2, 1, 16, 64)
+    cache = torch.zeros((1, 16, 16, 64), dtype=BF, device=gpu)
+    table, lens = torch.zeros(((1 << 22) + 2, 1), dtype=torch.int32, device=gpu), torch.ones((1 << 22) + 2, dtype=torch.int32, device=gpu)
+    with pytest.raises(ValueError, match="one launch"):
+        svdmlp.cache_attention(many, cache, cache, table, lens)
