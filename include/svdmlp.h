@@ -296,7 +296,8 @@ int svdmlp_noalloc_status(int32_t reset, int64_t wait_bound, void* stream);
  * (RMSNorm, attention) and add the decode half that it has not.  dtype is
  * SVDMLP_BF16 or SVDMLP_F32, of every tensor but gains (fp32) and indices.
  * Softmax statistics and sums are in 32 bits.  Strides are host arrays, in
- * elements, in the order named (NULL: dense); the last dimension is contiguous.
+ * elements, in the order named (NULL: dense); the last dimension is contiguous,
+ * and the stride of a dimension of one element is not looked at by attention.
  * Query head h belongs to key/value head h / (Hq / Hk).  They need no
  * workspace but cache attention's, hold no state between calls, and can be
  * captured into graphs.  Indices are read on the device: one that points

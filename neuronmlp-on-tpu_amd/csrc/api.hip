@@ -2545,11 +2545,16 @@ int device_cus() {
 
 int act_size(int32_t dtype) { return dtype == SVDMLP_BF16 ? 2 : dtype == SVDMLP_F32 ? 4 : 0; }
 
-// Strides of the attention entry points: not negative.
-bool no_negative(const int64_t* s, int n) {
-  for (int i = 0; i < n; ++i)
-    if (s[i] < 0) return false;
-  return true;
+// Strides of the attention entry points: false if one is negative.  That of a
+// dimension of one element, which may be anything, becomes 0.
+bool plain_strides(const int64_t* from, std::initializer_list<int64_t> sizes, int64_t* to) {
+  bool ok = true;
+  for (int64_t n : sizes) {
+    *to = n == 1 ? 0 : *from;
+    ok = ok && *to >= 0;
+    ++from, ++to;
+  }
+  return ok;
 }
 
 bool pieces16(std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> elements, int es) {
@@ -2649,9 +2654,9 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
   if (flags & ~SVDMLP_CAUSAL) return fail("prompt_attention: unsupported flags 0x%x", flags);
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail("prompt_attention: scale must be positive and finite");
   const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hk * D, D, Hq * D, D};
-  const int64_t* s = strides ? strides : dense;
+  int64_t s[8];
   const int es = act_size(dtype);
-  if (!no_negative(s, 8)) return fail("prompt_attention: strides must not be negative");
+  if (!plain_strides(strides ? strides : dense, {T, Hq, T, Hk, T, Hk, T, Hq}, s)) return fail("prompt_attention: strides must not be negative");
   if (s[2] > kTokenStrideMost || s[4] > kTokenStrideMost) return fail("prompt_attention: keys or values are more than %lld elements apart", (long long)kTokenStrideMost);
   if (!pieces16({q, k, v, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]}, es))
     return fail("prompt_attention: the head size, strides and addresses must be whole 16-byte pieces");
@@ -2690,9 +2695,9 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
   if (!(scale > 0.f) || !std::isfinite(scale)) return fail("cache_attention: scale must be positive and finite");
   const int64_t dense[15] = {n * Hq * D, Hq * D, D, page * Hk * D, Hk * D, D, page * Hk * D, Hk * D, D,
                              n * Hq * D, Hq * D, D, width, n * n, n};
-  const int64_t* s = strides ? strides : dense;
+  int64_t s[15];
   const int es = act_size(dtype);
-  if (!no_negative(s, 15)) return fail("cache_attention: strides must not be negative");
+  if (!plain_strides(strides ? strides : dense, {B, n, Hq, pages, page, Hk, pages, page, Hk, B, n, Hq, B, B, n}, s)) return fail("cache_attention: strides must not be negative");
   if (!pieces16({q, k_cache, v_cache, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10], s[11]}, es))
     return fail("cache_attention: the head size, strides and addresses must be whole 16-byte pieces");
   if (s[4] > kTokenStrideMost || s[7] > kTokenStrideMost) return fail("cache_attention: rows of the cache are more than %lld elements apart", (long long)kTokenStrideMost);

@@ -72,12 +72,13 @@ def _launch(index: int, fn, *args) -> None:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself where the kernels can read it in place (last dimension
-    contiguous, rows in whole 16-byte pieces), else a contiguous copy."""
+    contiguous, rows in whole 16-byte pieces), else a contiguous copy.  (The
+    stride of a dimension of one element may be anything.)"""
     step = 8 if t.dtype is _BF16 else 4
     st = t.stride()
     if st[-1] == 1 and not t.data_ptr() % 16:
-        for s in st[:-1]:
-            if s % step:
+        for s, n in zip(st[:-1], t.shape):
+            if s % step and n > 1:
                 break
         else:
             return t
@@ -406,7 +407,7 @@ def prompt_attention(q, k, v, cu_seqlens=None, *, causal: bool = True, scale: fl
     if T == 0:
         return out
     q, k, v = _rows(q), _rows(k), _rows(v)
-    if k.stride(0) > 1 << 23 or v.stride(0) > 1 << 23:  # farther apart than the kernels' offsets reach
+    if T > 1 and (k.stride(0) > 1 << 23 or v.stride(0) > 1 << 23):  # farther apart than the kernels' offsets reach
         k, v = k.contiguous(), v.contiguous()
     st = _Strides8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2])
     _launch(index, _lib.load().svdmlp_prompt_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu, out.data_ptr(),

@@ -28,6 +28,37 @@ def _laid_out(t, strides, gpu):
     return out.copy_(t)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,K,strides", [
+    (1, 1, (132, 130, 1)), (1, 2, (3, 128, 1)), (1, 1, (1 << 24, 128, 1)), (3, 1, (136, 7, 1)), (1, 1, (0, 0, 1))])
+def test_prompt_attention_dimensions_of_one(gpu, dtype, T, K, strides):
+    """The stride of a dimension of one element says nothing: the same bits as from dense tensors."""
+    H, D = 4, 128
+    q, k, v = _randn(1, T, H, D, dtype=dtype), _randn(2, T, K, D, dtype=dtype), _randn(3, T, K, D, dtype=dtype)
+    want = svdmlp.prompt_attention(*(t.to(gpu) for t in (q, k, v)))
+    qs = (strides[0] if T == 1 else H * D, D, 1)
+    out = _laid_out(torch.zeros(T, H, D, dtype=dtype), qs, gpu)
+    got = svdmlp.prompt_attention(_laid_out(q, qs, gpu), _laid_out(k, strides, gpu), _laid_out(v, strides, gpu), out=out)
+    assert got is out and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("pages,page,K,strides", [
+    (1, 16, 2, (3, 128, 64, 1)), (5, 1, 2, (128, 7, 64, 1)), (5, 1, 2, (128, 1 << 24, 64, 1)), (3, 16, 1, (1024, 64, 5, 1)), (1, 1, 1, (1, 1, 1, 1))])
+def test_cache_attention_dimensions_of_one(gpu, dtype, pages, page, K, strides):
+    H, D = 4, 64
+    q, kc, vc = _randn(4, 1, 1, H, D, dtype=dtype), _randn(5, pages, page, K, D, dtype=dtype), _randn(6, pages, page, K, D, dtype=dtype)
+    table, lens = torch.arange(pages, dtype=torch.int32, device=gpu)[None], torch.tensor([pages * page], dtype=torch.int32, device=gpu)
+    want = svdmlp.cache_attention(*(t.to(gpu) for t in (q, kc, vc)), table, lens)
+    out = _laid_out(torch.zeros(1, 1, H, D, dtype=dtype), (5, 3, D, 1), gpu)
+    got = svdmlp.cache_attention(_laid_out(q, (7, 9, D, 1), gpu), _laid_out(kc, strides, gpu), _laid_out(vc, strides, gpu), table, lens, out=out)
+    assert got is out and torch.equal(got, want)
+    one = _laid_out(_randn(7, 1, 1, 1, D, dtype=dtype), (1, 1, 1, 1), gpu)  # one head too
+    if K == 1:
+        assert torch.equal(svdmlp.cache_attention(one, kc.to(gpu), vc.to(gpu), table, lens),
+                           svdmlp.cache_attention(one.contiguous().clone(), kc.to(gpu), vc.to(gpu), table, lens))
+
+
 @pytest.mark.parametrize("T,d,dtype", [((1 << 24) + 5, 8, BF), ((1 << 23) + 3, 6, F32)])
 def test_residual_norm_of_many_rows(gpu, T, d, dtype):
     """More rows than one launch can have (2^32 threads): the same bits as of the rows alone."""
