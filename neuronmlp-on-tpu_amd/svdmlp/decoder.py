@@ -155,14 +155,19 @@ def _apart(name: str, out: torch.Tensor, *tensors, own=()) -> None:
 
 
 def _index(name: str, t: torch.Tensor, shape, dtype, device) -> torch.Tensor:
-    """An index tensor as the kernels take it: t itself, or a copy of the type and layout."""
+    """An index tensor as the kernels take it: t itself, or a copy of the type and layout (what 32 bits
+    do not hold stays beyond every table and row, or negative)."""
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be an int32 or int64 tensor")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.get_device() != device:
         raise ValueError("all inputs must be on the same device")
-    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
+    if t.dtype is dtype and t.is_contiguous():
+        return t
+    if dtype is torch.int32 and t.dtype is torch.int64:
+        t = t.clamp(-1, 2 ** 31 - 1)
+    return t.to(dtype).contiguous()
 
 
 def _refuse_heads(q, k, *more) -> None:
@@ -449,6 +454,8 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
         raise ValueError("block_table must have shape (sequences, pages of the longest)")
     width = block_table.shape[1]
     if block_table.stride(1) != 1 or block_table.dtype is not torch.int32:
+        if block_table.dtype is torch.int64:
+            block_table = block_table.masked_fill((block_table < 0) | (block_table >= min(pages, 1 << 31)), -1)
         block_table = _index("block_table", block_table, (B, width), torch.int32, index)
     elif block_table.shape[0] != B or block_table.get_device() != index:
         raise ValueError(f"block_table must have shape ({B}, pages of the longest) on {q.device}")

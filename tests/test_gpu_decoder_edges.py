@@ -59,6 +59,26 @@ def test_cache_attention_dimensions_of_one(gpu, dtype, pages, page, K, strides):
                            svdmlp.cache_attention(one.contiguous().clone(), kc.to(gpu), vc.to(gpu), table, lens))
 
 
+def test_cache_attention_indices_beyond_32_bits(gpu):
+    """Pages of 64 bits that lie outside the cache hold no keys, and lengths are cut at the table, whatever their low 32 bits say."""
+    page, K, D, pages = 16, 2, 64, 6
+    q, kc, vc = (t.to(gpu) for t in (_randn(8, 4, 1, 4, D), _randn(9, pages, page, K, D), _randn(10, pages, page, K, D)))
+    table = torch.tensor([[0, (1 << 32) + 3, 1], [-(1 << 32) + 2, 2, 1 << 31], [3, 4, (1 << 40) + 5], [1, 1, -1]], device=gpu)
+    lens = torch.tensor([48, 1 << 31, (1 << 32) + 5, -(1 << 32) + 7], device=gpu)
+    inside = torch.where((table >= 0) & (table < pages), table, -1).int()
+    want = svdmlp.cache_attention(q, kc, vc, inside, lens.clamp(0, 48).int())
+    assert torch.equal(svdmlp.cache_attention(q, kc, vc, table, lens), want)
+    assert (want[3] == 0).all() and (want[:3] != 0).any()
+
+
+def test_prompt_attention_bounds_beyond_32_bits(gpu):
+    q, k, v = (_randn(s, 50, 2, 64).to(gpu) for s in (11, 12, 13))
+    want = svdmlp.prompt_attention(q, k, v, torch.tensor([0, 20, 50], dtype=torch.int32, device=gpu))
+    for cu in ([-(1 << 32) + 9, 20, (1 << 32) + 30], [0, 20, 1 << 31]):
+        got = svdmlp.prompt_attention(q, k, v, torch.tensor(cu, device=gpu), out=torch.zeros_like(q))
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("T,d,dtype", [((1 << 24) + 5, 8, BF), ((1 << 23) + 3, 6, F32)])
 def test_residual_norm_of_many_rows(gpu, T, d, dtype):
     """More rows than one launch can have (2^32 threads): the same bits as of the rows alone."""
