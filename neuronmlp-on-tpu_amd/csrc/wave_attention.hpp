@@ -146,9 +146,9 @@ __global__ __launch_bounds__(64 * C::NW, 1) void cache_kernel(CacheParams p) {
     at_chunk = SHARE && p.chunk == p.chunk_most ? b * p.splits + split : id;
     const int len = held(p, b);
     r0 = rt * C::ROWS;
-    kbeg = split * chunk, kend = min(len, kbeg + chunk);
     used = chunks_of(len, chunk);
     if (split >= used) return;
+    kbeg = split * chunk, kend = kbeg + min(len - kbeg, chunk);  // (kbeg + chunk may pass 2^31)
     context = len - p.n;
     // The chunk's pages.
     pg0 = kbeg / p.page;

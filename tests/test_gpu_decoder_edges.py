@@ -79,6 +79,22 @@ def test_prompt_attention_bounds_beyond_32_bits(gpu):
         assert torch.equal(got, want)
 
 
+def test_cache_attention_longest_sequence(gpu):
+    """A sequence near 2^31 tokens: its last chunk would end beyond (2^25 keys a chunk, 64 of them).  Keys of one page there
+    outweigh all others by e^60, so that the result is the mean of their values, all 1.5: sums of up to 2^21 weights of 1
+    and values of 1.5 are exact in 32 bits."""
+    page, width, D = 2097150, 1024, 8
+    kc, vc = torch.zeros((2, page, 1, D), dtype=BF, device=gpu), torch.full((2, page, 1, D), -2.0, dtype=BF, device=gpu)
+    kc[1, :, 0, 0], vc[1] = 60.0, 1.5
+    q = torch.zeros((1, 1, 1, D), dtype=BF, device=gpu)
+    q[..., 0] = 1.0
+    table = torch.zeros((1, width), dtype=torch.int32, device=gpu)
+    table[0, 1020] = 1
+    assert page * 1020 >= 63 * 2 ** 25 and page * width > 2 ** 31 - 8192
+    got = svdmlp.cache_attention(q, kc, vc, table, torch.tensor([page * width], device=gpu), scale=1.0)
+    assert (got == 1.5).all()
+
+
 @pytest.mark.parametrize("T,d,dtype", [((1 << 24) + 5, 8, BF), ((1 << 23) + 3, 6, F32)])
 def test_residual_norm_of_many_rows(gpu, T, d, dtype):
     """More rows than one launch can have (2^32 threads): the same bits as of the rows alone."""
