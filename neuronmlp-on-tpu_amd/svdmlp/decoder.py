@@ -13,8 +13,9 @@ are bfloat16 or float32 on a ROCm GPU; queries are (rows, Hq, D), keys and value
 of a fused projection are read in place (last dimension contiguous, 16-byte
 aligned rows); others are copied first.  Work goes to the current stream.
 
-As everywhere in this package the operators are for inference: tensors that
-ask for a gradient are refused (wrap the call in ``torch.no_grad()``).
+The operators are for inference: tensors that ask for a gradient, or carry a
+forward-mode tangent, are refused (wrap the call in ``torch.no_grad()``, or
+detach them).
 Every call goes to libsvdmlp.so; there is no CPU or PyTorch fallback.
 """
 
@@ -25,6 +26,7 @@ import math
 import threading
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _lib
 from .ops import _ACT_CODES, _PARTIALS_CACHE
@@ -53,10 +55,20 @@ def _refuse_dtype(*dtypes) -> None:
     raise TypeError("supported dtypes are bfloat16 and float32")
 
 
+def _gradients() -> bool:
+    """Whether a tensor may ask for a gradient here: in grad mode, or where forward-mode tangents live."""
+    return torch.is_grad_enabled() or _forward._current_level >= 0
+
+
 def _refuse_grad(name: str, *tensors) -> None:
+    backward, forward = torch.is_grad_enabled(), _forward._current_level >= 0
     for t in tensors:
-        if t is not None and t.requires_grad:
+        if t is None:
+            continue
+        if backward and t.requires_grad:
             raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), or on detached tensors")
+        if forward and _forward.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} has no gradient: call it on tensors without forward-mode tangents")
 
 
 def _launch(index: int, fn, *args) -> None:
@@ -261,10 +273,10 @@ def _rope_args(name, q, k, v, positions, inv_freq, scale):
         _refuse_dtype(dtype, k.dtype, *(() if v is None else (v.dtype,)))
     if index < 0 or k.get_device() != index or (v is not None and v.get_device() != index):
         _refuse_device(name, q, k, v)
-    if torch.is_grad_enabled():
-        _refuse_grad(name, q, k, v)
     if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or inv_freq.get_device() != index:
         raise ValueError("inv_freq must be a 1-D floating point tensor on the inputs' device")
+    if _gradients():
+        _refuse_grad(name, q, k, v, inv_freq)
     rot = 2 * inv_freq.shape[0]
     if not 0 < rot <= D:
         raise ValueError(f"{rot} turned values (two a frequency) of a head of {D}")
@@ -289,6 +301,8 @@ def rope(q, k, positions, inv_freq, *, interleaved: bool = False, scale: float =
         qo, ko = q.new_empty((T, Hq, D)), q.new_empty((T, Hk, D))
     else:
         qo, ko = out
+        if _gradients():
+            _refuse_grad("rope", qo, ko)
         _writable("out[0]", qo, (T, Hq, D), q)
         _writable("out[1]", ko, (T, Hk, D), q)
         _apart("out[0]", qo, q, k, ko, own=(q,))
@@ -323,8 +337,8 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interl
         _refuse_dtype(q.dtype, k_cache.dtype, v_cache.dtype)
     if k_cache.get_device() != index or v_cache.get_device() != index:
         _refuse_device("rope_append", q, k_cache, v_cache)
-    if torch.is_grad_enabled():
-        _refuse_grad("rope_append", k_cache, v_cache)
+    if _gradients():
+        _refuse_grad("rope_append", k_cache, v_cache, out)
     if not k_cache.is_contiguous():
         _writable("k_cache", k_cache, cs, q)
     if not v_cache.is_contiguous():
@@ -392,8 +406,8 @@ def prompt_attention(q, k, v, cu_seqlens=None, *, causal: bool = True, scale: fl
         _refuse_dtype(dtype, k.dtype, v.dtype)
     if index < 0 or k.get_device() != index or v.get_device() != index:
         _refuse_device("prompt_attention", q, k, v)
-    if torch.is_grad_enabled():
-        _refuse_grad("prompt_attention", q, k, v)
+    if _gradients():
+        _refuse_grad("prompt_attention", q, k, v, out)
     _head_size(D, dtype)
     scale = _attention_scale(scale, D)
     B, cu = 1, None
@@ -446,8 +460,8 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
         _refuse_dtype(dtype, k_cache.dtype, v_cache.dtype)
     if index < 0 or k_cache.get_device() != index or v_cache.get_device() != index:
         _refuse_device("cache_attention", q, k_cache, v_cache)
-    if torch.is_grad_enabled():
-        _refuse_grad("cache_attention", q, k_cache, v_cache)
+    if _gradients():
+        _refuse_grad("cache_attention", q, k_cache, v_cache, out)
     _head_size(D, dtype)
     scale = _attention_scale(scale, D)
     if block_table.dim() != 2 or block_table.shape[1] == 0:
@@ -572,9 +586,8 @@ def residual_norm(x, branch, weight, *, post_weight=None, gate=None, scale: floa
     index = x.get_device()
     if index < 0 or (branch is not None and branch.get_device() != index) or (gate is not None and gate.get_device() != index):
         _refuse_device("residual_norm", x, branch, gate)
-    if torch.is_grad_enabled() and (x.requires_grad or (branch is not None and branch.requires_grad) or gate is not None
-                                    or post_weight is not None or (weight is not None and weight.requires_grad)):
-        _refuse_grad("residual_norm", x, branch, gate, weight, post_weight)
+    if _gradients():
+        _refuse_grad("residual_norm", x, branch, gate, weight, post_weight, *(out or ()))
     if branch is not None and branch.shape != shape:
         raise ValueError(f"branch must have x's shape {tuple(shape)}, got {tuple(branch.shape)}")
     if gate is not None and tuple(gate.shape) not in ((d,), (T, d)):

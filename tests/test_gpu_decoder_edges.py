@@ -134,3 +134,45 @@ def test_attention_of_more_blocks_than_a_launch_has(gpu):
     table, lens = torch.zeros(((1 << 22) + 2, 1), dtype=torch.int32, device=gpu), torch.ones((1 << 22) + 2, dtype=torch.int32, device=gpu)
     with pytest.raises(ValueError, match="one launch"):
         svdmlp.cache_attention(many, cache, cache, table, lens)
+
+
+def test_gradients_of_every_tensor_are_refused(gpu):
+    """Frequencies, outputs, gains and forward-mode tangents too: nothing that asks for a gradient is used without one."""
+    import torch.autograd.forward_ad as fwd
+
+    q, k, pos = torch.randn(4, 2, 8, device=gpu), torch.randn(4, 1, 8, device=gpu), torch.arange(4, device=gpu)
+    f, x, w = torch.ones(4, device=gpu), torch.randn(4, 16, device=gpu), torch.ones(16, device=gpu)
+    c, qc = torch.zeros(2, 16, 1, 8, device=gpu), q.view(4, 1, 2, 8)
+    table, lens = torch.zeros(4, 2, dtype=torch.int32, device=gpu), torch.ones(4, dtype=torch.int32, device=gpu)
+
+    def calls(ask):
+        return [
+            lambda: svdmlp.rope(ask(q), k, pos, f), lambda: svdmlp.rope(q, k, pos, ask(f)),
+            lambda: svdmlp.rope(q, k, pos, f, out=(ask(torch.empty_like(q)), torch.empty_like(k))),
+            lambda: svdmlp.rope(q, k, pos, f, out=(torch.empty_like(q), ask(torch.empty_like(k)))),
+            lambda: svdmlp.rope_append(q, k, ask(k), pos, f, c.clone(), c.clone(), pos),
+            lambda: svdmlp.rope_append(q, k, k, pos, ask(f), c.clone(), c.clone(), pos),
+            lambda: svdmlp.rope_append(q, k, k, pos, f, c.clone(), ask(c.clone()), pos),
+            lambda: svdmlp.rope_append(q, k, k, pos, f, c.clone(), c.clone(), pos, out=ask(torch.empty_like(q))),
+            lambda: svdmlp.prompt_attention(q, ask(k), k), lambda: svdmlp.prompt_attention(q, k, k, out=ask(torch.empty_like(q))),
+            lambda: svdmlp.cache_attention(qc, c, ask(c.clone()), table, lens),
+            lambda: svdmlp.cache_attention(qc, c, c, table, lens, out=ask(torch.empty_like(qc))),
+            lambda: svdmlp.residual_norm(x, x, ask(w)), lambda: svdmlp.residual_norm(x, ask(x), w),
+            lambda: svdmlp.residual_norm(x, x, w, post_weight=ask(w)), lambda: svdmlp.residual_norm(x, x, w, gate=ask(w)),
+            lambda: svdmlp.residual_norm(x, x, w, out=(ask(torch.empty_like(x)), None)),
+            lambda: svdmlp.residual_norm(x, x, w, out=(None, ask(torch.empty_like(x)))),
+        ]
+
+    for call in calls(lambda t: t.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with fwd.dual_level():
+        for call in calls(lambda t: fwd.make_dual(t.clone(), torch.ones_like(t))):
+            with pytest.raises(ValueError, match="no gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="no gradient"):  # which does not end tangents
+                call()
+        for call in calls(lambda t: t):
+            call()
