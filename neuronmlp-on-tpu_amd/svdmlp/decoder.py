@@ -547,8 +547,12 @@ def _partials(index: int, nbytes: int, counters: int) -> tuple[torch.Tensor, tor
     key = (index, _raw_stream(index))
     held = _PARTIALS_CACHE.get(key)
     if held is None or held[0].numel() < nbytes or held[1].numel() < counters:
-        held = _PARTIALS_CACHE[key] = (torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device),
-                                       torch.zeros(max(counters, 4096), dtype=torch.int32, device=device))
+        room, zeros = held or (None, None)  # each grown by itself
+        if room is None or room.numel() < nbytes:
+            room = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        if zeros is None or zeros.numel() < counters:
+            zeros = torch.zeros(max(counters, 4096), dtype=torch.int32, device=device)
+        held = _PARTIALS_CACHE[key] = (room, zeros)
     return held
 
 

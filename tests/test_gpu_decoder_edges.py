@@ -176,3 +176,15 @@ def test_gradients_of_every_tensor_are_refused(gpu):
                 call()
         for call in calls(lambda t: t):
             call()
+
+
+def test_room_for_partial_sums_does_not_shrink(gpu):
+    """Calls of more counters and fewer bytes, and of fewer counters and more bytes, in turn: one pair of buffers serves both."""
+    svdmlp.clear_workspace_cache()
+    decoder._partials(0, 1 << 22, 10)
+    wide = decoder._partials(0, 1 << 10, 9000)
+    assert wide[0].numel() >= 1 << 22 and wide[1].numel() >= 9000
+    again = decoder._partials(0, 1 << 22, 10)
+    assert again[0] is wide[0] and again[1] is wide[1]
+    assert (wide[1] == 0).all()
+    svdmlp.clear_workspace_cache()
