@@ -536,13 +536,21 @@ def _sizes(lib, index, *sizes) -> tuple[int, int]:
     return plan
 
 
+def _capturing(index: int) -> bool:
+    """Whether device `index`'s current stream is being captured (torch asks for the current device's)."""
+    if torch.cuda.current_device() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _partials(index: int, nbytes: int, counters: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Room for partial sums and zeroed counters.  One pair a (device, stream),
     grown on demand and kept until :func:`svdmlp.clear_workspace_cache`: every
     call leaves the counters zero for the next on its stream.  A captured call
     gets its own from the graph's pool, its counters cleared by the graph."""
     device = f"cuda:{index}"
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(index):
         return torch.empty(nbytes, dtype=torch.uint8, device=device), torch.zeros(counters, dtype=torch.int32, device=device)
     key = (index, _raw_stream(index))
     held = _PARTIALS_CACHE.get(key)
