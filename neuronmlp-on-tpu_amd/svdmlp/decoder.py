@@ -305,8 +305,8 @@ def rope(q, k, positions, inv_freq, *, interleaved: bool = False, scale: float =
             _refuse_grad("rope", qo, ko)
         _writable("out[0]", qo, (T, Hq, D), q)
         _writable("out[1]", ko, (T, Hk, D), q)
-        _apart("out[0]", qo, q, k, ko, own=(q,))
-        _apart("out[1]", ko, k, q, own=(k,))
+        _apart("out[0]", qo, q, k, ko, positions, inv_freq, own=(q,))
+        _apart("out[1]", ko, k, q, positions, inv_freq, own=(k,))
     if T == 0:
         return qo, ko
     q, k = _last(q), _last(k)
@@ -346,7 +346,7 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interl
     slots = _index("slots", slots, (T,), torch.int64, index)
     if out is not None:
         _writable("out", out, (T, Hq, D), q)
-        _apart("out", out, q, k, v, k_cache, v_cache, own=(q,))
+        _apart("out", out, q, k, v, k_cache, v_cache, positions, inv_freq, slots, own=(q,))
     if T == 0:
         return q.new_empty((0, Hq, D)) if out is None else out
     q, k, v = _last(q), _last(k), _last(v)
@@ -362,11 +362,17 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interl
     if (kcp < vce and vcp < kce) or (low < kce and kcp < high) or (low < vce and vcp < high):
         _apart("k_cache", k_cache, v_cache, q, k, v)
         _apart("v_cache", v_cache, q, k, v)
+    pp, fp, sp = positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr()
+    pe, fe, se = pp + 8 * T, fp + 4 * rot, sp + 8 * T
+    if ((pp < kce and kcp < pe) or (sp < kce and kcp < se) or (fp < kce and kcp < fe) or (pp < vce and vcp < pe)
+            or (sp < vce and vcp < se) or (fp < vce and vcp < fe)):
+        _apart("k_cache", k_cache, positions, inv_freq, slots)
+        _apart("v_cache", v_cache, positions, inv_freq, slots)
     if out is None:
         out = q.new_empty((T, Hq, D))
     o = out.stride()
     st = _Strides14(a[0], a[1], b[0], b[1], c[0], c[1], o[0], o[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2])
-    _launch(index, _lib.load().svdmlp_rope_append, qp, kp, vp, positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(),
+    _launch(index, _lib.load().svdmlp_rope_append, qp, kp, vp, pp, fp, sp,
             out.data_ptr(), kcp, vcp, _address(st), T, cs[0], cs[1], Hq, Hk, D, rot, scale, _ACT_CODES[q.dtype],
             1 if interleaved else 0)
     return out
@@ -422,7 +428,7 @@ def prompt_attention(q, k, v, cu_seqlens=None, *, causal: bool = True, scale: fl
     else:
         _writable("out", out, (T, Hq, D), q)
         _aligned("out", out)
-        _apart("out", out, q, k, v)
+        _apart("out", out, q, k, v, *(() if cu is None else (cu_seqlens,)))
     if T == 0:
         return out
     q, k, v = _rows(q), _rows(k), _rows(v)
@@ -495,7 +501,7 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
     else:
         _writable("out", out, (B, n, Hq, D), q)
         _aligned("out", out)
-        _apart("out", out, q, k_cache, v_cache)
+        _apart("out", out, q, k_cache, v_cache, block_table, lengths, *(() if tree is None else (tree,)))
     if B == 0:
         return out
     q = _rows(q)
@@ -628,7 +634,7 @@ def residual_norm(x, branch, weight, *, post_weight=None, gate=None, scale: floa
     r = n = None
     if out is not None:
         r, n = out
-        inputs = [a for a in (x, branch, gate) if a is not None]
+        inputs = [a for a in (x, branch, gate, w, pw) if a is not None]
         for name, t in (("out[0]", r), ("out[1]", n)):
             if t is not None:
                 _writable(name, t, (T, d), x)

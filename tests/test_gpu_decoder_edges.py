@@ -188,3 +188,45 @@ def test_room_for_partial_sums_does_not_shrink(gpu):
     assert again[0] is wide[0] and again[1] is wide[1]
     assert (wide[1] == 0).all()
     svdmlp.clear_workspace_cache()
+
+
+def test_outputs_apart_from_everything_read(gpu):
+    """Outputs that share memory with gains, frequencies, positions, slots, bounds, tables, lengths or a tree are refused."""
+    room = torch.zeros(4096, device=gpu)
+    q, k, v = torch.randn(4, 2, 8, device=gpu), torch.randn(4, 1, 8, device=gpu), torch.randn(4, 1, 8, device=gpu)
+    pos, f, slots = torch.arange(4, device=gpu), torch.ones(4, dtype=torch.float64, device=gpu), torch.arange(4, device=gpu)
+    whole = room[:64].view(4, 2, 8)
+    half = room[64:96].view(4, 1, 8)
+    as_i64, as_i32, as_f64, as_u8 = room.view(torch.int64), room.view(torch.int32), room.view(torch.float64), room.view(torch.uint8)
+    caches = [torch.zeros(2, 16, 1, 8, device=gpu) for _ in range(2)]
+    x, b, w, g = torch.randn(4, 8, device=gpu), torch.randn(4, 8, device=gpu), torch.ones(8, device=gpu), torch.ones(8, device=gpu)
+    qc = q.view(4, 1, 2, 8)
+    table, lens = torch.zeros(4, 2, dtype=torch.int32, device=gpu), torch.ones(4, dtype=torch.int32, device=gpu)
+    tree = torch.ones(4, 1, 1, dtype=torch.bool, device=gpu)
+    cases = [
+        lambda: svdmlp.rope(q, k, as_i64[:4], f, out=(whole, half)),
+        lambda: svdmlp.rope(q, k, as_i64[32:36], f, out=(whole, half)),
+        lambda: svdmlp.rope(q, k, pos, as_f64[:4], out=(whole, half)),
+        lambda: svdmlp.rope_append(q, k, v, as_i64[:4], f, *caches, slots, out=whole),
+        lambda: svdmlp.rope_append(q, k, v, pos, as_f64[:4], *caches, slots, out=whole),
+        lambda: svdmlp.rope_append(q, k, v, pos, f, *caches, as_i64[:4], out=whole),
+        lambda: svdmlp.rope_append(q, k, v, pos, f, room[:256].view(2, 16, 1, 8), caches[1], as_i64[:4]),
+        lambda: svdmlp.rope_append(q, k, v, as_i64[100:104], f, caches[0], room[:256].view(2, 16, 1, 8), slots),
+        lambda: svdmlp.rope_append(q, k, v, pos, as_f64[100:104], caches[0], room[:256].view(2, 16, 1, 8), slots),
+        lambda: svdmlp.prompt_attention(q, k, v, as_i32[:2], out=whole),
+        lambda: svdmlp.cache_attention(qc, *caches, as_i32[:8].view(4, 2), lens, out=whole.view(4, 1, 2, 8)),
+        lambda: svdmlp.cache_attention(qc, *caches, table, as_i32[60:64], out=whole.view(4, 1, 2, 8)),
+        lambda: svdmlp.cache_attention(qc, *caches, table, lens, tree=as_u8[:4].view(4, 1, 1), out=whole.view(4, 1, 2, 8)),
+        lambda: svdmlp.residual_norm(x, b, room[8:16], out=(room[:32].view(4, 8), None)),
+        lambda: svdmlp.residual_norm(x, b, w, post_weight=room[8:16], out=(None, room[:32].view(4, 8))),
+        lambda: svdmlp.residual_norm(x, b, w, gate=room[8:16], out=(None, room[:32].view(4, 8))),
+    ]
+    for call in cases:
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    # beside each other in one buffer they are fine
+    svdmlp.rope(q, k, as_i64[512:516], as_f64[600:604], out=(whole, half))
+    svdmlp.prompt_attention(q, k, v, as_i32[64:66], out=whole)
+    svdmlp.cache_attention(qc, *caches, as_i32[64:72].view(4, 2), as_i32[72:76], tree=as_u8[400:404].view(4, 1, 1), out=whole.view(4, 1, 2, 8))
+    svdmlp.residual_norm(x, b, room[128:136], post_weight=room[136:144], gate=room[144:152], out=(whole.view(8, 8)[:4], whole.view(8, 8)[4:]))
+    assert torch.equal(g, torch.ones_like(g)) and not tree.logical_not().any()
