@@ -12,9 +12,16 @@
 // product's sum over keys may take them in any order, so key 8 b + 4 h + r is
 // given the place that its weight already has.
 //
-// Statistics are in 32 bits, in the log2 domain: p = exp2(c s - m).  The weights
-// are rounded to the values' type for the second product (bf16: their relative
-// error 2^-9 averages out over the keys); their sum is of the unrounded ones.
+// Statistics are in 32 bits, in the log2 domain: p = exp2(c s - m), c the scale
+// times log2(e), off by at most 3 2^-24 of itself (both factors' rounding and
+// the product's), beside the D roundings of the score's own sum.
+// bf16: the weights are rounded to bf16 for the second product, whose operands
+// are of that type (two parts a weight, for 16 bits, would make it half as many
+// products again in all).  Each is off by at most 2^-8 of itself, so a result by
+// 2^-8 of the weighted mean of |v - out|; with random keys and values results
+// are off by 0.0020 to 0.0023 rms, by 0.0016 to 0.0017 from their own rounding
+// alone.  The sum is of the rounded weights: values that all keys share come out
+// as they are.
 #pragma once
 
 #include "common.hpp"

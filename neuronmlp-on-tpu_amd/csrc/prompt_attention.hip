@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           pf[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], p.c, -m));
-          st[g].l += pf[g][i];
+          if constexpr (!BF16) st[g].l += pf[g][i];
         }
       }
       if constexpr (BF16) {
@@ -163,7 +163,10 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
 #pragma unroll
           for (int g = 0; g < QG; ++g)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) pb[g][w] = pack_bf16x2(pf[g][8 * t + 2 * w], pf[g][8 * t + 2 * w + 1]);
+            for (int w = 0; w < 4; ++w) {
+              pb[g][w] = pack_bf16x2(pf[g][8 * t + 2 * w], pf[g][8 * t + 2 * w + 1]);
+              st[g].l = add_pair(pb[g][w], st[g].l);
+            }
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
             u32x4 vf = at.values(lv + 32 * u * RB, t, d);

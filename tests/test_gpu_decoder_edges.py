@@ -190,6 +190,30 @@ def test_room_for_partial_sums_does_not_shrink(gpu):
     svdmlp.clear_workspace_cache()
 
 
+def _equal_values(D, K, T, dtype, gpu):
+    """Queries and keys whose weights are 1 and exp(-t), many t, and values alike for all keys."""
+    q, k = torch.zeros(T, K, D), torch.zeros(T, K, D)
+    q[:, :, 0] = torch.linspace(0.05, 1.4, T)[:, None]
+    k[1:, :, 0] = -1.0
+    v = _randn(20, 1, K, D, dtype=dtype).expand(T, K, D).contiguous()
+    return q.to(dtype).to(gpu), k.to(dtype).to(gpu), v.to(gpu)
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 200, 256])
+@pytest.mark.parametrize("T,K", [(64, 2), (257, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_weights_are_summed_as_rounded(gpu, D, T, K, causal):
+    """Values that all keys share come out as they are: the sum is of the weights as the products take them, rounded to
+    bf16.  What is left are sums in 32 bits, T + 8 roundings of at most 2^-23 each: 2^-14 for 257 tokens, less than half a
+    step of bf16 (2^-9 of a value at least), so the result rounds to the value itself."""
+    q, k, v = _equal_values(D, K, T, BF, gpu)
+    assert torch.equal(svdmlp.prompt_attention(q, k, v, causal=causal, scale=1.0), v)
+    table, lens = torch.arange(T, dtype=torch.int32, device=gpu)[None], torch.tensor([T], dtype=torch.int32, device=gpu)
+    for n in (1, 9):
+        got = svdmlp.cache_attention(q[None, -n:], k[:, None], v[:, None], table, lens, scale=1.0)
+        assert torch.equal(got[0], v[-n:])
+
+
 def test_outputs_apart_from_everything_read(gpu):
     """Outputs that share memory with gains, frequencies, positions, slots, bounds, tables, lengths or a tree are refused."""
     room = torch.zeros(4096, device=gpu)
