@@ -68,7 +68,7 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   const int row = D * (bf16 ? 2 : 4), waves = row <= 256 ? 4 : row <= 512 ? 2 : 1;  // of a block that shares a chunk
   // One wave a block, of chunks of 256 keys, where those give every SIMD one.
   // Else, and where a wave has 64 rows (whose partial sums, written and read,
-  // would be a quarter of such a chunk's keys and values), blocks that share a
+  // would be half of such a chunk's keys and values), blocks that share a
   // chunk, of chunks that give every CU one; or three, of different lengths, if
   // the chunks stay long.  Blocks that share their tiles: two a CU, which is what
   // fits (trees of 16 over up to 16384 tokens, one, two, three, four a CU: 131,
@@ -77,6 +77,11 @@ CachePlan plan_cache_attention(int B, int n, int Hq, int Hk, int D, bool bf16, i
   plan.waves = rt == 32 && base * ((capacity + kSolo - 1) / kSolo) >= 4 * (int64_t)cus ? 1 : waves;
   int64_t c = kSolo;
   if (plan.waves > 1 || waves == 1) c = std::max(capacity * base / cus / 3, std::min<int64_t>(1024, capacity * base / cus));
+  // Over four waves a SIMD, chunks of at least as many keys as keep all row tiles'
+  // partial sums to a quarter of the keys and values (512 rows of heads of 256, 96
+  // sequences of up to 21800 tokens: 2.89 GB of them and 3.21 ms by chunks of 384
+  // keys, 0.56 GB and 2.10 ms by 2048; 128 rows, 32 of 16384: 454 and 344 us).
+  else c = std::max(c, std::min(rows * (bf16 ? 4 : 2), capacity * base / (16 * cus)));
   // Of few sequences, whose lengths may be any part of the table's width, from
   // the lengths (shared_chunk), 512 at least; many even out by themselves (heads
   // of 128, 8 of keys, 16 new tokens; 4 sequences of up to 32768 tokens 75 us from

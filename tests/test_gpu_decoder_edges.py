@@ -254,3 +254,21 @@ def test_outputs_apart_from_everything_read(gpu):
     svdmlp.cache_attention(qc, *caches, as_i32[64:72].view(4, 2), as_i32[72:76], tree=as_u8[400:404].view(4, 1, 1), out=whole.view(4, 1, 2, 8))
     svdmlp.residual_norm(x, b, room[128:136], post_weight=room[136:144], gate=room[144:152], out=(whole.view(8, 8)[:4], whole.view(8, 8)[4:]))
     assert torch.equal(g, torch.ones_like(g)) and not tree.logical_not().any()
+
+
+@pytest.mark.parametrize("dtype,B,n,H,K,D,page,most", [(BF, 24, 64, 8, 1, 256, 16, 3000), (BF, 40, 20, 8, 1, 200, 48, 4000), (F32, 24, 40, 16, 2, 128, 16, 2500)])
+def test_cache_attention_many_rows_of_large_heads(gpu, dtype, B, n, H, K, D, page, most):
+    """Many row tiles of 32 over longer chunks than 256 keys."""
+    import test_gpu_decoder as base
+
+    g = base._gen(B + n)
+    lens = [most, 0, n - 1, n] + [int(x) for x in torch.randint(1, most, (B - 4,), generator=g)]
+    table, pages = base._pages(g, lens, page)
+    q, kc, vc = (base._randn(g, *shape, dtype=dtype) for shape in ((B, n, H, D), (pages, page, K, D), (pages, page, K, D)))
+    tree = base._random_tree(g, B, n)
+    some = [0, 1, 2, 3, B - 1]
+    out, tol = base._cache_ref(q[some], kc, vc, table[some], [lens[b] for b in some], tree[some], 1 / math.sqrt(D))
+    args = [t.to(gpu) for t in (q, kc, vc, table)] + [torch.tensor(lens, device=gpu)]
+    got = svdmlp.cache_attention(*args, tree=tree.to(gpu))
+    base._close(got[some], out, tol)
+    assert torch.equal(got, svdmlp.cache_attention(*args, tree=tree.to(gpu)))
