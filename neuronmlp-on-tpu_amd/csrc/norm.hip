@@ -22,7 +22,6 @@ namespace {
 template <int NT>
 __device__ __forceinline__ float block_sum(float v, float* part) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  if constexpr (NT == 64) return v;
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
   float t = 0.f;

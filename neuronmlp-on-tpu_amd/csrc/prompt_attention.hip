@@ -19,26 +19,26 @@ namespace {
 
 // The kernel of heads over 128: four waves of 32 rows share tiles of 32 keys in
 // LDS; the registers' loads of the next tile wait while one is computed.  Bound by
-// its LDS reads (a piece feeds one product) and registers: 8 heads of 256, 4000
-// tokens causal 230 us, 285 TFLOP/s.
+// its LDS reads (a piece feeds one product) and registers: 8 heads of 256, 8 of
+// keys, 4000 tokens causal 247 us, 265 TFLOP/s (6 us of it for the sum of the
+// weights as rounded).
 template <bool BF16_>
 struct PromptCfg {
   static constexpr bool BF16 = BF16_;
   static constexpr int DP = 256;  // head elements held (D rounded up)
-  static constexpr int QG = 1;    // 32-row groups a wave
   static constexpr int ES = BF16 ? 2 : 4;
   static constexpr int RB = DP * ES;         // bytes of a key row in LDS
   static constexpr int PIECES = RB / 16;
   static constexpr int STEPS = RB / 32;      // 32-byte steps of the head
   static constexpr int KB = 32;              // keys a tile
-  static constexpr int BM = 128 * QG;        // rows a block
+  static constexpr int BM = 128;             // rows a block
   static constexpr int TILE = KB * RB;
 };
 
 template <class C>
 __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
   constexpr bool BF16 = C::BF16;
-  constexpr int ES = C::ES, RB = C::RB, QG = C::QG, KB = C::KB, DB = C::DP / 32;
+  constexpr int ES = C::ES, RB = C::RB, KB = C::KB, DB = C::DP / 32;
   __shared__ __attribute__((aligned(1024))) char lds[2 * C::TILE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
   const int G = p.Hq / p.Hk;
@@ -51,33 +51,24 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
   const int nkeys = p.causal ? tok_last + 1 : len;
 
   // Q: lane half h holds the 16-byte piece 2 s + h of its row at step s.
-  u32x4 qf[QG][C::STEPS];
-  int tok[QG];
+  u32x4 qf[C::STEPS];
   const int npieces = p.D * ES / 16;
+  const int r = row0 + wave * 32 + col;
+  const bool in = r < rows;
+  const int tok = in ? r / G : 0;
+  const char* const qp = static_cast<const char*>(p.q) + ((int64_t)(start + tok) * p.q_t + (int64_t)(hk * G + (in ? r - tok * G : 0)) * p.q_h) * ES;
 #pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int r = row0 + (wave * QG + g) * 32 + col;
-    const bool in = r < rows;
-    tok[g] = in ? r / G : 0;
-    const char* qp = static_cast<const char*>(p.q) +
-                     ((int64_t)(start + tok[g]) * p.q_t + (int64_t)(hk * G + (in ? r - tok[g] * G : 0)) * p.q_h) * ES;
-#pragma unroll
-    for (int s = 0; s < C::STEPS; ++s) {
-      const int c = 2 * s + half;
-      qf[g][s] = in && c < npieces ? *reinterpret_cast<const u32x4*>(qp + 16 * c) : u32x4{0u, 0u, 0u, 0u};
-    }
+  for (int s = 0; s < C::STEPS; ++s) {
+    const int c = 2 * s + half;
+    qf[s] = in && c < npieces ? *reinterpret_cast<const u32x4*>(qp + 16 * c) : u32x4{0u, 0u, 0u, 0u};
   }
 
-  f32x16 o[QG][DB];
-  RowState st[QG];
+  f32x16 o[DB];
+  RowState st = {-INFINITY, 0.f};
 #pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    st[g] = {-INFINITY, 0.f};
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[g][d][i] = 0.f;
-  }
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   const char* const kbase = static_cast<const char*>(p.k) + ((int64_t)start * p.k_t + (int64_t)hk * p.k_h) * ES;
   const char* const vbase = static_cast<const char*>(p.v) + ((int64_t)start * p.v_t + (int64_t)hk * p.v_h) * ES;
   const attn_lds lk = (attn_lds)lds, lv = lk + C::TILE;
@@ -109,106 +100,79 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
     if (k0 + KB < nkeys) fetch(k0 + KB);
     const bool masked = p.causal && k0 + KB - 1 > tok_first;  // not every row sees every key
     const bool edge = masked || k0 + KB > nkeys;
+    f32x16 s = {};
 #pragma unroll
-    for (int u = 0; u < KB / 32; ++u) {
-      const int ku = k0 + 32 * u;
-      if (ku >= nkeys) break;
-      f32x16 s[QG];
+    for (int t = 0; t < C::STEPS; ++t) s = attn_mfma<BF16>(at.key(lk, t), qf[t], s);
+    if (edge) {
+      const int last = p.causal ? min(tok, nkeys - 1) : nkeys - 1;
 #pragma unroll
-      for (int g = 0; g < QG; ++g)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[g][i] = 0.f;
-#pragma unroll
-      for (int t = 0; t < C::STEPS; ++t) {
-        const u32x4 kf = at.key(lk + 32 * u * RB, t);
-#pragma unroll
-        for (int g = 0; g < QG; ++g) s[g] = attn_mfma<BF16>(kf, qf[g][t], s[g]);
+      for (int i = 0; i < 16; ++i) {
+        const int key = k0 + 8 * (i >> 2) + 4 * half + (i & 3);
+        s[i] = key <= last ? s[i] : -INFINITY;
       }
-      float pf[QG][16];
+    }
+    float mx = s[0];
 #pragma unroll
-      for (int g = 0; g < QG; ++g) {
-        if (edge) {
-          const int last = p.causal ? min(tok[g], nkeys - 1) : nkeys - 1;
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * p.c;
+    if (__any(mx > st.m + kSlack)) {
+      const float m = fmaxf(st.m, mx);
+      const float a = m == -INFINITY ? 1.f : exp2f(st.m - m);
+      st.m = m;
+      st.l *= a;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = ku + 8 * (i >> 2) + 4 * half + (i & 3);
-            s[g][i] = key <= last ? s[g][i] : -INFINITY;
-          }
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= a;
+    }
+    const float m = st.m == -INFINITY ? 0.f : st.m;
+    float pf[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      pf[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -m));
+      if constexpr (!BF16) st.l += pf[i];
+    }
+    if constexpr (BF16) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {  // 16 keys each
+        u32x4 pb;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          pb[w] = pack_bf16x2(pf[8 * t + 2 * w], pf[8 * t + 2 * w + 1]);
+          st.l = add_pair(pb[w], st.l);
         }
-        float mx = s[g][0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[g][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * p.c;
-        if (__any(mx > st[g].m + kSlack)) {
-          const float m = fmaxf(st[g].m, mx);
-          const float a = m == -INFINITY ? 1.f : exp2f(st[g].m - m);
-          st[g].m = m;
-          st[g].l *= a;
+        for (int d = 0; d < DB; ++d) {
+          u32x4 vf = at.values(lv, t, d);
+          if (masked)
 #pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[g][d][i] *= a;
-        }
-        const float m = st[g].m == -INFINITY ? 0.f : st[g].m;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          pf[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], p.c, -m));
-          if constexpr (!BF16) st[g].l += pf[g][i];
+            for (int w = 0; w < 4; ++w) vf[w] = scrub<true>(vf[w], bad);
+          o[d] = attn_mfma<true>(vf, pb, o[d]);
         }
       }
-      if constexpr (BF16) {
+    } else {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {  // 16 keys each
-          u32x4 pb[QG];
+      for (int i = 0; i < 16; ++i)
 #pragma unroll
-          for (int g = 0; g < QG; ++g)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              pb[g][w] = pack_bf16x2(pf[g][8 * t + 2 * w], pf[g][8 * t + 2 * w + 1]);
-              st[g].l = add_pair(pb[g][w], st[g].l);
-            }
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            u32x4 vf = at.values(lv + 32 * u * RB, t, d);
-            if (masked)
-#pragma unroll
-              for (int w = 0; w < 4; ++w) vf[w] = scrub<true>(vf[w], bad);
-#pragma unroll
-            for (int g = 0; g < QG; ++g) o[g][d] = attn_mfma<true>(vf, pb[g], o[g][d]);
-          }
+        for (int d = 0; d < DB; ++d) {
+          uint32_t w = at.value(lv, i, d);
+          if (masked) w = scrub<false>(w, bad);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w), pf[i], o[d], 0, 0, 0);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            uint32_t w = at.value(lv + 32 * u * RB, i, d);
-            if (masked) w = scrub<false>(w, bad);
-#pragma unroll
-            for (int g = 0; g < QG; ++g)
-              o[g][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w), pf[g][i], o[g][d], 0, 0, 0);
-          }
-      }
     }
   }
 
+  const float inv = inverse_sum(st.l + __shfl_xor(st.l, 32));
 #pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const float l = st[g].l + __shfl_xor(st[g].l, 32);
-    const float inv = inverse_sum(l);
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[g][d][i] *= inv;
-  }
+    for (int i = 0; i < 16; ++i) o[d][i] *= inv;
   // Infinities and NaN among the values of the masked tiles were taken as
   // zeros, for the rows that do not see them; the rows that do get them here.
   if (__any(bad != 0)) {
     for (int key = (tok_first + 1) / KB * KB; key < nkeys; ++key) {
       const char* const vp = vbase + (int64_t)key * p.v_t * ES;
-      uint32_t see[QG];
-#pragma unroll
-      for (int g = 0; g < QG; ++g) see[g] = key <= tok[g] ? 0xffffffffu : 0u;
+      const uint32_t see = key <= tok ? 0xffffffffu : 0u;
       int D = p.D;
       asm volatile("" : "+s"(D));  // its comparisons stay in the loop: hoisted, they spill
 #pragma unroll
@@ -217,30 +181,19 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(PromptParams p) {
         for (int i = 0; i < 16; ++i) {
           const int e = 32 * d + 8 * (i >> 2) + 4 * half + (i & 3);
           const uint32_t w = e >= D ? 0u : BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(vp)[e] << 16 : reinterpret_cast<const uint32_t*>(vp)[e];
-          const uint32_t mask = not_finite<false>(w);
-#pragma unroll
-          for (int g = 0; g < QG; ++g) o[g][d][i] += __uint_as_float(w & mask & see[g]);
+          o[d][i] += __uint_as_float(w & not_finite<false>(w) & see);
         }
     }
   }
+  if (!in) return;
+  const int64_t op = (int64_t)(start + tok) * p.o_t + (int64_t)(hk * G + (r - tok * G)) * p.o_h;
 #pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int r = row0 + (wave * QG + g) * 32 + col;
-    if (r >= rows) continue;
-    char* op = static_cast<char*>(p.out) +
-               ((int64_t)(start + tok[g]) * p.o_t + (int64_t)(hk * G + (r - tok[g] * G)) * p.o_h) * ES;
+  for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int e = 32 * d + 8 * b + 4 * half;
-        if (e >= p.D) continue;
-        if constexpr (BF16)
-          *reinterpret_cast<u32x2*>(op + e * 2) = u32x2{pack_bf16x2(o[g][d][4 * b], o[g][d][4 * b + 1]), pack_bf16x2(o[g][d][4 * b + 2], o[g][d][4 * b + 3])};
-        else
-          *reinterpret_cast<f32x4*>(op + e * 4) = f32x4{o[g][d][4 * b], o[g][d][4 * b + 1], o[g][d][4 * b + 2], o[g][d][4 * b + 3]};
-      }
-  }
+    for (int b = 0; b < 4; ++b) {
+      const int e = 32 * d + 8 * b + 4 * half;
+      if (e < p.D) store4<BF16>(p.out, op + e, f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]});
+    }
 }
 
 // The bf16 kernel for many rows: 4 waves of 64 rows, whose walk over the keys
