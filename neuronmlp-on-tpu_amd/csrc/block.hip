@@ -215,16 +215,23 @@ hipError_t launch_rmsnorm(const void* x, const float* gain, void* y, int64_t T, 
                           hipStream_t st) {
   if (T <= 0) return hipSuccess;
   const bool vec = d % (bf16 ? 8 : 4) == 0 && aligned16(x) && aligned16(y) && aligned16(gain);
-  const dim3 grid((unsigned)T), block(256);
-  if (bf16 && vec)
-    hipLaunchKernelGGL((rmsnorm_kernel<true, true>), grid, block, 0, st, x, gain, y, d, eps);
-  else if (bf16)
-    hipLaunchKernelGGL((rmsnorm_kernel<true, false>), grid, block, 0, st, x, gain, y, d, eps);
-  else if (vec)
-    hipLaunchKernelGGL((rmsnorm_kernel<false, true>), grid, block, 0, st, x, gain, y, d, eps);
-  else
-    hipLaunchKernelGGL((rmsnorm_kernel<false, false>), grid, block, 0, st, x, gain, y, d, eps);
-  return hipGetLastError();
+  constexpr int64_t kRows = 1 << 23;  // a launch: HIP cuts a grid of 2^32 threads or more, without an error
+  for (int64_t row = 0; row < T; row += kRows) {
+    const int64_t from = row * d * (bf16 ? 2 : 4);
+    const void* const xr = static_cast<const char*>(x) + from;
+    void* const yr = static_cast<char*>(y) + from;
+    const dim3 grid((unsigned)std::min(kRows, T - row)), block(256);
+    if (bf16 && vec)
+      hipLaunchKernelGGL((rmsnorm_kernel<true, true>), grid, block, 0, st, xr, gain, yr, d, eps);
+    else if (bf16)
+      hipLaunchKernelGGL((rmsnorm_kernel<true, false>), grid, block, 0, st, xr, gain, yr, d, eps);
+    else if (vec)
+      hipLaunchKernelGGL((rmsnorm_kernel<false, true>), grid, block, 0, st, xr, gain, yr, d, eps);
+    else
+      hipLaunchKernelGGL((rmsnorm_kernel<false, false>), grid, block, 0, st, xr, gain, yr, d, eps);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_residual_add(const void* x, void* y, int64_t n, bool bf16, hipStream_t st) {

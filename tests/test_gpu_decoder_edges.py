@@ -272,3 +272,20 @@ def test_cache_attention_many_rows_of_large_heads(gpu, dtype, B, n, H, K, D, pag
     got = svdmlp.cache_attention(*args, tree=tree.to(gpu))
     base._close(got[some], out, tol)
     assert torch.equal(got, svdmlp.cache_attention(*args, tree=tree.to(gpu)))
+
+
+def test_svd_mlp_block_of_many_rows(gpu):
+    """The block's RMSNorm too: rows beyond a launch's 2^24 come out as in a call of their own.  The two calls may sum in
+    other orders: a row's elements are compared as a whole, within 2^-6 of its size (four roundings to bf16 on the way)."""
+    T, d, r = (1 << 24) + 300, 64, 64
+    g = torch.Generator(device=gpu)
+    g.manual_seed(3)
+    x = torch.randn((T, d), device=gpu, generator=g).to(BF)
+    w = [(torch.randn(s, device=gpu, generator=g) / 8).to(BF) for s in ((d, r), (r, 128), (d, r), (r, 128), (128, r), (r, d))]
+    gain = torch.ones(d, device=gpu)
+    y = svdmlp.svd_mlp_block(x, gain, *w, eps=1e-5)
+    for at in (0, (1 << 23) - 150, T - 300):
+        s = slice(at, at + 300)
+        a, b = y[s].float(), svdmlp.svd_mlp_block(x[s].contiguous(), gain, *w, eps=1e-5).float()
+        assert ((a - b).norm(dim=1) <= 2.0 ** -6 * b.norm(dim=1)).all()
+    svdmlp.clear_workspace_cache()
