@@ -289,3 +289,22 @@ def test_svd_mlp_block_of_many_rows(gpu):
         a, b = y[s].float(), svdmlp.svd_mlp_block(x[s].contiguous(), gain, *w, eps=1e-5).float()
         assert ((a - b).norm(dim=1) <= 2.0 ** -6 * b.norm(dim=1)).all()
     svdmlp.clear_workspace_cache()
+
+
+@pytest.mark.parametrize("D", [4, 12, 36, 68, 132, 252])
+def test_attention_of_fp32_heads_of_odd_pieces(gpu, D):
+    """Heads of an odd number of 16-byte pieces, prompts and cache, one token and many rows."""
+    import test_gpu_decoder as base
+
+    g = base._gen(D)
+    lens, H, K = [37, 1, 150], 6, 2
+    (q, k, v), dev = base._qkv(g, sum(lens), H, K, D, F32, gpu)
+    for causal in (True, False):
+        base._close(svdmlp.prompt_attention(*dev, base._cu(lens, gpu), causal=causal), *base._prompt_ref(q, k, v, lens, causal, 1 / math.sqrt(D)))
+    for page, lens in ((16, [300, 31]), (5, [41, 700])):
+        table, pages = base._pages(g, lens, page)
+        kc, vc = base._randn(g, pages, page, K, D, dtype=F32), base._randn(g, pages, page, K, D, dtype=F32)
+        for n in (1, 7, 30):
+            q = base._randn(g, 2, n, H, D, dtype=F32)
+            got = svdmlp.cache_attention(*(t.to(gpu) for t in (q, kc, vc, table)), torch.tensor(lens, device=gpu))
+            base._close(got, *base._cache_ref(q, kc, vc, table, lens, None, 1 / math.sqrt(D)))
