@@ -358,7 +358,8 @@ int svdmlp_prompt_attention(const void* q, const void* k, const void* v, const i
  * long contexts and needs no clearing.  With one go `counters` int32 counters
  * (*counters of svdmlp_cache_attention_workspace_bytes, if not NULL; may be 0), zero
  * before the call, which leaves them zero: calls in flight at the same time
- * (other streams, graphs) need workspaces and counters of their own.
+ * (other streams, graphs) need workspaces and counters of their own.  A call
+ * of more chunks (times heads and row tiles) than a launch can have is refused.
  */
 size_t svdmlp_cache_attention_workspace_bytes(int64_t B, int64_t n, int64_t page, int64_t width, int64_t Hq,
                                               int64_t Hk, int64_t D, int32_t dtype, int64_t* counters);
