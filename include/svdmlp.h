@@ -85,6 +85,9 @@ extern "C" {
 
 /* svdmlp_rope, svdmlp_rope_append: pairs (2p, 2p + 1) instead of (p, p + rot / 2) */
 #define SVDMLP_ROPE_INTERLEAVED 0x1u
+/* svdmlp_norm_rope, svdmlp_norm_rope_append: gains of each head, (Hq, D) or (Hk, D), instead of (D) */
+#define SVDMLP_Q_HEAD_GAINS 0x2u
+#define SVDMLP_K_HEAD_GAINS 0x4u
 /* svdmlp_prompt_attention: a token sees the keys up to its own */
 #define SVDMLP_CAUSAL 0x1u
 
@@ -381,6 +384,53 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
 int svdmlp_residual_norm(const void* x, const void* branch, const float* post_w, const void* gate,
                          const float* norm_w, void* r_out, void* n_out, const int64_t* strides /* 5 or NULL */,
                          int64_t T, int64_t d, float scale, float eps, int32_t dtype, void* stream);
+
+/*
+ * svdmlp_rope and svdmlp_rope_append of heads that are normalised first:
+ *   y = w * x / sqrt(mean(x^2) + eps)
+ * over each head of q (gains q_w) and of k (k_w), the sum in 32 bits; y is turned
+ * before it is rounded.  Values v go to the cache as they are.  Gains are fp32,
+ * (D) for all heads or, with SVDMLP_Q_HEAD_GAINS / SVDMLP_K_HEAD_GAINS,
+ * (heads, D) row by row.
+ */
+int svdmlp_norm_rope(const void* q, const void* k, const int64_t* positions, const double* inv_freq, const float* q_w,
+                     const float* k_w, void* q_out, void* k_out, const int64_t* strides /* 8 or NULL */, int64_t T,
+                     int64_t Hq, int64_t Hk, int64_t D, int64_t rot, float scale, float eps, int32_t dtype,
+                     uint32_t flags, void* stream);
+int svdmlp_norm_rope_append(const void* q, const void* k, const void* v, const int64_t* positions,
+                            const double* inv_freq, const float* q_w, const float* k_w, const int64_t* slots,
+                            void* q_out, void* k_cache, void* v_cache, const int64_t* strides /* 14 or NULL */,
+                            int64_t T, int64_t pages, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t rot,
+                            float scale, float eps, int32_t dtype, uint32_t flags, void* stream);
+
+/*
+ * Pages of a paged cache to other pages of it, in n caches at once (the keys'
+ * and values' of all layers: a host array of device addresses, each cache
+ * (pages, page, Hk, D) with the same strides: page, row, head): the first
+ * rows[i] rows (int32; NULL: all) of page dst[i] become those of page src[i],
+ * i < m.  A pair with a page outside the cache, or of a page and itself, is
+ * skipped.  The pages of dst have to differ from each other and from those
+ * of src: with a page twice its rows are of neither pair for sure.
+ */
+int svdmlp_copy_pages(void* const* caches, int64_t n, const int64_t* strides /* 3 or NULL */, const int32_t* src,
+                      const int32_t* dst, const int32_t* rows, int64_t m, int64_t pages, int64_t page, int64_t Hk,
+                      int64_t D, int32_t dtype, void* stream);
+
+/*
+ * After a tree of drafts has been verified (svdmlp_cache_attention): the accepted
+ * ones' rows to behind the context, in n caches at once (as svdmlp_copy_pages).
+ * The last `drafts` (1 to 64) of a sequence's lengths[b] tokens are its drafts;
+ * path (B, m), dense, names the accepted ones, m <= drafts: draft path[b][i]
+ * becomes the i-th token behind the context, and new_lengths[b] counts the
+ * context and them.  The numbers increase along a path; it ends before the
+ * first that does not, is negative, or is not below `drafts` (-1 behind a
+ * short path).  A sequence of fewer tokens than drafts stays as it is, with
+ * its length; a row in a page outside the cache is not moved.
+ */
+int svdmlp_keep_drafts(void* const* caches, int64_t n, const int64_t* strides /* 3 or NULL */,
+                       const int32_t* block_table, const int32_t* lengths, const int32_t* path, int32_t* new_lengths,
+                       int64_t table_stride, int64_t B, int64_t width, int64_t m, int64_t drafts, int64_t pages,
+                       int64_t page, int64_t Hk, int64_t D, int32_t dtype, void* stream);
 
 /*
  * Per-stage GPU timing (no counterpart in the reference, whose timing is host

@@ -114,13 +114,17 @@ enum Stage : int {
   ST_PROMPT_ATTENTION,
   ST_CACHE_ATTENTION,
   ST_RESIDUAL_NORM,
+  ST_NORM_ROPE,
+  ST_COPY_PAGES,
+  ST_KEEP_DRAFTS,
   ST_COUNT
 };
 const char* const kStageNames[ST_COUNT] = {
     "zero_fill",        "gate_up_xu",       "gate_up_xuv_swiglu", "down_xu",           "down_xuv",
     "decode_gate_up_xu", "decode_gate_up_xuv", "decode_down_xu",   "decode_down_xuv", "finalize",
     "gate_up_xuv_g",    "decode_layer",       "decode_gemv_layer",  "decode_layer_contracted", "quant_h_e4m3", "down_xu_fp8",
-    "gate_up_xuv_dual", "rope", "prompt_attention", "cache_attention", "residual_norm"
+    "gate_up_xuv_dual", "rope", "prompt_attention", "cache_attention", "residual_norm",
+    "norm_rope", "copy_pages", "keep_drafts"
 };
 
 struct Profiler {
@@ -2574,8 +2578,9 @@ int check_heads(const char* what, int64_t T, int64_t Hq, int64_t Hk, int64_t D, 
   return SVDMLP_OK;
 }
 
-int rope_call(const char* what, RopeParams& p, int64_t Hq, int64_t Hk, int64_t D, int64_t rot, float scale,
-              int32_t dtype, uint32_t flags, void* stream) {
+// The checks that rotary positions share, and p's sizes; vec: whether everything lies in whole 16-byte pieces.
+int rope_check(const char* what, RopeParams& p, int64_t Hq, int64_t Hk, int64_t D, int64_t rot, float scale,
+               int32_t dtype, uint32_t flags, bool* vec) {
   int rc = check_heads(what, p.T, Hq, Hk, D, dtype, 1024);
   if (rc) return rc;
   if (!p.q || !p.k || !p.pos || !p.inv_freq || !p.qo || !p.ko) return fail("%s: null pointer", what);
@@ -2588,12 +2593,67 @@ int rope_call(const char* what, RopeParams& p, int64_t Hq, int64_t Hk, int64_t D
   p.rot = (int)rot;
   p.scale = scale;
   p.interleaved = (flags & SVDMLP_ROPE_INTERLEAVED) != 0;
-  const int es = act_size(dtype);
-  const bool vec = pieces16({p.q, p.k, p.v, p.qo, p.ko, p.vo},
-                            {D, p.interleaved ? rot : rot / 2, rot, p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h, p.qo_t,
-                             p.qo_h, p.ko_p, p.ko_t, p.ko_h, p.vo_p, p.vo_t, p.vo_h}, es);
+  *vec = pieces16({p.q, p.k, p.v, p.qo, p.ko, p.vo},
+                  {D, p.interleaved ? rot : rot / 2, rot, p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h, p.qo_t,
+                   p.qo_h, p.ko_p, p.ko_t, p.ko_h, p.vo_p, p.vo_t, p.vo_h}, act_size(dtype));
+  return SVDMLP_OK;
+}
+
+int rope_call(const char* what, RopeParams& p, int64_t Hq, int64_t Hk, int64_t D, int64_t rot, float scale,
+              int32_t dtype, uint32_t flags, void* stream) {
+  bool vec = false;
+  const int rc = rope_check(what, p, Hq, Hk, D, rot, scale, dtype, flags, &vec);
+  if (rc) return rc;
   StageScope s(ST_ROPE, (hipStream_t)stream);
   return check(launch_rope(p, dtype == SVDMLP_BF16, vec, (hipStream_t)stream), what);
+}
+
+int norm_rope_call(const char* what, NormRopeParams& p, int64_t Hq, int64_t Hk, int64_t D, int64_t rot, float scale,
+                   float eps, int32_t dtype, uint32_t flags, void* stream) {
+  constexpr uint32_t kGains = SVDMLP_Q_HEAD_GAINS | SVDMLP_K_HEAD_GAINS;
+  bool vec = false;
+  const int rc = rope_check(what, p.r, Hq, Hk, D, rot, scale, dtype, flags & ~kGains, &vec);
+  if (rc) return rc;
+  if (!p.q_w || !p.k_w) return fail("%s: null pointer", what);
+  if (!(eps > 0.f) || !std::isfinite(eps)) return fail("%s: eps must be positive", what);
+  p.qw_h = flags & SVDMLP_Q_HEAD_GAINS ? D : 0;
+  p.kw_h = flags & SVDMLP_K_HEAD_GAINS ? D : 0;
+  p.eps = eps;
+  vec = vec && pieces16({p.q_w, p.k_w}, {D}, 4);
+  StageScope s(ST_NORM_ROPE, (hipStream_t)stream);
+  return check(launch_norm_rope(p, dtype == SVDMLP_BF16, vec, (hipStream_t)stream), what);
+}
+
+// The caches of an entry point that moves rows: their sizes and strides; the
+// addresses are filled in launch by launch.
+int cache_set(const char* what, CacheSet& c, void* const* caches, int64_t n, const int64_t* strides, int64_t pages,
+              int64_t page, int64_t Hk, int64_t D, int32_t dtype, bool* vec) {
+  if (!act_size(dtype)) return fail("%s: dtype must be bf16 or fp32, got %d", what, (int)dtype);
+  if (!caches || n <= 0) return fail("%s: no caches", what);
+  if (pages <= 0 || page <= 0 || Hk <= 0 || D <= 0) return fail("%s: sizes must be positive", what);
+  constexpr int64_t most = 1 << 30;  // elements of a page
+  if (pages > 0x7fffffff || page > most || Hk > most / page || D > most / page / Hk) return fail("%s: pages are too large", what);
+  const int64_t dense[3] = {page * Hk * D, Hk * D, D};
+  int64_t s[3];
+  if (!plain_strides(strides ? strides : dense, {pages, page, Hk}, s)) return fail("%s: strides must not be negative", what);
+  c.p_s = s[0], c.t_s = s[1], c.h_s = s[2];
+  c.pages = pages, c.es = act_size(dtype), c.page = (int)page, c.Hk = (int)Hk, c.D = (int)D;
+  *vec = pieces16({}, {D, s[0], s[1], s[2]}, c.es);
+  for (int64_t i = 0; i < n; ++i) {
+    if (!caches[i]) return fail("%s: null pointer", what);
+    *vec = *vec && ((uintptr_t)caches[i] & 15u) == 0;
+  }
+  return SVDMLP_OK;
+}
+// Calls go(set) for every kCachesMost of the caches.
+template <class F>
+hipError_t each_cache_set(CacheSet& c, void* const* caches, int64_t n, F go) {
+  for (int64_t i = 0; i < n; i += kCachesMost) {
+    c.n = (int)std::min<int64_t>(kCachesMost, n - i);
+    std::copy(caches + i, caches + i + c.n, c.base);
+    if (const hipError_t e = go(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
@@ -2742,6 +2802,72 @@ int svdmlp_residual_norm(const void* x, const void* branch, const float* post_w,
   const bool vec = pieces16({x, branch, post_w, gate, norm_w, r_out, n_out}, {d, s[0], s[1], s[2], s[3], s[4]}, es);
   StageScope sc(ST_RESIDUAL_NORM, (hipStream_t)stream);
   return check(launch_residual_norm(p, dtype == SVDMLP_BF16, vec, (hipStream_t)stream), "residual_norm");
+}
+
+int svdmlp_norm_rope(const void* q, const void* k, const int64_t* positions, const double* inv_freq, const float* q_w,
+                     const float* k_w, void* q_out, void* k_out, const int64_t* strides, int64_t T, int64_t Hq,
+                     int64_t Hk, int64_t D, int64_t rot, float scale, float eps, int32_t dtype, uint32_t flags,
+                     void* stream) {
+  NormRopeParams p = {};
+  p.r.q = q, p.r.k = k, p.r.pos = positions, p.r.inv_freq = inv_freq, p.r.qo = q_out, p.r.ko = k_out, p.r.T = T;
+  p.q_w = q_w, p.k_w = k_w;
+  const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hq * D, D, Hk * D, D};
+  const int64_t* s = strides ? strides : dense;
+  p.r.q_t = s[0], p.r.q_h = s[1], p.r.k_t = s[2], p.r.k_h = s[3], p.r.qo_t = s[4], p.r.qo_h = s[5], p.r.ko_t = s[6], p.r.ko_h = s[7];
+  return norm_rope_call("norm_rope", p, Hq, Hk, D, rot, scale, eps, dtype, flags, stream);
+}
+
+int svdmlp_norm_rope_append(const void* q, const void* k, const void* v, const int64_t* positions,
+                            const double* inv_freq, const float* q_w, const float* k_w, const int64_t* slots,
+                            void* q_out, void* k_cache, void* v_cache, const int64_t* strides, int64_t T,
+                            int64_t pages, int64_t page, int64_t Hq, int64_t Hk, int64_t D, int64_t rot, float scale,
+                            float eps, int32_t dtype, uint32_t flags, void* stream) {
+  if (!v || !slots || !v_cache) return fail("norm_rope_append: null pointer");
+  if (pages <= 0 || page <= 0 || page > 0x7fffffff || pages > INT64_MAX / page) return fail("norm_rope_append: pages and page size must be positive");
+  NormRopeParams p = {};
+  p.r.q = q, p.r.k = k, p.r.v = v, p.r.pos = positions, p.r.inv_freq = inv_freq, p.r.slots = slots;
+  p.r.qo = q_out, p.r.ko = k_cache, p.r.vo = v_cache, p.r.T = T, p.r.pages = pages, p.r.page = (int)page;
+  p.q_w = q_w, p.k_w = k_w;
+  const int64_t dense[14] = {Hq * D, D, Hk * D, D, Hk * D, D, Hq * D, D, page * Hk * D, Hk * D, D, page * Hk * D, Hk * D, D};
+  const int64_t* s = strides ? strides : dense;
+  p.r.q_t = s[0], p.r.q_h = s[1], p.r.k_t = s[2], p.r.k_h = s[3], p.r.v_t = s[4], p.r.v_h = s[5], p.r.qo_t = s[6], p.r.qo_h = s[7];
+  p.r.ko_p = s[8], p.r.ko_t = s[9], p.r.ko_h = s[10], p.r.vo_p = s[11], p.r.vo_t = s[12], p.r.vo_h = s[13];
+  return norm_rope_call("norm_rope_append", p, Hq, Hk, D, rot, scale, eps, dtype, flags, stream);
+}
+
+int svdmlp_copy_pages(void* const* caches, int64_t n, const int64_t* strides, const int32_t* src, const int32_t* dst,
+                      const int32_t* rows, int64_t m, int64_t pages, int64_t page, int64_t Hk, int64_t D,
+                      int32_t dtype, void* stream) {
+  PageCopyParams p = {};
+  bool vec = false;
+  const int rc = cache_set("copy_pages", p.c, caches, n, strides, pages, page, Hk, D, dtype, &vec);
+  if (rc) return rc;
+  if (!src || !dst) return fail("copy_pages: null pointer");
+  if (m <= 0 || m > 0x7fffffff) return fail("copy_pages: %lld pages", (long long)m);
+  p.src = src, p.dst = dst, p.rows = rows;
+  StageScope s(ST_COPY_PAGES, (hipStream_t)stream);
+  return check(each_cache_set(p.c, caches, n, [&] { return launch_copy_pages(p, m, vec, (hipStream_t)stream); }), "copy_pages",
+               "pages are too large for one launch");
+}
+
+int svdmlp_keep_drafts(void* const* caches, int64_t n, const int64_t* strides, const int32_t* block_table,
+                       const int32_t* lengths, const int32_t* path, int32_t* new_lengths, int64_t table_stride,
+                       int64_t B, int64_t width, int64_t m, int64_t drafts, int64_t pages, int64_t page, int64_t Hk,
+                       int64_t D, int32_t dtype, void* stream) {
+  DraftKeepParams p = {};
+  bool vec = false;
+  const int rc = cache_set("keep_drafts", p.c, caches, n, strides, pages, page, Hk, D, dtype, &vec);
+  if (rc) return rc;
+  if (!block_table || !lengths || !path || !new_lengths) return fail("keep_drafts: null pointer");
+  if (B <= 0 || width <= 0 || B > 0x7fffffff || page > 0x7fffff00 / width) return fail("keep_drafts: sizes must be positive, with less than 2^31 tokens a sequence");
+  if (drafts <= 0 || drafts > kDraftsMost || m <= 0 || m > drafts)
+    return fail("keep_drafts: 1 to %d drafts, and a path of at most as many, got %lld and %lld", kDraftsMost, (long long)drafts, (long long)m);
+  if (table_stride < 0) return fail("keep_drafts: strides must not be negative");
+  p.table = block_table, p.lengths = lengths, p.path = path, p.new_lengths = new_lengths;
+  p.table_b = table_stride, p.width = (int)width, p.B = (int)B, p.m = (int)m, p.drafts = (int)drafts;
+  StageScope s(ST_KEEP_DRAFTS, (hipStream_t)stream);
+  return check(each_cache_set(p.c, caches, n, [&] { return launch_keep_drafts(p, vec, (hipStream_t)stream); }), "keep_drafts",
+               "too many sequences for one launch");
 }
 
 }  // extern "C"

@@ -1,7 +1,8 @@
 // Parameters and launchers of the operators around the MLP block of a decoder
-// layer: rotary positions (rope.hip), attention over packed prompts
-// (prompt_attention.hip), attention over a paged cache (cache_attention.hip),
-// and the residual sum with the norms on both sides of a block (norm.hip).
+// layer: rotary positions (rope.hip) and head norms before them (norm_rope.hip),
+// attention over packed prompts (prompt_attention.hip), attention over a paged
+// cache (cache_attention.hip), the residual sum with the norms on both sides of a
+// block (norm.hip), and moves within a cache (cache_pages.hip).
 // Strides are in elements; the last dimension of every tensor is contiguous.
 #pragma once
 
@@ -33,6 +34,14 @@ struct RopeParams {
   int interleaved;
 };
 hipError_t launch_rope(const RopeParams& p, bool bf16, bool vec, hipStream_t st);
+
+struct NormRopeParams {
+  RopeParams r;
+  const float *q_w, *k_w;  // gains: (D) or, with a stride, (heads, D)
+  int64_t qw_h, kw_h;
+  float eps;
+};
+hipError_t launch_norm_rope(const NormRopeParams& p, bool bf16, bool vec, hipStream_t st);
 
 struct ResidualNormParams {
   const void* x;       // (T, d) the residual stream
@@ -102,5 +111,34 @@ inline int64_t cache_counters(const CachePlan& plan, int B, int Hk) {
   return plan.splits > 1 && !plan.shared ? (int64_t)B * Hk * plan.rtiles : 0;
 }
 hipError_t launch_cache_attention(const CacheParams& p, bool bf16, const CachePlan& plan, hipStream_t st);
+
+// The caches (pages, page, Hk, D) of a model's layers, all laid out alike: as many
+// as a launch's arguments hold.
+constexpr int kCachesMost = 128;
+struct CacheSet {
+  void* base[kCachesMost];
+  int64_t pages, p_s, t_s, h_s;  // strides in elements
+  int n, es, page, Hk, D;        // es: bytes of an element
+};
+struct PageCopyParams {
+  CacheSet c;
+  const int *src, *dst, *rows;  // pages, and how many of a page's rows, or null: all
+  int64_t first;                // of the launch's pages
+  int row_units, head_units, parts;  // set by the launcher
+};
+hipError_t launch_copy_pages(const PageCopyParams& p, int64_t m, bool vec, hipStream_t st);
+
+constexpr int kDraftsMost = 64;
+struct DraftKeepParams {
+  CacheSet c;
+  const int* table;    // (B, width)
+  const int* lengths;  // (B), the drafts last among the tokens
+  const int* path;     // (B, m)
+  int* new_lengths;    // (B)
+  int64_t table_b;
+  int width, B, m, drafts;
+  int row_units, head_units, parts;  // set by the launcher
+};
+hipError_t launch_keep_drafts(const DraftKeepParams& p, bool vec, hipStream_t st);
 
 }  // namespace svdmlp

@@ -5,9 +5,11 @@ Host package over libsvdmlp.so (hand-written HIP kernels for gfx950):
 * :mod:`svdmlp.ops`     -- kernels/reference.py operator API
   (``fused_gate_up``, ``fused_xuv``, ``svd_mlp``) on ROCm tensors.
 * :mod:`svdmlp.decoder` -- the operators around the MLP block of a decoder
-  layer: ``rope`` / ``rope_append``, ``prompt_attention``,
-  ``cache_attention`` (decode and drafted trees on a paged cache) and
-  ``residual_norm``.
+  layer: ``rope`` / ``rope_append`` and ``norm_rope`` / ``norm_rope_append``,
+  ``prompt_attention``, ``cache_attention`` (decode and drafted trees on a
+  paged cache) and ``residual_norm``.
+* :mod:`svdmlp.pages`   -- rows moved within a paged cache: ``copy_pages``,
+  ``keep_drafts``, and ``PagePool``, the host's books of its pages.
 * :mod:`svdmlp.compat`  -- the test_speedup.py launcher API
   (``fused_mlp_up_T``, ``fused_three_mm_XTUV``, ``svd_mlp_with_fused_kernel``,
   ``nki_mm``, ``get_fused_*_params`` ...).
@@ -29,6 +31,8 @@ Host package over libsvdmlp.so (hand-written HIP kernels for gfx950):
 from ._lib import SvdMlpError, load, version, workspace_bytes  # noqa: F401
 from .decoder import (  # noqa: F401
     cache_attention,
+    norm_rope,
+    norm_rope_append,
     prompt_attention,
     residual_norm,
     rope,
@@ -47,5 +51,6 @@ from .ops import (  # noqa: F401
     svd_mlp_workspace,
     workspace_status,
 )
+from .pages import PagePool, copy_pages, keep_drafts  # noqa: F401
 
 __version__ = "1.0.0"

@@ -27,6 +27,8 @@ SVDMLP_X_T = 0x8
 SVDMLP_CONTRACT = 0x10
 SVDMLP_FP8_ACT = 0x20
 SVDMLP_ROPE_INTERLEAVED = 0x1
+SVDMLP_Q_HEAD_GAINS = 0x2
+SVDMLP_K_HEAD_GAINS = 0x4
 SVDMLP_CAUSAL = 0x1
 SVDMLP_OK = 0
 SVDMLP_EINVAL = -1
@@ -55,6 +57,10 @@ EXPORTED = (
     "svdmlp_cache_attention_workspace_bytes",
     "svdmlp_cache_attention",
     "svdmlp_residual_norm",
+    "svdmlp_norm_rope",
+    "svdmlp_norm_rope_append",
+    "svdmlp_copy_pages",
+    "svdmlp_keep_drafts",
     "svdmlp_profile_enable",
     "svdmlp_profile_read",
     "svdmlp_stage_name",
@@ -123,6 +129,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.svdmlp_cache_attention.argtypes = [_vp] * 8 + [_i64] * 8 + [f32, _i32, _vp, _sz, _vp, _i64, _vp]
     lib.svdmlp_residual_norm.restype = ctypes.c_int
     lib.svdmlp_residual_norm.argtypes = [_vp] * 8 + [_i64] * 2 + [f32, f32, _i32, _vp]
+    lib.svdmlp_norm_rope.restype = ctypes.c_int
+    lib.svdmlp_norm_rope.argtypes = [_vp] * 9 + [_i64] * 5 + [f32, f32, _i32, _u32, _vp]
+    lib.svdmlp_norm_rope_append.restype = ctypes.c_int
+    lib.svdmlp_norm_rope_append.argtypes = [_vp] * 12 + [_i64] * 7 + [f32, f32, _i32, _u32, _vp]
+    lib.svdmlp_copy_pages.restype = ctypes.c_int
+    lib.svdmlp_copy_pages.argtypes = [_vp, _i64] + [_vp] * 4 + [_i64] * 5 + [_i32, _vp]
+    lib.svdmlp_keep_drafts.restype = ctypes.c_int
+    lib.svdmlp_keep_drafts.argtypes = [_vp, _i64] + [_vp] * 5 + [_i64] * 9 + [_i32, _vp]
     lib.svdmlp_profile_enable.restype = ctypes.c_int
     lib.svdmlp_profile_enable.argtypes = [ctypes.c_int]
     lib.svdmlp_profile_read.restype = ctypes.c_int

@@ -2,6 +2,7 @@
 
     rope(q, k, positions, inv_freq)                 rotary positions
     rope_append(q, k, v, ..., k_cache, v_cache, slots)   ... into a paged cache
+    norm_rope, norm_rope_append                     both, of normalised heads
     prompt_attention(q, k, v, cu_seqlens)           attention over packed prompts
     cache_attention(q, k_cache, v_cache, table, lengths)  decode, drafted trees
     residual_norm(x, branch, weight)                sum after a block, next norm
@@ -128,6 +129,14 @@ def _extent(t: torch.Tensor, first: int = 0) -> int:
     return (sum(s * (n - 1) for s, n in zip(t.stride()[first:], t.shape[first:])) + 1) * t.element_size()
 
 
+def _bytes(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses of a nonempty tensor's first byte and behind its last."""
+    p, es = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        return p, p + es * t.numel()
+    return p, p + _extent(t)
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two nonempty tensors may share memory (slices side by side in the rows of one buffer do not)."""
     pa, pb = a.data_ptr(), b.data_ptr()
@@ -194,6 +203,7 @@ def _refuse_heads(q, k, *more) -> None:
     raise ValueError(f"{Hq} query heads are no multiple of {Hk} key/value heads")
 
 
+_Strides3 = ctypes.c_int64 * 3
 _Strides5 = ctypes.c_int64 * 5
 _Strides8 = ctypes.c_int64 * 8
 _Strides14 = ctypes.c_int64 * 14
@@ -375,6 +385,97 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interl
     _launch(index, _lib.load().svdmlp_rope_append, qp, kp, vp, pp, fp, sp,
             out.data_ptr(), kcp, vcp, _address(st), T, cs[0], cs[1], Hq, Hk, D, rot, scale, _ACT_CODES[q.dtype],
             1 if interleaved else 0)
+    return out
+
+
+def _head_gains(name, w, heads, D, index):
+    """(gains in fp32, whether each head has its own)."""
+    if w.get_device() != index or not w.is_floating_point() or tuple(w.shape) not in ((D,), (heads, D)):
+        raise ValueError(f"{name} must be a ({D},) or ({heads}, {D}) tensor on q.device")
+    return w if w.dtype is torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous(), w.dim() == 2
+
+
+def _norm_rope_args(name, q, k, q_weight, k_weight, eps, interleaved, D, Hq, Hk, index):
+    if not (eps > 0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be positive, got {eps}")
+    qw, q_own = _head_gains("q_weight", q_weight, Hq, D, index)
+    kw, k_own = _head_gains("k_weight", k_weight, Hk, D, index)
+    if _gradients():
+        _refuse_grad(name, q_weight, k_weight)
+    flags = ((_lib.SVDMLP_ROPE_INTERLEAVED if interleaved else 0) | (_lib.SVDMLP_Q_HEAD_GAINS if q_own else 0)
+             | (_lib.SVDMLP_K_HEAD_GAINS if k_own else 0))
+    return qw, kw, flags
+
+
+def norm_rope(q, k, positions, inv_freq, q_weight, k_weight, *, eps: float = 1e-5, interleaved: bool = False,
+              scale: float = 1.0, out: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`rope` of heads that are normalised first, in the same pass: each head
+    x of q becomes ``q_weight * x / sqrt(mean(x^2) + eps)``, each of k the same
+    with ``k_weight``, and is turned before it is rounded.  The gains are (D,) for
+    all heads or (heads, D), of any float dtype (used in fp32)."""
+    T, Hq, Hk, D, index, rot, positions, inv_freq = _rope_args("norm_rope", q, k, None, positions, inv_freq, scale)
+    qw, kw, flags = _norm_rope_args("norm_rope", q, k, q_weight, k_weight, eps, interleaved, D, Hq, Hk, index)
+    if out is None:
+        qo, ko = q.new_empty((T, Hq, D)), q.new_empty((T, Hk, D))
+    else:
+        qo, ko = out
+        if _gradients():
+            _refuse_grad("norm_rope", qo, ko)
+        _writable("out[0]", qo, (T, Hq, D), q)
+        _writable("out[1]", ko, (T, Hk, D), q)
+        _apart("out[0]", qo, q, k, ko, positions, inv_freq, qw, kw, own=(q,))
+        _apart("out[1]", ko, k, q, positions, inv_freq, qw, kw, own=(k,))
+    if T == 0:
+        return qo, ko
+    q, k = _last(q), _last(k)
+    st = _Strides8(*q.stride()[:2], *k.stride()[:2], *qo.stride()[:2], *ko.stride()[:2])
+    _launch(index, _lib.load().svdmlp_norm_rope, q.data_ptr(), k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), qw.data_ptr(),
+            kw.data_ptr(), qo.data_ptr(), ko.data_ptr(), _address(st), T, Hq, Hk, D, rot, scale, eps, _ACT_CODES[q.dtype], flags)
+    return qo, ko
+
+
+def norm_rope_append(q, k, v, positions, inv_freq, q_weight, k_weight, k_cache, v_cache, slots, *, eps: float = 1e-5,
+                     interleaved: bool = False, scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`norm_rope` on the way into a paged cache, as :func:`rope_append`:
+    returns the turned q, and writes the normalised and turned k, and v as it
+    is, to their slots of the caches."""
+    name = "norm_rope_append"
+    T, Hq, Hk, D, index, rot, positions, inv_freq = _rope_args(name, q, k, v, positions, inv_freq, scale)
+    qw, kw, flags = _norm_rope_args(name, q, k, q_weight, k_weight, eps, interleaved, D, Hq, Hk, index)
+    cs = k_cache.shape
+    if len(cs) != 4 or v_cache.shape != cs or cs[2] != Hk or cs[3] != D or not cs[0] or not cs[1]:
+        _refuse_caches(k_cache, v_cache, Hk, D)
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        _refuse_dtype(q.dtype, k_cache.dtype, v_cache.dtype)
+    if k_cache.get_device() != index or v_cache.get_device() != index:
+        _refuse_device(name, q, k_cache, v_cache)
+    if _gradients():
+        _refuse_grad(name, k_cache, v_cache, out)
+    _writable("k_cache", k_cache, cs, q)
+    _writable("v_cache", v_cache, cs, q)
+    slots = _index("slots", slots, (T,), torch.int64, index)
+    if out is not None:
+        _writable("out", out, (T, Hq, D), q)
+        _apart("out", out, q, k, v, k_cache, v_cache, positions, inv_freq, slots, qw, kw, own=(q,))
+    if T == 0:
+        return q.new_empty((0, Hq, D)) if out is None else out
+    q, k, v = _last(q), _last(k), _last(v)
+    # The caches apart from each other and from what is read: by their first and
+    # last bytes, exactly where those meet.
+    kp, ke, vp, ve = *_bytes(k_cache), *_bytes(v_cache)
+    meet = kp < ve and vp < ke
+    for t in (q, k, v, positions, inv_freq, slots, qw, kw):
+        p, e = _bytes(t)
+        meet = meet or (p < ke and kp < e) or (p < ve and vp < e)
+    if meet:
+        _apart("k_cache", k_cache, v_cache, q, k, v, positions, inv_freq, slots, qw, kw)
+        _apart("v_cache", v_cache, q, k, v, positions, inv_freq, slots, qw, kw)
+    if out is None:
+        out = q.new_empty((T, Hq, D))
+    st = _Strides14(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3])
+    _launch(index, _lib.load().svdmlp_norm_rope_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
+            inv_freq.data_ptr(), qw.data_ptr(), kw.data_ptr(), slots.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            _address(st), T, cs[0], cs[1], Hq, Hk, D, rot, scale, eps, _ACT_CODES[q.dtype], flags)
     return out
 
 
