@@ -373,6 +373,29 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
                            void* workspace, size_t ws_bytes, int32_t* counters, int64_t n_counters, void* stream);
 
 /*
+ * Attention of packed chunks of new tokens of B sequences onto a paged cache that
+ * holds lengths[b] tokens of each, the new ones last among them: those of
+ * sequence b are rows cu_seqlens[b] .. cu_seqlens[b + 1] of q (int32, B + 1), any
+ * number of them, and each sees the keys up to itself.  Key x of sequence b
+ * is row x % page of page block_table[b][x / page] (int32, width pages a sequence, at
+ * most 65536, and at most 2^31 - 2^17 tokens); a page outside the cache holds no
+ * keys.  A token without keys gets zeros; more new tokens than lengths[b]
+ * leave the first ones without any.  Rows of no sequence are left as they were.
+ * D, strides and addresses as svdmlp_cache_attention.  strides: q token, head;
+ * k_cache page, row, head; v_cache page, row, head; out token, head; block_table
+ * sequence.  The workspace (svdmlp_chunk_attention_workspace_bytes; may be 0)
+ * holds the sums of long contexts' chunks and needs no clearing; calls in
+ * flight at the same time need workspaces of their own.
+ */
+size_t svdmlp_chunk_attention_workspace_bytes(int64_t T, int64_t B, int64_t page, int64_t width, int64_t Hq,
+                                              int64_t Hk, int64_t D, int32_t dtype);
+int svdmlp_chunk_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                           const int32_t* lengths, const int32_t* cu_seqlens, void* out,
+                           const int64_t* strides /* 11 or NULL */, int64_t T, int64_t B, int64_t pages, int64_t page,
+                           int64_t width, int64_t Hq, int64_t Hk, int64_t D, float scale, int32_t dtype,
+                           void* workspace, size_t ws_bytes, void* stream);
+
+/*
  * The sum after a block and the norm before the next:
  *   b = branch, or post_w * branch / sqrt(mean(branch^2) + eps) with post_w
  *   r = x + scale * gate * b      (gate (T, d), or (d) with row stride 0, or NULL)

@@ -117,6 +117,7 @@ enum Stage : int {
   ST_NORM_ROPE,
   ST_COPY_PAGES,
   ST_KEEP_DRAFTS,
+  ST_CHUNK_ATTENTION,
   ST_COUNT
 };
 const char* const kStageNames[ST_COUNT] = {
@@ -124,7 +125,7 @@ const char* const kStageNames[ST_COUNT] = {
     "decode_gate_up_xu", "decode_gate_up_xuv", "decode_down_xu",   "decode_down_xuv", "finalize",
     "gate_up_xuv_g",    "decode_layer",       "decode_gemv_layer",  "decode_layer_contracted", "quant_h_e4m3", "down_xu_fp8",
     "gate_up_xuv_dual", "rope", "prompt_attention", "cache_attention", "residual_norm",
-    "norm_rope", "copy_pages", "keep_drafts"
+    "norm_rope", "copy_pages", "keep_drafts", "chunk_attention"
 };
 
 struct Profiler {
@@ -2868,6 +2869,56 @@ int svdmlp_keep_drafts(void* const* caches, int64_t n, const int64_t* strides, c
   StageScope s(ST_KEEP_DRAFTS, (hipStream_t)stream);
   return check(each_cache_set(p.c, caches, n, [&] { return launch_keep_drafts(p, vec, (hipStream_t)stream); }), "keep_drafts",
                "too many sequences for one launch");
+}
+
+size_t svdmlp_chunk_attention_workspace_bytes(int64_t T, int64_t B, int64_t page, int64_t width, int64_t Hq, int64_t Hk,
+                                              int64_t D, int32_t dtype) {
+  if (check_heads("chunk_attention", T, Hq, Hk, D, dtype, 256) || B <= 0 || B > 0x7fffffff || page <= 0 || width <= 0 ||
+      width > kCachePagesMost || page > kChunkTokensMost / width)
+    return 0;
+  return (size_t)plan_chunk_attention(T, B, Hq, Hk, D, dtype == SVDMLP_BF16, page * width, device_cus()).floats * 4;
+}
+
+int svdmlp_chunk_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                           const int32_t* lengths, const int32_t* cu_seqlens, void* out, const int64_t* strides,
+                           int64_t T, int64_t B, int64_t pages, int64_t page, int64_t width, int64_t Hq, int64_t Hk,
+                           int64_t D, float scale, int32_t dtype, void* workspace, size_t ws_bytes, void* stream) {
+  const int rc = check_heads("chunk_attention", T, Hq, Hk, D, dtype, 256);
+  if (rc) return rc;
+  if (!q || !k_cache || !v_cache || !block_table || !lengths || !cu_seqlens || !out) return fail("chunk_attention: null pointer");
+  if (B <= 0 || B > 0x7fffffff - 64) return fail("chunk_attention: %lld sequences", (long long)B);
+  if (pages <= 0 || page <= 0 || width <= 0 || page > kChunkTokensMost / width)
+    return fail("chunk_attention: pages, page size and the table's width must be positive, with at most %lld tokens a sequence", (long long)kChunkTokensMost);
+  if (width > kCachePagesMost) return fail("chunk_attention: %lld pages a sequence, at most %lld", (long long)width, (long long)kCachePagesMost);
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail("chunk_attention: scale must be positive and finite");
+  const int64_t dense[11] = {Hq * D, D, page * Hk * D, Hk * D, D, page * Hk * D, Hk * D, D, Hq * D, D, width};
+  int64_t s[11];
+  if (!plain_strides(strides ? strides : dense, {T, Hq, pages, page, Hk, pages, page, Hk, T, Hq, B}, s)) return fail("chunk_attention: strides must not be negative");
+  if (!pieces16({q, k_cache, v_cache, out}, {D, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9]}, act_size(dtype)))
+    return fail("chunk_attention: the head size, strides and addresses must be whole 16-byte pieces");
+  if (s[3] > kTokenStrideMost || s[6] > kTokenStrideMost) return fail("chunk_attention: rows of the cache are more than %lld elements apart", (long long)kTokenStrideMost);
+  ChunkParams p = {};
+  p.q = q, p.kc = k_cache, p.vc = v_cache, p.table = block_table, p.lengths = lengths, p.cu = cu_seqlens, p.out = out;
+  p.q_t = s[0], p.q_h = s[1], p.k_p = s[2], p.k_t = s[3], p.k_h = s[4], p.v_p = s[5], p.v_t = s[6], p.v_h = s[7];
+  p.o_t = s[8], p.o_h = s[9], p.table_b = s[10], p.pages = pages;
+  p.page = (int)page, p.width = (int)width, p.T = (int)T, p.B = (int)B, p.Hq = (int)Hq, p.Hk = (int)Hk, p.D = (int)D;
+  if (page > 1) {
+    int log = 0;
+    while (((int64_t)1 << log) < page) ++log;
+    p.page_mul = (uint32_t)((((uint64_t)1 << (31 + log)) + page - 1) / page);
+    p.page_shift = log - 1;
+  }
+  p.alike = s[2] == s[5] && s[3] == s[6];
+  p.c = scale * 1.44269504088896340736f;
+  const int cus = device_cus();
+  const ChunkPlan plan = plan_chunk_attention(T, B, Hq, Hk, D, dtype == SVDMLP_BF16, page * width, cus);
+  const size_t need = (size_t)plan.floats * 4;
+  if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15u)))
+    return fail("chunk_attention: workspace too small: %zu bytes needed, 16-byte aligned, got %zu", need, ws_bytes);
+  p.part = static_cast<float*>(workspace);
+  StageScope sc(ST_CHUNK_ATTENTION, (hipStream_t)stream);
+  return check(launch_chunk_attention(p, dtype == SVDMLP_BF16, plan, cus, (hipStream_t)stream), "chunk_attention",
+               "too many rows or sequences for one launch");
 }
 
 }  // extern "C"

@@ -112,6 +112,38 @@ inline int64_t cache_counters(const CachePlan& plan, int B, int Hk) {
 }
 hipError_t launch_cache_attention(const CacheParams& p, bool bf16, const CachePlan& plan, hipStream_t st);
 
+// Sequences whose rows (new tokens x heads of a group) number from .. upto take
+// tiles of `rows` rows.
+struct ChunkClass {
+  int from, upto, rows;
+  int slots, least;        // chunks of keys: about so many, of at least so many keys
+  int64_t blocks;          // at most; 0: no sequence can be of the class
+  int64_t parts, part_at;  // room for the sums of so many chunks, from which float on
+};
+struct ChunkParams {
+  const void* q;        // (T, Hq, D), sequence b's new tokens in rows cu[b] .. cu[b + 1]
+  const void *kc, *vc;  // (pages, page, Hk, D)
+  const int* table;     // (B, width)
+  const int* lengths;   // (B) tokens held, the new ones last among them
+  const int* cu;        // (B + 1)
+  void* out;            // (T, Hq, D)
+  float* part;
+  int64_t q_t, q_h, k_p, k_t, k_h, v_p, v_t, v_h, o_t, o_h, table_b, pages;
+  int page, width, T, B, Hq, Hk, D;
+  uint32_t page_mul;  // x / page = umulhi(x, page_mul) >> page_shift, for x < 2^31 and a page of over one token
+  int page_shift;
+  int alike;  // keys and values have the same page and token strides
+  float c;    // softmax scale * log2(e)
+};
+constexpr int kFewRows = 128;
+constexpr int64_t kChunkTokensMost = 0x7ffe0000;  // of a sequence: room for the last tiles' ends
+struct ChunkPlan {
+  ChunkClass many, few;
+  int64_t floats;  // of the workspace
+};
+ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, bool bf16, int64_t capacity, int64_t cus);
+hipError_t launch_chunk_attention(const ChunkParams& p, bool bf16, const ChunkPlan& plan, int cus, hipStream_t st);
+
 // The caches (pages, page, Hk, D) of a model's layers, all laid out alike: as many
 // as a launch's arguments hold.
 constexpr int kCachesMost = 128;

@@ -7,7 +7,8 @@ Host package over libsvdmlp.so (hand-written HIP kernels for gfx950):
 * :mod:`svdmlp.decoder` -- the operators around the MLP block of a decoder
   layer: ``rope`` / ``rope_append`` and ``norm_rope`` / ``norm_rope_append``,
   ``prompt_attention``, ``cache_attention`` (decode and drafted trees on a
-  paged cache) and ``residual_norm``.
+  paged cache), ``chunk_attention`` (chunks of prompts on it) and
+  ``residual_norm``.
 * :mod:`svdmlp.pages`   -- rows moved within a paged cache: ``copy_pages``,
   ``keep_drafts``, and ``PagePool``, the host's books of its pages.
 * :mod:`svdmlp.compat`  -- the test_speedup.py launcher API
@@ -31,6 +32,7 @@ Host package over libsvdmlp.so (hand-written HIP kernels for gfx950):
 from ._lib import SvdMlpError, load, version, workspace_bytes  # noqa: F401
 from .decoder import (  # noqa: F401
     cache_attention,
+    chunk_attention,
     norm_rope,
     norm_rope_append,
     prompt_attention,

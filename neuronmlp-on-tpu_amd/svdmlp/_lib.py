@@ -61,6 +61,8 @@ EXPORTED = (
     "svdmlp_norm_rope_append",
     "svdmlp_copy_pages",
     "svdmlp_keep_drafts",
+    "svdmlp_chunk_attention_workspace_bytes",
+    "svdmlp_chunk_attention",
     "svdmlp_profile_enable",
     "svdmlp_profile_read",
     "svdmlp_stage_name",
@@ -137,6 +139,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.svdmlp_copy_pages.argtypes = [_vp, _i64] + [_vp] * 4 + [_i64] * 5 + [_i32, _vp]
     lib.svdmlp_keep_drafts.restype = ctypes.c_int
     lib.svdmlp_keep_drafts.argtypes = [_vp, _i64] + [_vp] * 5 + [_i64] * 9 + [_i32, _vp]
+    lib.svdmlp_chunk_attention_workspace_bytes.restype = _sz
+    lib.svdmlp_chunk_attention_workspace_bytes.argtypes = [_i64] * 7 + [_i32]
+    lib.svdmlp_chunk_attention.restype = ctypes.c_int
+    lib.svdmlp_chunk_attention.argtypes = [_vp] * 8 + [_i64] * 8 + [f32, _i32, _vp, _sz, _vp]
     lib.svdmlp_profile_enable.restype = ctypes.c_int
     lib.svdmlp_profile_enable.argtypes = [ctypes.c_int]
     lib.svdmlp_profile_read.restype = ctypes.c_int

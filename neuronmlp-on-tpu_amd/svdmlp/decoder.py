@@ -5,6 +5,7 @@
     norm_rope, norm_rope_append                     both, of normalised heads
     prompt_attention(q, k, v, cu_seqlens)           attention over packed prompts
     cache_attention(q, k_cache, v_cache, table, lengths)  decode, drafted trees
+    chunk_attention(q, k_cache, v_cache, table, lengths, cu_seqlens)   chunks of prompts, and decode among them
     residual_norm(x, branch, weight)                sum after a block, next norm
 
 With the projections and :func:`svdmlp.svd_mlp` they make a decoder layer
@@ -206,6 +207,7 @@ def _refuse_heads(q, k, *more) -> None:
 _Strides3 = ctypes.c_int64 * 3
 _Strides5 = ctypes.c_int64 * 5
 _Strides8 = ctypes.c_int64 * 8
+_Strides11 = ctypes.c_int64 * 11
 _Strides14 = ctypes.c_int64 * 14
 _Strides15 = ctypes.c_int64 * 15
 _address = ctypes.addressof
@@ -622,6 +624,82 @@ def cache_attention(q, k_cache, v_cache, block_table, lengths, *, tree=None, sca
         _launch(index, lib.svdmlp_cache_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
                 lengths.data_ptr(), tree_ptr, out.data_ptr(), _address(st), B, n, pages, page, width, Hq, Hk, D, scale, code,
                 None, 0, None, 0)
+    return out
+
+
+def chunk_attention(q, k_cache, v_cache, block_table, lengths, cu_seqlens, *, scale: float | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed chunks of new tokens onto a paged cache: q (T, Hq, D), rows
+    cu_seqlens[b] to cu_seqlens[b + 1] of it are the last of the ``lengths[b]``
+    tokens that the cache (pages, page size, Hk, D) holds of sequence b, any number
+    of them: one where it generates, a chunk of its prompt where that is being read.
+    Each sees the keys of its sequence up to itself.  block_table and lengths as
+    :func:`cache_attention`, cu_seqlens as :func:`prompt_attention`.  A token
+    without keys (a sequence with more new tokens than its length) gets zeros; pages outside the cache hold
+    no keys; rows behind the last sequence are not written."""
+    qs, cs = q.shape, k_cache.shape
+    if len(qs) != 3:
+        raise ValueError(f"expected q (new tokens, heads, head size), got {tuple(qs)}")
+    T, Hq, D = qs
+    if len(cs) != 4 or v_cache.shape != cs or cs[3] != D or not cs[0] or not cs[1]:
+        _refuse_caches(k_cache, v_cache, cs[2] if len(cs) == 4 else "kv heads", D)
+    pages, page, Hk, _ = cs
+    if not Hq or not Hk or not D or Hq % Hk:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hk} key/value heads")
+    dtype, index = q.dtype, q.get_device()
+    if k_cache.dtype != dtype or v_cache.dtype != dtype or dtype not in _ACT_CODES:
+        _refuse_dtype(dtype, k_cache.dtype, v_cache.dtype)
+    if index < 0 or k_cache.get_device() != index or v_cache.get_device() != index:
+        _refuse_device("chunk_attention", q, k_cache, v_cache)
+    if _gradients():
+        _refuse_grad("chunk_attention", q, k_cache, v_cache, out)
+    _head_size(D, dtype)
+    scale = _attention_scale(scale, D)
+    if block_table.dim() != 2 or block_table.shape[1] == 0:
+        raise ValueError("block_table must have shape (sequences, pages of the longest)")
+    B, width = block_table.shape
+    if block_table.stride(1) != 1 or block_table.dtype is not torch.int32:
+        if block_table.dtype is torch.int64:
+            block_table = block_table.masked_fill((block_table < 0) | (block_table >= min(pages, 1 << 31)), -1)
+        block_table = _index("block_table", block_table, (B, width), torch.int32, index)
+    elif block_table.get_device() != index:
+        raise ValueError("all inputs must be on the same device")
+    lengths = _index("lengths", lengths, (B,), torch.int32, index)
+    cu_seqlens = _index("cu_seqlens", cu_seqlens, (B + 1,), torch.int32, index)
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.stride(3) != 1:
+            raise ValueError(f"the last dimension of {name} must be contiguous")
+        _aligned(name, c)
+    if out is None:
+        out = q.new_empty((T, Hq, D))
+    else:
+        _writable("out", out, (T, Hq, D), q)
+        _aligned("out", out)
+        _apart("out", out, q, k_cache, v_cache, block_table, lengths, cu_seqlens)
+    if T == 0 or B == 0:
+        return out
+    q = _rows(q)
+    lib, code = _lib.load(), _ACT_CODES[dtype]
+    qst, kst, vst, ost = q.stride(), k_cache.stride(), v_cache.stride(), out.stride()
+    st = _Strides11(qst[0], qst[1], kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], ost[0], ost[1], block_table.stride(0))
+
+    def launch(room, nbytes):
+        _launch(index, lib.svdmlp_chunk_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                lengths.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr(), _address(st), T, B, pages, page, width, Hq, Hk, D, scale, code,
+                room, nbytes)
+
+    key = ("chunk", index, T, B, page, width, Hq, Hk, D, code)
+    nbytes = _SIZES.get(key)
+    if nbytes is None:
+        if len(_SIZES) > 4096:
+            _SIZES.clear()
+        with torch.cuda.device(index):
+            nbytes = _SIZES[key] = int(lib.svdmlp_chunk_attention_workspace_bytes(T, B, page, width, Hq, Hk, D, code))
+    if nbytes:
+        with _partials_lock:  # a call may be several launches: no other thread's between them
+            launch(_partials(index, nbytes, 0)[0].data_ptr(), nbytes)
+    else:
+        launch(None, 0)
     return out
 
 
