@@ -2876,7 +2876,10 @@ size_t svdmlp_chunk_attention_workspace_bytes(int64_t T, int64_t B, int64_t page
   if (check_heads("chunk_attention", T, Hq, Hk, D, dtype, 256) || B <= 0 || B > 0x7fffffff || page <= 0 || width <= 0 ||
       width > kCachePagesMost || page > kChunkTokensMost / width)
     return 0;
-  return (size_t)plan_chunk_attention(T, B, Hq, Hk, D, dtype == SVDMLP_BF16, page * width, device_cus()).floats * 4;
+  int64_t floats = 0;  // of caches laid out alike, or not
+  for (bool alike : {false, true})
+    floats = std::max(floats, plan_chunk_attention(T, B, Hq, Hk, D, dtype == SVDMLP_BF16, alike, page, page * width, device_cus()).floats);
+  return (size_t)floats * 4;
 }
 
 int svdmlp_chunk_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -2908,16 +2911,16 @@ int svdmlp_chunk_attention(const void* q, const void* k_cache, const void* v_cac
     p.page_mul = (uint32_t)((((uint64_t)1 << (31 + log)) + page - 1) / page);
     p.page_shift = log - 1;
   }
-  p.alike = s[2] == s[5] && s[3] == s[6];
+  constexpr int64_t kStrideMost = (int64_t)1 << 30;  // elements, of 4 bytes at most
+  p.alike = s[2] == s[5] && s[3] == s[6] && s[2] < kStrideMost && s[3] < kStrideMost / page;
   p.c = scale * 1.44269504088896340736f;
-  const int cus = device_cus();
-  const ChunkPlan plan = plan_chunk_attention(T, B, Hq, Hk, D, dtype == SVDMLP_BF16, page * width, cus);
+  const ChunkPlan plan = plan_chunk_attention(T, B, Hq, Hk, D, dtype == SVDMLP_BF16, p.alike, page, page * width, device_cus());
   const size_t need = (size_t)plan.floats * 4;
   if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 15u)))
     return fail("chunk_attention: workspace too small: %zu bytes needed, 16-byte aligned, got %zu", need, ws_bytes);
   p.part = static_cast<float*>(workspace);
   StageScope sc(ST_CHUNK_ATTENTION, (hipStream_t)stream);
-  return check(launch_chunk_attention(p, dtype == SVDMLP_BF16, plan, cus, (hipStream_t)stream), "chunk_attention",
+  return check(launch_chunk_attention(p, dtype == SVDMLP_BF16, plan, (hipStream_t)stream), "chunk_attention",
                "too many rows or sequences for one launch");
 }
 

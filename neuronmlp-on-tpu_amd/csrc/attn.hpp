@@ -113,6 +113,13 @@ struct TileLane {
   }
 };
 
+__device__ __forceinline__ float most_of(const f32x16& s) {
+  float m = fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) m = fmaxf(fmaxf(m, s[i]), s[i + 1]);
+  return m;
+}
+
 // All ones where a value (one fp32 or two bf16 a word) is an infinity or NaN;
 // in integer arithmetic, since comparisons keep a scalar register pair each.
 template <bool BF16>
@@ -203,6 +210,13 @@ __device__ __forceinline__ void load_lds16(const void* p, uint32_t offset, uint3
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"((uint32_t)__builtin_amdgcn_readfirstlane((int)base)), "v"(offset), "s"(u)
+               : "memory");
+}
+// 4 bytes a lane, lane i's to base + 4 i.
+__device__ __forceinline__ void load_lds4(const void* p, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"((uint32_t)__builtin_amdgcn_readfirstlane((int)base)), "v"(p)
                : "memory");
 }
 // Until at most N of the wave's loads are on their way.

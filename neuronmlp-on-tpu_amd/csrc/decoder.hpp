@@ -113,12 +113,16 @@ inline int64_t cache_counters(const CachePlan& plan, int B, int Hk) {
 hipError_t launch_cache_attention(const CacheParams& p, bool bf16, const CachePlan& plan, hipStream_t st);
 
 // Sequences whose rows (new tokens x heads of a group) number from .. upto take
-// tiles of `rows` rows.
+// tiles of `rows` rows; their work is a line of units of 2^unit_log keys, of which a
+// block takes at least `least`.
 struct ChunkClass {
-  int from, upto, rows;
-  int slots, least;        // chunks of keys: about so many, of at least so many keys
-  int64_t blocks;          // at most; 0: no sequence can be of the class
-  int64_t parts, part_at;  // room for the sums of so many chunks, from which float on
+  int from, upto, rows, rows_log;
+  int unit_log, slope, start, least;  // slope: a tile has so many units more than the one before it; start: as many as a tile's start and end take
+  int step;                    // keys that a block takes at once
+  int blocks, grid;            // parts of the line, blocks of the launch; 0: no sequence can be of the class
+  int joins, join_units;       // blocks that join the sums of tiles in several parts, of a cut
+  int fits;                    // whether units and tiles fit the kernels' numbers
+  int64_t part_at;             // room for two tiles' sums a block, from which float on
 };
 struct ChunkParams {
   const void* q;        // (T, Hq, D), sequence b's new tokens in rows cu[b] .. cu[b + 1]
@@ -132,7 +136,7 @@ struct ChunkParams {
   int page, width, T, B, Hq, Hk, D;
   uint32_t page_mul;  // x / page = umulhi(x, page_mul) >> page_shift, for x < 2^31 and a page of over one token
   int page_shift;
-  int alike;  // keys and values have the same page and token strides
+  int alike;  // keys and values have the same page and token strides, and those and a page are below 2^32 bytes
   float c;    // softmax scale * log2(e)
 };
 constexpr int kFewRows = 128;
@@ -141,8 +145,10 @@ struct ChunkPlan {
   ChunkClass many, few;
   int64_t floats;  // of the workspace
 };
-ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, bool bf16, int64_t capacity, int64_t cus);
-hipError_t launch_chunk_attention(const ChunkParams& p, bool bf16, const ChunkPlan& plan, int cus, hipStream_t st);
+// alike: ChunkParams::alike; a workspace for calls of either kind takes the larger plan.
+ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, bool bf16, bool alike, int64_t page, int64_t capacity, int64_t cus);
+void launch_chunk_waves(const ChunkParams& p, const ChunkClass& k, bool bf16, hipStream_t st);  // tiles of 32 rows
+hipError_t launch_chunk_attention(const ChunkParams& p, bool bf16, const ChunkPlan& plan, hipStream_t st);
 
 // The caches (pages, page, Hk, D) of a model's layers, all laid out alike: as many
 // as a launch's arguments hold.

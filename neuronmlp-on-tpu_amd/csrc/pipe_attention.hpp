@@ -40,13 +40,6 @@ struct PipeCfg {
   static_assert(FRAGS % AHEAD == 0 && PER * SLOTS == 16 * QG, "slots");
 };
 
-__device__ __forceinline__ float lane_max(const f32x16& s) {
-  float m = fmaxf(s[0], s[1]);
-#pragma unroll
-  for (int i = 2; i < 16; i += 2) m = fmaxf(fmaxf(m, s[i]), s[i + 1]);
-  return m;
-}
-
 // What a wave holds of its 64 rows, and its part of the walk.
 template <class C>
 struct PipeWave {
@@ -111,7 +104,7 @@ struct PipeWave {
     bool over = false;
 #pragma unroll
     for (int g = 0; g < QG; ++g) {
-      mx[g] = lane_max(s[g]) * c;
+      mx[g] = most_of(s[g]) * c;
       over |= mx[g] > m[g] + kSlack;
     }
     if (!__any(over)) return false;
@@ -149,11 +142,12 @@ struct PipeWave {
   }
 
   // Tiles 0 to full - 1 (at least one), of keys that every row sees; arrive(t)
-  // returns when tile t can be read.  Before the first step the values of the
+  // returns when tile t can be read, and beside(n) is what a slot n of its first
+  // step may do with what the matrix unit leaves it.  again: rows have sums already.  Before the first step the values of the
   // last stage's second unit are multiplied by zero weights: they have to be
   // finite.
-  template <class Arrive>
-  __device__ __forceinline__ void whole_tiles(attn_lds base, int full, int& t, Arrive arrive) {
+  template <class Arrive, class Beside>
+  __device__ __forceinline__ void whole_tiles(attn_lds base, int full, int& t, bool again, Arrive arrive, Beside beside) {
     f32x16 s0[QG], s1[QG];
     u32x4 p0[QG][2], p1[QG][2], frag[C::AHEAD];
     float scale[QG], over[QG];  // over: the score beyond which the reference moves
@@ -230,6 +224,7 @@ struct PipeWave {
             pc[wg][wi / 8][wi % 8 / 2] = both;
           }
         }
+        if constexpr (U == 0) beside(n);
       }
       __builtin_amdgcn_sched_barrier(0);
       bool any = moved;
@@ -245,7 +240,7 @@ struct PipeWave {
     };
     arrive(0);
     scores(base, base, s0);
-    if (reference(s0, scale)) {}  // nothing has been summed yet
+    if (reference(s0, scale) && again) rescale(scale);  // (else nothing has been summed yet)
 #pragma unroll
     for (int g = 0; g < QG; ++g) {
       if (m[g] == -INFINITY) m[g] = -1e30f;  // no finite score yet: a finite reference that any will move

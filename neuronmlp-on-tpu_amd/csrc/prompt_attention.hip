@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256, 1) void prompt_pipe_kernel(PromptParams p) {
   };
 
   int t = 0;
-  if (full > 0) w.whole_tiles(base, full, t, arrive);
+  if (full > 0) w.whole_tiles(base, full, t, false, arrive, [](int) {});
   for (; t < tiles; ++t) {
     arrive(t);
     const attn_lds cur = base + (t % C::NS) * C::STAGE;
