@@ -53,6 +53,8 @@ class Line {
       if (b0 == 0) first_ = s;
       tiles += sum(s.tiles);
     }
+    slope_ = k_.slope;
+    if (p_.B <= 64 && (int64_t)tiles * p_.Hk * 2 <= k_.blocks && alone(tiles)) return;
     // Tiles that are blocks of their own: whole rounds of them, all but the last.
     const int rounds = MANY ? (int)((int64_t)tiles * p_.Hk / k_.blocks) - 1 : 0;
     from_ = max(rounds, 0) * (int64_t)k_.blocks / p_.Hk;
@@ -69,6 +71,29 @@ class Line {
     }
     total = units * p_.Hk;
     part = max((total + k_.blocks - 1) / k_.blocks, k_.least);
+  }
+  // Few tiles: where each can be cut into equal pieces, one a block, that are hardly
+  // longer than equal parts of the line, no block takes the time of two pieces'
+  // starts and ends.  A tile's units are then those pieces.
+  __device__ __forceinline__ bool alone(int tiles) {
+    const int most = first_.a + slope_ * max(first_.tiles - 1, 0), n = tiles * p_.Hk;
+    const int line = sum(upto(first_.a, first_.tiles, first_.tiles)) * p_.Hk;
+    const int even = max((line + k_.blocks - 1) / k_.blocks, k_.least);
+    int best = 0;
+    for (int i = 0; i < 8 && !best; ++i) {
+      const int length = max((int)((float)line / (float)(k_.blocks - n * i / 8)) + 1, k_.least);
+      if (length > even + k_.start) break;
+      if (sum(first_.tiles * ((most + length - 1) / length)) * p_.Hk <= k_.blocks) best = length;
+    }
+    if (!best) return false;
+    first_.a = (most + best - 1) / best;
+    slope_ = 0;
+    from_ = whole = 0;
+    Carry c = {};
+    order(first_, 0, c);
+    total = sum(first_.mine) * p_.Hk;
+    part = 1;
+    return true;
   }
   // Tile `id` of those that are blocks of their own.
   __device__ __forceinline__ void tile(int id, Place& w) const {
@@ -130,7 +155,7 @@ class Line {
   // Units of the first m tiles of a sequence, the last rows' first.
   __device__ __forceinline__ int upto(int a, int tiles, int m) const {
     const uint32_t n = m;  // (where the slope is 0 the other factor may be anything)
-    return (int)(n * a + (uint32_t)k_.slope * (n * (uint32_t)(tiles - 1) - n * (n - 1) / 2));
+    return (int)(n * a + (uint32_t)slope_ * (n * (uint32_t)(tiles - 1) - n * (n - 1) / 2));
   }
   // Bounds that leave the rows or run backwards are cut, so that no row is of two
   // sequences; lengths beyond the table too.  c.ends: rows up to there are taken.
@@ -157,29 +182,29 @@ class Line {
   // among 64.
   __device__ __forceinline__ void order(Some& s, int b0, Carry& c) const {
     if constexpr (MANY) {
-      const int n = min(64, p_.B - b0);
-      s.before = c.tiles;
-      for (int j = 0; j < n; ++j) {
-        const int len = __builtin_amdgcn_readlane(s.len, j);
-        if (len > s.len || (len == s.len && j < lane_)) s.before += __builtin_amdgcn_readlane(s.tiles, j);
-      }
+      s.before = c.tiles + sum_before(s, s.tiles);
     } else {
       s.before = c.tiles + sums_upto(s.tiles) - s.tiles;
     }
     const int z0 = min(max(from_ - s.before, 0), s.tiles);
     s.mine = upto(s.a, s.tiles, s.tiles) - upto(s.a, s.tiles, z0);
     if constexpr (MANY) {
-      const int n = min(64, p_.B - b0);
-      s.units_before = c.units;
-      for (int j = 0; j < n; ++j) {
-        const int len = __builtin_amdgcn_readlane(s.len, j);
-        if (len > s.len || (len == s.len && j < lane_)) s.units_before += __builtin_amdgcn_readlane(s.mine, j);
-      }
+      s.units_before = c.units + sum_before(s, s.mine);
     } else {
       s.units_before = c.units + sums_upto(s.mine) - s.mine;
     }
     c.tiles += sum(s.tiles);
     c.units += sum(s.mine);
+  }
+  // The sum of v over the sequences longer than a lane's (of the same length, of a
+  // lower number), of those that have tiles.
+  __device__ __forceinline__ int sum_before(const Some& s, int v) const {
+    int total = 0;
+    for (uint64_t left = __ballot(s.tiles > 0); left; left &= left - 1) {
+      const int j = __builtin_ctzll(left), len = __builtin_amdgcn_readlane(s.len, j), x = __builtin_amdgcn_readlane(v, j);
+      total += len > s.len || (len == s.len && j < lane_) ? x : 0;
+    }
+    return total;
   }
   __device__ __forceinline__ Some batch(int b0, Carry& c) const {
     if (b0 == 0) {
@@ -196,14 +221,14 @@ class Line {
     w.n = __builtin_amdgcn_readlane(s.n, i);
     w.len = __builtin_amdgcn_readlane(s.len, i);
     w.tile = __builtin_amdgcn_readlane(s.tiles, i) - 1 - (q - __builtin_amdgcn_readlane(s.before, i));
-    w.units = __builtin_amdgcn_readlane(s.a, i) + k_.slope * w.tile;
+    w.units = __builtin_amdgcn_readlane(s.a, i) + slope_ * w.tile;
   }
 
   const ChunkParams& p_;
   const ChunkClass& k_;
   const int lane_;
   Some first_;
-  int from_;  // tiles (in order, without their heads) before those of the line
+  int from_, slope_;  // from_: tiles (in order, without their heads) before those of the line
 };
 
 // What a block does of a tile: units from .. upto of it, keys kbeg .. kend.

@@ -273,11 +273,11 @@ __global__ __launch_bounds__(256, 1) void chunk_pipe_kernel(ChunkParams p, Chunk
 
 // Joins the sums of a tile that cuts lie in, at the first of them: the block before
 // the cut has the tile's start, the block behind it what follows, and so on.  A
-// thread takes 16 bytes (four elements) of a row's sums, for every `units` th of them.
+// block takes 32 rows of it, a thread every eighth 16 bytes (four elements) of one.
 template <bool BF16, bool MANY>
 __device__ __forceinline__ void join(const ChunkParams& p, const ChunkClass& k, int id) {
-  const int lane = threadIdx.x & 63, G = p.Hq / p.Hk;
-  const int cut = id / k.join_units, unit = id - cut * k.join_units, block = cut + 1;
+  const int lane = threadIdx.x & 63, G = p.Hq / p.Hk, groups = k.rows / 32;
+  const int cut = id / groups, group = id - cut * groups, block = cut + 1;
   const Line<MANY> line(p, k, lane);
   const int64_t part = line.part;
   Place w;
@@ -288,15 +288,17 @@ __device__ __forceinline__ void join(const ChunkParams& p, const ChunkClass& k, 
   // The last block with a piece of it.
   int last = (int)((tile_at + w.units - 1) / part);
   if (last > block && line.cut((int)(last * part - tile_at), w.units) == w.units) --last;
-  const int cols = 256 >> k.rows_log, rr = threadIdx.x & (k.rows - 1), r = w.tile * k.rows + rr;
+  const int rr = group * 32 + (threadIdx.x & 31), r = w.tile * k.rows + rr;
   if (r >= w.n * G) return;
   const int64_t ml_at = (int64_t)k.rows * p.D + 2 * rr;
-  auto sums = [&](int b) { return sums_of(p, k, min(b, last), b < block); };
+  // (block - 1's second sums, then the others' first ones)
+  auto sums = [&](int j) { return sums_of(p, k, min(block - 1 + j, last), j == 0); };
+  const int pieces = last - block + 2;
   float m = -INFINITY, l = 0.f;
-  for (int b0 = block - 1; b0 <= last; b0 += 8) {
+  for (int j0 = 0; j0 < pieces; j0 += 8) {
     f32x2 v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const f32x2*>(sums(b0 + j) + ml_at);
+    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const f32x2*>(sums(j0 + j) + ml_at);
     float most = m;
 #pragma unroll
     for (int j = 0; j < 8; ++j) most = fmaxf(most, v[j].x);
@@ -305,26 +307,35 @@ __device__ __forceinline__ void join(const ChunkParams& p, const ChunkClass& k, 
     // (a piece without a score over -infinity: its sums are zeros, or not finite and stay so)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (b0 + j <= last) l += v[j].y * (v[j].x == -INFINITY ? 1.f : exp2f(v[j].x - m));
+      if (j0 + j < pieces) l += v[j].y * (v[j].x == -INFINITY ? 1.f : exp2f(v[j].x - m));
   }
   const float inv = inverse_sum(l);
   const int t = r / G;
   const int64_t out = (int64_t)(w.start + t) * p.o_t + (int64_t)(w.hk * G + r - t * G) * p.o_h;
-  for (int c = unit * cols + (threadIdx.x >> k.rows_log); 4 * c < p.D; c += k.join_units * cols) {
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int b0 = block - 1; b0 <= last; b0 += 8) {
-      float v[8];
-      f32x4 x[8];
+  constexpr int kCols = 4;  // of a thread's, on their way at once
+  for (int c0 = threadIdx.x / 32; 4 * c0 < p.D; c0 += 8 * kCols) {
+    f32x4 o[kCols] = {};
+    for (int j0 = 0; j0 < pieces; j0 += 4) {
+      float v[4];
+      f32x4 x[4][kCols];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = sums(b0 + j)[ml_at];
-        x[j] = reinterpret_cast<const f32x4*>(sums(b0 + j))[c * k.rows + rr];
+      for (int j = 0; j < 4; ++j) {
+        const float* const from = sums(j0 + j);
+        v[j] = from[ml_at];
+#pragma unroll
+        for (int q = 0; q < kCols; ++q) x[j][q] = reinterpret_cast<const f32x4*>(from)[min(c0 + 8 * q, p.D / 4 - 1) * k.rows + rr];
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (b0 + j <= last) o += x[j] * (v[j] == -INFINITY ? 1.f : exp2f(v[j] - m));
+      for (int j = 0; j < 4; ++j) {
+        const float a = j0 + j >= pieces ? 0.f : v[j] == -INFINITY ? 1.f : exp2f(v[j] - m);
+        if (j0 + j < pieces)
+#pragma unroll
+          for (int q = 0; q < kCols; ++q) o[q] += x[j][q] * a;
+      }
     }
-    store4<BF16>(p.out, out + 4 * c, o * inv);
+#pragma unroll
+    for (int q = 0; q < kCols; ++q)
+      if (4 * (c0 + 8 * q) < p.D) store4<BF16>(p.out, out + 4 * (c0 + 8 * q), o[q] * inv);
   }
 }
 template <bool BF16>
@@ -353,7 +364,7 @@ ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int
     const int64_t tile = (int64_t)1 << tile_log, G = Hq / Hk;
     k.from = (int)std::min<int64_t>(from, 0x7fffffff), k.upto = (int)std::min<int64_t>(upto, 0x7fffffff);
     k.rows = (int)tile, k.rows_log = tile_log, k.step = step;
-    if (rows < from) return;
+    if (upto < from) return;
     // Sequences of the class, and their tiles: at most one short tile each.
     const int64_t n = std::min(B, rows / from);
     int64_t tiles = rows / tile + n;
@@ -371,22 +382,20 @@ ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int
     k.least = (int)std::max<int64_t>(least >> log, 1);
     k.blocks = (int)std::max<int64_t>(std::min<int64_t>(blocks, (int64_t)std::min(units() / (double)k.least, 1e9) + 1), 1);
     k.grid = k.blocks + (tile_log == 8 ? (int)std::min<int64_t>(tiles * Hk, 1 << 23) : 0);
-    const int64_t cols = 256 / tile;
-    k.join_units = (int)std::max<int64_t>(1, (D / 4 + 4 * cols - 1) / (4 * cols));
-    k.joins = (k.blocks - 1) * k.join_units;
+    k.joins = (k.blocks - 1) * (int)(tile / 32);
     k.part_at = plan.floats;
     if (k.blocks > 1) plan.floats += (int64_t)k.blocks * 2 * tile * (D + 2);
   };
   const int wave = 32 * wave_block(D, bf16);
-  const bool pipe = bf16 && D <= 128 && alike && page % (D <= 64 ? PipeCfg<64>::RPL : PipeCfg<128>::RPL) == 0;
-  if (pipe && B == 1 && rows > kFewRows) {
-    fill(plan.many, 1, rows, 8, 64, cus, 512, 384);
-  } else if (pipe) {
-    fill(plan.many, kFewRows + 1, rows, 8, 64, cus, 512, 384);
-    fill(plan.few, 1, kFewRows, 5, wave, 2 * cus, 256, 256);
-  } else {
-    fill(plan.few, 1, rows, 5, wave, 2 * cus, 256, 256);
-  }
+  // Blocks of 32-row tiles that a CU holds at once.
+  const int64_t held = !bf16 ? (D <= 128 ? 2 : 1) : D <= 64 ? 3 : D <= 128 ? 2 : 1;
+  // A call of up to one tile of 256 rows has no use for them; of one sequence of
+  // more rows for nothing else.  A start and an end of a tile take as long as 384 and
+  // 448 keys of it.
+  int64_t few = bf16 && D <= 128 && alike && page % (D <= 64 ? PipeCfg<64>::RPL : PipeCfg<128>::RPL) == 0 && rows > 256 ? kFewRows : rows;
+  if (few < rows && B == 1) few = 0;
+  fill(plan.many, few + 1, rows, 8, 64, cus, 512, 384);
+  fill(plan.few, 1, few, 5, wave, held * cus, 256, 448);
   return plan;
 }
 

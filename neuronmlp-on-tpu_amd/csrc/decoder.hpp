@@ -120,7 +120,7 @@ struct ChunkClass {
   int unit_log, slope, start, least;  // slope: a tile has so many units more than the one before it; start: as many as a tile's start and end take
   int step;                    // keys that a block takes at once
   int blocks, grid;            // parts of the line, blocks of the launch; 0: no sequence can be of the class
-  int joins, join_units;       // blocks that join the sums of tiles in several parts, of a cut
+  int joins;                   // blocks that join the sums of tiles in several parts
   int fits;                    // whether units and tiles fit the kernels' numbers
   int64_t part_at;             // room for two tiles' sums a block, from which float on
 };
