@@ -231,6 +231,15 @@ class Line {
   int from_, slope_;  // from_: tiles (in order, without their heads) before those of the line
 };
 
+// What chunk_join_kernel reads of a tile that begins in a block and goes on in others:
+// its pieces (0: there is none) and where its rows go.
+struct JoinNote {
+  int pieces, row0, rows, start, hk, pad[3];
+};
+__device__ __forceinline__ JoinNote* note_of(const ChunkParams& p, const ChunkClass& k, int block) {
+  return reinterpret_cast<JoinNote*>(p.part + k.notes_at) + block;
+}
+
 // What a block does of a tile: units from .. upto of it, keys kbeg .. kend.
 struct Piece {
   int from, upto, kbeg, kend;
@@ -271,7 +280,10 @@ __device__ __forceinline__ bool next_piece(const ChunkParams& p, const ChunkClas
   const int64_t begin = (int64_t)block * line.part;
   const int end = (int)min((int64_t)line.total, begin + line.part);
   bool first = at < 0;
-  if (first) at = (int)min(begin, (int64_t)line.total);
+  if (first) {
+    at = (int)min(begin, (int64_t)line.total);
+    if (threadIdx.x == 0 && k.blocks > 1) note_of(p, k, block)->pieces = 0;
+  }
   while (at < end && line.find(at, w)) {
     const int tile_at = at - w.u;
     piece.from = first ? line.cut(w.u, w.units) : 0;
@@ -280,6 +292,12 @@ __device__ __forceinline__ bool next_piece(const ChunkParams& p, const ChunkClas
     at = tile_at + w.units;
     if (piece.from >= piece.upto) continue;  // its neighbour takes it
     keys_of(p, k, w, piece);
+    if (piece.from == 0 && piece.upto < w.units && threadIdx.x == 0) {
+      // The last block with a piece of it.
+      int last = (tile_at + w.units - 1) / line.part;
+      if (last > block + 1 && line.cut((int)((int64_t)last * line.part - tile_at), w.units) == w.units) --last;
+      *note_of(p, k, block) = {last - block + 1, w.tile * k.rows, w.n * (p.Hq / p.Hk), w.start, w.hk, {}};
+    }
     return true;
   }
   return false;

@@ -271,68 +271,54 @@ __global__ __launch_bounds__(256, 1) void chunk_pipe_kernel(ChunkParams p, Chunk
 // Tiles in several parts
 // ---------------------------------------------------------------------------
 
-// Joins the sums of a tile that cuts lie in, at the first of them: the block before
-// the cut has the tile's start, the block behind it what follows, and so on.  A
-// block takes 32 rows of it, a thread every eighth 16 bytes (four elements) of one.
-template <bool BF16, bool MANY>
+// Joins the sums of the tile that begins in a block and goes on in those behind it.
+// A block takes 32 rows of it, a thread every eighth 16 bytes (four elements) of one.
+template <bool BF16>
 __device__ __forceinline__ void join(const ChunkParams& p, const ChunkClass& k, int id) {
-  const int lane = threadIdx.x & 63, G = p.Hq / p.Hk, groups = k.rows / 32;
-  const int cut = id / groups, group = id - cut * groups, block = cut + 1;
-  const Line<MANY> line(p, k, lane);
-  const int64_t part = line.part;
-  Place w;
-  if (block * part >= line.total || !line.find((int)(block * part), w)) return;
-  if (w.u == 0 || line.cut(w.u, w.units) != w.u) return;  // the cut lies between tiles
-  const int64_t tile_at = block * part - w.u, before = (block - 1) * part - tile_at;
-  if (before > 0 && line.cut((int)before, w.units) == (int)before) return;  // the tile's first cut is an earlier one
-  // The last block with a piece of it.
-  int last = (int)((tile_at + w.units - 1) / part);
-  if (last > block && line.cut((int)(last * part - tile_at), w.units) == w.units) --last;
-  const int rr = group * 32 + (threadIdx.x & 31), r = w.tile * k.rows + rr;
-  if (r >= w.n * G) return;
+  const int G = p.Hq / p.Hk, block = id >> (k.rows_log - 5), group = id - (block << (k.rows_log - 5));
+  const JoinNote w = *note_of(p, k, block);
+  const int pieces = w.pieces;
+  if (pieces == 0) return;
+  const int rr = group * 32 + (threadIdx.x & 31), r = w.row0 + rr;
+  if (r >= w.rows) return;
   const int64_t ml_at = (int64_t)k.rows * p.D + 2 * rr;
-  // (block - 1's second sums, then the others' first ones)
-  auto sums = [&](int j) { return sums_of(p, k, min(block - 1 + j, last), j == 0); };
-  const int pieces = last - block + 2;
-  float m = -INFINITY, l = 0.f;
-  for (int j0 = 0; j0 < pieces; j0 += 8) {
-    f32x2 v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const f32x2*>(sums(j0 + j) + ml_at);
-    float most = m;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) most = fmaxf(most, v[j].x);
-    l *= m == most ? 1.f : exp2f(m - most);
-    m = most;
-    // (a piece without a score over -infinity: its sums are zeros, or not finite and stay so)
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j0 + j < pieces) l += v[j].y * (v[j].x == -INFINITY ? 1.f : exp2f(v[j].x - m));
-  }
-  const float inv = inverse_sum(l);
+  // The block's second sums, then the others' first ones.
+  auto sums = [&](int j) { return sums_of(p, k, block + min(j, pieces - 1), j == 0); };
   const int t = r / G;
   const int64_t out = (int64_t)(w.start + t) * p.o_t + (int64_t)(w.hk * G + r - t * G) * p.o_h;
-  constexpr int kCols = 4;  // of a thread's, on their way at once
+  constexpr int kCols = 4, kPieces = 4;  // on their way at once
   for (int c0 = threadIdx.x / 32; 4 * c0 < p.D; c0 += 8 * kCols) {
     f32x4 o[kCols] = {};
-    for (int j0 = 0; j0 < pieces; j0 += 4) {
-      float v[4];
-      f32x4 x[4][kCols];
+    float m = -INFINITY, l = 0.f;
+    for (int j0 = 0; j0 < pieces; j0 += kPieces) {
+      f32x2 v[kPieces];
+      f32x4 x[kPieces][kCols];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kPieces; ++j) {
         const float* const from = sums(j0 + j);
-        v[j] = from[ml_at];
+        v[j] = *reinterpret_cast<const f32x2*>(from + ml_at);
 #pragma unroll
         for (int q = 0; q < kCols; ++q) x[j][q] = reinterpret_cast<const f32x4*>(from)[min(c0 + 8 * q, p.D / 4 - 1) * k.rows + rr];
       }
+      float most = m;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = j0 + j >= pieces ? 0.f : v[j] == -INFINITY ? 1.f : exp2f(v[j] - m);
-        if (j0 + j < pieces)
+      for (int j = 0; j < kPieces; ++j) most = fmaxf(most, v[j].x);
+      const float a = m == most ? 1.f : exp2f(m - most);
+      m = most;
+      l *= a;
 #pragma unroll
-          for (int q = 0; q < kCols; ++q) o[q] += x[j][q] * a;
-      }
+      for (int q = 0; q < kCols; ++q) o[q] *= a;
+      // (a piece without a score over -infinity: its sums are zeros, or not finite and stay so)
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+        if (j0 + j < pieces) {
+          const float b = v[j].x == -INFINITY ? 1.f : exp2f(v[j].x - m);
+          l += v[j].y * b;
+#pragma unroll
+          for (int q = 0; q < kCols; ++q) o[q] += x[j][q] * b;
+        }
     }
+    const float inv = inverse_sum(l);
 #pragma unroll
     for (int q = 0; q < kCols; ++q)
       if (4 * (c0 + 8 * q) < p.D) store4<BF16>(p.out, out + 4 * (c0 + 8 * q), o[q] * inv);
@@ -341,8 +327,8 @@ __device__ __forceinline__ void join(const ChunkParams& p, const ChunkClass& k, 
 template <bool BF16>
 __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkParams p, ChunkClass many, ChunkClass few) {
   const int id = blockIdx.x;
-  if (id < many.joins) join<BF16, true>(p, many, id);
-  else join<BF16, false>(p, few, id - many.joins);
+  if (id < many.joins) join<BF16>(p, many, id);
+  else join<BF16>(p, few, id - many.joins);
 }
 
 template <int DP>
@@ -382,20 +368,22 @@ ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int
     k.least = (int)std::max<int64_t>(least >> log, 1);
     k.blocks = (int)std::max<int64_t>(std::min<int64_t>(blocks, (int64_t)std::min(units() / (double)k.least, 1e9) + 1), 1);
     k.grid = k.blocks + (tile_log == 8 ? (int)std::min<int64_t>(tiles * Hk, 1 << 23) : 0);
-    k.joins = (k.blocks - 1) * (int)(tile / 32);
-    k.part_at = plan.floats;
-    if (k.blocks > 1) plan.floats += (int64_t)k.blocks * 2 * tile * (D + 2);
+    if (k.blocks == 1) return;
+    k.joins = (k.blocks - 1) * (int)(tile / 32);  // (no tile begins in the last block and goes on)
+    k.notes_at = plan.floats;
+    k.part_at = plan.floats + (int64_t)k.blocks * (sizeof(JoinNote) / 4);
+    plan.floats = k.part_at + (int64_t)k.blocks * 2 * tile * (D + 2);
   };
   const int wave = 32 * wave_block(D, bf16);
   // Blocks of 32-row tiles that a CU holds at once.
   const int64_t held = !bf16 ? (D <= 128 ? 2 : 1) : D <= 64 ? 3 : D <= 128 ? 2 : 1;
   // A call of up to one tile of 256 rows has no use for them; of one sequence of
   // more rows for nothing else.  A start and an end of a tile take as long as 384 and
-  // 448 keys of it.
+  // 256 keys of it.
   int64_t few = bf16 && D <= 128 && alike && page % (D <= 64 ? PipeCfg<64>::RPL : PipeCfg<128>::RPL) == 0 && rows > 256 ? kFewRows : rows;
   if (few < rows && B == 1) few = 0;
   fill(plan.many, few + 1, rows, 8, 64, cus, 512, 384);
-  fill(plan.few, 1, few, 5, wave, held * cus, 256, 448);
+  fill(plan.few, 1, few, 5, wave, held * cus, 512, 256);
   return plan;
 }
 

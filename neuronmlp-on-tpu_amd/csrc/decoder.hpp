@@ -122,7 +122,7 @@ struct ChunkClass {
   int blocks, grid;            // parts of the line, blocks of the launch; 0: no sequence can be of the class
   int joins;                   // blocks that join the sums of tiles in several parts
   int fits;                    // whether units and tiles fit the kernels' numbers
-  int64_t part_at;             // room for two tiles' sums a block, from which float on
+  int64_t notes_at, part_at;   // from which float of the workspace on: a note a block, two tiles' sums a block
 };
 struct ChunkParams {
   const void* q;        // (T, Hq, D), sequence b's new tokens in rows cu[b] .. cu[b + 1]
