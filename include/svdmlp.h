@@ -428,15 +428,16 @@ int svdmlp_norm_rope_append(const void* q, const void* k, const void* v, const i
 
 /*
  * Pages of a paged cache to other pages of it, in n caches at once (the keys'
- * and values' of all layers: a host array of device addresses, each cache
- * (pages, page, Hk, D) with the same strides: page, row, head): the first
+ * and values' of all layers: a host array of device addresses or, with `apart`
+ * not 0, the first one alone, the others `apart` elements behind each other; each
+ * cache (pages, page, Hk, D) with the same strides: page, row, head): the first
  * rows[i] rows (int32; NULL: all) of page dst[i] become those of page src[i],
  * i < m.  A pair with a page outside the cache, or of a page and itself, is
  * skipped.  The pages of dst have to differ from each other and from those
  * of src: with a page twice its rows are of neither pair for sure.
  */
-int svdmlp_copy_pages(void* const* caches, int64_t n, const int64_t* strides /* 3 or NULL */, const int32_t* src,
-                      const int32_t* dst, const int32_t* rows, int64_t m, int64_t pages, int64_t page, int64_t Hk,
+int svdmlp_copy_pages(void* const* caches, int64_t n, int64_t apart, const int64_t* strides /* 3 or NULL */,
+                      const int32_t* src, const int32_t* dst, const int32_t* rows, int64_t m, int64_t pages, int64_t page, int64_t Hk,
                       int64_t D, int32_t dtype, void* stream);
 
 /*
@@ -450,7 +451,7 @@ int svdmlp_copy_pages(void* const* caches, int64_t n, const int64_t* strides /* 
  * short path).  A sequence of fewer tokens than drafts stays as it is, with
  * its length; a row in a page outside the cache is not moved.
  */
-int svdmlp_keep_drafts(void* const* caches, int64_t n, const int64_t* strides /* 3 or NULL */,
+int svdmlp_keep_drafts(void* const* caches, int64_t n, int64_t apart, const int64_t* strides /* 3 or NULL */,
                        const int32_t* block_table, const int32_t* lengths, const int32_t* path, int32_t* new_lengths,
                        int64_t table_stride, int64_t B, int64_t width, int64_t m, int64_t drafts, int64_t pages,
                        int64_t page, int64_t Hk, int64_t D, int32_t dtype, void* stream);

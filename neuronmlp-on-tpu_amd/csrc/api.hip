@@ -2627,8 +2627,8 @@ int norm_rope_call(const char* what, NormRopeParams& p, int64_t Hq, int64_t Hk, 
 
 // The caches of an entry point that moves rows: their sizes and strides; the
 // addresses are filled in launch by launch.
-int cache_set(const char* what, CacheSet& c, void* const* caches, int64_t n, const int64_t* strides, int64_t pages,
-              int64_t page, int64_t Hk, int64_t D, int32_t dtype, bool* vec) {
+int cache_set(const char* what, CacheSet& c, void* const* caches, int64_t n, int64_t apart, const int64_t* strides,
+              int64_t pages, int64_t page, int64_t Hk, int64_t D, int32_t dtype, bool* vec) {
   if (!act_size(dtype)) return fail("%s: dtype must be bf16 or fp32, got %d", what, (int)dtype);
   if (!caches || n <= 0) return fail("%s: no caches", what);
   if (pages <= 0 || page <= 0 || Hk <= 0 || D <= 0) return fail("%s: sizes must be positive", what);
@@ -2640,18 +2640,20 @@ int cache_set(const char* what, CacheSet& c, void* const* caches, int64_t n, con
   c.p_s = s[0], c.t_s = s[1], c.h_s = s[2];
   c.pages = pages, c.es = act_size(dtype), c.page = (int)page, c.Hk = (int)Hk, c.D = (int)D;
   *vec = pieces16({}, {D, s[0], s[1], s[2]}, c.es);
-  for (int64_t i = 0; i < n; ++i) {
+  if (apart < 0) return fail("%s: strides must not be negative", what);
+  for (int64_t i = 0; i < (apart ? 1 : n); ++i) {
     if (!caches[i]) return fail("%s: null pointer", what);
     *vec = *vec && ((uintptr_t)caches[i] & 15u) == 0;
   }
+  *vec = *vec && apart * c.es % 16 == 0;
   return SVDMLP_OK;
 }
 // Calls go(set) for every kCachesMost of the caches.
 template <class F>
-hipError_t each_cache_set(CacheSet& c, void* const* caches, int64_t n, F go) {
+hipError_t each_cache_set(CacheSet& c, void* const* caches, int64_t n, int64_t apart, F go) {
   for (int64_t i = 0; i < n; i += kCachesMost) {
     c.n = (int)std::min<int64_t>(kCachesMost, n - i);
-    std::copy(caches + i, caches + i + c.n, c.base);
+    for (int j = 0; j < c.n; ++j) c.base[j] = apart ? static_cast<char*>(caches[0]) + (i + j) * apart * c.es : caches[i + j];
     if (const hipError_t e = go(); e != hipSuccess) return e;
   }
   return hipSuccess;
@@ -2836,28 +2838,28 @@ int svdmlp_norm_rope_append(const void* q, const void* k, const void* v, const i
   return norm_rope_call("norm_rope_append", p, Hq, Hk, D, rot, scale, eps, dtype, flags, stream);
 }
 
-int svdmlp_copy_pages(void* const* caches, int64_t n, const int64_t* strides, const int32_t* src, const int32_t* dst,
+int svdmlp_copy_pages(void* const* caches, int64_t n, int64_t apart, const int64_t* strides, const int32_t* src, const int32_t* dst,
                       const int32_t* rows, int64_t m, int64_t pages, int64_t page, int64_t Hk, int64_t D,
                       int32_t dtype, void* stream) {
   PageCopyParams p = {};
   bool vec = false;
-  const int rc = cache_set("copy_pages", p.c, caches, n, strides, pages, page, Hk, D, dtype, &vec);
+  const int rc = cache_set("copy_pages", p.c, caches, n, apart, strides, pages, page, Hk, D, dtype, &vec);
   if (rc) return rc;
   if (!src || !dst) return fail("copy_pages: null pointer");
   if (m <= 0 || m > 0x7fffffff) return fail("copy_pages: %lld pages", (long long)m);
   p.src = src, p.dst = dst, p.rows = rows;
   StageScope s(ST_COPY_PAGES, (hipStream_t)stream);
-  return check(each_cache_set(p.c, caches, n, [&] { return launch_copy_pages(p, m, vec, (hipStream_t)stream); }), "copy_pages",
+  return check(each_cache_set(p.c, caches, n, apart, [&] { return launch_copy_pages(p, m, vec, (hipStream_t)stream); }), "copy_pages",
                "pages are too large for one launch");
 }
 
-int svdmlp_keep_drafts(void* const* caches, int64_t n, const int64_t* strides, const int32_t* block_table,
+int svdmlp_keep_drafts(void* const* caches, int64_t n, int64_t apart, const int64_t* strides, const int32_t* block_table,
                        const int32_t* lengths, const int32_t* path, int32_t* new_lengths, int64_t table_stride,
                        int64_t B, int64_t width, int64_t m, int64_t drafts, int64_t pages, int64_t page, int64_t Hk,
                        int64_t D, int32_t dtype, void* stream) {
   DraftKeepParams p = {};
   bool vec = false;
-  const int rc = cache_set("keep_drafts", p.c, caches, n, strides, pages, page, Hk, D, dtype, &vec);
+  const int rc = cache_set("keep_drafts", p.c, caches, n, apart, strides, pages, page, Hk, D, dtype, &vec);
   if (rc) return rc;
   if (!block_table || !lengths || !path || !new_lengths) return fail("keep_drafts: null pointer");
   if (B <= 0 || width <= 0 || B > 0x7fffffff || page > 0x7fffff00 / width) return fail("keep_drafts: sizes must be positive, with less than 2^31 tokens a sequence");
@@ -2867,7 +2869,7 @@ int svdmlp_keep_drafts(void* const* caches, int64_t n, const int64_t* strides, c
   p.table = block_table, p.lengths = lengths, p.path = path, p.new_lengths = new_lengths;
   p.table_b = table_stride, p.width = (int)width, p.B = (int)B, p.m = (int)m, p.drafts = (int)drafts;
   StageScope s(ST_KEEP_DRAFTS, (hipStream_t)stream);
-  return check(each_cache_set(p.c, caches, n, [&] { return launch_keep_drafts(p, vec, (hipStream_t)stream); }), "keep_drafts",
+  return check(each_cache_set(p.c, caches, n, apart, [&] { return launch_keep_drafts(p, vec, (hipStream_t)stream); }), "keep_drafts",
                "too many sequences for one launch");
 }
 

@@ -21,17 +21,6 @@ namespace svdmlp {
 
 namespace {
 
-// E values from element `at` on.
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void take(const char* p, int at, float* x) {
-  if constexpr (VEC) unpack<BF16>(*reinterpret_cast<const u32x4*>(p + at * (BF16 ? 2 : 4)), x);
-  else x[0] = ld1<BF16>(p, at);
-}
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void give(char* p, int at, const float* x) {
-  if constexpr (VEC) *reinterpret_cast<u32x4*>(p + at * (BF16 ? 2 : 4)) = pack<BF16>(x);
-  else st1<BF16>(p, at, x[0]);
-}
 template <int E>
 __device__ __forceinline__ void scaled(float* x, float by, const float* w) {
   if constexpr (E == 1) {
@@ -49,116 +38,142 @@ __device__ __forceinline__ void scaled(float* x, float by, const float* w) {
 // VEC: D, rot, every stride and every base in whole 16-byte pieces (half layout:
 // rot / 2 too); a unit of a head is then a piece of its first half with its
 // partner (half layout) or a piece (interleaved, and behind rot), else a pair or,
-// behind rot, a value.
-template <bool BF16, bool VEC, int L, int TOK>
+// behind rot, a value.  BATCH heads of a group of lanes are on their way at once.
+template <bool BF16, bool VEC, int L, int TOK, int BATCH>
 __global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
-  constexpr int ES = BF16 ? 2 : 4, E = VEC ? 16 / ES : 1;
+  constexpr int ES = BF16 ? 2 : 4, E = VEC ? 16 / ES : 1, GROUPS = 256 / L;
+  using Raw = std::conditional_t<VEC, u32x4, float>;
   extern __shared__ float cs[];  // [TOK][rot / 2] cosines, then as many sines
   const RopeParams& r = p.r;
   const int half = r.rot / 2;
   const int64_t t0 = (int64_t)blockIdx.x * TOK;
+  const int tokens = (int)min((int64_t)TOK, r.T - t0);
   float* const sn = cs + TOK * half;
   const bool append = r.slots != nullptr, inside = VEC && r.interleaved;  // inside: both of a pair in one piece
-  const int heads = r.Hq + r.Hk * (append ? 2 : 1);
   const int turned = inside ? r.rot / E : half / E, units = turned + (r.D - r.rot) / E;
-  const int lane = threadIdx.x % L;
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
   // The places of unit u's values in the head.
   auto first = [&](int u) { return u >= turned ? r.rot + (u - turned) * E : !VEC && r.interleaved ? 2 * u : u * E; };
   auto second = [&](int u) { return !VEC && r.interleaved ? 2 * u + 1 : half + u * E; };
   auto paired = [&](int u) { return u < turned && !inside; };
-  float x[2 * E];
-  auto load = [&](const char* src, int u) {
-    take<BF16, VEC>(src, first(u), x);
-    if (paired(u)) take<BF16, VEC>(src, second(u), x + E);
-    else
+  auto raw = [&](const char* src, int at) -> Raw {
+    if constexpr (VEC) return *reinterpret_cast<const u32x4*>(src + at * ES);
+    else return ld1<BF16>(src, at);
+  };
+  auto values = [&](Raw v, float* x) {
+    if constexpr (VEC) unpack<BF16>(v, x);
+    else x[0] = v;
+  };
+  auto give = [&](char* dst, int at, const float* x) {
+    if constexpr (VEC) *reinterpret_cast<u32x4*>(dst + at * ES) = pack<BF16>(x);
+    else st1<BF16>(dst, at, x[0]);
+  };
+  // Unit u of a head: normalised, turned and stored.
+  auto finish = [&](int tt, char* dst, int u, Raw va, Raw vb, float rstd, const float* w) {
+    const int a = first(u), b = second(u);
+    float x[E], y[E];
+    values(va, x);
+    scaled<E>(x, rstd, w + a);
+    if (paired(u)) {
+      values(vb, y);
+      scaled<E>(y, rstd, w + b);
+      const float *c = cs + tt * half + u * E, *s = sn + tt * half + u * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[E + e] = 0.f;
-  };
-  auto squares = [&] {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 2 * E; ++e) ss += x[e] * x[e];
-    return ss;
-  };
-  auto source = [&](int64_t t, int hh) -> const char* {
-    if (hh < r.Hq) return static_cast<const char*>(r.q) + (t * r.q_t + hh * r.q_h) * ES;
-    const int h = hh - r.Hq;
-    return h < r.Hk ? static_cast<const char*>(r.k) + (t * r.k_t + h * r.k_h) * ES
-                    : static_cast<const char*>(r.v) + (t * r.v_t + (h - r.Hk) * r.v_h) * ES;
-  };
-  // The first head's values are on their way while the angles are computed.
-  int item = threadIdx.x / L;
-  bool loaded = false;
-  if (item < TOK * heads && t0 + item / heads < r.T && lane < units) {
-    load(source(t0 + item / heads, item % heads), lane);
-    loaded = true;
-  }
-  for (int i = threadIdx.x; i < TOK * half; i += 256) {
-    const int64_t t = t0 + i / half;
-    if (t < r.T) turn(r.pos[t], r.inv_freq[i % half], r.scale, &cs[i], &sn[i]);
-  }
-  __syncthreads();
-  for (; item < TOK * heads; item += 256 / L) {
-    const int tt = TOK == 1 ? 0 : item / heads, hh = item - tt * heads;
-    const int64_t t = t0 + tt;
-    if (t >= r.T) break;
-    const char* const src = source(t, hh);
-    const int h = hh < r.Hq ? hh : hh < r.Hq + r.Hk ? hh - r.Hq : hh - r.Hq - r.Hk;
-    const bool val = hh >= r.Hq + r.Hk;  // a value's head: copied
-    if (!loaded && lane < units) load(src, lane);
-    loaded = false;
-    float rstd = 1.f;
-    if (!val) {
-      float ss = lane < units ? squares() : 0.f;
-      for (int u = lane + L; u < units; u += L) {
-        load(src, u);
-        ss += squares();
+      for (int e = 0; e < E; ++e) {
+        const float f = x[e], g = y[e];
+        x[e] = f * c[e] - g * s[e];
+        y[e] = g * c[e] + f * s[e];
       }
+      give(dst, b, y);
+    } else if (VEC && u < turned) {
+      const float *c = cs + tt * half + u * (E / 2), *s = sn + tt * half + u * (E / 2);
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-      rstd = 1.0f / sqrtf(ss / (float)r.D + p.eps);
-      if (units > L && lane < units) load(src, lane);
+      for (int e = 0; e < E / 2; ++e) {
+        const float f = x[2 * e], g = x[2 * e + 1];
+        x[2 * e] = f * c[e] - g * s[e];
+        x[2 * e + 1] = g * c[e] + f * s[e];
+      }
     }
-    char* dst;
-    if (hh < r.Hq) {
-      dst = static_cast<char*>(r.qo) + (t * r.qo_t + h * r.qo_h) * ES;
-    } else if (append) {
-      const int64_t slot = r.slots[t];
-      if (slot < 0 || slot >= r.pages * r.page) continue;  // no row of the cache
-      const int64_t pg = slot / r.page, row = slot - pg * r.page;
-      dst = val ? static_cast<char*>(r.vo) + (pg * r.vo_p + row * r.vo_t + h * r.vo_h) * ES
-                : static_cast<char*>(r.ko) + (pg * r.ko_p + row * r.ko_t + h * r.ko_h) * ES;
-    } else {
-      dst = static_cast<char*>(r.ko) + (t * r.ko_t + h * r.ko_h) * ES;
-    }
-    const float* const w = hh < r.Hq ? p.q_w + (int64_t)h * p.qw_h : p.k_w + (int64_t)h * p.kw_h;
-    for (int u = lane; u < units; u += L) {
-      if (u != lane) load(src, u);  // (behind what this lane has written, and nobody else writes)
-      const int a = first(u), b = second(u);
-      if (!val) {
-        scaled<E>(x, rstd, w + a);
-        if (paired(u)) {
-          scaled<E>(x + E, rstd, w + b);
-          const float *c = cs + tt * half + u * E, *s = sn + tt * half + u * E;
+    give(dst, a, x);
+  };
+  // Heads of q or of k of the block's tokens, BATCH a group of lanes: their first
+  // units are loaded, then (before the first of them) the angles are awaited.
+  bool waited = false;
+  auto pass = [&](auto is_q, int heads) {
+    constexpr bool Q = decltype(is_q)::value;
+    for (int i0 = group; i0 < tokens * heads || !waited; i0 += GROUPS * BATCH) {
+      Raw va[BATCH], vb[BATCH];
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float f = x[e], g = x[E + e];
-            x[e] = f * c[e] - g * s[e];
-            x[E + e] = g * c[e] + f * s[e];
-          }
-        } else if (VEC && u < turned) {
-          const float *c = cs + tt * half + u * (E / 2), *s = sn + tt * half + u * (E / 2);
-#pragma unroll
-          for (int e = 0; e < E / 2; ++e) {
-            const float f = x[2 * e], g = x[2 * e + 1];
-            x[2 * e] = f * c[e] - g * s[e];
-            x[2 * e + 1] = g * c[e] + f * s[e];
-          }
+      for (int j = 0; j < BATCH; ++j) {
+        const int i = min(i0 + GROUPS * j, tokens * heads - 1), tt = TOK == 1 ? 0 : i / heads, h = i - tt * heads;
+        const char* const src = Q ? static_cast<const char*>(r.q) + ((t0 + tt) * r.q_t + h * r.q_h) * ES
+                                  : static_cast<const char*>(r.k) + ((t0 + tt) * r.k_t + h * r.k_h) * ES;
+        va[j] = vb[j] = Raw{};
+        if (lane < units) {
+          va[j] = raw(src, first(lane));
+          if (paired(lane)) vb[j] = raw(src, second(lane));
         }
       }
-      give<BF16, VEC>(dst, a, x);
-      if (paired(u)) give<BF16, VEC>(dst, b, x + E);
+      if (!waited) {
+        for (int i = threadIdx.x; i < tokens * half; i += 256) turn(r.pos[t0 + i / half], r.inv_freq[i % half], r.scale, &cs[i], &sn[i]);
+        __syncthreads();
+        waited = true;
+      }
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int i = i0 + GROUPS * j;
+        if (i >= tokens * heads) break;
+        const int tt = TOK == 1 ? 0 : i / heads, h = i - tt * heads;
+        const int64_t t = t0 + tt;
+        const char* const src = Q ? static_cast<const char*>(r.q) + (t * r.q_t + h * r.q_h) * ES : static_cast<const char*>(r.k) + (t * r.k_t + h * r.k_h) * ES;
+        float ss = 0.f, x[E];
+        auto add = [&](Raw v) {
+          values(v, x);
+#pragma unroll
+          for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+        };
+        add(va[j]);  // (zeros where there is no unit or partner)
+        add(vb[j]);
+        for (int u = lane + L; u < units; u += L) {
+          add(raw(src, first(u)));
+          if (paired(u)) add(raw(src, second(u)));
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+        const float rstd = 1.0f / sqrtf(ss / (float)r.D + p.eps);
+        char* dst;
+        if constexpr (Q) {
+          dst = static_cast<char*>(r.qo) + (t * r.qo_t + h * r.qo_h) * ES;
+        } else if (append) {
+          const int64_t slot = r.slots[t];
+          if (slot < 0 || slot >= r.pages * r.page) continue;  // no row of the cache
+          const int64_t pg = slot / r.page;
+          dst = static_cast<char*>(r.ko) + (pg * r.ko_p + (slot - pg * r.page) * r.ko_t + h * r.ko_h) * ES;
+        } else {
+          dst = static_cast<char*>(r.ko) + (t * r.ko_t + h * r.ko_h) * ES;
+        }
+        const float* const w = Q ? p.q_w + (int64_t)h * p.qw_h : p.k_w + (int64_t)h * p.kw_h;
+        if (lane < units) finish(tt, dst, lane, va[j], vb[j], rstd, w);
+        // (an output may be its input: a unit's values are read before they are written, by the same lane)
+        for (int u = lane + L; u < units; u += L) finish(tt, dst, u, raw(src, first(u)), paired(u) ? raw(src, second(u)) : Raw{}, rstd, w);
+      }
     }
+  };
+  pass(std::true_type{}, r.Hq);
+  pass(std::false_type{}, r.Hk);
+  if (!append) return;
+  // Values: copied.
+  const int pieces = r.D / E, all = tokens * r.Hk * pieces;
+  for (int i = threadIdx.x; i < all; i += 256) {
+    const int head = i / pieces, tt = head / r.Hk, h = head - tt * r.Hk, at = (i - head * pieces) * E;
+    const int64_t t = t0 + tt, slot = r.slots[t];
+    if (slot < 0 || slot >= r.pages * r.page) continue;
+    const int64_t pg = slot / r.page;
+    const char* const src = static_cast<const char*>(r.v) + (t * r.v_t + h * r.v_h) * ES;
+    char* const dst = static_cast<char*>(r.vo) + (pg * r.vo_p + (slot - pg * r.page) * r.vo_t + h * r.vo_h) * ES;
+    if constexpr (VEC) *reinterpret_cast<u32x4*>(dst + at * ES) = *reinterpret_cast<const u32x4*>(src + at * ES);
+    else if constexpr (BF16) reinterpret_cast<uint16_t*>(dst)[at] = reinterpret_cast<const uint16_t*>(src)[at];
+    else reinterpret_cast<uint32_t*>(dst)[at] = reinterpret_cast<const uint32_t*>(src)[at];
   }
 }
 
@@ -167,7 +182,7 @@ hipError_t run(const NormRopeParams& p, hipStream_t st) {
   const RopeParams& r = p.r;
   // (one token a block while those are few, as rope.hip)
   if (r.T < 4096) {
-    hipLaunchKernelGGL((head_norm_turn_kernel<BF16, VEC, L, 1>), dim3((unsigned)r.T), dim3(256), r.rot * 4, st, p);
+    hipLaunchKernelGGL((head_norm_turn_kernel<BF16, VEC, L, 1, 1>), dim3((unsigned)r.T), dim3(256), r.rot * 4, st, p);
     return hipGetLastError();
   }
   constexpr int64_t kTokens = 1 << 24;  // a launch
@@ -181,7 +196,7 @@ hipError_t run(const NormRopeParams& p, hipStream_t st) {
     c.qo = static_cast<char*>(r.qo) + t * r.qo_t * ES, c.pos = r.pos + t;
     if (r.slots) c.v = static_cast<const char*>(r.v) + t * r.v_t * ES, c.slots = r.slots + t;
     else c.ko = static_cast<char*>(r.ko) + t * r.ko_t * ES;
-    hipLaunchKernelGGL((head_norm_turn_kernel<BF16, VEC, L, 4>), dim3((unsigned)((c.T + 3) / 4)), dim3(256), 4 * r.rot * 4, st, n);
+    hipLaunchKernelGGL((head_norm_turn_kernel<BF16, VEC, L, 4, 4>), dim3((unsigned)((c.T + 3) / 4)), dim3(256), 4 * r.rot * 4, st, n);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -136,9 +136,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.svdmlp_norm_rope_append.restype = ctypes.c_int
     lib.svdmlp_norm_rope_append.argtypes = [_vp] * 12 + [_i64] * 7 + [f32, f32, _i32, _u32, _vp]
     lib.svdmlp_copy_pages.restype = ctypes.c_int
-    lib.svdmlp_copy_pages.argtypes = [_vp, _i64] + [_vp] * 4 + [_i64] * 5 + [_i32, _vp]
+    lib.svdmlp_copy_pages.argtypes = [_vp, _i64, _i64] + [_vp] * 4 + [_i64] * 5 + [_i32, _vp]
     lib.svdmlp_keep_drafts.restype = ctypes.c_int
-    lib.svdmlp_keep_drafts.argtypes = [_vp, _i64] + [_vp] * 5 + [_i64] * 9 + [_i32, _vp]
+    lib.svdmlp_keep_drafts.argtypes = [_vp, _i64, _i64] + [_vp] * 5 + [_i64] * 9 + [_i32, _vp]
     lib.svdmlp_chunk_attention_workspace_bytes.restype = _sz
     lib.svdmlp_chunk_attention_workspace_bytes.argtypes = [_i64] * 7 + [_i32]
     lib.svdmlp_chunk_attention.restype = ctypes.c_int

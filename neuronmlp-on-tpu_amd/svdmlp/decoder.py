@@ -392,7 +392,7 @@ def rope_append(q, k, v, positions, inv_freq, k_cache, v_cache, slots, *, interl
 
 def _head_gains(name, w, heads, D, index):
     """(gains in fp32, whether each head has its own)."""
-    if w.get_device() != index or not w.is_floating_point() or tuple(w.shape) not in ((D,), (heads, D)):
+    if w.get_device() != index or not w.is_floating_point() or w.shape not in ((D,), (heads, D)):
         raise ValueError(f"{name} must be a ({D},) or ({heads}, {D}) tensor on q.device")
     return w if w.dtype is torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous(), w.dim() == 2
 
@@ -453,8 +453,10 @@ def norm_rope_append(q, k, v, positions, inv_freq, q_weight, k_weight, k_cache, 
         _refuse_device(name, q, k_cache, v_cache)
     if _gradients():
         _refuse_grad(name, k_cache, v_cache, out)
-    _writable("k_cache", k_cache, cs, q)
-    _writable("v_cache", v_cache, cs, q)
+    if not k_cache.is_contiguous():
+        _writable("k_cache", k_cache, cs, q)
+    if not v_cache.is_contiguous():
+        _writable("v_cache", v_cache, cs, q)
     slots = _index("slots", slots, (T,), torch.int64, index)
     if out is not None:
         _writable("out", out, (T, Hq, D), q)
@@ -464,19 +466,25 @@ def norm_rope_append(q, k, v, positions, inv_freq, q_weight, k_weight, k_cache, 
     q, k, v = _last(q), _last(k), _last(v)
     # The caches apart from each other and from what is read: by their first and
     # last bytes, exactly where those meet.
-    kp, ke, vp, ve = *_bytes(k_cache), *_bytes(v_cache)
-    meet = kp < ve and vp < ke
-    for t in (q, k, v, positions, inv_freq, slots, qw, kw):
-        p, e = _bytes(t)
-        meet = meet or (p < ke and kp < e) or (p < ve and vp < e)
+    a, b, c, kc, vc = q.stride(), k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    qp, kp, vp, kcp, vcp = q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    pp, fp, sp, qwp, kwp = positions.data_ptr(), inv_freq.data_ptr(), slots.data_ptr(), qw.data_ptr(), kw.data_ptr()
+    es, n0, n1, n2 = 2 if q.dtype is _BF16 else 4, cs[0] - 1, cs[1] - 1, Hk - 1
+    kce, vce = kcp + es * (n0 * kc[0] + n1 * kc[1] + n2 * kc[2] + D), vcp + es * (n0 * vc[0] + n1 * vc[1] + n2 * vc[2] + D)
+    meet = kcp < vce and vcp < kce
+    for p, e in ((min(qp, kp, vp), max(qp + es * (a[0] * (T - 1) + a[1] * (Hq - 1) + D), kp + es * (b[0] * (T - 1) + b[1] * n2 + D),
+                                       vp + es * (c[0] * (T - 1) + c[1] * n2 + D))),
+                 (pp, pp + 8 * T), (sp, sp + 8 * T), (fp, fp + 4 * rot), (qwp, qwp + 4 * D * Hq), (kwp, kwp + 4 * D * Hk)):
+        if (p < kce and kcp < e) or (p < vce and vcp < e):
+            meet = True
     if meet:
         _apart("k_cache", k_cache, v_cache, q, k, v, positions, inv_freq, slots, qw, kw)
         _apart("v_cache", v_cache, q, k, v, positions, inv_freq, slots, qw, kw)
     if out is None:
         out = q.new_empty((T, Hq, D))
-    st = _Strides14(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3])
-    _launch(index, _lib.load().svdmlp_norm_rope_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
-            inv_freq.data_ptr(), qw.data_ptr(), kw.data_ptr(), slots.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+    o = out.stride()
+    st = _Strides14(a[0], a[1], b[0], b[1], c[0], c[1], o[0], o[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2])
+    _launch(index, _lib.load().svdmlp_norm_rope_append, qp, kp, vp, pp, fp, qwp, kwp, sp, out.data_ptr(), kcp, vcp,
             _address(st), T, cs[0], cs[1], Hq, Hk, D, rot, scale, eps, _ACT_CODES[q.dtype], flags)
     return out
 

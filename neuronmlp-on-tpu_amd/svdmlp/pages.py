@@ -24,17 +24,19 @@ from .decoder import (_Strides3, _address, _apart, _bytes, _extent, _gradients, 
 from .ops import _ACT_CODES
 
 
+_Pointer = ctypes.c_void_p * 1
+
+
 def _cache_set(name: str, caches):
-    """(first cache, addresses, n, device index, strides) of the caches, checked."""
+    """(shape of a cache, dtype code, all of them, addresses, n, elements apart, device index, strides) of the caches, checked."""
     if isinstance(caches, torch.Tensor):
-        if caches.dim() != 5 or not caches.numel():
-            raise ValueError(f"caches must have shape (caches, pages, page size, heads, head size), got {tuple(caches.shape)}")
-        one, every, n = caches[0], (caches,), caches.shape[0]
+        shape = caches.shape
+        if len(shape) != 5 or 0 in shape:
+            raise ValueError(f"caches must have shape (caches, pages, page size, heads, head size), got {tuple(shape)}")
         _check_cache(name, caches)
-        base, step = caches.data_ptr(), caches.stride(0) * caches.element_size()
-        if n == 1:
-            step = 0
-        pointers = range(base, base + n * step, step) if step else (base,)
+        st = caches.stride()
+        return (shape[1:], _ACT_CODES[caches.dtype], (caches,), _Pointer(caches.data_ptr()), shape[0], st[0] if shape[0] > 1 else 0,
+                caches.get_device(), _Strides3(st[1], st[2], st[3]))
     else:
         every = tuple(caches)
         if not every or not all(isinstance(c, torch.Tensor) for c in every):
@@ -58,8 +60,7 @@ def _cache_set(name: str, caches):
                         break
                     if _overlap(a, b):
                         raise ValueError("the caches must not overlap")
-    s = one.stride()
-    return one, every, (ctypes.c_void_p * n)(*pointers), n, one.get_device(), _Strides3(*s[:3])
+    return shape, _ACT_CODES[dtype], every, (ctypes.c_void_p * n)(*pointers), n, 0, index, _Strides3(*strides[:3])
 
 
 def _check_cache(name: str, c: torch.Tensor) -> None:
@@ -74,14 +75,12 @@ def _check_cache(name: str, c: torch.Tensor) -> None:
 
 def _indices_apart(every, *tensors) -> None:
     """No cache shares memory with the index tensors."""
-    for t in tensors:
-        if t is None or not t.numel():
-            continue
-        p, e = _bytes(t)
-        for c in every:
-            a, b = _bytes(c)
+    spans = [_bytes(t) for t in tensors if t is not None and t.numel()]
+    for c in every:
+        a, b = _bytes(c)
+        for p, e in spans:
             if p < b and a < e:
-                _apart("caches", c, t)
+                _apart("caches", c, *(t for t in tensors if t is not None))
 
 
 def copy_pages(caches, src, dst, rows=None) -> None:
@@ -90,7 +89,7 @@ def copy_pages(caches, src, dst, rows=None) -> None:
     device, one value a pair.  A pair with a page outside the cache, or of a page
     and itself, is skipped.  The pages of dst have to differ from each other and
     from those of src."""
-    one, every, pointers, n, index, strides = _cache_set("copy_pages", caches)
+    (pages, page, Hk, D), code, every, pointers, n, apart, index, strides = _cache_set("copy_pages", caches)
     if not isinstance(src, torch.Tensor) or src.dim() != 1:
         raise ValueError("src must hold the pages to copy")
     m = src.shape
@@ -99,9 +98,8 @@ def copy_pages(caches, src, dst, rows=None) -> None:
     if not m[0]:
         return
     _indices_apart(every, src, dst, rows)
-    pages, page, Hk, D = one.shape
-    _launch(index, _lib.load().svdmlp_copy_pages, _address(pointers), n, _address(strides), src.data_ptr(), dst.data_ptr(),
-            None if rows is None else rows.data_ptr(), m[0], pages, page, Hk, D, _ACT_CODES[one.dtype])
+    _launch(index, _lib.load().svdmlp_copy_pages, _address(pointers), n, apart, _address(strides), src.data_ptr(), dst.data_ptr(),
+            None if rows is None else rows.data_ptr(), m[0], pages, page, Hk, D, code)
 
 
 def keep_drafts(caches, block_table, lengths, path, drafts: int) -> torch.Tensor:
@@ -116,8 +114,7 @@ def keep_drafts(caches, block_table, lengths, path, drafts: int) -> torch.Tensor
     increase or is no draft.  A sequence of fewer tokens than ``drafts`` keeps
     them and its length.  block_table and lengths are those of
     cache_attention; rows in pages outside the cache are not moved."""
-    one, every, pointers, n, index, strides = _cache_set("keep_drafts", caches)
-    pages, page, Hk, D = one.shape
+    (pages, page, Hk, D), code, every, pointers, n, apart, index, strides = _cache_set("keep_drafts", caches)
     if isinstance(drafts, bool) or not isinstance(drafts, int) or not 1 <= drafts <= 64:
         raise ValueError(f"1 to 64 drafts a sequence, got {drafts}")
     if block_table.dim() != 2 or block_table.shape[1] == 0:
@@ -129,13 +126,13 @@ def keep_drafts(caches, block_table, lengths, path, drafts: int) -> torch.Tensor
     if block_table.stride(1) != 1 or block_table.dtype is not torch.int32 or block_table.get_device() != index:
         block_table = _index("block_table", block_table, (B, width), torch.int32, index)
     lengths = _index("lengths", lengths, (B,), torch.int32, index)
-    out = torch.empty(B, dtype=torch.int32, device=one.device)
+    out = lengths.new_empty(B)
     if not B:
         return out
     _indices_apart(every, block_table, lengths, path)
-    _launch(index, _lib.load().svdmlp_keep_drafts, _address(pointers), n, _address(strides), block_table.data_ptr(), lengths.data_ptr(),
+    _launch(index, _lib.load().svdmlp_keep_drafts, _address(pointers), n, apart, _address(strides), block_table.data_ptr(), lengths.data_ptr(),
             path.data_ptr(), out.data_ptr(), block_table.stride(0), B, width, path.shape[1], drafts, pages, page, Hk, D,
-            _ACT_CODES[one.dtype])
+            code)
     return out
 
 
@@ -148,9 +145,9 @@ class PagePool:
     refused call changes nothing."""
 
     def __init__(self, caches):
-        one, _, _, _, index, _ = _cache_set("PagePool", caches)
+        shape, _, _, _, _, _, index, _ = _cache_set("PagePool", caches)
         self.caches = caches if isinstance(caches, torch.Tensor) else tuple(caches)
-        self.pages, self.page = one.shape[:2]
+        self.pages, self.page = shape[:2]
         self.device = torch.device("cuda", index)
         self._holders = [0] * self.pages
         self._free = list(range(self.pages))  # a heap: the lowest page goes first

@@ -49,9 +49,10 @@ def _caches(n=2, hole=False):
     (dict(n=0), b"no caches"), (dict(caches=None), b"no caches"), (dict(caches=_caches(hole=True)), b"null"), (dict(src=None), b"null"),
     (dict(m=0), b"0 pages"), (dict(pages=0), b"positive"), (dict(page=0), b"positive"), (dict(D=0), b"positive"), (dict(dtype=2), b"dtype"),
     (dict(page=1 << 20, D=1 << 20), b"too large"), (dict(strides=(ctypes.c_int64 * 3)(64, -16, 16)), b"negative"), (dict(pages=1 << 31), b"too large"),
+    (dict(apart=-8), b"negative"),
 ])
 def test_copy_pages_refusals(lib, kw, msg):
-    a = dict(caches=_caches(), n=2, strides=None, src=P, dst=P, rows=None, m=3, pages=4, page=16, Hk=2, D=16, dtype=1) | kw
+    a = dict(caches=_caches(), n=2, apart=0, strides=None, src=P, dst=P, rows=None, m=3, pages=4, page=16, Hk=2, D=16, dtype=1) | kw
     assert lib.svdmlp_copy_pages(*a.values(), None) == BAD
     assert msg in lib.svdmlp_last_error()
 
@@ -62,7 +63,7 @@ def test_copy_pages_refusals(lib, kw, msg):
     (dict(m=5), b"as many"), (dict(m=0), b"as many"), (dict(table_stride=-1), b"negative"), (dict(Hk=0), b"positive"),
 ])
 def test_keep_drafts_refusals(lib, kw, msg):
-    a = dict(caches=_caches(), n=2, strides=None, table=P, lengths=P, path=P, out=P, table_stride=4, B=2, width=4, m=3, drafts=4, pages=4,
+    a = dict(caches=_caches(), n=2, apart=0, strides=None, table=P, lengths=P, path=P, out=P, table_stride=4, B=2, width=4, m=3, drafts=4, pages=4,
              page=16, Hk=2, D=16, dtype=1) | kw
     assert lib.svdmlp_keep_drafts(*a.values(), None) == BAD
     assert msg in lib.svdmlp_last_error()
