@@ -10,7 +10,10 @@
 // turn would read and write them twice.  L lanes hold a head between its sum of
 // squares and its turn, a 16-byte piece and its partner each, so that the sum is
 // a few exchanges of lanes and pairs never leave their lane.  A block takes a
-// token, four where those are many.
+// token: more of them a block, or heads on their way ahead of others, cost
+// registers and so waves (6007 tokens of 32 + 8 heads of 128 in bf16 24 us, 5.1
+// TB/s, a copy's rate; by four tokens a block 28, two 26).  16 tokens into a
+// cache: 5.4 us, latency.
 #include <algorithm>
 #include <type_traits>
 
@@ -38,17 +41,16 @@ __device__ __forceinline__ void scaled(float* x, float by, const float* w) {
 // VEC: D, rot, every stride and every base in whole 16-byte pieces (half layout:
 // rot / 2 too); a unit of a head is then a piece of its first half with its
 // partner (half layout) or a piece (interleaved, and behind rot), else a pair or,
-// behind rot, a value.  BATCH heads of a group of lanes are on their way at once.
-template <bool BF16, bool VEC, int L, int TOK, int BATCH>
+// behind rot, a value.
+template <bool BF16, bool VEC, int L>
 __global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
   constexpr int ES = BF16 ? 2 : 4, E = VEC ? 16 / ES : 1, GROUPS = 256 / L;
   using Raw = std::conditional_t<VEC, u32x4, float>;
-  extern __shared__ float cs[];  // [TOK][rot / 2] cosines, then as many sines
+  extern __shared__ float cs[];  // rot / 2 cosines, then as many sines
   const RopeParams& r = p.r;
   const int half = r.rot / 2;
-  const int64_t t0 = (int64_t)blockIdx.x * TOK;
-  const int tokens = (int)min((int64_t)TOK, r.T - t0);
-  float* const sn = cs + TOK * half;
+  const int64_t t = blockIdx.x;
+  float* const sn = cs + half;
   const bool append = r.slots != nullptr, inside = VEC && r.interleaved;  // inside: both of a pair in one piece
   const int turned = inside ? r.rot / E : half / E, units = turned + (r.D - r.rot) / E;
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
@@ -69,7 +71,7 @@ __global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
     else st1<BF16>(dst, at, x[0]);
   };
   // Unit u of a head: normalised, turned and stored.
-  auto finish = [&](int tt, char* dst, int u, Raw va, Raw vb, float rstd, const float* w) {
+  auto finish = [&](char* dst, int u, Raw va, Raw vb, float rstd, const float* w) {
     const int a = first(u), b = second(u);
     float x[E], y[E];
     values(va, x);
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
     if (paired(u)) {
       values(vb, y);
       scaled<E>(y, rstd, w + b);
-      const float *c = cs + tt * half + u * E, *s = sn + tt * half + u * E;
+      const float *c = cs + u * E, *s = sn + u * E;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float f = x[e], g = y[e];
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
       }
       give(dst, b, y);
     } else if (VEC && u < turned) {
-      const float *c = cs + tt * half + u * (E / 2), *s = sn + tt * half + u * (E / 2);
+      const float *c = cs + u * (E / 2), *s = sn + u * (E / 2);
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) {
         const float f = x[2 * e], g = x[2 * e + 1];
@@ -96,81 +98,61 @@ __global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
     }
     give(dst, a, x);
   };
-  // Heads of q or of k of the block's tokens, BATCH a group of lanes: their first
-  // units are loaded, then (before the first of them) the angles are awaited.
+  const int64_t slot = append ? r.slots[t] : 0;
+  const bool stored = slot >= 0 && (!append || slot < r.pages * r.page);  // (else no row of the cache)
+  const int64_t pg = append && stored ? slot / r.page : 0, row = slot - pg * r.page;
+  // Heads of q or of k, one a group of lanes; the first of them is loaded before
+  // the angles are computed.
   bool waited = false;
   auto pass = [&](auto is_q, int heads) {
     constexpr bool Q = decltype(is_q)::value;
-    for (int i0 = group; i0 < tokens * heads || !waited; i0 += GROUPS * BATCH) {
-      Raw va[BATCH], vb[BATCH];
-#pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        const int i = min(i0 + GROUPS * j, tokens * heads - 1), tt = TOK == 1 ? 0 : i / heads, h = i - tt * heads;
-        const char* const src = Q ? static_cast<const char*>(r.q) + ((t0 + tt) * r.q_t + h * r.q_h) * ES
-                                  : static_cast<const char*>(r.k) + ((t0 + tt) * r.k_t + h * r.k_h) * ES;
-        va[j] = vb[j] = Raw{};
-        if (lane < units) {
-          va[j] = raw(src, first(lane));
-          if (paired(lane)) vb[j] = raw(src, second(lane));
-        }
+    for (int h = group; h < heads || !waited; h += GROUPS) {
+      const char* const src = Q ? static_cast<const char*>(r.q) + (t * r.q_t + min(h, heads - 1) * r.q_h) * ES
+                                : static_cast<const char*>(r.k) + (t * r.k_t + h * r.k_h) * ES;
+      Raw va{}, vb{};
+      if (lane < units) {
+        va = raw(src, first(lane));
+        if (paired(lane)) vb = raw(src, second(lane));
       }
       if (!waited) {
-        for (int i = threadIdx.x; i < tokens * half; i += 256) turn(r.pos[t0 + i / half], r.inv_freq[i % half], r.scale, &cs[i], &sn[i]);
+        for (int i = threadIdx.x; i < half; i += 256) turn(r.pos[t], r.inv_freq[i], r.scale, &cs[i], &sn[i]);
         __syncthreads();
         waited = true;
+        if (h >= heads) break;
+      }
+      float ss = 0.f, x[E];
+      auto add = [&](Raw v) {
+        values(v, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+      };
+      add(va);  // (zeros where there is no unit or partner)
+      add(vb);
+      for (int u = lane + L; u < units; u += L) {
+        add(raw(src, first(u)));
+        if (paired(u)) add(raw(src, second(u)));
       }
 #pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        const int i = i0 + GROUPS * j;
-        if (i >= tokens * heads) break;
-        const int tt = TOK == 1 ? 0 : i / heads, h = i - tt * heads;
-        const int64_t t = t0 + tt;
-        const char* const src = Q ? static_cast<const char*>(r.q) + (t * r.q_t + h * r.q_h) * ES : static_cast<const char*>(r.k) + (t * r.k_t + h * r.k_h) * ES;
-        float ss = 0.f, x[E];
-        auto add = [&](Raw v) {
-          values(v, x);
-#pragma unroll
-          for (int e = 0; e < E; ++e) ss += x[e] * x[e];
-        };
-        add(va[j]);  // (zeros where there is no unit or partner)
-        add(vb[j]);
-        for (int u = lane + L; u < units; u += L) {
-          add(raw(src, first(u)));
-          if (paired(u)) add(raw(src, second(u)));
-        }
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-        const float rstd = 1.0f / sqrtf(ss / (float)r.D + p.eps);
-        char* dst;
-        if constexpr (Q) {
-          dst = static_cast<char*>(r.qo) + (t * r.qo_t + h * r.qo_h) * ES;
-        } else if (append) {
-          const int64_t slot = r.slots[t];
-          if (slot < 0 || slot >= r.pages * r.page) continue;  // no row of the cache
-          const int64_t pg = slot / r.page;
-          dst = static_cast<char*>(r.ko) + (pg * r.ko_p + (slot - pg * r.page) * r.ko_t + h * r.ko_h) * ES;
-        } else {
-          dst = static_cast<char*>(r.ko) + (t * r.ko_t + h * r.ko_h) * ES;
-        }
-        const float* const w = Q ? p.q_w + (int64_t)h * p.qw_h : p.k_w + (int64_t)h * p.kw_h;
-        if (lane < units) finish(tt, dst, lane, va[j], vb[j], rstd, w);
-        // (an output may be its input: a unit's values are read before they are written, by the same lane)
-        for (int u = lane + L; u < units; u += L) finish(tt, dst, u, raw(src, first(u)), paired(u) ? raw(src, second(u)) : Raw{}, rstd, w);
-      }
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+      const float rstd = 1.0f / sqrtf(ss / (float)r.D + p.eps);
+      if (!Q && !stored) continue;
+      char* const dst = Q ? static_cast<char*>(r.qo) + (t * r.qo_t + h * r.qo_h) * ES
+                          : static_cast<char*>(r.ko) + (append ? pg * r.ko_p + row * r.ko_t + h * r.ko_h : t * r.ko_t + h * r.ko_h) * ES;
+      const float* const w = Q ? p.q_w + (int64_t)h * p.qw_h : p.k_w + (int64_t)h * p.kw_h;
+      if (lane < units) finish(dst, lane, va, vb, rstd, w);
+      // (an output may be its input: a unit's values are read before they are written, by the same lane)
+      for (int u = lane + L; u < units; u += L) finish(dst, u, raw(src, first(u)), paired(u) ? raw(src, second(u)) : Raw{}, rstd, w);
     }
   };
   pass(std::true_type{}, r.Hq);
   pass(std::false_type{}, r.Hk);
-  if (!append) return;
+  if (!append || !stored) return;
   // Values: copied.
-  const int pieces = r.D / E, all = tokens * r.Hk * pieces;
-  for (int i = threadIdx.x; i < all; i += 256) {
-    const int head = i / pieces, tt = head / r.Hk, h = head - tt * r.Hk, at = (i - head * pieces) * E;
-    const int64_t t = t0 + tt, slot = r.slots[t];
-    if (slot < 0 || slot >= r.pages * r.page) continue;
-    const int64_t pg = slot / r.page;
+  const int pieces = r.D / E;
+  for (int i = threadIdx.x; i < r.Hk * pieces; i += 256) {
+    const int h = i / pieces, at = (i - h * pieces) * E;
     const char* const src = static_cast<const char*>(r.v) + (t * r.v_t + h * r.v_h) * ES;
-    char* const dst = static_cast<char*>(r.vo) + (pg * r.vo_p + (slot - pg * r.page) * r.vo_t + h * r.vo_h) * ES;
+    char* const dst = static_cast<char*>(r.vo) + (pg * r.vo_p + row * r.vo_t + h * r.vo_h) * ES;
     if constexpr (VEC) *reinterpret_cast<u32x4*>(dst + at * ES) = *reinterpret_cast<const u32x4*>(src + at * ES);
     else if constexpr (BF16) reinterpret_cast<uint16_t*>(dst)[at] = reinterpret_cast<const uint16_t*>(src)[at];
     else reinterpret_cast<uint32_t*>(dst)[at] = reinterpret_cast<const uint32_t*>(src)[at];
@@ -179,15 +161,10 @@ __global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
 
 template <bool BF16, bool VEC, int L>
 hipError_t run(const NormRopeParams& p, hipStream_t st) {
-  const RopeParams& r = p.r;
-  // (one token a block while those are few, as rope.hip)
-  if (r.T < 4096) {
-    hipLaunchKernelGGL((head_norm_turn_kernel<BF16, VEC, L, 1, 1>), dim3((unsigned)r.T), dim3(256), r.rot * 4, st, p);
-    return hipGetLastError();
-  }
-  constexpr int64_t kTokens = 1 << 24;  // a launch
-  static_assert(kTokens / 4 * 256 < (int64_t)1 << 32, "threads of a launch");
+  constexpr int64_t kTokens = 1 << 23;  // a launch
+  static_assert(kTokens * 256 < (int64_t)1 << 32, "threads of a launch");
   constexpr int ES = BF16 ? 2 : 4;
+  const RopeParams& r = p.r;
   for (int64_t t = 0; t < r.T; t += kTokens) {
     NormRopeParams n = p;
     RopeParams& c = n.r;
@@ -196,7 +173,7 @@ hipError_t run(const NormRopeParams& p, hipStream_t st) {
     c.qo = static_cast<char*>(r.qo) + t * r.qo_t * ES, c.pos = r.pos + t;
     if (r.slots) c.v = static_cast<const char*>(r.v) + t * r.v_t * ES, c.slots = r.slots + t;
     else c.ko = static_cast<char*>(r.ko) + t * r.ko_t * ES;
-    hipLaunchKernelGGL((head_norm_turn_kernel<BF16, VEC, L, 4, 4>), dim3((unsigned)((c.T + 3) / 4)), dim3(256), 4 * r.rot * 4, st, n);
+    hipLaunchKernelGGL((head_norm_turn_kernel<BF16, VEC, L>), dim3((unsigned)c.T), dim3(256), r.rot * 4, st, n);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;
