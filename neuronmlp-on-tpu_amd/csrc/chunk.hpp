@@ -119,17 +119,27 @@ class Line {
         const int i = __builtin_ctzll(hit);
         const int before = __builtin_amdgcn_readlane(s.before, i), tiles = __builtin_amdgcn_readlane(s.tiles, i);
         const int a = __builtin_amdgcn_readlane(s.a, i), z0 = max(from_ - before, 0), base = upto(a, tiles, z0);
-        const int rest = at - __builtin_amdgcn_readlane(begin, i);
+        int rest = at - __builtin_amdgcn_readlane(begin, i);
+        // MANY: tile by tile, each for all heads; else head by head, each with all its
+        // tiles, whose keys then stay in an XCD's L2.
+        const int each = MANY ? p_.Hk : 1;
+        if constexpr (!MANY) {
+          const int mine = __builtin_amdgcn_readlane(s.mine, i);
+          w.hk = rest / mine;
+          rest -= w.hk * mine;
+        }
         int lo = z0, hi = tiles - 1;  // the last tile (in order) that begins at or before `rest`
         while (lo < hi) {
           const int mid = (lo + hi + 1) / 2;
-          if ((upto(a, tiles, mid) - base) * p_.Hk <= rest) lo = mid;
+          if ((upto(a, tiles, mid) - base) * each <= rest) lo = mid;
           else hi = mid - 1;
         }
         take(s, b0, i, before + lo, w);
-        const int in = rest - (upto(a, tiles, lo) - base) * p_.Hk;
-        w.hk = in / w.units;
-        w.u = in - w.hk * w.units;
+        w.u = rest - (upto(a, tiles, lo) - base) * each;
+        if constexpr (MANY) {
+          w.hk = w.u / w.units;
+          w.u -= w.hk * w.units;
+        }
         return true;
       }
     }

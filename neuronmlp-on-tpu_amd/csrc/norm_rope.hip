@@ -12,8 +12,9 @@
 // a few exchanges of lanes and pairs never leave their lane.  A block takes a
 // token: more of them a block, or heads on their way ahead of others, cost
 // registers and so waves (6007 tokens of 32 + 8 heads of 128 in bf16 24 us, 5.1
-// TB/s, a copy's rate; by four tokens a block 28, two 26).  16 tokens into a
-// cache: 5.4 us, latency.
+// TB/s, a copy's rate; by four tokens a block 28, two 26).  Seven waves a SIMD: 72
+// registers, without the bound 96 and 25 us, by eight (24 bytes spilled) 32.  16 tokens into
+// a cache: 5.2 us, latency.
 #include <algorithm>
 #include <type_traits>
 
@@ -43,7 +44,7 @@ __device__ __forceinline__ void scaled(float* x, float by, const float* w) {
 // partner (half layout) or a piece (interleaved, and behind rot), else a pair or,
 // behind rot, a value.
 template <bool BF16, bool VEC, int L>
-__global__ __launch_bounds__(256) void head_norm_turn_kernel(NormRopeParams p) {
+__global__ __launch_bounds__(256, 7) void head_norm_turn_kernel(NormRopeParams p) {
   constexpr int ES = BF16 ? 2 : 4, E = VEC ? 16 / ES : 1, GROUPS = 256 / L;
   using Raw = std::conditional_t<VEC, u32x4, float>;
   extern __shared__ float cs[];  // rot / 2 cosines, then as many sines
