@@ -4,17 +4,18 @@
 // one new token (it generates) or thousands (a chunk of its prompt), all in one
 // call.
 //
-// A row is a new token and one of the heads that share a key/value head.  Two
+// A row is a new token and one of the heads that share a key/value head.  Three
 // kernels share a call's sequences by their rows a key/value head, which only the
-// device knows: chunk_pipe_kernel takes tiles of 256 rows (bf16, heads up to 128,
-// sequences of over kFewRows rows), chunk_wave_kernel of 32.
+// device knows: chunk_wave_kernel takes tiles of 32 rows (chunk_wave.hip), those of
+// sequences that generate; chunk_share_kernel of 128 (chunk_share.hip);
+// chunk_pipe_kernel of 256 (bf16, heads up to 128).
 //
 // The work of a class of sequences is a line: for every row tile and key/value head
 // as many units as the tile has keys, about.  It is cut into equal parts, one a
 // block, whatever the lengths are: a block takes the end of a tile, some whole
 // ones, the start of another.  chunk_join_kernel adds the sums of the tiles that
-// lie in several parts, of which there are fewer than blocks.  Where tiles of 256
-// rows are many, the first ones are blocks of their own, the longest first, and
+// lie in several parts, of which there are fewer than blocks.  Where tiles of 128
+// or 256 rows are many, the first ones are blocks of their own, the longest first, and
 // only the last one or two a CU are such a line: blocks that start together on
 // tiles of one head read the same keys at the same time, from one XCD's L2.
 #include "chunk.hpp"
@@ -325,10 +326,11 @@ __device__ __forceinline__ void join(const ChunkParams& p, const ChunkClass& k, 
   }
 }
 template <bool BF16>
-__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkParams p, ChunkClass many, ChunkClass few) {
-  const int id = blockIdx.x;
-  if (id < many.joins) join<BF16>(p, many, id);
-  else join<BF16>(p, few, id - many.joins);
+__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkParams p, ChunkPlan plan) {
+  const int id = blockIdx.x, some = id - plan.many.joins, few = some - plan.some.joins;
+  if (some < 0) join<BF16>(p, plan.many, id);
+  else if (few < 0) join<BF16>(p, plan.some, some);
+  else join<BF16>(p, plan.few, few);
 }
 
 template <int DP>
@@ -339,7 +341,7 @@ void run_pipe(const ChunkParams& p, const ChunkClass& k, hipStream_t st) {
 }
 
 // Waves of a block of 32-row tiles: as many as have stages in half of a CU's LDS.
-int wave_block(int64_t D, bool bf16) { return D * (bf16 ? 2 : 4) <= 256 ? 4 : D * (bf16 ? 2 : 4) <= 512 ? 2 : 1; }
+int wave_block(int64_t D, bool bf16) { return D * (bf16 ? 2 : 4) <= 256 ? 4 : 2; }
 
 }  // namespace
 
@@ -367,7 +369,9 @@ ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int
     k.fits = units() < (double)(1 << 30) && tiles * Hk < (int64_t)1 << 23;
     k.least = (int)std::max<int64_t>(least >> log, 1);
     k.blocks = (int)std::max<int64_t>(std::min<int64_t>(blocks, (int64_t)std::min(units() / (double)k.least, 1e9) + 1), 1);
-    k.grid = k.blocks + (tile_log == 8 ? (int)std::min<int64_t>(tiles * Hk, 1 << 23) : 0);
+    // (blocks without work cost their share too: the tiles that have blocks of their own
+    // are whole rounds, one less than all)
+    k.grid = k.blocks + (tile_log > 5 ? (int)std::max<int64_t>(std::min<int64_t>(tiles * Hk, 1 << 23) / k.blocks - 1, 0) * k.blocks : 0);
     if (k.blocks == 1) return;
     k.joins = (k.blocks - 1) * (int)(tile / 32);  // (no tile begins in the last block and goes on)
     k.notes_at = plan.floats;
@@ -375,26 +379,42 @@ ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int
     plan.floats = k.part_at + (int64_t)k.blocks * 2 * tile * (D + 2);
   };
   const int wave = 32 * wave_block(D, bf16);
-  // Blocks of 32-row tiles that a CU holds at once.
-  const int64_t held = !bf16 ? (D <= 128 ? 2 : 1) : D <= 64 ? 3 : D <= 128 ? 2 : 1;
-  // A call of up to one tile of 256 rows has no use for them; of one sequence of
-  // more rows for nothing else.  A start and an end of a tile take as long as 384 and
-  // 256 keys of it.
-  int64_t few = bf16 && D <= 128 && alike && page % (D <= 64 ? PipeCfg<64>::RPL : PipeCfg<128>::RPL) == 0 && rows > 256 ? kFewRows : rows;
-  if (few < rows && B == 1) few = 0;
-  fill(plan.many, few + 1, rows, 8, 64, cus, 512, 384);
-  fill(plan.few, 1, few, 5, wave, held * cus, 512, 256);
+  const bool pipe = bf16 && D <= 128 && alike && page % (D <= 64 ? PipeCfg<64>::RPL : PipeCfg<128>::RPL) == 0;
+  // The largest sequences of each class, in rows a key/value head (of 3000 keys each,
+  // 32 over 8 heads of 128 unless said; us by tiles of 32, 128 and 256 rows).  Tiles
+  // of 32 rows read the keys again for each, from L2 as long as a head's tiles run
+  // together, which they do while all fit the card: 16 bf16 sequences of 64 rows 63,
+  // 82, 92; 64 of 48 rows and 2000 keys 201, 160, 215; of 256 rows and 1000 keys 313,
+  // 190, 182.  One sequence gains most from them: 120 rows of 4000 keys 27, 35, 37,
+  // 512 rows 35, 47, 38.  fp32 is bound by its products: 8 of 128 rows 135, 168; 48
+  // of 128 rows 835, 873, of 512 rows 3403, 2964.  Heads of 256 in bf16, 16 over 2:
+  // 8 sequences of 64 rows 36, 43; 64 of 128 rows 194, 164; in fp32, where a CU
+  // holds a single wave that shares nothing, one sequence of 8 rows 221, 115.
+  // A class takes some 5 us where it has nothing to do: small calls have one, and most
+  // two, where most sequences must be of few rows.
+  const bool full = B * Hk > cus && rows > 32 * B;
+  int64_t few = bf16 ? (D <= 128 && full ? 32 : 64) : D <= 128 ? rows : 0, some = !pipe ? rows : full ? 128 : few;
+  if (bf16 && rows <= 256) few = rows;
+  else if (bf16 && B == 1) few = 0, some = pipe ? 0 : rows;  // (whose rows are the call's)
+  few = std::min(few, rows), some = std::max(few, std::min(some, rows));
+  // Blocks that a CU holds at once, and the keys that a tile's start and end take
+  // as long as.
+  fill(plan.many, some + 1, rows, 8, 64, cus, 512, 384);
+  fill(plan.some, few + 1, some, 7, 32, cus * (D <= 128 ? 2 : 1), 256, 256);
+  fill(plan.few, 1, few, 5, wave, cus * (!bf16 ? 2 : D <= 64 ? 3 : D <= 128 ? 2 : 1), 512, 256);
   return plan;
 }
 
 hipError_t launch_chunk_attention(const ChunkParams& p, bool bf16, const ChunkPlan& plan, hipStream_t st) {
   if (p.T <= 0 || p.B <= 0) return hipSuccess;
-  if ((plan.many.blocks && !plan.many.fits) || (plan.few.blocks && !plan.few.fits)) return hipErrorInvalidValue;
+  for (const ChunkClass* k : {&plan.many, &plan.some, &plan.few})
+    if (k->blocks && !k->fits) return hipErrorInvalidValue;
   if (plan.many.blocks) p.D <= 64 ? run_pipe<64>(p, plan.many, st) : run_pipe<128>(p, plan.many, st);
+  if (plan.some.blocks) launch_chunk_shared(p, plan.some, bf16, st);
   if (plan.few.blocks) launch_chunk_waves(p, plan.few, bf16, st);
-  if (const int joins = plan.many.joins + plan.few.joins) {
-    if (bf16) hipLaunchKernelGGL((chunk_join_kernel<true>), dim3((unsigned)joins), dim3(256), 0, st, p, plan.many, plan.few);
-    else hipLaunchKernelGGL((chunk_join_kernel<false>), dim3((unsigned)joins), dim3(256), 0, st, p, plan.many, plan.few);
+  if (const int joins = plan.many.joins + plan.some.joins + plan.few.joins) {
+    if (bf16) hipLaunchKernelGGL((chunk_join_kernel<true>), dim3((unsigned)joins), dim3(256), 0, st, p, plan);
+    else hipLaunchKernelGGL((chunk_join_kernel<false>), dim3((unsigned)joins), dim3(256), 0, st, p, plan);
   }
   return hipGetLastError();
 }

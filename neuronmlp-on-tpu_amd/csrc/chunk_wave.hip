@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void chunk_wave_kernel(ChunkParams p
     // do not, and the others get them at the end.
     auto unit = [&](auto masked_) {
       constexpr bool masked = decltype(masked_)::value;
-      constexpr int kAhead = RB < 1024 ? 4 : 2, VF = BF16 ? 2 * DB : 16 * DB;  // VF: pieces of V
+      constexpr int kAhead = 4, VF = BF16 ? 2 * DB : 16 * DB;  // VF: pieces of V
       u32x4 kf[kAhead], vf[kAhead], qa[kAhead];
       auto read_query = [&](int t) { return *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>((attn_lds)qlds + (t * 64 + lane) * 16); };
       auto read_value = [&](int f) {
@@ -249,8 +249,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void chunk_wave_kernel(ChunkParams p
     };
     // Whole tiles that every row sees, up to the first that is not; then the others,
     // masked.  (Two loops: a branch in one kept the registers of both.)
-    if constexpr (RB < 1024)  // (else two copies of a tile's code do not fit the registers)
-      while (ku + 31 < min(shared, kend) && seen == 0xffffffffu) unit(std::false_type{});
+    while (ku + 31 < min(shared, kend) && seen == 0xffffffffu) unit(std::false_type{});
     const int masked_from = ku;
     while (ku < kend) unit(std::true_type{});
 
@@ -340,7 +339,7 @@ void run(const ChunkParams& p, const ChunkClass& k, hipStream_t st) {
 
 void launch_chunk_waves(const ChunkParams& p, const ChunkClass& k, bool bf16, hipStream_t st) {
   if (bf16) p.D <= 64 ? run<true, 64, 4>(p, k, st) : p.D <= 128 ? run<true, 128, 4>(p, k, st) : run<true, 256, 2>(p, k, st);
-  else p.D <= 64 ? run<false, 64, 4>(p, k, st) : p.D <= 128 ? run<false, 128, 2>(p, k, st) : run<false, 256, 1>(p, k, st);
+  else p.D <= 64 ? run<false, 64, 4>(p, k, st) : run<false, 128, 2>(p, k, st);  // (heads of over 128: chunk_share_kernel)
 }
 
 }  // namespace svdmlp

@@ -139,15 +139,15 @@ struct ChunkParams {
   int alike;  // keys and values have the same page and token strides, and those and a page are below 2^32 bytes
   float c;    // softmax scale * log2(e)
 };
-constexpr int kFewRows = 128;
 constexpr int64_t kChunkTokensMost = 0x7ffe0000;  // of a sequence: room for the last tiles' ends
 struct ChunkPlan {
-  ChunkClass many, few;
-  int64_t floats;  // of the workspace
+  ChunkClass many, some, few;  // tiles of 256, 128 and 32 rows
+  int64_t floats;              // of the workspace
 };
 // alike: ChunkParams::alike; a workspace for calls of either kind takes the larger plan.
 ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, bool bf16, bool alike, int64_t page, int64_t capacity, int64_t cus);
-void launch_chunk_waves(const ChunkParams& p, const ChunkClass& k, bool bf16, hipStream_t st);  // tiles of 32 rows
+void launch_chunk_waves(const ChunkParams& p, const ChunkClass& k, bool bf16, hipStream_t st);
+void launch_chunk_shared(const ChunkParams& p, const ChunkClass& k, bool bf16, hipStream_t st);
 hipError_t launch_chunk_attention(const ChunkParams& p, bool bf16, const ChunkPlan& plan, hipStream_t st);
 
 // The caches (pages, page, Hk, D) of a model's layers, all laid out alike: as many

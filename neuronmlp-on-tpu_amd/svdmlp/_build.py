@@ -53,7 +53,7 @@ HIPCC_FLAGS = [
 # Flags of single translation units.  Attention: results of MFMAs in vector
 # registers where they fit (by itself the compiler puts them all into
 # accumulation registers, from which the softmax would copy every score).
-UNIT_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("prompt_attention", "cache_attention", "chunk_attention", "chunk_wave")}
+UNIT_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("prompt_attention", "cache_attention", "chunk_attention", "chunk_wave", "chunk_share")}
 
 
 def _hipcc() -> str:

@@ -90,7 +90,8 @@ def test_chunk_attention_long_contexts(gpu, dtype, lens, news, H, K, D, page):
 
 
 @pytest.mark.parametrize("dtype,B,most,longest,H,K,D,page", [
-    (BF, 200, 900, 3, 8, 2, 128, 16), (BF, 70, 2500, 60, 8, 2, 64, 16), (F32, 130, 300, 9, 4, 2, 64, 32), (BF, 66, 700, 5, 4, 4, 256, 16), (BF, 90, 400, 200, 4, 1, 128, 16)])
+    (BF, 200, 900, 3, 8, 2, 128, 16), (BF, 70, 2500, 60, 8, 2, 64, 16), (F32, 130, 300, 9, 4, 2, 64, 32), (BF, 66, 700, 5, 4, 4, 256, 16), (BF, 90, 400, 200, 4, 1, 128, 16),
+    (BF, 140, 700, 45, 8, 2, 128, 16), (BF, 260, 500, 90, 3, 1, 64, 16), (BF, 130, 300, 50, 6, 2, 80, 8), (BF, 40, 700, 150, 4, 2, 128, 5)])
 def test_chunk_attention_many_sequences(gpu, dtype, B, most, longest, H, K, D, page):
     """More sequences than a wave looks at at once, most with a token or none, some with chunks."""
     g = _gen(B + most)
