@@ -18,6 +18,9 @@ X ~ 0.02 N(0, 1)).  The arms differ only in how the SVD MLP runs:
   rotary positions, all but the projections in the library's kernels
   (:mod:`svdmlp.decoder`): a prompt of S tokens that fills a paged cache, and
   one more token onto it.
+* ``served_step`` (``--serve-arm``, not in the reference's report): a step of the
+  same layers for several sequences (:class:`SequenceModel`), the first prompts read
+  in chunks: each generates a token onto S, and one reads a chunk of its prompt.
 
 Attention is the same in the other arms and is not the subject of the comparison:
 torch's scaled_dot_product_attention, restricted to its flash and
@@ -40,6 +43,8 @@ import sys
 _SHAPES = {
     "llama3-3b": dict(hidden=3072, intermediate=8192, heads=24, kv_heads=8, layers=28),
     "llama3-8b": dict(hidden=4096, intermediate=14336, heads=32, kv_heads=8, layers=32),
+    # queries and keys normalised head by head (by the decoder and the server only)
+    "qwen3-8b": dict(hidden=4096, intermediate=12288, heads=32, kv_heads=8, layers=36, head_norms=True),
 }
 _DEFAULT_COMPRESS_RATIO = 0.8
 RMS_EPS = 1e-6
@@ -117,6 +122,8 @@ def load_checkpoint_weights(model_path, layer_indices, device, dtype):
     missing = [k for k in keys if k not in weight_map]
     if missing:
         raise KeyError(f"checkpoint missing key: {missing[0]}")
+    norms = ("self_attn.q_norm.weight", "self_attn.k_norm.weight")  # of models that have them
+    keys += [k for layer in layer_indices for k in (f"model.layers.{layer}.{n}" for n in norms) if k in weight_map]
     raw = {}
     with ExitStack() as stack:
         shards = {name: stack.enter_context(safe_open(str(model_path / name), framework="pt"))
@@ -132,6 +139,8 @@ def load_checkpoint_weights(model_path, layer_indices, device, dtype):
                         wq=raw[p + "self_attn.q_proj.weight"], wk=raw[p + "self_attn.k_proj.weight"],
                         wv=raw[p + "self_attn.v_proj.weight"], wo=raw[p + "self_attn.o_proj.weight"],
                         ug=ug, vg=vg, uu=uu, vu=vu, ud=ud, vd=vd))
+        if p + norms[0] in raw and p + norms[1] in raw:
+            out[-1].update(q_norm_w=raw[p + norms[0]], k_norm_w=raw[p + norms[1]])
     return out
 
 
@@ -163,18 +172,16 @@ def dense_block(x, w, dense, num_heads: int, num_kv_heads: int):
     return x + compat.nki_baseline(rmsnorm(x, w["norm2_w"]), *dense)
 
 
-class DecoderModel:
+class _Layers:
     """The layers of ``weights`` as a served model runs them, on the library's
-    kernels: q, k, v from one product, rotary positions, a paged cache a layer,
-    causal attention, the SVD MLP, and each residual sum with the norm after it.
-
-    ``prompt(x)`` runs one sequence and fills the caches; ``step(x, position)``
-    runs one token at ``position``, whose keys and values go into the caches, onto
-    what they hold before it.  ``capacity``: tokens the caches can hold."""
+    kernels: q, k, v from one product, rotary positions (of heads that are normalised
+    first where the weights have ``q_norm_w`` and ``k_norm_w``), a paged cache a
+    layer, causal attention, the SVD MLP, and each residual sum with the norm after
+    it.  ``caches[i]`` (2, pages, PAGE, kv heads, head size): layer i's keys and values."""
 
     PAGE = 64
 
-    def __init__(self, weights, num_heads: int, num_kv_heads: int, capacity: int, theta: float = 500000.0, workspace=None):
+    def __init__(self, weights, num_heads: int, num_kv_heads: int, pages: int, theta: float, workspace):
         import torch
 
         from . import decoder
@@ -183,49 +190,145 @@ class DecoderModel:
         self.heads = (num_heads, num_kv_heads, num_kv_heads)
         H, like = weights[0]["wq"].shape[0], weights[0]["wq"]
         self.head_dim = H // num_heads
-        pages = -(-capacity // self.PAGE)
         self.qkv = [torch.cat([w["wq"], w["wk"], w["wv"]], dim=1) for w in weights]
         self.gains = [(w["norm1_w"].float(), w["norm2_w"].float()) for w in weights]
-        self.caches = [like.new_zeros((2, pages, self.PAGE, num_kv_heads, self.head_dim)) for _ in weights]
-        # one sequence: its pages lie in order, so a prompt's keys are the cache's first rows
-        self.table = torch.arange(pages, dtype=torch.int32, device=like.device)[None]
-        self.places = torch.arange(pages * self.PAGE, device=like.device)
-        self.lengths = torch.arange(pages * self.PAGE + 1, dtype=torch.int32, device=like.device)
+        self.head_gains = [(w["q_norm_w"].float(), w["k_norm_w"].float()) if "q_norm_w" in w else None for w in weights]
+        self.caches = like.new_zeros((len(weights), 2, pages, self.PAGE, num_kv_heads, self.head_dim))
         self.inv_freq, self.rope_scale = decoder.rope_frequencies(self.head_dim, theta, device=like.device)
+
+    def _layers(self, x, positions, slots, attend):
+        from . import decoder, ops
+
+        T = x.shape[0]
+        _, n = decoder.residual_norm(x, None, self.gains[0][0], eps=RMS_EPS)
+        for i, w in enumerate(self.weights):
+            q, k, v = (n @ self.qkv[i]).view(T, -1, self.head_dim).split(self.heads, dim=1)
+            keys, values = self.caches[i]
+            if self.head_gains[i] is None:
+                q = decoder.rope_append(q, k, v, positions, self.inv_freq, keys, values, slots, scale=self.rope_scale)
+            else:
+                q = decoder.norm_rope_append(q, k, v, positions, self.inv_freq, *self.head_gains[i], keys, values, slots, eps=RMS_EPS,
+                                             scale=self.rope_scale)
+            x, n = decoder.residual_norm(x, attend(q, keys, values).reshape(T, -1) @ w["wo"], self.gains[i][1], eps=RMS_EPS)
+            y = ops.svd_mlp(n, w["ug"], w["vg"], w["uu"], w["vu"], w["ud"], w["vd"], workspace=self.workspace)
+            x, n = decoder.residual_norm(x, y, self.gains[i + 1][0] if i + 1 < len(self.weights) else None, eps=RMS_EPS)
+        return x
+
+
+class DecoderModel(_Layers):
+    """:class:`_Layers` for one sequence, its pages in order.
+
+    ``prompt(x)`` runs a sequence and fills the caches; ``extend(x, first)`` runs the
+    tokens from position ``first`` on, a chunk of a prompt, whose keys and values go
+    into the caches, onto what they hold before them; ``step(x, position)`` one token.
+    ``capacity``: tokens the caches can hold."""
+
+    def __init__(self, weights, num_heads: int, num_kv_heads: int, capacity: int, theta: float = 500000.0, workspace=None):
+        import torch
+
+        pages = -(-capacity // self.PAGE)
+        super().__init__(weights, num_heads, num_kv_heads, pages, theta, workspace)
+        device = self.caches.device
+        # one sequence: its pages lie in order, so a prompt's keys are the cache's first rows
+        self.table = torch.arange(pages, dtype=torch.int32, device=device)[None]
+        self.places = torch.arange(pages * self.PAGE, device=device)
+        self.lengths = torch.arange(pages * self.PAGE + 1, dtype=torch.int32, device=device)
 
     def prompt(self, x):
         from . import decoder
 
         rows = x.shape[0]
 
-        def attend(q, cache):
-            k, v = cache.flatten(1, 2)[:, :rows]
-            return decoder.prompt_attention(q, k, v)
+        def attend(q, keys, values):
+            return decoder.prompt_attention(q, keys.flatten(0, 1)[:rows], values.flatten(0, 1)[:rows])
 
-        return self._layers(x, 0, attend)
+        return self._at(x, 0, attend)
+
+    def extend(self, x, first: int):
+        from . import decoder
+
+        rows = x.shape[0]
+        if not rows:
+            return x
+        lengths, cu = self.lengths[first + rows:first + rows + 1], self.lengths[:rows + 1:rows]
+        return self._at(x, first, lambda q, keys, values: decoder.chunk_attention(q, keys, values, self.table, lengths, cu))
 
     def step(self, x, position: int):
         from . import decoder
 
         lengths = self.lengths[position + 1:position + 2]
-        return self._layers(x, position, lambda q, cache: decoder.cache_attention(q[None], cache[0], cache[1], self.table, lengths)[0])
+        return self._at(x, position, lambda q, keys, values: decoder.cache_attention(q[None], keys, values, self.table, lengths)[0])
 
-    def _layers(self, x, first: int, attend):
-        from . import decoder, ops
-
+    def _at(self, x, first: int, attend):
         T = x.shape[0]
-        if first + T > self.places.shape[0]:
-            raise ValueError(f"positions up to {first + T - 1} of caches for {self.places.shape[0]} tokens")
+        if first < 0 or first + T > self.places.shape[0]:
+            raise ValueError(f"positions {first} to {first + T - 1} of caches for {self.places.shape[0]} tokens")
         at = self.places[first:first + T]
-        _, n = decoder.residual_norm(x, None, self.gains[0][0], eps=RMS_EPS)
-        for i, w in enumerate(self.weights):
-            q, k, v = (n @ self.qkv[i]).view(T, -1, self.head_dim).split(self.heads, dim=1)
-            cache = self.caches[i]
-            q = decoder.rope_append(q, k, v, at, self.inv_freq, cache[0], cache[1], at, scale=self.rope_scale)
-            x, n = decoder.residual_norm(x, attend(q, cache).reshape(T, -1) @ w["wo"], self.gains[i][1], eps=RMS_EPS)
-            y = ops.svd_mlp(n, w["ug"], w["vg"], w["uu"], w["vu"], w["ud"], w["vd"], workspace=self.workspace)
-            x, n = decoder.residual_norm(x, y, self.gains[i + 1][0] if i + 1 < len(self.weights) else None, eps=RMS_EPS)
-        return x
+        return self._layers(x, at, at, attend)
+
+
+class SequenceModel(_Layers):
+    """:class:`_Layers` for sequences side by side in caches of ``pages`` pages, whose
+    books :class:`svdmlp.PagePool` keeps (``pool``: sequences are added, forked,
+    trimmed and freed there).
+
+    ``step(x, sequences, tokens)`` runs the next tokens[i] tokens of sequence
+    sequences[i], rows of x in this order: one where it generates, a chunk of its
+    prompt where that is being read, in one call.  ``verify(x, sequences, tree)``
+    runs a tree of drafts of each, and ``keep(sequences, paths, drafts)`` puts the
+    accepted ones behind the context."""
+
+    def __init__(self, weights, num_heads: int, num_kv_heads: int, pages: int, theta: float = 500000.0, workspace=None):
+        from .pages import PagePool
+
+        super().__init__(weights, num_heads, num_kv_heads, pages, theta, workspace)
+        self.pool = PagePool(self.caches.flatten(0, 1))
+
+    def step(self, x, sequences, tokens):
+        from . import decoder
+
+        tokens = [int(t) for t in tokens]
+        if sum(tokens) != x.shape[0]:
+            raise ValueError(f"{sum(tokens)} tokens in {x.shape[0]} rows")
+        if not sum(tokens):
+            return x
+        slots, positions, cu = self.pool.reserve(sequences, tokens)
+        table, lengths = self.pool.table(sequences)
+        return self._layers(x, positions, slots, lambda q, keys, values: decoder.chunk_attention(q, keys, values, table, lengths, cu))
+
+    def verify(self, x, sequences, tree):
+        """x (sequences, n, hidden): n drafts of each sequence, their states.  tree
+        (n, n), bool: whose row i names the drafts that draft i follows, and itself,
+        which all come before it.  Those are in the caches until keep says which stay."""
+        from . import decoder
+
+        B, n, H = x.shape
+        if len(sequences) != B or tuple(tree.shape) != (n, n):
+            raise ValueError(f"{len(sequences)} sequences and a tree {tuple(tree.shape)} for {B} x {n} drafts")
+        slots, positions, _ = self.pool.reserve(sequences, [n] * B)
+        table, lengths = self.pool.table(sequences)
+        # a draft's position: the context, and the drafts it follows
+        positions = (positions.view(B, n)[:, :1] + tree.sum(1) - 1).flatten()
+
+        def attend(q, keys, values):
+            return decoder.cache_attention(q.view(B, n, -1, self.head_dim), keys, values, table, lengths, tree=tree)
+
+        return self._layers(x.reshape(B * n, H), positions, slots, attend).view(B, n, H)
+
+    def keep(self, sequences, paths, drafts: int):
+        """paths[i]: the numbers of the drafts of sequences[i], of ``drafts``, that are
+        accepted, increasing."""
+        from .pages import keep_drafts
+
+        paths = [[int(d) for d in path] for path in paths]
+        if len(paths) != len(sequences) or any(sorted(set(p)) != p or any(not 0 <= d < drafts for d in p) for p in paths):
+            raise ValueError(f"paths must hold increasing numbers of drafts below {drafts}, one path a sequence")
+        table, lengths = self.pool.table(sequences)
+        width = max([1, *map(len, paths)])
+        path = self.pool._tensor([p + [-1] * (width - len(p)) for p in paths], lengths.dtype)
+        keep_drafts(self.pool.caches, table, lengths, path.view(len(paths), width), drafts)
+        for s, p in zip(sequences, paths):
+            self.pool.trim(s, self.pool.length(s) - drafts + len(p))
 
 
 def _stats(samples) -> dict:
@@ -259,6 +362,9 @@ def bench_model(S: int, cfg: dict, args) -> dict:
     from . import compat, ops
 
     compat._positive("S", S)
+    if getattr(args, "serve_arm", False):
+        compat._positive("serve-sequences", args.serve_sequences)
+        compat._positive("serve-chunk", args.serve_chunk)
     H, I, n_heads, kv_heads = cfg["hidden"], cfg["intermediate"], cfg["heads"], cfg["kv_heads"]
     n_layers = args.layers if args.layers is not None else cfg["layers"]
     dev = torch.device("cuda:0")
@@ -274,6 +380,9 @@ def bench_model(S: int, cfg: dict, args) -> dict:
         gen = torch.Generator(device=dev)
         gen.manual_seed(args.seed)
         weights = [make_layer_weights(gen, dev, H, I, R, n_heads, kv_heads, dtype) for _ in range(n_layers)]
+        if cfg.get("head_norms"):
+            for w in weights:
+                w.update(q_norm_w=torch.ones(H // n_heads, device=dev, dtype=dtype), k_norm_w=torch.ones(H // n_heads, device=dev, dtype=dtype))
     xgen = torch.Generator(device=dev)
     xgen.manual_seed(args.seed ^ 0xDEAD)
     x = (torch.randn((S, H), generator=xgen, device=dev, dtype=torch.float32) * 0.02).to(dtype)
@@ -322,8 +431,37 @@ def bench_model(S: int, cfg: dict, args) -> dict:
         rec["decoder_step_vs_block_relative_l2"] = float(torch.linalg.norm(got - want) / torch.clamp(torch.linalg.norm(want), min=1e-12))
         rec["decoder_block"] = _time_model(torch, model.prompt, x, args.warmup, args.repeats)
         rec["decoder_step"] = _time_model(torch, lambda x: model.step(x, S), x[:1].contiguous(), args.warmup, args.repeats)
+    if getattr(args, "serve_arm", False):
+        rec["served_step"] = _serve(torch, weights, n_heads, kv_heads, x, args, workspace)
     del weights
     return rec
+
+
+def _serve(torch, weights, n_heads: int, kv_heads: int, x, args, workspace) -> dict:
+    """A server's step: args.serve_sequences sequences of S tokens generate one each, and
+    one reads the chunk of args.serve_chunk behind its S tokens."""
+    from . import ops
+
+    S, n, chunk = x.shape[0], args.serve_sequences, args.serve_chunk
+    model = SequenceModel(weights, n_heads, kv_heads, -(-S // SequenceModel.PAGE) + (n + 1) * (1 + -(-chunk // SequenceModel.PAGE)),
+                          workspace=workspace)
+    first = model.pool.add()
+    for at in range(0, S, chunk):
+        out = model.step(x[at:at + chunk], [first], [x[at:at + chunk].shape[0]])
+    alone = DecoderModel(weights, n_heads, kv_heads, S, workspace=workspace).prompt(x)[-1].float()
+    others = [model.pool.fork(first) for _ in range(n)]  # the same S tokens, in the same pages
+    rows = x[torch.arange(n + chunk, device=x.device) % S].contiguous()
+    sequences, tokens = others + [first], [1] * n + [chunk]
+    model.workspace = ops.svd_mlp_workspace(rows, r=max(max(w["ug"].shape[1], w["ud"].shape[1]) for w in weights), ff=weights[0]["vg"].shape[1])
+
+    def step(rows):
+        model.step(rows, sequences, tokens)
+        for s in sequences:
+            model.pool.trim(s, S)
+
+    stats = _time_model(torch, step, rows, args.warmup, args.repeats)
+    return dict(stats, sequences=n, chunk=chunk,
+                chunks_vs_prompt_relative_l2=float(torch.linalg.norm(out[-1].float() - alone) / torch.clamp(torch.linalg.norm(alone), min=1e-12)))
 
 
 def _parser() -> argparse.ArgumentParser:
@@ -342,6 +480,10 @@ def _parser() -> argparse.ArgumentParser:
     p.add_argument("--dense-arm", action="store_true", help="also time the dense SwiGLU block (weights rebuilt as U.V)")
     p.add_argument("--decoder-arm", action="store_true",
                    help="also time the causal decoder with rotary positions and a paged cache: a prompt, and one more token")
+    p.add_argument("--serve-arm", action="store_true",
+                   help="also time a step of several sequences side by side: each generates a token, one reads a chunk of its prompt")
+    p.add_argument("--serve-sequences", type=int, default=32, metavar="N", help="sequences that generate in the step")
+    p.add_argument("--serve-chunk", type=int, default=256, metavar="T", help="tokens of a prompt's chunk")
     return p
 
 

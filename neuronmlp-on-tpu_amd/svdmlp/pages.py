@@ -141,8 +141,9 @@ class PagePool:
     many hold each.  Sequences are numbers that :meth:`add` and :meth:`fork` give
     out.  The books are kept on the host, without waiting for the device; the rows
     that they move (:meth:`reserve`, :meth:`compact`) move on the current stream by
-    :func:`copy_pages`, so calls on other streams have to be ordered with it.  A
-    refused call changes nothing."""
+    :func:`copy_pages`, so calls on other streams have to be ordered with it.  What
+    it gives out is of the moment, and is refused to a stream that is being
+    captured.  A refused call changes nothing."""
 
     def __init__(self, caches):
         shape, _, _, _, _, _, index, _ = _cache_set("PagePool", caches)
@@ -204,25 +205,26 @@ class PagePool:
                 heapq.heappush(self._free, p)
 
     def reserve(self, sequences, tokens) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """Room for tokens[i] more tokens of sequence sequences[i]: (slots,
+        """Room for tokens[i] more tokens of sequence sequences[i], each once: (slots,
         positions, cu_seqlens) of the packed new tokens, as the operators take them.
         A partly filled last page that others hold too is copied first."""
+        self._uncaptured()
         sequences, tokens = [self._known(s) for s in sequences], [int(t) for t in tokens]
         if len(sequences) != len(tokens) or any(t < 0 for t in tokens):
             raise ValueError("reserve takes a number of tokens, not negative, for each sequence")
+        if len(set(sequences)) < len(sequences):
+            raise ValueError("reserve takes a sequence once")
         # What it takes: pages behind the last, and copies of shared ones.
-        lengths, left, own, need = {}, {}, set(), 0
+        left, need = {}, 0
         for s, t in zip(sequences, tokens):
-            length = lengths.get(s, self._lengths[s])
-            if t and length % self.page and length == self._lengths[s] and s not in own:
+            length = self._lengths[s]
+            if t and length % self.page:
                 last = self._held[s][-1]
                 holders = left.get(last, self._holders[last])
                 if holders > 1:
                     need += 1
                     left[last] = holders - 1
-                own.add(s)
             need += -(-(length + t) // self.page) - -(-length // self.page)
-            lengths[s] = length + t
         if need > len(self._free):
             raise RuntimeError(f"{need} pages needed, {len(self._free)} of {self.pages} free")
         slots, positions, cu, copies = [], [], [0], []
@@ -243,13 +245,20 @@ class PagePool:
             self._copy(*zip(*copies))
         return self._tensor(slots, torch.int64), self._tensor(positions, torch.int64), self._tensor(cu, torch.int32)
 
+    def _uncaptured(self) -> None:
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the books of pages are not for a stream that is being captured")
+
     def _take(self) -> int:
         p = heapq.heappop(self._free)
         self._holders[p] = 1
         return p
 
     def _tensor(self, values, dtype) -> torch.Tensor:
-        return torch.tensor(values, dtype=dtype, device=self.device)
+        if self.device.type != "cuda":
+            return torch.tensor(values, dtype=dtype)
+        # (pinned: a copy from other memory waits for the stream)
+        return torch.tensor(values, dtype=dtype, pin_memory=True).to(self.device, non_blocking=True)
 
     def _copy(self, src, dst, rows=None) -> None:
         with torch.no_grad():
@@ -258,6 +267,7 @@ class PagePool:
 
     def table(self, sequences) -> tuple[torch.Tensor, torch.Tensor]:
         """(block_table, lengths) of the sequences, as the operators take them."""
+        self._uncaptured()
         held = [self._held[self._known(s)] for s in sequences]
         width = max([1, *map(len, held)])
         return (self._tensor([h + [-1] * (width - len(h)) for h in held], torch.int32).view(len(held), width),
@@ -267,6 +277,7 @@ class PagePool:
         """Moves pages from the end to free ones at the front; returns how many are
         held, all of them now before the free ones.  Block tables from before are
         stale."""
+        self._uncaptured()
         used = self.pages - len(self._free)
         dst = sorted(p for p in self._free if p < used)
         src = [p for p in range(used, self.pages) if self._holders[p]]

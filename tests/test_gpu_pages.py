@@ -221,7 +221,7 @@ def test_page_pool(gpu):
         if what < 0.5 or not told:
             if not told or rng.random() < 0.2:
                 told[pool.add()] = torch.zeros(n, 0, K, D)
-            seqs = [rng.choice(list(told)) for _ in range(rng.randint(1, 3))]
+            seqs = rng.sample(list(told), min(len(told), rng.randint(1, 3)))
             grow = [rng.randint(0, 9) for _ in seqs]
             free = pool.free_pages
             try:

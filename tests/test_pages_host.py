@@ -127,7 +127,9 @@ def test_books_copy_after_a_cut_into_a_shared_page(monkeypatch):
     pool.reserve([a], [8])
     b = pool.fork(a)
     pool.trim(b, 7)
-    slots, _, _ = pool.reserve([b, b], [1, 1])  # the same sequence twice: one copy, then a page of its own
+    with pytest.raises(ValueError, match="once"):
+        pool.reserve([b, b], [1, 1])
+    slots, _, _ = pool.reserve([b], [2])  # a copy, then a page of its own
     assert calls == [([1], [2], [3])] and slots.tolist() == [11, 12] and pool.free_pages == 0
     with pytest.raises(RuntimeError, match="1 pages needed"):
         pool.reserve([a], [1])
