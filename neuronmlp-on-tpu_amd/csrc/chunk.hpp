@@ -40,16 +40,34 @@ struct Place {
   int hk, b, tile, start, n, len, u, units;
 };
 
+// The bounds of the first 64 sequences, which a block keeps in LDS for its later
+// pieces: read again while other blocks load keys, they took 4 us.
+struct Kept {
+  int start[64], n[64], len[64], ends[64];
+};
+
 // The work of a class (all of a wave's lanes together).  Units fit 31 bits: the host
 // chooses their size so.
 template <bool MANY>
 class Line {
  public:
-  __device__ __forceinline__ Line(const ChunkParams& p, const ChunkClass& k, int lane) : p_(p), k_(k), lane_(lane) {
+  // first: the block's first one, whose bounds are read and kept; all of its threads are here.
+  __device__ __forceinline__ Line(const ChunkParams& p, const ChunkClass& k, int lane, SVDMLP_ATTN_LDS Kept* kept, bool first)
+      : p_(p), k_(k), lane_(lane) {
     int tiles = 0;
     Carry c = {};
     for (int b0 = 0; b0 < p_.B; b0 += 64) {
-      const Some s = some(b0, c);
+      Some s;
+      if (b0 == 0 && !first) {
+        s = tiles_of({kept->start[lane], kept->n[lane], kept->len[lane], 0, __builtin_amdgcn_readfirstlane(kept->ends[lane])});
+        c.ends = s.ends;
+      } else {
+        s = some(b0, c);
+      }
+      if (b0 == 0 && first) {
+        if (threadIdx.x < 64) kept->start[lane] = s.start, kept->n[lane] = s.n, kept->len[lane] = s.len, kept->ends[lane] = s.ends;
+        __syncthreads();
+      }
       if (b0 == 0) first_ = s;
       tiles += sum(s.tiles);
     }
@@ -76,12 +94,14 @@ class Line {
   // longer than equal parts of the line, no block takes the time of two pieces'
   // starts and ends.  A tile's units are then those pieces.  Tiles of one sequence that
   // are cut alike also read the same keys at the same time, from L2, which is worth
-  // half a part (160 rows over 120000 keys, 8 heads of 128: 401 us by the line).
+  // half a part in bf16 (160 rows over 120000 keys, 8 heads of 128: 401 us by the
+  // line, 233 alike); fp32 is bound by its products (701 tokens of three sequences,
+  // 16 heads of 64: 65 us by the line, 68 alike).
   __device__ __forceinline__ bool alone(int tiles) {
     const int most = first_.a + slope_ * max(first_.tiles - 1, 0), n = tiles * p_.Hk;
     const int line = sum(upto(first_.a, first_.tiles, first_.tiles)) * p_.Hk;
     const int even = max((line + k_.blocks - 1) / k_.blocks, k_.least);
-    const int slack = tiles > __builtin_popcountll(__ballot(first_.tiles > 0)) ? max(even / 2, k_.start) : k_.start;
+    const int slack = k_.alike && tiles > __builtin_popcountll(__ballot(first_.tiles > 0)) ? max(even / 2, k_.start) : k_.start;
     int best = 0;
     for (int i = 0; i < 8 && !best; ++i) {
       const int length = max((int)((float)line / (float)(k_.blocks - n * i / 8)) + 1, k_.least);
@@ -185,10 +205,13 @@ class Line {
     const int before = __builtin_amdgcn_update_dpp(0, upto, 0x138, 0xf, 0xf, false);  // the lane before's
     s.start = max(from, lane_ == 0 ? c.ends : before);
     s.n = max(to - s.start, 0);
+    c.ends = s.ends = __builtin_amdgcn_readlane(upto, 63);
+    return tiles_of(s);
+  }
+  __device__ __forceinline__ Some tiles_of(Some s) const {
     const int rows = s.n * (p_.Hq / p_.Hk);
     s.tiles = rows >= k_.from && rows <= k_.upto ? (rows + k_.rows - 1) >> k_.rows_log : 0;
     s.a = (max(s.len - s.n, 0) >> k_.unit_log) + k_.slope + k_.start;
-    c.ends = s.ends = __builtin_amdgcn_readlane(upto, 63);
     return s;
   }
   // The order of tiles: by index, or (MANY) by the sequences' lengths, the longest first,
@@ -272,31 +295,38 @@ __device__ __forceinline__ void keys_of(const ChunkParams& p, const ChunkClass& 
   piece.kbeg = piece.from ? keys_upto(k, w, keys, piece.from) : 0;
   piece.kend = keys_upto(k, w, keys, piece.upto);
 }
-// The block's next piece; `at` is its place in the line behind it, -1 before its first
-// and the line's end behind its last.  (The line is read again for each piece:
-// kept, it takes registers that the products need.)  block: its part of the line.
+// A block's way along the line: where it is (-1 before its first piece), where its
+// part ends, and which part that is.
+struct Walk {
+  int at = -1, end = 0, block = 0;
+};
+// The block's next piece.  (The line is computed again for each: kept, it takes
+// registers that the products need.)
 template <bool MANY>
-__device__ __forceinline__ bool next_piece(const ChunkParams& p, const ChunkClass& k, int lane, int& at, int& block, Place& w, Piece& piece) {
-  const Line<MANY> line(p, k, lane);
+__device__ __forceinline__ bool next_piece(const ChunkParams& p, const ChunkClass& k, int lane, SVDMLP_ATTN_LDS Kept* kept, Walk& walk, Place& w, Piece& piece) {
+  const bool first_piece = walk.at < 0;
+  if (!first_piece && walk.at >= walk.end) return false;
+  const Line<MANY> line(p, k, lane, kept, first_piece);
   if (MANY && (int)blockIdx.x < line.whole) {
-    if (at >= 0) return false;
-    at = 0;
+    walk.at = walk.end;
     line.tile(blockIdx.x, w);
     piece.from = 0, piece.upto = w.units;
     keys_of(p, k, w, piece);
     return true;
   }
-  // Parts that lie side by side go to one XCD.
-  block = blockIdx.x - line.whole;
-  if (block >= k.blocks) return false;
-  if constexpr (!MANY) block = xcd_remap(block, k.blocks);
-  const int64_t begin = (int64_t)block * line.part;
-  const int end = (int)min((int64_t)line.total, begin + line.part);
-  bool first = at < 0;
-  if (first) {
-    at = (int)min(begin, (int64_t)line.total);
-    if (threadIdx.x == 0 && k.blocks > 1) note_of(p, k, block)->pieces = 0;
+  if (first_piece) {
+    // Parts that lie side by side go to one XCD.
+    walk.block = blockIdx.x - line.whole;
+    if (walk.block >= k.blocks) return false;
+    if constexpr (!MANY) walk.block = xcd_remap(walk.block, k.blocks);
+    const int64_t begin = (int64_t)walk.block * line.part;
+    walk.end = (int)min((int64_t)line.total, begin + line.part);
+    walk.at = (int)min(begin, (int64_t)line.total);
+    if (threadIdx.x == 0 && k.blocks > 1) note_of(p, k, walk.block)->pieces = 0;
   }
+  const int block = walk.block, end = walk.end;
+  int& at = walk.at;
+  bool first = first_piece;
   while (at < end && line.find(at, w)) {
     const int tile_at = at - w.u;
     piece.from = first ? line.cut(w.u, w.units) : 0;

@@ -43,13 +43,14 @@ __global__ __launch_bounds__(256, 1) void chunk_pipe_kernel(ChunkParams p, Chunk
   if constexpr (!FULL)  // zeros where a head is shorter than its place (never loaded)
     for (int i = threadIdx.x; i < C::NS * C::STAGE / 16; i += 256) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(base + 16 * i) = u32x4{0u, 0u, 0u, 0u};
 
-  for (int now = -1, block = 0;;) {
+  __shared__ Kept kept;
+  for (Walk walk;;) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));  // what follows from it is not kept over the pieces
     const int col = lane & 31, half = lane >> 5;
     Place w;
     Piece part;
-    if (!next_piece<true>(p, k, lane, now, block, w, part)) return;
+    if (!next_piece<true>(p, k, lane, (SVDMLP_ATTN_LDS Kept*)&kept, walk, w, part)) return;
     const int G = p.Hq / p.Hk, npieces = p.D / 8, row0 = w.tile * C::BM, rows = w.n * G, context = w.len - w.n;
     const int all = part.kend - part.kbeg;  // keys of this piece, its first number 0 from here on
     const int token0 = context - part.kbeg;  // the first new token's key
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(256, 1) void chunk_pipe_kernel(ChunkParams p, Chunk
           }
       }
     }
-    float* const sums = part.whole ? nullptr : sums_of(e, k, block, part.from == 0);
+    float* const sums = part.whole ? nullptr : sums_of(e, k, walk.block, part.from == 0);
 #pragma unroll
     for (int g = 0; g < QG; ++g) {
       const int rr = (wave * QG + g) * 32 + col, r = row0 + rr;
@@ -351,7 +352,7 @@ ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int
   auto fill = [&](ChunkClass& k, int64_t from, int64_t upto, int tile_log, int step, int64_t blocks, int64_t least, int64_t start) {
     const int64_t tile = (int64_t)1 << tile_log, G = Hq / Hk;
     k.from = (int)std::min<int64_t>(from, 0x7fffffff), k.upto = (int)std::min<int64_t>(upto, 0x7fffffff);
-    k.rows = (int)tile, k.rows_log = tile_log, k.step = step;
+    k.rows = (int)tile, k.rows_log = tile_log, k.step = step, k.alike = bf16;
     if (upto < from) return;
     // Sequences of the class, and their tiles: at most one short tile each.
     const int64_t n = std::min(B, rows / from);

@@ -35,13 +35,14 @@ __global__ __launch_bounds__(256, 1) void chunk_share_kernel(ChunkParams p, Chun
   if (p.D < C::DP)  // pieces behind the head's end: never loaded, zeros
     for (int i = threadIdx.x; i < C::STAGES * C::STAGE / 16; i += 256) *reinterpret_cast<SVDMLP_ATTN_LDS u32x4*>(base + 16 * i) = u32x4{0u, 0u, 0u, 0u};
 
-  for (int now = -1, block = 0;;) {
+  __shared__ Kept kept;
+  for (Walk walk;;) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));  // what follows from it is not kept over the pieces
     const int col = lane & 31, half = lane >> 5;
     Place w;
     Piece piece;
-    if (!next_piece<true>(p, k, lane, now, block, w, piece)) return;
+    if (!next_piece<true>(p, k, lane, (SVDMLP_ATTN_LDS Kept*)&kept, walk, w, piece)) return;
     const int G = p.Hq / p.Hk, npieces = p.D * ES / 16, row0 = w.tile * C::ROWS, rows = w.n * G, context = w.len - w.n;
     const int shared = context + row0 / G + 1;     // keys that every row sees
     const int rr = wave * 32 + col, r = min(row0 + rr, rows - 1);  // rows behind the last repeat it, and are not stored
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(256, 1) void chunk_share_kernel(ChunkParams p, Chun
       }
     }
     if (row0 + rr < rows) {
-      float* const sums = piece.whole ? nullptr : sums_of(e, k, block, piece.from == 0);
+      float* const sums = piece.whole ? nullptr : sums_of(e, k, walk.block, piece.from == 0);
       const int64_t out = (int64_t)(w.start + tok) * e.o_t + (int64_t)(w.hk * G + (r - tok * G)) * e.o_h;
       if (sums && half == 0) reinterpret_cast<f32x2*>(sums + C::ROWS * e.D)[rr] = f32x2{st.m, l};
 #pragma unroll

@@ -38,13 +38,14 @@ __global__ __launch_bounds__(64 * C::NW, 1) void chunk_wave_kernel(ChunkParams p
   const int G = p.Hq / p.Hk, npieces = p.D * ES / 16;
   const attn_lds mine = (attn_lds)lds + wave * C::STAGE;
 
-  for (int now = -1, block = 0;;) {
+  __shared__ Kept kept;
+  for (Walk walk;;) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));  // what follows from it is not kept over the pieces
     const int col = lane & 31, half = lane >> 5;
     Place w;
     Piece piece;
-    if (!next_piece<false>(p, k, lane, now, block, w, piece)) return;
+    if (!next_piece<false>(p, k, lane, (SVDMLP_ATTN_LDS Kept*)&kept, walk, w, piece)) return;
     const TileLane<RB, BF16> at(lane);
     const int lrow = lane / C::PIECES, lc = lane % C::PIECES;
     const int kpiece0 = lc ^ k_swz<RB>(lrow), vpiece0 = lc ^ v_swz<RB, BF16>(lrow);
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(64 * C::NW, 1) void chunk_wave_kernel(ChunkParams p
     }
     __syncthreads();
     const ChunkParams& e = args_again();
-    float* const sums = piece.whole ? nullptr : sums_of(e, k, block, piece.from == 0);
+    float* const sums = piece.whole ? nullptr : sums_of(e, k, walk.block, piece.from == 0);
     for (int i = threadIdx.x; i < 32 * OP; i += 64 * NW) {
       // (sums go out row by row, results piece by piece of a row)
       const int rr = piece.whole ? i / OP : i % 32, c = piece.whole ? i % OP : i / 32, row = row0 + rr;

@@ -119,6 +119,7 @@ struct ChunkClass {
   int from, upto, rows, rows_log;
   int unit_log, slope, start, least;  // slope: a tile has so many units more than the one before it; start: as many as a tile's start and end take
   int step;                    // keys that a block takes at once
+  int alike;                   // whether tiles of a sequence gain from being cut alike (Line::alone)
   int blocks, grid;            // parts of the line, blocks of the launch; 0: no sequence can be of the class
   int joins;                   // blocks that join the sums of tiles in several parts
   int fits;                    // whether units and tiles fit the kernels' numbers
