@@ -302,8 +302,8 @@ int svdmlp_noalloc_status(int32_t reset, int64_t wait_bound, void* stream);
  * elements, in the order named (NULL: dense); the last dimension is contiguous,
  * and the stride of a dimension of one element is not looked at by attention.
  * Query head h belongs to key/value head h / (Hq / Hk).  They need no
- * workspace but cache attention's, hold no state between calls, and can be
- * captured into graphs.  Indices are read on the device: one that points
+ * workspace but cache and chunk attention's, hold no state between calls, and can
+ * be captured into graphs.  Indices are read on the device: one that points
  * nowhere (a slot or page outside the cache, a sequence outside the rows, a
  * length beyond the table) is skipped or cut, never followed.
  */
@@ -383,9 +383,11 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
  * leave the first ones without any.  Rows of no sequence are left as they were.
  * D, strides and addresses as svdmlp_cache_attention.  strides: q token, head;
  * k_cache page, row, head; v_cache page, row, head; out token, head; block_table
- * sequence.  The workspace (svdmlp_chunk_attention_workspace_bytes; may be 0)
- * holds the sums of long contexts' chunks and needs no clearing; calls in
- * flight at the same time need workspaces of their own.
+ * sequence.  The workspace (svdmlp_chunk_attention_workspace_bytes, which depends on
+ * the sizes and the current device's CUs; may be 0) holds the sums of long
+ * contexts' pieces and needs no clearing; calls in flight at the same time need
+ * workspaces of their own.  A call of more rows or sequences than the kernels'
+ * numbers hold is refused.
  */
 size_t svdmlp_chunk_attention_workspace_bytes(int64_t T, int64_t B, int64_t page, int64_t width, int64_t Hq,
                                               int64_t Hk, int64_t D, int32_t dtype);

@@ -14,10 +14,22 @@
 // as many units as the tile has keys, about.  It is cut into equal parts, one a
 // block, whatever the lengths are: a block takes the end of a tile, some whole
 // ones, the start of another.  chunk_join_kernel adds the sums of the tiles that
-// lie in several parts, of which there are fewer than blocks.  Where tiles of 128
-// or 256 rows are many, the first ones are blocks of their own, the longest first, and
-// only the last one or two a CU are such a line: blocks that start together on
-// tiles of one head read the same keys at the same time, from one XCD's L2.
+// lie in several parts, of which there are fewer than blocks, always in their
+// order.  Where tiles of 128 or 256 rows are many, the first ones are blocks of
+// their own, the longest first, and only the last one or two a CU are such a line:
+// blocks that start together on tiles of one head read the same keys at the same
+// time, from one XCD's L2.
+//
+// What bounds them: tiles of 32 rows the cache's bytes (96 sequences of 4000 tokens
+// that generate, heads of 128: 300 us, 5.2 TB/s, a copy's rate) and, in fp32, the
+// matrix unit (73% busy); tiles of 256 rows the matrix unit and the softmax beside
+// it in the one wave a SIMD (8192 tokens of four sequences onto 16384, 64 heads of
+// 128: 1.64 ms, 1.08 PFLOP/s of a product's 1.25; 512 onto 32768: 265 us, 1.03).  A
+// server's step, 63 sequences of up to 4096 that generate and a chunk of 449: 187 us =
+// 117 for the generating ones (4.5 TB/s), 53 for the chunk (five pieces of a tile, 15
+// of the 53 for their starts and ends), 17 to add them (34 MB of sums of pieces, at
+// 2.5 TB/s, whatever the registers, and so waves, of the join).  Few tokens: latency, a chain of
+// loads (bounds, pages, keys), the join a launch of its own: 37 tokens 16 us.
 #include "chunk.hpp"
 #include "pipe_attention.hpp"
 

@@ -7,6 +7,11 @@
 // of 32 rows the keys and values are read a quarter as often, and a start and an
 // end are shared by four times the rows; heads of over 128 fit their queries into
 // registers, with one wave a SIMD.
+// Bound there by LDS, which 32 rows a wave read as long as they multiply, and the
+// softmax behind it (the matrix unit is busy 28% of the time): 4000 tokens of 8
+// heads of 256 165 us, 396 TFLOP/s; 1000 tokens each of 8 sequences of 8000, 583.
+// fp32 heads of 256: 61% busy, 78 TFLOP/s.  64 sequences of 12 tokens, 2000 keys, heads of
+// 128: 160 us, 3.3 TB/s.
 #include "chunk.hpp"
 
 namespace svdmlp {
@@ -52,8 +57,12 @@ __global__ __launch_bounds__(256, 1) void chunk_share_kernel(ChunkParams p, Chun
     const int* const table = p.table + (int64_t)w.b * p.table_b;
     const uint32_t cache_pages = (uint32_t)min(p.pages, (int64_t)0x7fffffff);
     auto valid = [&](int pg) { return (uint32_t)pg < cache_pages; };
-    const TileLane<RB, BF16> at(lane);
-    const int lrow = wave * C::MINE * C::RPL + lane / C::PIECES, lc = lane % C::PIECES;
+    // Where registers are short, a lane's places in the tiles are computed for every tile.
+    auto here = [&] {
+      int x = lane;
+      if constexpr (RB >= 1024) asm volatile("" : "+v"(x));
+      return x;
+    };
 
     u32x4 qf[C::STEPS];
     f32x16 o[DB];
@@ -93,6 +102,7 @@ __global__ __launch_bounds__(256, 1) void chunk_share_kernel(ChunkParams p, Chun
       // This wave's loads of tile t: MINE of keys and as many of values in any case.
       auto issue = [&](int t) {
         const uint32_t to = (uint32_t)(uintptr_t)(base + t % C::STAGES * C::STAGE) + wave * C::MINE * 1024;
+        const int x = here(), lrow = wave * C::MINE * C::RPL + x / C::PIECES, lc = x % C::PIECES;
 #pragma unroll
         for (int j = 0; j < C::MINE; ++j) {
           const int row = lrow + j * C::RPL, key = min(kbeg + t * KB + row, kend - 1), pg = page_of(p, key);
@@ -117,6 +127,7 @@ __global__ __launch_bounds__(256, 1) void chunk_share_kernel(ChunkParams p, Chun
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (t + C::STAGES - 1 < tiles) issue(t + C::STAGES - 1);
         const attn_lds lk = base + t % C::STAGES * C::STAGE, lv = lk + C::TILE;
+        const TileLane<RB, BF16> at(here());
         const int ku = kbeg + t * KB;
         constexpr int kAhead = RB < 1024 ? 4 : 2, VF = BF16 ? 2 * DB : 16 * DB;  // VF: pieces of V
         u32x4 kf[kAhead], vf[kAhead];

@@ -1,4 +1,5 @@
-// Attention over chunks, of tiles of 32 rows (chunk_attention.hip).
+// Attention over chunks, of tiles of 32 rows (chunk_attention.hip): sequences that
+// generate, short chunks, and fp32 heads up to 128.
 #include "chunk.hpp"
 
 namespace svdmlp {
@@ -25,7 +26,11 @@ __device__ const u32x4 kNoKey = {0u, 0u, 0u, 0u};  // what lanes without a key l
 // A block's waves share its rows: each takes every NW-th tile of 32 keys through
 // LDS of its own, and their sums meet in LDS at the end.  A wave's next keys are on
 // their way while it multiplies the values, its next values while it multiplies
-// the keys, and the numbers of its pages a tile before.
+// the keys, and the numbers of its pages a tile before.  Two blocks a CU (three of
+// bf16 heads up to 64), so that one's start and end lie behind the other's
+// products.  Two waves a block, twice as many blocks: bf16 heads of 128, 37 tokens
+// 17.1 -> 20.4 us, 64 sequences that generate 149 -> 158; fp32 heads of 64, 701 tokens 66
+// -> 71, 3200 tokens 452 -> 396.
 template <class C>
 __global__ __launch_bounds__(64 * C::NW, 1) void chunk_wave_kernel(ChunkParams p, ChunkClass k) {
   constexpr bool BF16 = C::BF16, QREG = C::QREG;
