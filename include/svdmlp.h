@@ -451,7 +451,8 @@ int svdmlp_copy_pages(void* const* caches, int64_t n, int64_t apart, const int64
  * context and them.  The numbers increase along a path; it ends before the
  * first that does not, is negative, or is not below `drafts` (-1 behind a
  * short path).  A sequence of fewer tokens than drafts stays as it is, with
- * its length; a row in a page outside the cache is not moved.
+ * its length; a row in a page outside the cache is not moved.  Pages that hold
+ * drafts are of one sequence alone, once; new_lengths and lengths share no memory.
  */
 int svdmlp_keep_drafts(void* const* caches, int64_t n, int64_t apart, const int64_t* strides /* 3 or NULL */,
                        const int32_t* block_table, const int32_t* lengths, const int32_t* path, int32_t* new_lengths,

@@ -2866,6 +2866,9 @@ int svdmlp_keep_drafts(void* const* caches, int64_t n, int64_t apart, const int6
   if (drafts <= 0 || drafts > kDraftsMost || m <= 0 || m > drafts)
     return fail("keep_drafts: 1 to %d drafts, and a path of at most as many, got %lld and %lld", kDraftsMost, (long long)drafts, (long long)m);
   if (table_stride < 0) return fail("keep_drafts: strides must not be negative");
+  // (blocks read the lengths after another one has written the new ones)
+  const uintptr_t was = (uintptr_t)lengths, now = (uintptr_t)new_lengths, bytes = (uintptr_t)B * 4;
+  if (was < now + bytes && now < was + bytes) return fail("keep_drafts: new_lengths must not share memory with lengths");
   p.table = block_table, p.lengths = lengths, p.path = path, p.new_lengths = new_lengths;
   p.table_b = table_stride, p.width = (int)width, p.B = (int)B, p.m = (int)m, p.drafts = (int)drafts;
   StageScope s(ST_KEEP_DRAFTS, (hipStream_t)stream);

@@ -303,8 +303,10 @@ class SequenceModel(_Layers):
         from . import decoder
 
         B, n, H = x.shape
-        if len(sequences) != B or tuple(tree.shape) != (n, n):
-            raise ValueError(f"{len(sequences)} sequences and a tree {tuple(tree.shape)} for {B} x {n} drafts")
+        if len(sequences) != B or tuple(tree.shape) != (n, n) or not 1 <= n <= 64:
+            raise ValueError(f"{len(sequences)} sequences and a tree {tuple(tree.shape)} for {B} x {n} drafts (1 to 64)")
+        if str(tree.dtype) != "torch.bool" or tree.device != x.device:
+            raise ValueError(f"the tree must be a bool tensor on {x.device}, got {tree.dtype} on {tree.device}")
         slots, positions, _ = self.pool.reserve(sequences, [n] * B)
         table, lengths = self.pool.table(sequences)
         # a draft's position: the context, and the drafts it follows
@@ -321,6 +323,10 @@ class SequenceModel(_Layers):
         from .pages import keep_drafts
 
         paths = [[int(d) for d in path] for path in paths]
+        if len(set(sequences)) < len(sequences):
+            raise ValueError("keep takes a sequence once")
+        if any(self.pool.length(s) < drafts for s in sequences):
+            raise ValueError(f"a sequence has fewer than {drafts} tokens")
         if len(paths) != len(sequences) or any(sorted(set(p)) != p or any(not 0 <= d < drafts for d in p) for p in paths):
             raise ValueError(f"paths must hold increasing numbers of drafts below {drafts}, one path a sequence")
         table, lengths = self.pool.table(sequences)

@@ -113,7 +113,8 @@ def keep_drafts(caches, block_table, lengths, path, drafts: int) -> torch.Tensor
     behind the context.  A path ends before the first number that does not
     increase or is no draft.  A sequence of fewer tokens than ``drafts`` keeps
     them and its length.  block_table and lengths are those of
-    cache_attention; rows in pages outside the cache are not moved."""
+    cache_attention; rows in pages outside the cache are not moved.  A page that
+    holds drafts has to be of one sequence alone, as PagePool.reserve leaves it."""
     (pages, page, Hk, D), code, every, pointers, n, apart, index, strides = _cache_set("keep_drafts", caches)
     if isinstance(drafts, bool) or not isinstance(drafts, int) or not 1 <= drafts <= 64:
         raise ValueError(f"1 to 64 drafts a sequence, got {drafts}")

@@ -128,8 +128,15 @@ def test_sequences_side_by_side(gpu, head_norms):
         model.step(rows(2), [a, a], [1, 1])
     with pytest.raises(ValueError, match="increasing"):
         model.keep([a], [[1, 0]], 5)
-    with pytest.raises(ValueError, match="tree"):
-        model.verify(rows(2, 3), [a, c], tree.to(gpu))
+    held = pool.length(a), pool.length(c), pool.free_pages
+    for x, t in ((rows(2, 3), tree.to(gpu)), (rows(2, 5), tree), (rows(2, 5), tree.to(gpu).int()), (rows(1, 5), tree.to(gpu)), (rows(2, 0), tree[:0, :0].to(gpu))):
+        with pytest.raises(ValueError, match="tree"):
+            model.verify(x, [a, c], t)
+    with pytest.raises(ValueError, match="once"):
+        model.keep([a, a], [[0], [1]], 5)
+    with pytest.raises(ValueError, match="fewer"):
+        model.keep([pool.add()], [[0]], 5)
+    assert held == (pool.length(a), pool.length(c), pool.free_pages)
 
 
 def test_books_of_a_captured_stream(gpu):

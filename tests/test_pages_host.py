@@ -60,10 +60,11 @@ def test_copy_pages_refusals(lib, kw, msg):
 @pytest.mark.parametrize("kw,msg", [
     (dict(n=-1), b"no caches"), (dict(table=None), b"null"), (dict(path=None), b"null"), (dict(out=None), b"null"), (dict(B=0), b"positive"),
     (dict(width=0), b"positive"), (dict(width=1 << 40), b"2^31"), (dict(drafts=0), b"1 to 64"), (dict(drafts=65), b"1 to 64"),
+    (dict(out=ctypes.c_void_p(P.value - 4)), b"share memory"), (dict(lengths=ctypes.c_void_p(4096), out=ctypes.c_void_p(4100)), b"share memory"),
     (dict(m=5), b"as many"), (dict(m=0), b"as many"), (dict(table_stride=-1), b"negative"), (dict(Hk=0), b"positive"),
 ])
 def test_keep_drafts_refusals(lib, kw, msg):
-    a = dict(caches=_caches(), n=2, apart=0, strides=None, table=P, lengths=P, path=P, out=P, table_stride=4, B=2, width=4, m=3, drafts=4, pages=4,
+    a = dict(caches=_caches(), n=2, apart=0, strides=None, table=P, lengths=P, path=P, out=ctypes.c_void_p(4096), table_stride=4, B=2, width=4, m=3, drafts=4, pages=4,
              page=16, Hk=2, D=16, dtype=1) | kw
     assert lib.svdmlp_keep_drafts(*a.values(), None) == BAD
     assert msg in lib.svdmlp_last_error()
