@@ -410,8 +410,11 @@ ChunkPlan plan_chunk_attention(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int
   if (bf16 && rows <= 256) few = rows;
   else if (bf16 && B == 1) few = 0, some = pipe ? 0 : rows;  // (whose rows are the call's)
   few = std::min(few, rows), some = std::max(few, std::min(some, rows));
-  // Blocks that a CU holds at once, and the keys that a tile's start and end take
-  // as long as.
+  // Blocks that a CU holds at once, the keys a block takes at least, and those that a
+  // tile's start and end take as long as.  Half as many blocks again, or twice as
+  // many, that start as others end, lose to their starts: 64 sequences that generate
+  // 149, 164, 159 us; 701 fp32 tokens 66, 83, 81 (3200: 421, 454, 395).  Starts of 128 or
+  // 400 keys are within 2% of 256, but for fp32 (701 tokens 66, 71 by 128).
   fill(plan.many, some + 1, rows, 8, 64, cus, 512, 384);
   fill(plan.some, few + 1, some, 7, 32, cus * (D <= 128 ? 2 : 1), 256, 256);
   fill(plan.few, 1, few, 5, wave, cus * (!bf16 ? 2 : D <= 64 ? 3 : D <= 128 ? 2 : 1), 512, 256);

@@ -83,7 +83,8 @@ def test_chunk_attention(gpu, dtype, lens, news, H, K, D, page):
 @pytest.mark.parametrize("dtype,lens,news,H,K,D,page", [
     (BF, [9000], [40], 16, 4, 128, 4), (BF, [20000, 300], [70, 2], 8, 2, 128, 16), (BF, [6000], [90], 4, 2, 64, 1), (BF, [12000, 11000], [300, 1], 4, 1, 96, 8),
     (BF, [5000], [5000], 2, 1, 64, 64), (BF, [30000], [2], 8, 1, 128, 48), (BF, [9000, 100], [140, 90], 2, 1, 256, 16), (F32, [7000], [40], 4, 2, 64, 16),
-    (F32, [5000, 64], [3, 64], 4, 1, 128, 3), (F32, [3000], [300], 2, 1, 256, 32), (BF, [70000], [129], 1, 1, 128, 2), (BF, [40000, 3], [1, 3], 2, 2, 64, 16)])
+    (F32, [5000, 64], [3, 64], 4, 1, 128, 3), (F32, [3000], [300], 2, 1, 256, 32), (BF, [70000], [129], 1, 1, 128, 2), (BF, [40000, 3], [1, 3], 2, 2, 64, 16),
+    (BF, [7000, 300], [150, 4], 4, 2, 256, 1), (F32, [5000], [70], 2, 1, 256, 1), (BF, [6000, 40], [170, 2], 4, 2, 128, 1)])
 def test_chunk_attention_long_contexts(gpu, dtype, lens, news, H, K, D, page):
     """Contexts in several chunks, more pages than lie in LDS at once."""
     _run(_gen(sum(lens) + D), gpu, dtype, lens, news, H, K, D, page, heads=sorted({0, H - 1}))
@@ -205,7 +206,7 @@ def test_chunk_attention_large_scores(gpu, dtype):
             _close(got[:, [0, H - 1]], out, tol)
 
 
-@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 256), (F32, 64)])
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 256), (F32, 64), (F32, 128), (F32, 256)])
 @pytest.mark.parametrize("n", [2, 170])
 @pytest.mark.parametrize("page", [16, 3])
 def test_chunk_attention_pages_outside_the_cache(gpu, dtype, D, n, page):
