@@ -25,10 +25,10 @@
 // matrix unit (73% busy); tiles of 256 rows the matrix unit and the softmax beside
 // it in the one wave a SIMD (8192 tokens of four sequences onto 16384, 64 heads of
 // 128: 1.64 ms, 1.08 PFLOP/s of a product's 1.25; 512 onto 32768: 265 us, 1.03).  A
-// server's step, 63 sequences of up to 4096 that generate and a chunk of 449: 187 us =
+// server's step, 63 sequences of up to 4096 that generate and a chunk of 449, 187 us:
 // 117 for the generating ones (4.5 TB/s), 53 for the chunk (five pieces of a tile, 15
-// of the 53 for their starts and ends), 17 to add them (34 MB of sums of pieces, at
-// 2.5 TB/s, whatever the registers, and so waves, of the join).  Few tokens: latency, a chain of
+// of the 53 for their starts and ends), some 20 to add them (34 MB of sums of pieces
+// at 2.5 TB/s, whatever the registers, and so waves, of the join).  Few tokens: latency, a chain of
 // loads (bounds, pages, keys), the join a launch of its own: 37 tokens 16 us.
 #include "chunk.hpp"
 #include "pipe_attention.hpp"

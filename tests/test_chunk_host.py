@@ -80,3 +80,35 @@ def test_e2e_parser_has_the_serve_arm():
     args = e2e_block._parser().parse_args([])
     assert (args.serve_arm, args.serve_sequences, args.serve_chunk) == (False, 32, 256)
     assert e2e_block._parser().parse_args(["--serve-arm", "--model", "qwen3-8b", "--serve-chunk", "64"]).serve_chunk == 64
+
+
+@pytest.mark.parametrize("head_norms", [False, True])
+def test_checkpoint_weights_with_head_norms(tmp_path, head_norms):
+    """The layers' weights from a checkpoint: the gains of the heads too, where it has them."""
+    import json
+
+    from safetensors.torch import save_file
+    from svdmlp import checkpoint, e2e_block
+
+    D, FF, R, G = 64, 96, 32, torch.Generator().manual_seed(4)
+    rand = lambda *shape: torch.randn(shape, generator=G).bfloat16()
+    layers = [tuple(rand(*s) for s in ((D, R), (R, FF), (D, R), (R, FF), (FF, R), (R, D))) for _ in range(2)]
+    checkpoint.save_mlp_checkpoint(tmp_path, layers, hidden_size=D, intermediate_size=FF)
+    more = {}
+    for i in range(2):
+        p = f"model.layers.{i}."
+        more |= {p + "self_attn.q_proj.weight": rand(D, D), p + "self_attn.k_proj.weight": rand(32, D), p + "self_attn.v_proj.weight": rand(32, D),
+                 p + "self_attn.o_proj.weight": rand(D, D), p + "input_layernorm.weight": rand(D), p + "post_attention_layernorm.weight": rand(D)}
+        if head_norms:
+            more |= {p + "self_attn.q_norm.weight": rand(16), p + "self_attn.k_norm.weight": rand(16)}
+    save_file(more, str(tmp_path / "attention.safetensors"))
+    at = tmp_path / "model.safetensors.index.json"
+    index = json.loads(at.read_text())
+    index["weight_map"] |= {k: "attention.safetensors" for k in more}
+    at.write_text(json.dumps(index))
+    for i, w in enumerate(e2e_block.load_checkpoint_weights(tmp_path, [0, 1], "cpu", torch.bfloat16)):
+        assert torch.equal(w["wk"], more[f"model.layers.{i}.self_attn.k_proj.weight"].t()) and torch.equal(w["ug"], layers[i][0])
+        assert ("q_norm_w" in w) == ("k_norm_w" in w) == head_norms
+        if head_norms:
+            assert torch.equal(w["q_norm_w"], more[f"model.layers.{i}.self_attn.q_norm.weight"])
+            assert torch.equal(w["k_norm_w"], more[f"model.layers.{i}.self_attn.k_norm.weight"])

@@ -291,3 +291,11 @@ def test_page_pool_refusals(gpu):
         pool.free(a)
     pool.reserve([b], [3])  # alone again: no copy
     assert pool.free_pages == 1
+    slots, positions, cu = pool.reserve([], [])
+    assert slots.shape == positions.shape == (0,) and cu.tolist() == [0] and slots.is_cuda and cu.dtype is torch.int32
+    slots, positions, cu = pool.reserve([b], [0])
+    assert slots.shape == (0,) and cu.tolist() == [0, 0]
+    table, lengths = pool.table([])
+    assert table.shape == (0, 1) and lengths.shape == (0,) and table.is_cuda
+    path = torch.zeros(0, 1, dtype=torch.int32, device=gpu)
+    assert svdmlp.keep_drafts(pool.caches, table, lengths, path, 3).shape == (0,)
