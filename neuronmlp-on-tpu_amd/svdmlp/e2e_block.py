@@ -327,6 +327,8 @@ class SequenceModel(_Layers):
             raise ValueError("keep takes a sequence once")
         if any(self.pool.length(s) < drafts for s in sequences):
             raise ValueError(f"a sequence has fewer than {drafts} tokens")
+        if not all(self.pool.alone(s, drafts) for s in sequences):
+            raise ValueError("a fork holds the drafts' pages: keep comes before it")
         if len(paths) != len(sequences) or any(sorted(set(p)) != p or any(not 0 <= d < drafts for d in p) for p in paths):
             raise ValueError(f"paths must hold increasing numbers of drafts below {drafts}, one path a sequence")
         table, lengths = self.pool.table(sequences)

@@ -114,7 +114,8 @@ def keep_drafts(caches, block_table, lengths, path, drafts: int) -> torch.Tensor
     increase or is no draft.  A sequence of fewer tokens than ``drafts`` keeps
     them and its length.  block_table and lengths are those of
     cache_attention; rows in pages outside the cache are not moved.  A page that
-    holds drafts has to be of one sequence alone, as PagePool.reserve leaves it."""
+    holds drafts has to be of one sequence alone, as PagePool.reserve leaves it
+    (PagePool.alone)."""
     (pages, page, Hk, D), code, every, pointers, n, apart, index, strides = _cache_set("keep_drafts", caches)
     if isinstance(drafts, bool) or not isinstance(drafts, int) or not 1 <= drafts <= 64:
         raise ValueError(f"1 to 64 drafts a sequence, got {drafts}")
@@ -174,6 +175,11 @@ class PagePool:
         self._held[self._next], self._lengths[self._next] = [], 0
         self._next += 1
         return self._next - 1
+
+    def alone(self, sequence: int, tokens: int) -> bool:
+        """Whether no other sequence holds the pages of the sequence's last tokens."""
+        first = max(self.length(sequence) - tokens, 0) // self.page
+        return all(self._holders[p] == 1 for p in self._held[sequence][first:])
 
     def fork(self, sequence: int) -> int:
         """A new sequence of the same tokens, in the same pages: the last one, partly filled, is copied when one of its holders

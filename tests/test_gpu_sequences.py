@@ -115,6 +115,10 @@ def test_sequences_side_by_side(gpu, head_norms):
         sees[n:, n:] = tree
         positions = torch.cat([torch.arange(n), n + tree.sum(1) - 1])
         _close(got[i], _layers64(torch.cat([told[s], x[i]]), weights, positions, sees)[n:])
+    d = pool.fork(a)
+    with pytest.raises(ValueError, match="fork"):
+        model.keep([a, c], [[0, 3, 4], []], 5)
+    pool.free(d)
     model.keep([a, c], [[0, 3, 4], []], 5)
     told[a] = torch.cat([told[a], x[0, [0, 3, 4]]])
     assert pool.length(a) == told[a].shape[0] and pool.length(c) == told[c].shape[0]

@@ -102,10 +102,12 @@ def test_books_of_shared_pages(monkeypatch):
     a = pool.add()
     slots, positions, cu = pool.reserve([a], [6])
     assert slots.tolist() == [0, 1, 2, 3, 4, 5] and positions.tolist() == list(range(6)) and cu.tolist() == [0, 6]
+    assert pool.alone(a, 6)
     b, c = pool.fork(a), pool.fork(a)
-    assert pool.free_pages == 6
+    assert pool.free_pages == 6 and not pool.alone(a, 1) and not pool.alone(c, 6)
     slots, positions, cu = pool.reserve([c, b, a], [1, 0, 3])
     assert calls == [([1, 1], [2, 3], [2, 2])]          # c's copy, then a's, which needs one page more
+    assert pool.alone(c, 3) and not pool.alone(c, 4) and pool.alone(c, 0)
     assert slots.tolist() == [10, 14, 15, 16] and positions.tolist() == [6, 6, 7, 8] and cu.tolist() == [0, 1, 1, 4]
     assert pool.table([a, b, c])[0].tolist() == [[0, 3, 4], [0, 1, -1], [0, 2, -1]]
     pool.reserve([b], [1])                              # the last holder: no copy
