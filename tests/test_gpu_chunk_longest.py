@@ -40,3 +40,12 @@ def _longest(gpu, dtype, H, D, n):
 @pytest.mark.parametrize("dtype,H,D,n", [(F32, 1, 136, 5), (BF, 2, 136, 150)])
 def test_longest_sequence_by_tiles_of_128_rows(gpu, dtype, H, D, n):
     _longest(gpu, dtype, H, D, n)
+
+
+def test_longest_sequence_by_tiles_of_256_rows(gpu):
+    _longest(gpu, BF, 1, 128, 300)
+
+
+@pytest.mark.parametrize("dtype,H,D,n", [(BF, 4, 64, 3), (BF, 2, 128, 9), (F32, 2, 64, 20)])
+def test_longest_sequence_by_tiles_of_32_rows(gpu, dtype, H, D, n):
+    _longest(gpu, dtype, H, D, n)
