@@ -35,6 +35,7 @@ reference's keys (bench/e2e_block.py:338-352, 399-413).
 from __future__ import annotations
 
 import argparse
+import contextlib
 import json
 import math
 import statistics
@@ -276,7 +277,8 @@ class SequenceModel(_Layers):
     sequences[i], rows of x in this order: one where it generates, a chunk of its
     prompt where that is being read, in one call.  ``verify(x, sequences, tree)``
     runs a tree of drafts of each, and ``keep(sequences, paths, drafts)`` puts the
-    accepted ones behind the context."""
+    accepted ones behind the context.  A step or a tree that raises leaves the
+    sequences as long as they were."""
 
     def __init__(self, weights, num_heads: int, num_kv_heads: int, pages: int, theta: float = 500000.0, workspace=None):
         from .pages import PagePool
@@ -284,17 +286,29 @@ class SequenceModel(_Layers):
         super().__init__(weights, num_heads, num_kv_heads, pages, theta, workspace)
         self.pool = PagePool(self.caches.flatten(0, 1))
 
+    @contextlib.contextmanager
+    def _reserved(self, sequences, tokens):
+        """(slots, positions, cu_seqlens, block_table, lengths) of room for tokens[i] more of sequences[i], given back by
+        what raises."""
+        before = [self.pool.length(s) for s in sequences]
+        room = self.pool.reserve(sequences, tokens)
+        try:
+            yield *room, *self.pool.table(sequences)
+        except BaseException:
+            for s, length in zip(sequences, before):
+                self.pool.trim(s, length)
+            raise
+
     def step(self, x, sequences, tokens):
         from . import decoder
 
-        tokens = [int(t) for t in tokens]
+        sequences, tokens = list(sequences), [int(t) for t in tokens]
         if sum(tokens) != x.shape[0]:
             raise ValueError(f"{sum(tokens)} tokens in {x.shape[0]} rows")
         if not sum(tokens):
             return x
-        slots, positions, cu = self.pool.reserve(sequences, tokens)
-        table, lengths = self.pool.table(sequences)
-        return self._layers(x, positions, slots, lambda q, keys, values: decoder.chunk_attention(q, keys, values, table, lengths, cu))
+        with self._reserved(sequences, tokens) as (slots, positions, cu, table, lengths):
+            return self._layers(x, positions, slots, lambda q, keys, values: decoder.chunk_attention(q, keys, values, table, lengths, cu))
 
     def verify(self, x, sequences, tree):
         """x (sequences, n, hidden): n drafts of each sequence, their states.  tree
@@ -307,15 +321,14 @@ class SequenceModel(_Layers):
             raise ValueError(f"{len(sequences)} sequences and a tree {tuple(tree.shape)} for {B} x {n} drafts (1 to 64)")
         if str(tree.dtype) != "torch.bool" or tree.device != x.device:
             raise ValueError(f"the tree must be a bool tensor on {x.device}, got {tree.dtype} on {tree.device}")
-        slots, positions, _ = self.pool.reserve(sequences, [n] * B)
-        table, lengths = self.pool.table(sequences)
-        # a draft's position: the context, and the drafts it follows
-        positions = (positions.view(B, n)[:, :1] + tree.sum(1) - 1).flatten()
+        with self._reserved(sequences, [n] * B) as (slots, positions, _, table, lengths):
+            # a draft's position: the context, and the drafts it follows
+            positions = (positions.view(B, n)[:, :1] + tree.sum(1) - 1).flatten()
 
-        def attend(q, keys, values):
-            return decoder.cache_attention(q.view(B, n, -1, self.head_dim), keys, values, table, lengths, tree=tree)
+            def attend(q, keys, values):
+                return decoder.cache_attention(q.view(B, n, -1, self.head_dim), keys, values, table, lengths, tree=tree)
 
-        return self._layers(x.reshape(B * n, H), positions, slots, attend).view(B, n, H)
+            return self._layers(x.reshape(B * n, H), positions, slots, attend).view(B, n, H)
 
     def keep(self, sequences, paths, drafts: int):
         """paths[i]: the numbers of the drafts of sequences[i], of ``drafts``, that are
