@@ -19,7 +19,7 @@ import heapq
 import torch
 
 from . import _lib
-from .decoder import (_Strides3, _address, _apart, _bytes, _extent, _gradients, _index, _launch, _overlap, _refuse_device,
+from .decoder import (_Strides3, _address, _apart, _bytes, _capturing, _extent, _gradients, _index, _launch, _overlap, _refuse_device,
                       _refuse_dtype, _refuse_grad, _writable)
 from .ops import _ACT_CODES
 
@@ -253,7 +253,7 @@ class PagePool:
         return self._tensor(slots, torch.int64), self._tensor(positions, torch.int64), self._tensor(cu, torch.int32)
 
     def _uncaptured(self) -> None:
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        if self.device.type == "cuda" and _capturing(self.device.index):
             raise RuntimeError("the books of pages are not for a stream that is being captured")
 
     def _take(self) -> int:

@@ -47,3 +47,40 @@ def test_sequences_from_an_iterator():
     a, b = model.pool.add(), model.pool.add()
     model.step(torch.zeros(7, 8), (s for s in (b, a)), (t for t in (5, 2)))
     assert model.pool.asked == [b, a] and (model.pool.length(a), model.pool.length(b)) == (2, 5)
+
+
+def test_captured_stream_of_the_pools_device(monkeypatch):
+    """The stream that counts is the pool's device's, whichever device is the current one."""
+    now = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.index
+
+        def __exit__(self, *_):
+            now[0] = self.was
+
+    captured = set()
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] in captured)
+    pool = _Books(torch.zeros(2, 8, 4, 1, 2))
+    pool._tensor = lambda values, dtype: torch.tensor(values, dtype=dtype)
+    pool.device = torch.device("cuda", 1)
+    a = pool.add()
+    captured.add(0)  # a graph of another device
+    pool.reserve([a], [3])
+    captured.add(1)
+    for current in (0, 1):
+        now[0] = current
+        for call in (lambda: pool.reserve([a], [1]), lambda: pool.table([a]), pool.compact):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    captured.remove(0)
+    now[0] = 0
+    with pytest.raises(RuntimeError, match="captured"):
+        pool.table([a])
+    assert pool.length(a) == 3
