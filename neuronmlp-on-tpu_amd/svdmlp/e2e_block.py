@@ -460,17 +460,23 @@ def bench_model(S: int, cfg: dict, args) -> dict:
 
 def _serve(torch, weights, n_heads: int, kv_heads: int, x, args, workspace) -> dict:
     """A server's step: args.serve_sequences sequences of S tokens generate one each, and
-    one reads the chunk of args.serve_chunk behind its S tokens."""
+    one reads the chunk of args.serve_chunk behind its S tokens.  All have the same
+    tokens, each in pages of its own."""
     from . import ops
+    from .pages import copy_pages
 
     S, n, chunk = x.shape[0], args.serve_sequences, args.serve_chunk
-    model = SequenceModel(weights, n_heads, kv_heads, -(-S // SequenceModel.PAGE) + (n + 1) * (1 + -(-chunk // SequenceModel.PAGE)),
+    model = SequenceModel(weights, n_heads, kv_heads, n * -(-(S + 1) // SequenceModel.PAGE) + -(-(S + chunk) // SequenceModel.PAGE),
                           workspace=workspace)
     first = model.pool.add()
     for at in range(0, S, chunk):
         out = model.step(x[at:at + chunk], [first], [x[at:at + chunk].shape[0]])
     alone = DecoderModel(weights, n_heads, kv_heads, S, workspace=workspace).prompt(x)[-1].float()
-    others = [model.pool.fork(first) for _ in range(n)]  # the same S tokens, in the same pages
+    others = [model.pool.add() for _ in range(n)]
+    model.pool.reserve(others, [S] * n)
+    source, *copies = model.pool.table([first] + others)[0]
+    for pages in copies:
+        copy_pages(model.pool.caches, source, pages)
     rows = x[torch.arange(n + chunk, device=x.device) % S].contiguous()
     sequences, tokens = others + [first], [1] * n + [chunk]
     model.workspace = ops.svd_mlp_workspace(rows, r=max(max(w["ug"].shape[1], w["ud"].shape[1]) for w in weights), ff=weights[0]["vg"].shape[1])
