@@ -32,7 +32,6 @@
 // loads (bounds, pages, keys), the join a launch of its own: 37 tokens 16 us.
 #include "chunk.hpp"
 #include "pipe_attention.hpp"
-#include "segments.hpp"
 
 namespace svdmlp {
 
@@ -89,10 +88,11 @@ __global__ __launch_bounds__(256, 1) void chunk_pipe_kernel(ChunkParams p, Chunk
 #pragma unroll
     for (int g = 0; g < QG; ++g) tok[g] = min(row0 + (wave * QG + g) * 32 + col, rows - 1) / G;  // rows behind the last repeat it, and are not stored
 
-    for (Segments seg(all, segment_keys(kIds, p.page, KB)); seg.more(); seg.next()) {
-      const int done = all - seg.left;  // keys of the segments before
-      const int kbeg = part.kbeg + done, nkeys = seg.keys(), tiles = (nkeys + KB - 1) / KB;
-      const int first = token0 - done;
+    // Segments of as many keys as have their pages' numbers in LDS.
+    const int most = segment_keys(kIds, p.page, KB) / KB;  // tiles of a segment
+    for (int t0 = 0; t0 * KB < all; t0 += most) {
+      const int kbeg = part.kbeg + t0 * KB, nkeys = (int)min((int64_t)(all - t0 * KB), (int64_t)most * KB), tiles = (nkeys + KB - 1) / KB;
+      const int first = token0 - t0 * KB;
       __syncthreads();  // (with what the last segment left in LDS)
       // The pages' numbers, and whether all are pages of the cache.  One that is not
       // holds no keys: page 0 is read for it, and masked.
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256, 1) void chunk_pipe_kernel(ChunkParams p, Chunk
           qf[g][s] = FULL || c < npieces ? *reinterpret_cast<const u32x4*>(qp + 16 * c) : u32x4{0u, 0u, 0u, 0u};
         }
       }
-      const int full = holes ? 0 : min(max(whole - done / KB, 0), nkeys / KB);
+      const int full = holes ? 0 : min(max(whole - t0, 0), nkeys / KB);
 
       // Lane j's place of load j of a tile of keys, in bytes (behind the last key: rows
       // of its load's page).  Kept for the tile behind the last one asked for.
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256, 1) void chunk_pipe_kernel(ChunkParams p, Chunk
       for (int g = 0; g < QG; ++g)
 #pragma unroll
         for (int s = 0; s < C::STEPS; ++s) asm volatile("" : "+a"(qf[g][s]));
-      if (full > 0) pw.whole_tiles(base, full, t, done > 0, arrive, beside);
+      if (full > 0) pw.whole_tiles(base, full, t, t0 > 0, arrive, beside);
       for (; t < tiles; ++t) {
         arrive(t);
         next = places(t + 4);

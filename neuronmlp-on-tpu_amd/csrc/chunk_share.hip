@@ -13,7 +13,6 @@
 // fp32 heads of 256: 61% busy, 78 TFLOP/s.  64 sequences of 12 tokens, 2000 keys, heads of
 // 128: 160 us, 3.3 TB/s.
 #include "chunk.hpp"
-#include "segments.hpp"
 
 namespace svdmlp {
 
@@ -74,8 +73,10 @@ __global__ __launch_bounds__(256, 1) void chunk_share_kernel(ChunkParams p, Chun
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     uint32_t bad = 0;
 
-    for (Segments seg(piece.kend - piece.kbeg, segment_keys(kShareIds, p.page, KB)); seg.more(); seg.next()) {
-      const int kbeg = piece.kend - seg.left, kend = kbeg + seg.keys(), tiles = (kend - kbeg + KB - 1) / KB;
+    // Segments of as many keys as have their pages' numbers in LDS.
+    const int most = segment_keys(kShareIds, p.page, KB);
+    for (int kbeg = piece.kbeg; kbeg < piece.kend; kbeg += most) {
+      const int kend = (int)min((int64_t)piece.kend, (int64_t)kbeg + most), tiles = (kend - kbeg + KB - 1) / KB;
       __syncthreads();  // (with what the last segment left in LDS)
       // The pages' numbers, and whether all are pages of the cache.  One that is not
       // holds no keys: page 0 is read for it, and masked.

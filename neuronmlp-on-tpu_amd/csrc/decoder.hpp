@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "segments.hpp"
+
 namespace svdmlp {
 
 // Whether one launch can have so many blocks: HIP cuts a grid of 2^32 threads or
@@ -140,7 +142,6 @@ struct ChunkParams {
   int alike;  // keys and values have the same page and token strides, and those and a page are below 2^32 bytes
   float c;    // softmax scale * log2(e)
 };
-constexpr int64_t kChunkTokensMost = 0x7ffe0000;  // of a sequence: room for the last tiles' ends
 struct ChunkPlan {
   ChunkClass many, some, few;  // tiles of 256, 128 and 32 rows
   int64_t floats;              // of the workspace
