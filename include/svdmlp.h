@@ -376,7 +376,8 @@ int svdmlp_cache_attention(const void* q, const void* k_cache, const void* v_cac
  * Attention of packed chunks of new tokens of B sequences onto a paged cache that
  * holds lengths[b] tokens of each, the new ones last among them: those of
  * sequence b are rows cu_seqlens[b] .. cu_seqlens[b + 1] of q (int32, B + 1), any
- * number of them, and each sees the keys up to itself.  Key x of sequence b
+ * number of them, and each sees the keys up to itself.  Of bf16 the weights are
+ * rounded to bf16 before their product with the values.  Key x of sequence b
  * is row x % page of page block_table[b][x / page] (int32, width pages a sequence, at
  * most 65536, and at most 2^31 - 2^17 tokens); a page outside the cache holds no
  * keys.  A token without keys gets zeros; more new tokens than lengths[b]

@@ -1,5 +1,5 @@
 // What the kernels of attention over chunks share (chunk_attention.hip,
-// chunk_wave.hip): which block does what, and where its sums go.
+// chunk_share.hip, chunk_wave.hip): which block does what, and where its sums go.
 #pragma once
 
 #include <math.h>

@@ -30,6 +30,11 @@
 // of the 53 for their starts and ends), some 20 to add them (34 MB of sums of pieces
 // at 2.5 TB/s, whatever the registers, and so waves, of the join).  Few tokens: latency, a chain of
 // loads (bounds, pages, keys), the join a launch of its own: 37 tokens 16 us.
+//
+// bf16: the weights are rounded to bf16 for the second product and summed after it
+// (attn.hpp: why), so that results are off by 0.0020-0.0024 rms of the definition in 64 bits, of
+// which their own rounding is 0.0017; a second part of each weight would halve the rate of that
+// product.  fp32: 3e-7.
 #include "chunk.hpp"
 #include "pipe_attention.hpp"
 

@@ -259,8 +259,8 @@ void run(const ChunkParams& p, const ChunkClass& k, hipStream_t st) {
 
 }  // namespace
 
-// As many stages as leave room for two blocks a CU, or for one where a wave takes
-// over half of a SIMD's registers.
+// Stages for two blocks a CU (plan_chunk_attention takes two of heads up to 128), or
+// for one where a wave takes over half of a SIMD's registers.
 void launch_chunk_shared(const ChunkParams& p, const ChunkClass& k, bool bf16, hipStream_t st) {
   if (bf16) p.D <= 64 ? run<true, 64, 4>(p, k, st) : p.D <= 128 ? run<true, 128, 4>(p, k, st) : run<true, 256, 4>(p, k, st);
   else run<false, 256, 2>(p, k, st);  // (shorter heads: chunk_wave_kernel)

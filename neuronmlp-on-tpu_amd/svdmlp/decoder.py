@@ -644,7 +644,14 @@ def chunk_attention(q, k_cache, v_cache, block_table, lengths, cu_seqlens, *, sc
     Each sees the keys of its sequence up to itself.  block_table and lengths as
     :func:`cache_attention`, cu_seqlens as :func:`prompt_attention`.  A token
     without keys (a sequence with more new tokens than its length) gets zeros; pages outside the cache hold
-    no keys; rows behind the last sequence are not written."""
+    no keys; rows behind the last sequence are not written.
+
+    Sums and the softmax's statistics are held in 32 bits; of bfloat16, as in the other
+    attentions, the weights are rounded to bfloat16 for their product with the values
+    (2^-8 of each at most; results are off by 0.0024 rms, 0.0017 of it their own rounding).
+    Where every sequence has the same 1 to 64 new tokens :func:`cache_attention` takes them
+    too: faster for a few sequences (one of 4097 tokens that generates 13 us, here
+    22), slower for many (96 of 4000: 322, here 300)."""
     qs, cs = q.shape, k_cache.shape
     if len(qs) != 3:
         raise ValueError(f"expected q (new tokens, heads, head size), got {tuple(qs)}")
